@@ -424,6 +424,53 @@ int rdb_gemm_dense_scatter(void *const *dst_ptrs, int ndst, size_t dst_offset_by
                            const void *b, int64_t M, int64_t N, int64_t Kc, int64_t lda, int64_t ldb, int b_kmajor,
                            const rdb_call_options *options, int32_t *status, void *stream);
 
+/*
+ * AdamW over a list of tensors in one launch (no counterpart in the reference, which calls torch.optim: modded-nanogpt/
+ * train_gpt2.py:354-372).  For every element, with t the tensor's step count after this call has raised it by one:
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2          g: gradient times *grad_scale (1 when null)
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in float32.  `tensors` and `h` are HOST memory, read before the call returns; the pointers in them (`step`: the tensor's
+ * float32 count), `grad_scale` and `h->lr_dev` (one float32 each, may be null) are device memory, read and written on `stream`
+ * only, so a captured call replays with new gradients, counts and learning rates.
+ *   param_dtype   RDB_F32, or RDB_BF16 (rounded to nearest after each step; with `master` set -- for all tensors or none --
+ *                 the float32 master copy is what is updated and the parameter receives its rounding)
+ *   grad_dtype    RDB_F32 or RDB_BF16, one type for all tensors
+ *   state_bits    32: exp_avg and exp_avg_sq are float32.
+ *                 8: one byte per element and one float32 scale per RDB_ADAMW_BLOCK consecutive elements of a tensor
+ *                 (ceil(numel / RDB_ADAMW_BLOCK) of them).  exp_avg: float8 e4m3, rounded to nearest, scale = largest
+ *                 magnitude / 448.  exp_avg_sq: no sign, 4 exponent bits (bias 15) and 4 mantissa bits, scale = largest value /
+ *                 1.9375, rounded down or up at random with the odds that keep the expectation (nearest would never let it
+ *                 decay: 1 - beta2 is below half a step of any 8-bit format), never to 0 when positive.  The random bits are
+ *                 the upper 19 of the 1-D noise word of (element index mod 2^32) under the seed
+ *                 h->seed + t * 0x9E3779B1 + i * 0x85EBCA6B (tensor i of the list): the same call gives the same bytes.
+ * Tensors may start at any address their element type allows (vector accesses where all of a tensor's pointers allow them).
+ * Entries of the list must not overlap.  rdb_grad_norm (grads, numels, dtypes: HOST arrays): 2-norm over all gradients in float64 partial sums, repeatable;
+ * coef (may be null) = min(1, max_norm / (norm + 1e-6)), the factor to pass as grad_scale.  workspace: 8-byte aligned.
+ */
+#define RDB_ADAMW_BLOCK 256
+#define RDB_NORM_BLOCKS 1184
+typedef struct rdb_adamw_tensor {
+    void *param;
+    const void *grad;
+    float *master;
+    void *exp_avg;
+    void *exp_avg_sq;
+    float *exp_avg_scale;
+    float *exp_avg_sq_scale;
+    float *step;
+    int64_t numel;
+} rdb_adamw_tensor;
+typedef struct rdb_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    const float *lr_dev;      /* not null: read instead of lr */
+    uint32_t seed;
+} rdb_adamw_hyper;
+int rdb_adamw_step(const rdb_adamw_tensor *tensors, int n, int param_dtype, int grad_dtype, int state_bits,
+                   const rdb_adamw_hyper *h, const float *grad_scale, void *stream);
+size_t rdb_grad_norm_workspace_bytes(int n);
+int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int64_t *numels, const int32_t *dtypes, int n, float max_norm,
+                  void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,6 +41,15 @@ class CallOptions(ctypes.Structure):
         super().__init__(noise_tile, dense_pair, stage_noise, reserve_sms, fill_overlap, grads_beside)
 
 
+class AdamwHyper(ctypes.Structure):
+    """``rdb_adamw_hyper``."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("lr_dev", ctypes.c_void_p), ("seed", ctypes.c_uint32)]
+
+
+ADAMW_WORDS = 9            # rdb_adamw_tensor: eight pointers and an int64, nine 8-byte words
+ADAMW_BLOCK = 256          # RDB_ADAMW_BLOCK
+
 _op = ctypes.POINTER(CallOptions)
 
 # name -> (restype, argtypes); one entry per declaration in the header
@@ -88,6 +97,9 @@ PROTOTYPES = {
     "rdb_scale_bias_bwd_workspace_bytes": (_sz, [_i64]),
     "rdb_scale_bias_bwd": (_i32, [_vp, _vp, _vp, _i64, _u32, _vp]),
     "rdb_embed_fwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _u32, _vp]),
+    "rdb_adamw_step": (_i32, [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(AdamwHyper), _vp, _vp]),
+    "rdb_grad_norm_workspace_bytes": (_sz, [_i32]),
+    "rdb_grad_norm": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, ctypes.c_float, _vp, _sz, _vp]),
     "rdb_embed_bwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _u32, _vp]),
 }
 

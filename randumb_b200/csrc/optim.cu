@@ -1,0 +1,483 @@
+// AdamW over a list of tensors and the norm of a list of gradients (CUDA cores, HBM-bound).
+//
+// One launch walks up to ADAMW_TENSORS tensors: their pointers travel in the kernel's parameters, the elements are cut into
+// chunks of ADAMW_CHUNK, and a block finds the tensor of its chunk by bisection.  A warp owns 256 consecutive elements at a
+// time -- the block of elements that shares the scale of an 8-bit moment, so its maximum is one shuffle reduction and nothing
+// is read twice.  Arithmetic is float32 throughout, one rounding per operation as written (no contraction), so the bytes of
+// the 8-bit moments follow from the inputs alone.
+//
+//   m' = b1 m + (1 - b1) g        v' = b2 v + (1 - b2) g^2
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+#include <cuda_fp8.h>
+#include <math.h>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace rdb {
+
+constexpr int ADAMW_CHUNK = 8192;
+constexpr int ADAMW_THREADS = 256;
+constexpr int SEG = RDB_ADAMW_BLOCK;      // elements per warp pass, and per scale of an 8-bit moment
+static_assert(SEG == 256, "a warp pass is 32 lanes x 8 elements");
+
+struct AdamwDesc {
+    void *p;
+    const void *g;
+    float *master;
+    void *m, *v;
+    float *ms, *vs;
+    float *step;
+    int64_t n;
+};
+
+// NT tensors; first[i] is the first chunk of tensor i, first[count] the number of chunks
+template <int NT>
+struct AdamwTable {
+    AdamwDesc t[NT];
+    uint32_t first[NT + 1];
+    int32_t count;
+    int32_t index0;                       // position of t[0] in the caller's list
+};
+
+struct AdamwScalars {
+    float b1, omb1, b2, omb2, eps;
+    double lr, beta1, beta2;
+    const float *lr_dev;                  // one float32 in device memory, or null: `lr`
+    double weight_decay;
+    uint32_t seed;
+};
+
+// ---- loads and stores of the 8 elements a lane owns: two groups of four, 128 apart (vector form), or eight single elements
+// 32 apart (tensors that do not start on a vector boundary, and the ragged end of a tensor)
+template <typename T> struct Vec4;
+template <> struct Vec4<float> { using V = float4; };
+template <> struct Vec4<__nv_bfloat16> { using V = uint2; };
+template <> struct Vec4<uint8_t> { using V = uint32_t; };
+
+template <bool VEC> __device__ __forceinline__ int elem_of(int lane, int j) {
+    return VEC ? ((j >> 2) * 128 + lane * 4 + (j & 3)) : (j * 32 + lane);
+}
+
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(T (&r)[8], const T *__restrict__ base, int lane, int left) {
+    if (VEC) {
+        using V = typename Vec4<T>::V;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const V v = *reinterpret_cast<const V *>(base + h * 128 + lane * 4);
+            const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[h * 4 + k] = e[k];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int e = j * 32 + lane;
+            T zero{};
+            r[j] = e < left ? base[e] : zero;
+        }
+    }
+}
+
+template <bool VEC, typename T>
+__device__ __forceinline__ void store8(T *__restrict__ base, const T (&r)[8], int lane, int left) {
+    if (VEC) {
+        using V = typename Vec4<T>::V;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            V v;
+            T *e = reinterpret_cast<T *>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e[k] = r[h * 4 + k];
+            *reinterpret_cast<V *>(base + h * 128 + lane * 4) = v;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int e = j * 32 + lane;
+            if (e < left) base[e] = r[j];
+        }
+    }
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+
+// First moment in 8 bits: float8 e4m3 times the scale that puts the block's largest magnitude at 448, rounded to nearest
+// (off by at most 2^-4 of the value; b1 forgets it within a few steps).
+__device__ __forceinline__ float e4m3_value(uint8_t c) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
+    return __half2float(__half(h));
+}
+__device__ __forceinline__ uint8_t e4m3_code(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+
+// Second moment in 8 bits: no sign, 4 exponent bits (bias 15), 4 mantissa bits; byte 255 stands for 1.9375 and carries the
+// block's maximum.  Shifted into a float32 the byte sits on top of exponent and mantissa, so its value is that float32 times
+// 2^112 (subnormals included).  (1 - b2) is far below a step of any 8-bit format: rounding to nearest would leave v where it
+// is however small the gradients become, so v is rounded to one of its two neighbours at random with the odds that keep its
+// expectation: add 19 random bits below the byte and cut.  A positive v never becomes 0: it divides.
+__device__ __forceinline__ float ue4m4_value(uint8_t c) { return __fmul_rn(__uint_as_float((uint32_t)c << 19), 5.192296858534828e33f); }
+__device__ __forceinline__ uint8_t ue4m4_code(float q, float v, uint32_t r19) {
+    uint32_t c = (__float_as_uint(__fmul_rn(q, 1.925929944387236e-34f)) + r19) >> 19;
+    c = c > 255u ? 255u : c;
+    return (uint8_t)((c == 0u && v > 0.0f) ? 1u : c);
+}
+
+template <typename P, typename G, bool MASTER, bool BITS8, bool VEC>
+__device__ __forceinline__ void adamw_segment(const AdamwDesc &d, int64_t at, int left, int lane, const AdamwScalars &s, float gscale,
+                                              float size, float inv_root, float decay, uint32_t rseed) {
+    using S = typename std::conditional<BITS8, uint8_t, float>::type;
+    P p8[8];
+    G g8[8];
+    S m8[8], v8[8];
+    float w8[8];
+    float mscale = 0.0f, vscale = 0.0f;
+    load8<VEC>(g8, reinterpret_cast<const G *>(d.g) + at, lane, left);
+    load8<VEC>(m8, reinterpret_cast<const S *>(d.m) + at, lane, left);
+    load8<VEC>(v8, reinterpret_cast<const S *>(d.v) + at, lane, left);
+    if (MASTER) load8<VEC>(w8, const_cast<const float *>(d.master) + at, lane, left);
+    else load8<VEC>(p8, const_cast<const P *>(reinterpret_cast<P *>(d.p)) + at, lane, left);
+    if (BITS8) {
+        mscale = d.ms[at / SEG];
+        vscale = d.vs[at / SEG];
+    }
+    float m[8], v[8];
+    float mmax = 0.0f, vmax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float g = __fmul_rn(to_f32<G>(g8[j]), gscale);
+        float m0, v0;
+        if (BITS8) {
+            m0 = __fmul_rn(e4m3_value(*reinterpret_cast<uint8_t *>(&m8[j])), mscale);
+            v0 = __fmul_rn(ue4m4_value(*reinterpret_cast<uint8_t *>(&v8[j])), vscale);
+        } else {
+            m0 = *reinterpret_cast<float *>(&m8[j]);
+            v0 = *reinterpret_cast<float *>(&v8[j]);
+        }
+        m[j] = __fadd_rn(__fmul_rn(m0, s.b1), __fmul_rn(g, s.omb1));
+        v[j] = __fadd_rn(__fmul_rn(v0, s.b2), __fmul_rn(__fmul_rn(g, g), s.omb2));
+        mmax = fmaxf(mmax, fabsf(m[j]));
+        vmax = fmaxf(vmax, v[j]);
+        const float p = MASTER ? w8[j] : to_f32<P>(p8[j]);
+        const float upd = __fdiv_rn(m[j], __fadd_rn(__fmul_rn(__fsqrt_rn(v[j]), inv_root), s.eps));
+        const float q = __fsub_rn(__fmul_rn(p, decay), __fmul_rn(size, upd));
+        if (MASTER) w8[j] = q;
+        p8[j] = from_f32<P>(q);
+    }
+    store8<VEC>(reinterpret_cast<P *>(d.p) + at, p8, lane, left);
+    if (MASTER) store8<VEC>(d.master + at, w8, lane, left);
+    if (BITS8) {
+        mscale = __fdiv_rn(warp_max(mmax), 448.0f);
+        vscale = __fdiv_rn(warp_max(vmax), 1.9375f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float qm = mscale > 0.0f ? __fdiv_rn(m[j], mscale) : 0.0f;
+            const float qv = vscale > 0.0f ? __fdiv_rn(v[j], vscale) : 0.0f;
+            const uint32_t pos = (uint32_t)(at + elem_of<VEC>(lane, j));
+            const uint32_t r19 = sq5_tail(pos * SQ5_N1 + rseed) >> 13;
+            *reinterpret_cast<uint8_t *>(&m8[j]) = e4m3_code(qm);
+            *reinterpret_cast<uint8_t *>(&v8[j]) = ue4m4_code(qv, v[j], r19);
+        }
+        if (lane == 0) {
+            d.ms[at / SEG] = mscale;
+            d.vs[at / SEG] = vscale;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            *reinterpret_cast<float *>(&m8[j]) = m[j];
+            *reinterpret_cast<float *>(&v8[j]) = v[j];
+        }
+    }
+    store8<VEC>(reinterpret_cast<S *>(d.m) + at, m8, lane, left);
+    store8<VEC>(reinterpret_cast<S *>(d.v) + at, v8, lane, left);
+}
+
+template <typename Table>
+__device__ __forceinline__ int find_tensor(const Table &tab, uint32_t chunk) {
+    int lo = 0, hi = tab.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.first[mid] <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// every tensor's step count, one more; a launch of its own, before any block of the update reads a count
+template <int NT>
+struct StepTable {
+    float *step[NT];
+    int32_t count;
+};
+template <int NT>
+__global__ void adamw_count_kernel(const __grid_constant__ StepTable<NT> tab) {
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int i = threadIdx.x; i < tab.count; i += blockDim.x) *tab.step[i] += 1.0f;
+}
+
+template <typename P, typename G, bool MASTER, bool BITS8, int NT>
+__global__ void __launch_bounds__(ADAMW_THREADS)
+adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, const float *__restrict__ grad_scale) {
+    __shared__ float sh[3];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float gscale = grad_scale ? *grad_scale : 1.0f;
+    const uint32_t chunks = tab.first[tab.count];
+    int cur = -1;
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int ti = find_tensor(tab, c);
+        const AdamwDesc &d = tab.t[ti];
+        if (ti != cur) {                  // bias corrections of this tensor's step, in float64
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const double t = (double)*d.step;
+                const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
+                sh[0] = (float)(lr / (1.0 - pow(s.beta1, t)));
+                sh[1] = (float)(1.0 / sqrt(1.0 - pow(s.beta2, t)));
+                sh[2] = (float)(1.0 - lr * s.weight_decay);
+            }
+            __syncthreads();
+            cur = ti;
+        }
+        const float size = sh[0], inv_root = sh[1], decay = sh[2];
+        const uint32_t rseed = BITS8 ? s.seed + (uint32_t)(int64_t)*d.step * 0x9E3779B1u + (uint32_t)(tab.index0 + ti) * 0x85EBCA6Bu : 0u;
+        const int64_t lo = (int64_t)(c - tab.first[ti]) * ADAMW_CHUNK;
+        const int64_t hi = lo + ADAMW_CHUNK < d.n ? lo + ADAMW_CHUNK : d.n;
+        constexpr uintptr_t PV = sizeof(P) * 4 - 1, GV = sizeof(G) * 4 - 1, SV = BITS8 ? 3 : 15;
+        const bool vec = ((reinterpret_cast<uintptr_t>(d.p) & PV) | (reinterpret_cast<uintptr_t>(d.g) & GV) |
+                          (reinterpret_cast<uintptr_t>(d.m) & SV) | (reinterpret_cast<uintptr_t>(d.v) & SV) |
+                          (MASTER ? reinterpret_cast<uintptr_t>(d.master) & 15 : 0)) == 0;
+        for (int64_t at = lo + warp * SEG; at < hi; at += (ADAMW_THREADS / 32) * SEG) {
+            const int left = (int)(hi - at < SEG ? hi - at : SEG);
+            if (vec && left == SEG)
+                adamw_segment<P, G, MASTER, BITS8, true>(d, at, left, lane, s, gscale, size, inv_root, decay, rseed);
+            else
+                adamw_segment<P, G, MASTER, BITS8, false>(d, at, left, lane, s, gscale, size, inv_root, decay, rseed);
+        }
+    }
+}
+
+// ---- norm ----------------------------------------------------------------------------------------------------------------
+// Sum of squares: float32 within the 8 elements a lane reads at a time, float64 above; one partial sum per block in the
+// workspace, added in block order by one block, so the result repeats run to run.
+template <typename G, int NT>
+__global__ void __launch_bounds__(ADAMW_THREADS)
+sumsq_kernel(const __grid_constant__ AdamwTable<NT> tab, double *__restrict__ partial) {
+    __shared__ double sh[ADAMW_THREADS / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t chunks = tab.first[tab.count];
+    double acc = 0.0;
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int ti = find_tensor(tab, c);
+        const AdamwDesc &d = tab.t[ti];
+        const int64_t lo = (int64_t)(c - tab.first[ti]) * ADAMW_CHUNK;
+        const int64_t hi = lo + ADAMW_CHUNK < d.n ? lo + ADAMW_CHUNK : d.n;
+        const bool vec = (reinterpret_cast<uintptr_t>(d.g) & (sizeof(G) * 4 - 1)) == 0;
+        for (int64_t at = lo + warp * SEG; at < hi; at += (ADAMW_THREADS / 32) * SEG) {
+            const int left = (int)(hi - at < SEG ? hi - at : SEG);
+            G g8[8];
+            if (vec && left == SEG) load8<true>(g8, reinterpret_cast<const G *>(d.g) + at, lane, left);
+            else load8<false>(g8, reinterpret_cast<const G *>(d.g) + at, lane, left);
+            float f = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f += to_f32<G>(g8[j]) * to_f32<G>(g8[j]);
+            acc += (double)f;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (lane == 0) sh[warp] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < ADAMW_THREADS / 32; ++i) t += sh[i];
+        partial[blockIdx.x] = t;
+    }
+}
+
+// norm, and the factor that brings it down to max_norm (1 when it is below; max_norm < 0: none asked for)
+__global__ void __launch_bounds__(256) norm_finish_kernel(float *__restrict__ norm, float *__restrict__ coef, const double *__restrict__ partial,
+                                                          int n, float max_norm) {
+    __shared__ double sh[256];
+    pdl_launch_dependents();
+    pdl_wait();
+    double a = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) a += partial[i];
+    sh[threadIdx.x] = a;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const float nv = (float)sqrt(sh[0]);
+        if (norm) *norm = nv;
+        if (coef) {
+            const float c = max_norm / (nv + 1e-6f);
+            *coef = c > 1.0f ? 1.0f : c;          // not-a-number stays one
+        }
+    }
+}
+
+static int norm_blocks(uint32_t chunks) { return (int)(chunks < (uint32_t)RDB_NORM_BLOCKS ? (chunks ? chunks : 1) : RDB_NORM_BLOCKS); }
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+constexpr int NT_SMALL = 48, NT_LARGE = 384;      // tensors per launch: 3.5 KB or 26 KB of kernel parameters
+static_assert(sizeof(AdamwTable<NT_LARGE>) + 512 < 32764, "kernel parameters");
+
+template <int NT>
+static int fill_table(AdamwTable<NT> *tab, const rdb_adamw_tensor *t, int n, int index0) {
+    uint64_t c = 0;
+    for (int i = 0; i < n; ++i) {
+        tab->t[i] = AdamwDesc{t[i].param, t[i].grad, t[i].master, t[i].exp_avg, t[i].exp_avg_sq, t[i].exp_avg_scale, t[i].exp_avg_sq_scale, t[i].step, t[i].numel};
+        tab->first[i] = (uint32_t)c;
+        c += (uint64_t)cdiv64(t[i].numel, ADAMW_CHUNK);
+        if (c >= (1ull << 32)) return RDB_ERR_TOO_LARGE;
+    }
+    tab->first[n] = (uint32_t)c;
+    tab->count = n;
+    tab->index0 = index0;
+    return RDB_OK;
+}
+
+template <typename P, typename G, bool MASTER, bool BITS8, int NT>
+static int launch_adamw(const rdb_adamw_tensor *t, int n, int index0, const AdamwScalars &s, const float *gs, cudaStream_t st) {
+    AdamwTable<NT> tab;
+    StepTable<NT> steps;
+    int rc = fill_table(&tab, t, n, index0);
+    if (rc) return rc;
+    for (int i = 0; i < n; ++i) steps.step[i] = t[i].step;
+    steps.count = n;
+    rc = launch_pdl(adamw_count_kernel<NT>, dim3(1), 256, 0, st, steps);
+    if (rc) return rc;
+    const uint32_t chunks = tab.first[n];
+    if (chunks == 0) return RDB_OK;
+    const uint32_t cap = 148 * 8;
+    return launch_pdl(adamw_kernel<P, G, MASTER, BITS8, NT>, dim3(chunks < cap ? chunks : cap), ADAMW_THREADS, 0, st, tab, s, gs);
+}
+
+template <typename P, typename G, bool MASTER, bool BITS8>
+static int adamw_all(const rdb_adamw_tensor *t, int n, const AdamwScalars &s, const float *gs, cudaStream_t st) {
+    for (int i = 0; i < n;) {
+        const int k = n - i < NT_LARGE ? n - i : NT_LARGE;
+        const int rc = k <= NT_SMALL ? launch_adamw<P, G, MASTER, BITS8, NT_SMALL>(t + i, k, i, s, gs, st)
+                                     : launch_adamw<P, G, MASTER, BITS8, NT_LARGE>(t + i, k, i, s, gs, st);
+        if (rc) return rc;
+        i += k;
+    }
+    return RDB_OK;
+}
+
+template <typename G, int NT>
+static int launch_sumsq(const rdb_adamw_tensor *t, int n, double *partial, int *used, cudaStream_t st) {
+    AdamwTable<NT> tab;
+    int rc = fill_table(&tab, t, n, 0);
+    if (rc) return rc;
+    *used = norm_blocks(tab.first[n]);
+    return launch_pdl(sumsq_kernel<G, NT>, dim3(*used), ADAMW_THREADS, 0, st, tab, partial);
+}
+
+}  // namespace rdb
+
+using namespace rdb;
+
+extern "C" int rdb_adamw_step(const rdb_adamw_tensor *tensors, int n, int param_dtype, int grad_dtype, int state_bits,
+                              const rdb_adamw_hyper *h, const float *grad_scale, void *stream) {
+    if (n < 0 || !h) return n < 0 ? RDB_ERR_SHAPE : RDB_ERR_NULL;
+    if (n == 0) return RDB_OK;
+    if (!tensors) return RDB_ERR_NULL;
+    if ((param_dtype != RDB_F32 && param_dtype != RDB_BF16) || (grad_dtype != RDB_F32 && grad_dtype != RDB_BF16)) return RDB_ERR_DTYPE;
+    if (state_bits != 32 && state_bits != 8) return RDB_ERR_DTYPE;
+    if (!(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0) || !(h->eps >= 0.0)) return RDB_ERR_UNSUPPORTED;
+    bool master = false;
+    for (int i = 0; i < n; ++i) master = master || tensors[i].master != nullptr;
+    for (int i = 0; i < n; ++i) {
+        const rdb_adamw_tensor &t = tensors[i];
+        if (t.numel < 0) return RDB_ERR_SHAPE;
+        if (!t.step) return RDB_ERR_NULL;
+        if (t.numel == 0) continue;
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return RDB_ERR_NULL;
+        if (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return RDB_ERR_NULL;
+        if ((t.master != nullptr) != master || (master && param_dtype != RDB_BF16)) return RDB_ERR_UNSUPPORTED;
+        const uintptr_t pm = dtype_size(param_dtype) - 1, gm = dtype_size(grad_dtype) - 1, sm = state_bits == 8 ? 0 : 3;
+        if ((reinterpret_cast<uintptr_t>(t.param) & pm) || (reinterpret_cast<uintptr_t>(t.grad) & gm) || (reinterpret_cast<uintptr_t>(t.exp_avg) & sm) ||
+            (reinterpret_cast<uintptr_t>(t.exp_avg_sq) & sm) || (reinterpret_cast<uintptr_t>(t.master) & 3))
+            return RDB_ERR_ALIGN;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    AdamwScalars s;
+    s.b1 = (float)h->beta1;
+    s.omb1 = (float)(1.0 - h->beta1);
+    s.b2 = (float)h->beta2;
+    s.omb2 = (float)(1.0 - h->beta2);
+    s.eps = (float)h->eps;
+    s.lr = h->lr;
+    s.beta1 = h->beta1;
+    s.beta2 = h->beta2;
+    s.lr_dev = h->lr_dev;
+    s.weight_decay = h->weight_decay;
+    s.seed = h->seed;
+    const bool b8 = state_bits == 8;
+#define RDB_ADAMW(P, G, M) (b8 ? adamw_all<P, G, M, true>(tensors, n, s, grad_scale, st) : adamw_all<P, G, M, false>(tensors, n, s, grad_scale, st))
+    if (param_dtype == RDB_F32) return grad_dtype == RDB_F32 ? RDB_ADAMW(float, float, false) : RDB_ADAMW(float, __nv_bfloat16, false);
+    if (master) return grad_dtype == RDB_F32 ? RDB_ADAMW(__nv_bfloat16, float, true) : RDB_ADAMW(__nv_bfloat16, __nv_bfloat16, true);
+    return grad_dtype == RDB_F32 ? RDB_ADAMW(__nv_bfloat16, float, false) : RDB_ADAMW(__nv_bfloat16, __nv_bfloat16, false);
+#undef RDB_ADAMW
+}
+
+extern "C" size_t rdb_grad_norm_workspace_bytes(int n) {
+    const int64_t launches = (n > 0 ? cdiv64(n, NT_LARGE) : 0) + 1;     // one more: the two types' lists are filled apart
+    return (size_t)launches * RDB_NORM_BLOCKS * sizeof(double);
+}
+
+extern "C" int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int64_t *numels, const int32_t *dtypes, int n,
+                             float max_norm, void *workspace, size_t workspace_bytes, void *stream) {
+    if (n < 0) return RDB_ERR_SHAPE;
+    if (!norm && !coef) return RDB_ERR_NULL;
+    if (n > 0 && (!grads || !numels || !dtypes)) return RDB_ERR_NULL;
+    if (coef && !(max_norm >= 0.0f)) return RDB_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < rdb_grad_norm_workspace_bytes(n) || (reinterpret_cast<uintptr_t>(workspace) & 7)) return RDB_ERR_WORKSPACE;
+    for (int i = 0; i < n; ++i) {
+        if (dtypes[i] != RDB_F32 && dtypes[i] != RDB_BF16) return RDB_ERR_DTYPE;
+        if (numels[i] < 0) return RDB_ERR_SHAPE;
+        if (numels[i] > 0 && !grads[i]) return RDB_ERR_NULL;
+        if (reinterpret_cast<uintptr_t>(grads[i]) & (dtype_size(dtypes[i]) - 1)) return RDB_ERR_ALIGN;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    double *partial = reinterpret_cast<double *>(workspace);
+    int filled = 0;
+    rdb_adamw_tensor part[NT_LARGE];
+    for (int dtype = RDB_F32; dtype <= RDB_BF16; ++dtype) {       // one launch holds gradients of one type
+        int k = 0;
+        for (int i = 0; i <= n; ++i) {
+            if (i < n && (dtypes[i] != dtype || numels[i] == 0)) continue;
+            if (k == NT_LARGE || (i == n && k > 0)) {
+                int used = 0, rc;
+                if (dtype == RDB_F32)
+                    rc = k <= NT_SMALL ? launch_sumsq<float, NT_SMALL>(part, k, partial + filled, &used, st)
+                                       : launch_sumsq<float, NT_LARGE>(part, k, partial + filled, &used, st);
+                else
+                    rc = k <= NT_SMALL ? launch_sumsq<__nv_bfloat16, NT_SMALL>(part, k, partial + filled, &used, st)
+                                       : launch_sumsq<__nv_bfloat16, NT_LARGE>(part, k, partial + filled, &used, st);
+                if (rc) return rc;
+                filled += used;
+                k = 0;
+            }
+            if (i < n) {
+                part[k] = rdb_adamw_tensor{};
+                part[k].grad = grads[i];
+                part[k++].numel = numels[i];
+            }
+        }
+    }
+    return launch_pdl(norm_finish_kernel, dim3(1), 256, 0, st, norm, coef, (const double *)partial, filled, max_norm);
+}

@@ -1,0 +1,283 @@
+"""Optimiser of a training step: AdamW over all tensors in one launch, and the norm of all gradients.
+
+``adamw_step`` / ``grad_norm`` are the functional forms over lists of tensors; ``AdamW`` is the ``torch.optim.Optimizer`` on top of
+them.  Everything a step depends on that changes from step to step (gradients, step counts, clipping factor, optionally the
+learning rate) is read on the device, so a captured step replays correctly and nothing waits for the host.  The reference trains
+its coefficients with torch.optim (modded-nanogpt/train_gpt2.py:354-372).
+
+All tensors must be CUDA tensors: there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from . import kernels as K
+
+BLOCK = _lib.ADAMW_BLOCK
+
+
+def _uniform(what: str, ts: Sequence[torch.Tensor], dtypes, n: int, dev: torch.device) -> torch.dtype:
+    if len(ts) != n:
+        raise RuntimeError(f"adamw_step: {n} params but {len(ts)} {what}")
+    kinds = {t.dtype for t in ts}
+    if len(kinds) != 1 or next(iter(kinds)) not in dtypes:
+        raise RuntimeError(f"adamw_step: {what} must all have one type out of {sorted(str(d) for d in dtypes)}, got {sorted(str(d) for d in kinds)}")
+    if {t.device for t in ts} != {dev}:
+        raise RuntimeError(f"adamw_step: {what} must live on {dev}")
+    if not all([t.is_contiguous() for t in ts]):
+        raise RuntimeError(f"adamw_step: {what} must be contiguous")
+    return next(iter(kinds))
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+               exp_avg_sqs: Sequence[torch.Tensor], steps: Union[torch.Tensor, Sequence[torch.Tensor]], *,
+               lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, masters: Optional[Sequence[torch.Tensor]] = None,
+               exp_avg_scales: Optional[Sequence[torch.Tensor]] = None, exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
+               seed: int = 0, grad_scale: Optional[torch.Tensor] = None) -> None:
+    """One AdamW step over a list of contiguous tensors, in place (see rdb_adamw_step for the formula and the 8-bit formats).
+
+    params      float32, or bfloat16 (all of one type); grads: float32 or bfloat16, same sizes.
+    exp_avgs / exp_avg_sqs   float32 moments; or, with ``exp_avg_scales`` and ``exp_avg_sq_scales`` (float32, one per 256
+                consecutive elements of a tensor), 8-bit moments: float8_e4m3fn and uint8 (no sign, 4 exponent and 4 mantissa bits).
+    steps       float32 step counts on the device, raised by one here: one tensor with an element per param, or a list of
+                one-element tensors.
+    lr          a number, or a one-element float32 CUDA tensor that is read when the step runs.
+    masters     float32 copies of bfloat16 params: they are updated, the params receive their rounding.
+    seed        of the random rounding of the 8-bit second moments.
+    grad_scale  one-element float32 CUDA tensor the gradients are multiplied with (the factor ``grad_norm`` returns).
+    """
+    n = len(params)
+    if n == 0:
+        return
+    dev = K._need_cuda(*params)
+    pd = _uniform("params", params, (torch.float32, torch.bfloat16), n, dev)
+    gd = _uniform("grads", grads, (torch.float32, torch.bfloat16), n, dev)
+    eight = exp_avg_scales is not None or exp_avg_sq_scales is not None
+    if eight:
+        if exp_avg_scales is None or exp_avg_sq_scales is None:
+            raise RuntimeError("adamw_step: 8-bit moments need exp_avg_scales and exp_avg_sq_scales")
+        _uniform("exp_avg_scales", exp_avg_scales, (torch.float32,), n, dev)
+        _uniform("exp_avg_sq_scales", exp_avg_sq_scales, (torch.float32,), n, dev)
+    _uniform("exp_avgs", exp_avgs, (torch.float8_e4m3fn,) if eight else (torch.float32,), n, dev)
+    _uniform("exp_avg_sqs", exp_avg_sqs, (torch.uint8,) if eight else (torch.float32,), n, dev)
+    if masters is not None:
+        _uniform("masters", masters, (torch.float32,), n, dev)
+        if pd != torch.bfloat16:
+            raise RuntimeError("adamw_step: masters are the float32 copies of bfloat16 params")
+    numels = [t.numel() for t in params]
+    for what, ts in (("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs), ("masters", masters)):
+        if ts is not None and [t.numel() for t in ts] != numels:
+            raise RuntimeError(f"adamw_step: {what} and params differ in size")
+    if eight:
+        blocks = [-(-k // BLOCK) for k in numels]
+        if [t.numel() for t in exp_avg_scales] != blocks or [t.numel() for t in exp_avg_sq_scales] != blocks:
+            raise RuntimeError(f"adamw_step: scales hold one value per {BLOCK} elements of their tensor")
+    if isinstance(steps, torch.Tensor):
+        if steps.dtype != torch.float32 or steps.device != dev or steps.numel() != n or not steps.is_contiguous():
+            raise RuntimeError(f"adamw_step: steps must be {n} contiguous float32 counts on {dev}")
+        sp = range(steps.data_ptr(), steps.data_ptr() + 4 * n, 4)
+    else:
+        _uniform("steps", steps, (torch.float32,), n, dev)
+        if any([t.numel() != 1 for t in steps]):
+            raise RuntimeError("adamw_step: every tensor has one step count")
+        sp = [t.data_ptr() for t in steps]
+    pp = [t.data_ptr() for t in params]
+    if len(set(pp)) != n and len({a for a, k in zip(pp, numels) if k}) != sum(1 for k in numels if k):
+        raise RuntimeError("adamw_step: a param is in the list twice")
+    _one_float("grad_scale", grad_scale, dev)
+    lr_dev = None
+    if isinstance(lr, torch.Tensor):
+        _one_float("lr", lr, dev)
+        lr, lr_dev = 0.0, lr.data_ptr()
+    none = [0] * n
+    cols = (pp, [t.data_ptr() for t in grads], [t.data_ptr() for t in masters] if masters is not None else none,
+            [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
+            [t.data_ptr() for t in exp_avg_scales] if eight else none, [t.data_ptr() for t in exp_avg_sq_scales] if eight else none, sp, numels)
+    words = (ctypes.c_uint64 * (_lib.ADAMW_WORDS * n))()
+    for i, col in enumerate(cols):
+        words[i::_lib.ADAMW_WORDS] = col
+    h = _lib.AdamwHyper(float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), lr_dev, K._seed(seed))
+    with torch.cuda.device(dev):
+        rc = _lib.lib().rdb_adamw_step(words, n, K._dt(pd), K._dt(gd), 8 if eight else 32, ctypes.byref(h), K._ptr(grad_scale), K._stream(dev))
+    _lib.check(rc, "rdb_adamw_step")
+
+
+def _one_float(what: str, t: Optional[torch.Tensor], dev: torch.device) -> None:
+    if t is not None and (t.dtype != torch.float32 or t.numel() != 1 or t.device != dev):
+        raise RuntimeError(f"{what} must be a one-element float32 tensor on {dev}")
+
+
+def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(norm, factor): 2-norm over all gradients (float32 or bfloat16, contiguous, types may be mixed), and with ``max_norm`` the
+    factor ``min(1, max_norm / (norm + 1e-6))`` to pass to ``adamw_step`` as ``grad_scale``.  Both are 0-d float32 tensors on the
+    device; nothing is written to the gradients and nothing waits.  A gradient that holds a NaN or an infinity makes the norm
+    one too, and the factor NaN or 0."""
+    n = len(grads)
+    if n == 0:
+        raise RuntimeError("grad_norm: no gradients")
+    dev = K._need_cuda(*grads)
+    if not all([t.is_contiguous() for t in grads]):
+        raise RuntimeError("grad_norm: gradients must be contiguous")
+    if max_norm is not None and not max_norm >= 0.0:
+        raise RuntimeError(f"grad_norm: max_norm must not be negative, got {max_norm}")
+    out = torch.empty((2,), dtype=torch.float32, device=dev)
+    L = _lib.lib()
+    ptrs = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in grads])
+    numels = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
+    kinds = (ctypes.c_int32 * n)(*[K._dt(t.dtype) for t in grads])
+    ws = K._workspace(L.rdb_grad_norm_workspace_bytes(n), dev)
+    clip = max_norm is not None
+    with torch.cuda.device(dev):
+        rc = L.rdb_grad_norm(out.data_ptr(), out.data_ptr() + 4 if clip else None, ptrs, numels, kinds, n, float(max_norm) if clip else 0.0, K._ptr(ws),
+                             ws.numel(), K._stream(dev))
+    _lib.check(rc, "rdb_grad_norm")
+    return out[0], out[1] if clip else None
+
+
+def second_moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """float32 values of an 8-bit second moment (uint8 codes of ``adamw_step`` and their scales), in the shape of ``codes``."""
+    v = (codes.reshape(-1).to(torch.int32) << 19).view(torch.float32) * 2.0 ** 112
+    return (v * scales.repeat_interleave(BLOCK)[:v.numel()]).reshape(codes.shape)
+
+
+def first_moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """float32 values of an 8-bit first moment (float8_e4m3fn codes of ``adamw_step`` and their scales)."""
+    return (codes.reshape(-1).float() * scales.repeat_interleave(BLOCK)[:codes.numel()]).reshape(codes.shape)
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` on one launch per (parameter type, gradient type) and group, with 32-bit or 8-bit moments.
+
+    Args:
+        params, lr, betas, eps, weight_decay: as torch.optim.AdamW; ``lr`` may be a one-element float32 CUDA tensor, read when the
+            step runs (a schedule then works inside a captured step).
+        state_bits: 32 or 8 (2 bytes and a little per element instead of 8; formats at ``adamw_step``).
+        master_weights: keep a float32 copy of every bfloat16 parameter and update that (default True: with bfloat16 alone an
+            update below 2^-9 of the weight is lost).  float32 parameters have none.
+        max_grad_norm: clip the norm of all gradients of all groups to this value, without writing to the gradients.
+        seed: of the random rounding of 8-bit second moments.
+
+    ``step()`` returns the closure's loss; ``last_grad_norm`` holds the norm of the last step (a device tensor) with ``max_grad_norm``.
+    The first step creates the state and cannot be captured; later ones can.
+    """
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = True, max_grad_norm: Optional[float] = None,
+                 seed: int = 0):
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"invalid learning rate: {lr}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"invalid betas: {betas}")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"invalid eps or weight_decay: {eps}, {weight_decay}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"invalid max_grad_norm: {max_grad_norm}")
+        self.max_grad_norm, self.seed, self.last_grad_norm = max_grad_norm, int(seed), None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights))
+
+    def _new_state(self, p: torch.Tensor, group: dict) -> dict:
+        if p.dtype not in (torch.float32, torch.bfloat16) or not p.is_cuda:
+            raise RuntimeError(f"AdamW takes float32 and bfloat16 CUDA parameters, got {p.dtype} on {p.device}")
+        _flat(p)                                                    # refuses a parameter whose elements are not one block of memory
+        st = {"step": torch.zeros((), dtype=torch.float32, device=p.device)}
+        if group["state_bits"] == 32:
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        else:
+            blocks = -(-p.numel() // BLOCK)
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.uint8).view(torch.float8_e4m3fn)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.uint8)
+            st["exp_avg_scale"] = torch.zeros((blocks,), dtype=torch.float32, device=p.device)
+            st["exp_avg_sq_scale"] = torch.zeros((blocks,), dtype=torch.float32, device=p.device)
+        if p.dtype == torch.bfloat16 and group["master_weights"]:
+            st["master"] = p.detach().float()
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        todo, all_grads = [], {}
+        for gi, group in enumerate(self.param_groups):
+            kinds: dict = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                if not self.state[p]:
+                    self.state[p].update(self._new_state(p, group))
+                g = p.grad
+                if g.stride() != p.stride() or g.dtype not in (torch.float32, torch.bfloat16):
+                    g = torch.empty_like(p).copy_(g)               # the parameter's own order of elements
+                kinds.setdefault((p.device, p.dtype, g.dtype, "master" in self.state[p]), []).append((p, _flat(g)))
+            for kind, pairs in kinds.items():
+                todo.append((gi, group, kind, pairs))
+                all_grads.setdefault(kind[0], []).extend(g for _, g in pairs)
+        scales = {}
+        if self.max_grad_norm is not None and all_grads:
+            if len(all_grads) > 1:
+                raise RuntimeError("max_grad_norm: the parameters must live on one device")
+            for dev, grads in all_grads.items():
+                self.last_grad_norm, scales[dev] = grad_norm(grads, self.max_grad_norm)
+        for k, (gi, group, kind, pairs) in enumerate(todo):
+            states = [self.state[p] for p, _ in pairs]
+            eight = {}
+            if group["state_bits"] == 8:
+                eight = dict(exp_avg_scales=[s["exp_avg_scale"] for s in states], exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states],
+                             seed=self.seed + 0x632BE5AB * k)
+            adamw_step([_flat(p) for p, _ in pairs], [g for _, g in pairs], [_flat(s["exp_avg"]) for s in states],
+                       [_flat(s["exp_avg_sq"]) for s in states], [s["step"] for s in states], lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"], masters=[_flat(s["master"]) for s in states] if kind[3] else None,
+                       grad_scale=scales.get(kind[0]), **eight)
+        return loss
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, but every state tensor keeps its own type (moments and masters of a bfloat16 parameter are not bfloat16).  The
+        groups' hyperparameters, ``state_bits`` and ``master_weights`` among them, become the checkpoint's; what a checkpoint of
+        torch.optim.AdamW does not have keeps this optimiser's values, and its float32 moments load into 32-bit ones."""
+        here = [dict(g) for g in self.param_groups]
+        super().load_state_dict(state_dict)
+        for group, old in zip(self.param_groups, here):
+            for k in ("state_bits", "master_weights"):
+                group.setdefault(k, old[k])
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        places = [(p, g) for g in self.param_groups for p in g["params"]]
+        for i, (p, group) in zip(ids, places):
+            if i not in state_dict["state"]:
+                continue
+            src, dst = state_dict["state"][i], self._new_state(p, group)
+            if set(src) != set(dst):
+                raise RuntimeError(f"AdamW: the checkpoint holds {sorted(src)} for a parameter whose state is {sorted(dst)}: other state_bits or masters")
+            for k, t in dst.items():
+                v = src[k] if isinstance(src[k], torch.Tensor) else torch.tensor(float(src[k]))
+                if v.dtype != t.dtype or v.numel() != t.numel():
+                    raise RuntimeError(f"AdamW: {k} is {v.dtype} of {v.numel()} in the checkpoint, {t.dtype} of {t.numel()} here")
+                if "exp_avg_scale" in dst and v.dim() and not v.is_contiguous() == t.is_contiguous():
+                    raise RuntimeError("AdamW: the checkpoint's parameter has its elements in another order, which 8-bit moments cannot follow")
+                if t.dtype == torch.float8_e4m3fn:
+                    t, v = t.view(torch.uint8), v.view(torch.uint8)
+                t.copy_(v.reshape(t.shape))
+            self.state[p] = dst
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """The elements of a dense tensor in memory order (any permutation of its dimensions)."""
+    t = t.detach()
+    if t.is_contiguous():
+        return t
+    acc = 1
+    for size, stride in sorted(((n, st) for n, st in zip(t.shape, t.stride()) if n > 1), key=lambda x: x[1]):
+        if stride != acc:
+            raise RuntimeError("AdamW needs parameters whose elements are one block of memory")
+        acc *= size
+    return t.as_strided((t.numel(),), (1,))

@@ -1,0 +1,304 @@
+"""AdamW and the gradient norm on the GPU against plain 64-bit implementations.
+
+Tolerances.  One float32 operation is off by at most half a step, u = 2^-24 of its value.  A moment is a sum of two rounded products:
+|dm| <= 2 u (|b1 m| + |(1 - b1) g|) and one u more where the gradient is scaled first.  The update m / (sqrt(v) / root + eps) adds
+the roundings of v (3 u, halved by the root), sqrt, product, sum, quotient, size: below 10 u relative to the update's own terms.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+SIZES = [1, 3, 255, 256, 257, 1000, 8192, 8193, 20001]
+
+
+@pytest.fixture(scope="module")
+def rb():
+    import randumb_b200
+    assert torch.cuda.is_available()
+    return randumb_b200
+
+
+def make(sizes, pdtype, gdtype, seed, shift=0):
+    """Tensors carved out of one buffer, `shift` elements off its start: most of them begin on no vector boundary."""
+    g = torch.Generator().manual_seed(seed)
+    n = sum(sizes)
+
+    def carve(flat):
+        buf = torch.zeros(n + shift, dtype=flat.dtype, device="cuda")
+        buf[shift:] = flat.cuda()
+        out, at = [], shift
+        for k in sizes:
+            out.append(buf[at:at + k])
+            at += k
+        return out
+
+    p = torch.randn(n, generator=g) * 0.05
+    gr = torch.randn(n, generator=g) * torch.exp(2 * torch.randn(n, generator=g)) * 1e-3
+    m = torch.randn(n, generator=g) * 1e-3
+    v = torch.rand(n, generator=g) * 1e-6
+    return carve(p.to(pdtype)), carve(gr.to(gdtype)), carve(m), carve(v), carve
+
+
+def plain(p, g, m, v, t, lr, b1, b2, eps, wd, gs=1.0):
+    """The definition in 64 bits."""
+    g = g.double() * gs
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    upd = (m / (1 - b1 ** t)) / (torch.sqrt(v / (1 - b2 ** t)) + eps)
+    return p * (1 - lr * wd) - lr * upd, m, v, upd
+
+
+@pytest.mark.parametrize("pdtype,gdtype,master", [(torch.float32, torch.float32, False), (torch.float32, torch.bfloat16, False),
+                                                  (torch.bfloat16, torch.bfloat16, False), (torch.bfloat16, torch.float32, True),
+                                                  (torch.bfloat16, torch.bfloat16, True)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_adamw_32_bit_moments(rb, pdtype, gdtype, master, shift):
+    lr, b1, b2, eps, wd, gs = 3e-3, 0.9, 0.95, 1e-8, 0.1, 0.25
+    ps, grads, ms, vs, carve = make(SIZES, pdtype, gdtype, 3, shift)
+    masters = carve(torch.cat([p.float().cpu() * 1.001 for p in ps])) if master else None
+    steps = torch.tensor([float(7 * i) for i in range(len(SIZES))], device="cuda")
+    want = []
+    for i, (p, g, m, v) in enumerate(zip(masters or ps, grads, ms, vs)):
+        want.append(plain(p.double(), g, m.double(), v.double(), 7 * i + 1, lr, b1, b2, eps, wd, gs) + (m.double().abs(), g.double().abs() * gs, p.double().abs()))
+    before = [g.clone() for g in grads]
+    rb.optim.adamw_step(ps, grads, ms, vs, steps, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd, masters=masters,
+                        grad_scale=torch.full((1,), gs, device="cuda"))
+    assert steps.tolist() == [7 * i + 1 for i in range(len(SIZES))]
+    for i in range(len(SIZES)):
+        wp, wm, wv, upd, am, ag, ap = want[i]
+        assert torch.equal(before[i], grads[i])
+        # |m| can be far below its terms: the bound is on the terms.  eps of v: three roundings of its larger term
+        assert ((ms[i].double() - wm).abs() <= 4 * U * (am + ag)).all()
+        assert ((vs[i].double() - wv).abs() <= 5 * U * wv).all()
+        dm = 4 * U * (am + ag) / (1 - b1 ** (7 * i + 1)) / (torch.sqrt(wv / (1 - b2 ** (7 * i + 1))) + eps)
+        bound = lr * (dm + 16 * U * upd.abs()) + 4 * U * ap
+        got = (masters or ps)[i]
+        if pdtype == torch.float32 or master:
+            assert ((got.double() - wp).abs() <= bound).all()
+        if master:
+            assert torch.equal(ps[i], masters[i].to(torch.bfloat16))
+        elif pdtype == torch.bfloat16:
+            # rounded to bf16 at the end: half a step, 2^-8 of the value, on top
+            assert ((got.double() - wp).abs() <= bound + 2.0 ** -8 * (wp.abs() + bound)).all()
+
+
+def _v_values(codes):
+    return (codes.to(torch.int32) << 19).view(torch.float32).double() * 2.0 ** 112
+
+
+def _e4m3_neighbours_ok(code, q):
+    """Rounded to nearest: off by at most half a step -- 2^-4 of the value, or half the smallest step 2^-9 -- and 4 u of q."""
+    return (code.double() - q).abs() <= torch.clamp(q.abs() * 2.0 ** -4, min=2.0 ** -10) * (1 + 8 * U)
+
+
+@pytest.mark.parametrize("pdtype,gdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("shift", [0, 3])
+def test_adamw_8_bit_moments(rb, pdtype, gdtype, shift):
+    lr, b1, b2, eps, wd, seed = 1e-3, 0.9, 0.999, 1e-8, 0.01, 77
+    ps, grads, _, _, carve = make(SIZES, pdtype, gdtype, 5, shift)
+    n = sum(SIZES)
+    ms = carve(torch.zeros(n, dtype=torch.uint8))
+    ms = [t.view(torch.float8_e4m3fn) for t in ms]
+    vs = carve(torch.zeros(n, dtype=torch.uint8))
+    blocks = [-(-k // 256) for k in SIZES]
+    msc = [torch.zeros(b, device="cuda") for b in blocks]
+    vsc = [torch.zeros(b, device="cuda") for b in blocks]
+    steps = torch.zeros(len(SIZES), device="cuda")
+    for it in range(3):
+        for k, g in enumerate(grads):
+            g.copy_(torch.randn(g.shape, generator=torch.Generator().manual_seed(100 * it + k)).to(g.dtype) * 1e-3)
+        old = [(p.double().cpu(), rb.optim.first_moment_values(m, a).double().cpu(), rb.optim.second_moment_values(v, b).double().cpu())
+               for p, m, v, a, b in zip(ps, ms, vs, msc, vsc)]
+        rb.optim.adamw_step(ps, grads, ms, vs, steps, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd, exp_avg_scales=msc, exp_avg_sq_scales=vsc, seed=seed)
+        for i, k in enumerate(SIZES):
+            p0, m0, v0 = old[i]
+            wp, wm, wv, upd = plain(p0, grads[i].cpu(), m0, v0, it + 1, lr, b1, b2, eps, wd)
+            pad = blocks[i] * 256 - k
+            top = lambda x: torch.nn.functional.pad(x, (0, pad)).reshape(-1, 256).amax(1)
+            a, b = msc[i].double().cpu(), vsc[i].double().cpu()
+            at = (m0.abs() + grads[i].double().cpu().abs())
+            # the largest magnitude's own rounding error and the division's
+            assert ((a * 448 - top(wm.abs())).abs() <= 6 * U * top(at)).all() and ((b * 1.9375 - top(wv)).abs() <= 8 * U * top(wv)).all()
+            sa, sb = a.repeat_interleave(256)[:k], b.repeat_interleave(256)[:k]
+            q = torch.where(sa > 0, wm / sa, 0.0)
+            slack = 16 * U * torch.where(sa > 0, at / sa, 0.0)
+            assert (((ms[i].cpu().double() - q).abs() - slack) <= torch.clamp(q.abs() * 2.0 ** -4, min=2.0 ** -10)).all()
+            # second moment: one of the two neighbours, the one that the noise word picks (a value within 2^-20 of a border may fall either way)
+            qv = torch.where(sb > 0, wv / sb, 0.0)
+            word = O.noise_bits_1d(k, (seed + (it + 1) * 0x9E3779B1 + i * 0x85EBCA6B) & 0xFFFFFFFF) >> np.uint32(13)
+            frac = torch.from_numpy(word.astype(np.float64)) * 2.0 ** -19
+            lo = torch.where(qv >= 2.0 ** -14, torch.floor(torch.log2(qv.clamp(min=1e-300))), torch.full_like(qv, -14.0))
+            step = torch.exp2(lo - 4)
+            cell = torch.floor(qv / step + frac + 1e-9) * step
+            got = _v_values(vs[i].cpu())
+            border = ((qv / step + frac) - torch.round(qv / step + frac)).abs() < 2.0 ** -16
+            want = torch.where((wv > 0) & (cell == 0), torch.full_like(cell, 2.0 ** -18), cell).clamp(max=1.9375)
+            assert ((got == want) | border).all()
+            assert ((got > 0) == (wv > 0)).all()
+            bound = lr * 32 * U * (upd.abs() + 1) + 4 * U * p0.abs()
+            rnd = 0 if pdtype == torch.float32 else 2.0 ** -8 * (wp.abs() + bound)
+            slack_m = lr * 8 * U * at / (1 - b1 ** (it + 1)) / (torch.sqrt(wv / (1 - b2 ** (it + 1))) + eps)
+            assert ((ps[i].double().cpu() - wp).abs() <= bound + slack_m + rnd).all()
+
+
+def test_adamw_8_bit_second_moment_keeps_its_expectation(rb):
+    """With no gradient v decays by b2 each step, far below a step of the format: the random rounding follows it on average.
+    64 blocks of 256 equal values start at 1; after 400 steps of b2 = 0.998 the expectation is 0.998^400 = 0.449.  The first
+    element of each block is fed so that the scale stays; one rounding has variance below (step/2)^2, step <= 2^-4 of the value,
+    so 400 of them on 16320 values leave the mean within 400^0.5 * 2^-5 / 16320^0.5 * 5 sigma = 2.5 %."""
+    n, b2 = 64 * 256, 0.998
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    head = torch.zeros(n, dtype=torch.bool, device="cuda")
+    head[::256] = True
+    g[head] = 1.0
+    m = torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    v = torch.full((n,), 247, dtype=torch.uint8, device="cuda")
+    v[head] = 247
+    ms, vs = torch.zeros(64, device="cuda"), torch.full((64,), 1 / 1.4375, device="cuda")
+    steps = torch.zeros(1, device="cuda")
+    for _ in range(400):
+        rb.optim.adamw_step([p], [g], [m], [v], steps, lr=0.0, betas=(0.9, b2), exp_avg_scales=[ms], exp_avg_sq_scales=[vs], seed=5)
+    mean = rb.optim.second_moment_values(v, vs)[~head].double().mean().item()
+    assert abs(mean / b2 ** 400 - 1) < 0.025
+
+
+@pytest.mark.parametrize("dtypes", [(torch.float32,), (torch.bfloat16,), (torch.float32, torch.bfloat16)])
+def test_grad_norm(rb, dtypes):
+    g = torch.Generator().manual_seed(1)
+    grads = [(torch.randn(k, generator=g) * 10 ** (i % 5 - 2)).to(dtypes[i % len(dtypes)]).cuda() for i, k in enumerate(SIZES * 60)]   # 540 tensors: two launches
+    grads.append(torch.zeros(0, device="cuda", dtype=dtypes[0]))
+    want = math.sqrt(sum(float((t.double() ** 2).sum()) for t in grads))
+    norm, none = rb.optim.grad_norm(grads)
+    # the eight squares a lane adds in float32: 8 roundings of u each at most, halved by the root, and the result's own
+    assert none is None and abs(norm.item() / want - 1) <= 8 * U
+    n2, f = rb.optim.grad_norm(grads, max_norm=0.5)
+    assert torch.equal(n2, norm) and abs(f.item() * want / 0.5 - 1) <= 12 * U + 1e-6 / want
+    assert rb.optim.grad_norm(grads, max_norm=1e9)[1].item() == 1.0
+    bad = grads[:3] + [torch.full((5,), float("nan"), device="cuda", dtype=dtypes[0])]
+    nn, ff = rb.optim.grad_norm(bad, max_norm=1.0)
+    assert math.isnan(nn.item()) and math.isnan(ff.item())
+
+
+def test_step_on_a_side_stream_and_in_a_graph(rb):
+    sizes = [5000, 300, 77]
+    ps, grads, ms, vs, _ = make(sizes, torch.float32, torch.float32, 9)
+    ref = [[t.clone() for t in x] for x in (ps, ms, vs)]
+    steps, rsteps = torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda")
+    lr = torch.full((1,), 1e-2, device="cuda")
+    for k in range(3):
+        _, f = rb.optim.grad_norm(grads, 1.0)
+        rb.optim.adamw_step(ref[0], grads, ref[1], ref[2], rsteps, lr=1e-2 * (k + 1), grad_scale=f)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        _, f = rb.optim.grad_norm(grads, 1.0)
+        rb.optim.adamw_step(ps, grads, ms, vs, steps, lr=lr, grad_scale=f)
+    assert steps.tolist() == [0, 0, 0]
+    for k in range(3):
+        lr.fill_(1e-2 * (k + 1))
+        graph.replay()
+    torch.cuda.synchronize()
+    assert steps.tolist() == [3, 3, 3]
+    for a, b in zip(ps + ms + vs, ref[0] + ref[1] + ref[2]):
+        # the learning rate is 1e-2 in float32 here and in float64 there: u of the update
+        assert (a - b).abs().max() <= 1e-6
+
+
+def test_optimizer_class(rb):
+    """Two groups, bf16 with masters beside float32, a channels-last weight, a parameter whose gradient comes later, a checkpoint."""
+    torch.manual_seed(0)
+
+    def build():
+        g = torch.Generator().manual_seed(4)
+        a = torch.nn.Parameter(torch.randn(33, 65, generator=g).cuda().bfloat16())
+        b = torch.nn.Parameter(torch.randn(8, 3, 5, 5, generator=g).cuda().to(memory_format=torch.channels_last))
+        c = torch.nn.Parameter(torch.randn(70, generator=g).cuda())
+        return a, b, c
+
+    def grads(ps, k, skip_c):
+        g = torch.Generator().manual_seed(50 + k)
+        for i, p in enumerate(ps):
+            p.grad = None if (i == 2 and skip_c) else torch.randn(p.shape, generator=g).cuda().to(p.dtype)
+
+    for bits in (32, 8):
+        ps = build()
+        opt = rb.optim.AdamW([{"params": ps[:2], "lr": 1e-2}, {"params": ps[2:], "weight_decay": 0.0}], lr=1e-3, state_bits=bits, max_grad_norm=0.7, seed=3)
+        ref = [p.detach().float().clone().requires_grad_() for p in ps]
+        topt = torch.optim.AdamW([{"params": ref[:2], "lr": 1e-2}, {"params": ref[2:], "weight_decay": 0.0}], lr=1e-3)
+        for k in range(4):
+            grads(ps, k, k == 0)
+            for p, r in zip(ps, ref):
+                r.grad = None if p.grad is None else p.grad.float().clone()  # clip_grad_norm_ writes to it
+            want = torch.nn.utils.clip_grad_norm_([r for r in ref if r.grad is not None], 0.7)
+            opt.step()
+            topt.step()
+            assert abs(opt.last_grad_norm.item() / want.item() - 1) < 1e-5
+            if k == 1:                                             # save, rebuild, load
+                sd = opt.state_dict()
+                saved = [p.detach().clone() for p in ps]
+                ps2 = build()
+                for p, s in zip(ps2, saved):
+                    p.data.copy_(s)
+                opt = rb.optim.AdamW([{"params": ps2[:2], "lr": 1e-2}, {"params": ps2[2:], "weight_decay": 0.0}], lr=1e-3, state_bits=bits,
+                                     max_grad_norm=0.7, seed=3)
+                opt.load_state_dict(sd)
+                ps = ps2
+        assert opt.state[ps[0]]["step"].item() == 4 and opt.state[ps[2]]["step"].item() == 3
+        assert opt.state[ps[1]]["exp_avg"].stride() == ps[1].stride()
+        for i, (p, r) in enumerate(zip(ps, ref)):
+            got = opt.state[p]["master"] if "master" in opt.state[p] else p
+            # each of the four updates is at most lr * (1 + a few) in size; 8-bit moments are within 2^-4 (first), and the second's random rounding
+            # within 2^-4 a step, of the float32 ones: at most a quarter of the distance walked.  32 bits: roundings only
+            walked = 4 * (1e-2 if i < 2 else 1e-3) * 1.2
+            assert (got.float() - r).abs().max().item() <= (walked * 0.25 if bits == 8 else 1e-5)
+        other = rb.optim.AdamW([{"params": build()[:2]}, {"params": build()[2:]}], state_bits=40 - bits)
+        other.load_state_dict(opt.state_dict())                    # the checkpoint's format comes with it
+        assert [g["state_bits"] for g in other.param_groups] == [bits, bits]
+    ckpt = topt.state_dict()
+    c = [torch.nn.Parameter(r.detach().clone()) for r in ref]
+    mine = rb.optim.AdamW([{"params": c[:2]}, {"params": c[2:]}])
+    mine.load_state_dict(ckpt)                                     # torch's own AdamW
+    assert torch.equal(mine.state[c[0]]["exp_avg"], topt.state[ref[0]]["exp_avg"]) and mine.state[c[0]]["step"].item() == 4
+    low = build()
+    with pytest.raises(RuntimeError, match="other state_bits or masters"):
+        rb.optim.AdamW([{"params": low[:2]}, {"params": low[2:]}]).load_state_dict(ckpt)   # no masters for the bfloat16 parameter in it
+
+
+def test_refusals(rb):
+    p, g, m, v = (torch.zeros(4, device="cuda") for _ in range(4))
+    s = torch.zeros(1, device="cuda")
+    step = rb.optim.adamw_step
+    with pytest.raises(RuntimeError, match="twice"):
+        step([p, p], [g, g], [m, m], [v, v], torch.zeros(2, device="cuda"))
+    with pytest.raises(RuntimeError, match="differ in size"):
+        step([p], [torch.zeros(5, device="cuda")], [m], [v], s)
+    with pytest.raises(RuntimeError, match="one type"):
+        step([p], [g.half()], [m], [v], s)
+    with pytest.raises(RuntimeError, match="one type"):
+        step([p], [g], [m.bfloat16()], [v], s)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        step([torch.zeros(4, 2, device="cuda")[:, 0]], [g], [m], [v], s)
+    with pytest.raises(RuntimeError, match="live on"):
+        step([p], [g.cpu()], [m], [v], s)
+    with pytest.raises(RuntimeError, match="steps"):
+        step([p], [g], [m], [v], torch.zeros(2, device="cuda"))
+    with pytest.raises(RuntimeError, match="masters"):
+        step([p], [g], [m], [v], s, masters=[p.clone()])
+    with pytest.raises(RuntimeError, match="one-element"):
+        step([p], [g], [m], [v], s, grad_scale=torch.zeros(2, device="cuda"))
+    with pytest.raises(RuntimeError, match="not supported"):
+        step([p], [g], [m], [v], s, betas=(1.0, 0.9))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        step([p.cpu()], [g], [m], [v], s)
+    with pytest.raises(RuntimeError, match="scales"):
+        step([p], [g], [m.to(torch.float8_e4m3fn)], [v.to(torch.uint8)], s, exp_avg_scales=[m[:2]], exp_avg_sq_scales=[m[:1]])
+    step([], [], [], [], s)
+    assert p.abs().sum() == 0
