@@ -438,8 +438,8 @@ int rdb_gemm_dense_scatter(void *const *dst_ptrs, int ndst, size_t dst_offset_by
  *   state_bits    32: exp_avg and exp_avg_sq are float32.
  *                 8: one byte per element and one float32 scale per RDB_ADAMW_BLOCK consecutive elements of a tensor
  *                 (ceil(numel / RDB_ADAMW_BLOCK) of them).  exp_avg: float8 e4m3, rounded to nearest, scale = largest
- *                 magnitude / 448.  exp_avg_sq: no sign, 4 exponent bits (bias 15) and 4 mantissa bits, scale = largest value /
- *                 1.9375, rounded down or up at random with the odds that keep the expectation (nearest would never let it
+ *                 magnitude * float32(1/448).  exp_avg_sq: no sign, 4 exponent bits (bias 15) and 4 mantissa bits, scale = largest value *
+ *                 float32(1/1.9375), rounded down or up at random with the odds that keep the expectation (nearest would never let it
  *                 decay: 1 - beta2 is below half a step of any 8-bit format), never to 0 when positive.  The random bits are
  *                 the upper 19 of the 1-D noise word of (element index mod 2^32) under the seed
  *                 h->seed + t * 0x9E3779B1 + i * 0x85EBCA6B (tensor i of the list): the same call gives the same bytes.

@@ -171,8 +171,8 @@ __device__ __forceinline__ void adamw_segment(const AdamwDesc &d, int64_t at, in
     store8<VEC>(reinterpret_cast<P *>(d.p) + at, p8, lane, left);
     if (MASTER) store8<VEC>(d.master + at, w8, lane, left);
     if (BITS8) {
-        mscale = __fdiv_rn(warp_max(mmax), 448.0f);
-        vscale = __fdiv_rn(warp_max(vmax), 1.9375f);
+        mscale = __fmul_rn(warp_max(mmax), 1.0f / 448.0f);
+        vscale = __fmul_rn(warp_max(vmax), 1.0f / 1.9375f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float qm = mscale > 0.0f ? __fdiv_rn(m[j], mscale) : 0.0f;
