@@ -471,6 +471,41 @@ size_t rdb_grad_norm_workspace_bytes(int n);
 int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int64_t *numels, const int32_t *dtypes, int n, float max_norm,
                   void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Softmax cross entropy of rows x [T, R] over a vocabulary matrix of V rows, without keeping the logits x W^T:
+ *   w not null   the stored matrix W [V, R], row pitch ldw
+ *   w null       W = S[row0 : row0 + V, 0 : R], the noise of `seed` in x's type (the head of a pseudorandom-weight layer, with
+ *                x standing for z = input C^T)
+ * target: int64 [T], the row's column in [0, V); with use_ignore, rows whose target equals ignore_index count for nothing: their
+ * contents (infinities and NaN included) reach no result, their loss and gradient are 0.  Any other target outside [0, V) makes
+ * the row's loss and gradient NaN.  reduction RDB_CE_NONE: loss per row; RDB_CE_SUM; RDB_CE_MEAN: over the rows that count (NaN
+ * when none does).  x, w and the gradients are of type dtype, losses float32.
+ *
+ * rdb_ce_fwd   loss (one float32; ignored for RDB_CE_NONE) and aux, float32 [2T + 1]: log-sum-exp per row, loss per row, number
+ *              of rows that count.  dx_unit (may be null, only with w null): d(row's loss)/dx, contiguous [T, R].
+ * rdb_ce_scale dz = dx_unit times the gradient of the loss: *dloss (RDB_CE_SUM), *dloss / count (RDB_CE_MEAN), dloss[row] (NONE).
+ * rdb_ce_bwd   gradients for a stored matrix from the forward's aux: dx [T, R] and dw [V, R], contiguous, either may be null.
+ * workspace: 256-byte aligned, rdb_ce_workspace_bytes(op, ...) bytes with op RDB_CE_LOSS (fwd), RDB_CE_LOSS_GRAD (fwd with
+ * dx_unit) or RDB_CE_GRADS (bwd), and the same w and ldw (w only says whether it is null and how it is aligned); contents need
+ * not survive between calls.  Results repeat run to run.  The reference ends in F.cross_entropy on the full logits
+ * (modded-nanogpt/train_gpt2.py:236-240).
+ */
+#define RDB_CE_LOSS 0
+#define RDB_CE_LOSS_GRAD 1
+#define RDB_CE_GRADS 2
+#define RDB_CE_NONE 0
+#define RDB_CE_MEAN 1
+#define RDB_CE_SUM 2
+size_t rdb_ce_workspace_bytes(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw);
+int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
+               void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t V, int64_t row0, uint32_t seed, int64_t ignore_index,
+               int use_ignore, int dtype, int reduction, int32_t *status, void *stream);
+int rdb_ce_scale(void *dz, const void *dx_unit, const float *dloss, const float *aux, int64_t T, int64_t R, int dtype, int reduction,
+                 void *stream);
+int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
+               const float *aux, void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t V, int64_t ignore_index,
+               int use_ignore, int dtype, int reduction, int32_t *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,8 +15,8 @@ Importing the package does not need a GPU; running any kernel does, and there is
 """
 from . import kernels, ops, optim, parallel  # noqa: F401
 from .layers import RandumbLinear, SillyConv2d, SillyEmbedding, SillyLinear, listgen, stepgen  # noqa: F401
-from .ops import rlinear  # noqa: F401
+from .ops import linear_cross_entropy, noise_cross_entropy, rlinear, rlinear_cross_entropy  # noqa: F401
 from .tensor import CreateRandumbTensor, RandumbTensor  # noqa: F401
 
-__all__ = ["kernels", "ops", "optim", "parallel", "RandumbLinear", "SillyLinear", "SillyEmbedding", "SillyConv2d", "listgen", "stepgen", "rlinear",
+__all__ = ["kernels", "ops", "optim", "parallel", "RandumbLinear", "SillyLinear", "SillyEmbedding", "SillyConv2d", "listgen", "stepgen", "rlinear", "rlinear_cross_entropy", "noise_cross_entropy", "linear_cross_entropy",
            "CreateRandumbTensor", "RandumbTensor"]

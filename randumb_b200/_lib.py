@@ -25,6 +25,8 @@ OPT_GEMV_FUSED = 6
 OPT_GRADS_BESIDE = 7
 MAX_RESERVE_SMS = 64
 MAX_PEERS = 8
+CE_LOSS, CE_LOSS_GRAD, CE_GRADS = 0, 1, 2
+CE_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 STATUS_NAMES = {0: "ok", 1: "producer wait expired", 2: "mma wait expired", 3: "epilogue wait expired",
                 4: "generator wait expired", 5: "peer wait expired"}
 
@@ -100,6 +102,10 @@ PROTOTYPES = {
     "rdb_adamw_step": (_i32, [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(AdamwHyper), _vp, _vp]),
     "rdb_grad_norm_workspace_bytes": (_sz, [_i32]),
     "rdb_grad_norm": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, ctypes.c_float, _vp, _sz, _vp]),
+    "rdb_ce_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64, _i32, _vp, _i64]),
+    "rdb_ce_fwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _u32, _i64, _i32, _i32, _i32, _vp, _vp]),
+    "rdb_ce_scale": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
+    "rdb_ce_bwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp]),
     "rdb_embed_bwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _u32, _vp]),
 }
 

@@ -1,0 +1,1206 @@
+// Softmax cross entropy over a vocabulary matrix W [V, R] (stored, or noise regenerated from a seed), loss and gradients, without
+// keeping the logits l = x W^T.
+//
+// Everything is taken relative to the logit of the row's own target t, which a small kernel computes first:
+//
+//   e_v = exp(l_v - l_t),  s = sum over v != t of e_v        loss = log(1 + s)            lse = l_t + loss
+//   d loss / dx = (sum over v != t of e_v w_v  -  s w_t) / (1 + s)
+//
+// so no running maximum is needed: the sum never falls below the target's own 1, and small losses and the gradients of tokens
+// the model already knows come out of log1p and of a sum without the target, not of a difference of nearly equal numbers.  e_v
+// exceeds float32 only where another logit lies more than 69 above the target's (s beyond 2^100); such rows are counted as
+// they are found and done again, one by one, with their true maximum (ce_rescue_kernel).
+//
+// Rows whose target is ignored are left out: the remaining rows are gathered to the front, and every later kernel works on that
+// many rows, a number that only the device knows.
+//
+//   gradient of x only (noise matrix): one pass over the vocabulary in pieces, E = exp(..) of a piece in bf16, O += E W_piece in
+//       float32; the gradient is finished from O, s and the target's row.  Two products per (row, vocabulary, R).
+//   stored matrix: the forward needs only s (one product); the backward recomputes each piece's logits with the final lse,
+//       P = w (softmax - onehot), and takes dx += P W_piece and dW_piece = P^T x.  Four products in all.
+//
+// float32 operands are split into three bf16 parts each (3 x 8 = 24 significant bits) and multiplied as the six products of
+// parts whose orders add up to at most two, accumulated in the same float32 accumulator: exact products, terms below 2^-24
+// left out.
+//
+// The products run on CTA pairs (cta_group::2), 256 x 256 tiles, six 32 KB stages of TMA-fed operands, two accumulators in TMEM
+// so that the exponentials of one tile run under the next tile's MMAs.  The x-gradient product is cut by k-blocks: every pair
+// takes an equal run of the (tile, k-block) sequence and leaves its part of a tile in a slot of its own; the slots are added in
+// order, so results repeat run to run whatever the number of tiles.
+#include <cmath>
+
+#include "umma.cuh"
+#include "umma_pipe.cuh"
+
+namespace rdb {
+
+using namespace ptx;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float S_LIMIT = 1.2676506e30f;       // 2^100: rows above are redone with their maximum
+constexpr int CE_TILE = 256;
+constexpr int CE_STAGES = 6;
+constexpr int CE_STAGE = 2 * SUB_BYTES;        // this CTA's 128 rows of A and its half (128 rows) of B
+constexpr int CE_EPI = 8;
+constexpr int CE_THREADS = (2 + CE_EPI) * 32;
+constexpr int CE_SMEM = CE_STAGES * CE_STAGE + CE_EPI * 4096 + 1024;
+static_assert(CE_SMEM <= 232448 - 512, "shared memory");
+
+enum { EPI_SUM, EPI_EXP, EPI_PROB, EPI_SLOT, EPI_BF16, EPI_F32 };
+
+struct CeArgs {
+    const int32_t *count;         // rows left after gathering
+    int64_t M, N;                 // output extents in tiles' terms (M ignored where the rows are counted on the device)
+    int m_counted, k_counted;     // M, or the contraction, is *count
+    int kbs;                      // 64-wide k-blocks per term
+    int nterm;
+    int a_off[6], b_off[6];       // column offsets of the parts a term multiplies
+    int m_fast;
+    int accumulate;               // EPI_SLOT: add to the slots instead of storing
+    const float *off2, *scale, *tval;   // per row: exponent offset in powers of two; EPI_PROB: factor and the target's value
+    const int32_t *tcol;          // per row: target column, -1 for none
+    int32_t v0, ncols;            // first column of this piece, columns of it that exist
+    float *partial;               // EPI_SUM / EPI_EXP: row sums, [2 per column tile][ld_partial]
+    int64_t ld_partial;
+    int part_cols;                // columns between the parts of the output (three parts: float32)
+    int32_t *status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *m, uint32_t smem_src, int32_t x, int32_t y) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_src), "r"(x), "r"(y) : "memory");
+}
+
+// ---- the equal cut of `total` k-blocks over `pairs`: pair p owns [total p / pairs, total (p + 1) / pairs) ----------------
+// As many pairs take part as get four k-blocks each (a part of a tile costs a 256 x 256 float32 slot, written and read back).
+__host__ __device__ __forceinline__ int64_t cut_pairs(int64_t total, int64_t pairs) {
+    const int64_t p = total / 4;
+    return p < 1 ? 1 : (p < pairs ? p : pairs);
+}
+__host__ __device__ __forceinline__ int64_t cut_begin(int64_t total, int64_t pairs, int64_t p) { return total * p / pairs; }
+__host__ __device__ __forceinline__ int64_t cut_owner(int64_t total, int64_t pairs, int64_t g) {
+    int64_t p = ((g + 1) * pairs + total - 1) / total - 1;
+    return p;
+}
+
+// Part of tile `tile` computed by pair `p`: one 256 x 256 float32 slot.  tile + p grows from each part to the next, so the parts
+// need (tiles + pairs) slots whatever the cut.
+__host__ __device__ __forceinline__ int64_t slot_of(int64_t tile, int64_t p) { return tile + p; }
+
+struct WorkItem {
+    int64_t m, n, slot;
+    int kb0, kb1;
+};
+
+// The sequence of work items of one pair; every role walks it by itself.
+struct Walk {
+    int64_t tiles_m, tiles_n, total, next, end, pairs, pair;
+    int KB, m_fast;
+    bool cut;
+    __device__ __forceinline__ void start(const CeArgs &a, bool cut_, int64_t rows, int kb_total, int64_t pair_, int64_t pairs_) {
+        tiles_m = (rows + CE_TILE - 1) / CE_TILE;
+        tiles_n = (a.N + CE_TILE - 1) / CE_TILE;
+        KB = kb_total;
+        m_fast = a.m_fast;
+        cut = cut_;
+        pairs = pairs_;
+        pair = pair_;
+        if (cut) {
+            total = tiles_m * tiles_n * KB;
+            pairs = cut_pairs(total, pairs_);
+            next = pair < pairs ? cut_begin(total, pairs, pair) : total;
+            end = pair < pairs ? cut_begin(total, pairs, pair + 1) : total;
+        } else {
+            total = tiles_m * tiles_n;
+            next = pair;
+            end = total;
+        }
+    }
+    __device__ __forceinline__ bool take(WorkItem &w) {
+        if (next >= end) return false;
+        int64_t tile;
+        if (cut) {
+            tile = next / KB;
+            w.kb0 = (int)(next - tile * KB);
+            const int64_t left = end - next;
+            w.kb1 = left < KB - w.kb0 ? w.kb0 + (int)left : KB;
+            w.slot = slot_of(tile, pair);
+            next += w.kb1 - w.kb0;
+        } else {
+            tile = next;
+            w.kb0 = 0;
+            w.kb1 = KB;
+            w.slot = 0;
+            next += pairs;
+        }
+        w.m = m_fast ? tile % tiles_m : tile / tiles_n;
+        w.n = m_fast ? tile / tiles_m : tile % tiles_n;
+        return true;
+    }
+};
+
+template <int A_MN, int B_MN, int EPI, int PARTS>
+__global__ void __launch_bounds__(CE_THREADS, 1)
+ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+               const __grid_constant__ CUtensorMap tmap_d, const __grid_constant__ CeArgs args) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bar_full[CE_STAGES], bar_free[CE_STAGES], bar_tmem_full[2], bar_tmem_empty[2];
+    __shared__ uint32_t tmem_holder;
+    __shared__ int abort_flag;
+    constexpr bool CUT = EPI == EPI_SLOT;
+
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const uint32_t half = rank & 1;
+    const bool leader = half == 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < CE_STAGES; ++s) {
+            mbar_init(smem_u32(&bar_full[s]), 1);      // the even CTA's TMA thread; both CTAs' loads complete their bytes here
+            mbar_init(smem_u32(&bar_free[s]), 1);      // one tcgen05.commit from the pair's MMA thread
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(smem_u32(&bar_tmem_full[s]), 1);
+            mbar_init(smem_u32(&bar_tmem_empty[s]), 2 * CE_EPI);
+        }
+        abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(&tmem_holder), TMEM_COLS);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_holder;
+    volatile int *abortp = &abort_flag;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int64_t counted = (args.m_counted || args.k_counted) ? (int64_t)*args.count : 0;
+    const int64_t rows = args.m_counted ? counted : args.M;
+    const int kbs = args.k_counted ? (int)((counted + BK - 1) / BK) : args.kbs;
+    const int KB = kbs * args.nterm;
+    Walk walk;
+    walk.start(args, CUT, rows, KB, blockIdx.x >> 1, gridDim.x >> 1);
+    WorkItem w;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            prefetch_tmap(&tmap_a);
+            prefetch_tmap(&tmap_b);
+            PipeState st;
+            bool ok = true;
+            while (ok && walk.take(w)) {
+                const int32_t m0 = (int32_t)(w.m * CE_TILE + half * BM);
+                const int32_t n0 = (int32_t)(w.n * CE_TILE + half * BM);
+                int term = kbs ? w.kb0 / kbs : 0, kk = w.kb0 - term * kbs;
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    if (!mbar_wait_cluster(smem_u32(&bar_free[st.idx]), st.phase ^ 1, abortp)) {
+                        raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_PRODUCER);
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb = mapa(smem_u32(&bar_full[st.idx]), rank & ~1u);
+                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[st.idx]), 2 * CE_STAGE);
+                    const uint32_t sa = smem_base + st.idx * CE_STAGE, sb = sa + SUB_BYTES;
+                    const int32_t ax = args.a_off[term], bx = args.b_off[term], k0 = kk * BK;
+                    if (A_MN) {
+#pragma unroll
+                        for (int i = 0; i < BM / 64; ++i) tma_load_2d_pair(sa + i * (64 * BK * 2), &tmap_a, fb, ax + m0 + i * 64, k0);
+                    } else {
+                        tma_load_2d_pair(sa, &tmap_a, fb, ax + k0, m0);
+                    }
+                    if (B_MN) {
+#pragma unroll
+                        for (int i = 0; i < BM / 64; ++i) tma_load_2d_pair(sb + i * (64 * BK * 2), &tmap_b, fb, bx + n0 + i * 64, k0);
+                    } else {
+                        tma_load_2d_pair(sb, &tmap_b, fb, bx + k0, n0);
+                    }
+                    st.advance<CE_STAGES>();
+                    if (++kk == kbs) { kk = 0; ++term; }
+                }
+            }
+            if (!ok) {
+                // gave up: let the loads already in flight land before the CTA may retire
+                const long long t0 = clock64();
+                while (clock64() - t0 < 4000000LL) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer (even CTA of the pair)
+        if (lane == 0 && leader) {
+            constexpr uint32_t idesc = idesc_bf16_f32(2 * BM, CE_TILE, A_MN, B_MN);
+            constexpr uint32_t desc_hi = smem_desc_hi_sw128(1024);
+            constexpr uint32_t A_LBO = A_MN ? 64 * BK * 2 : 0, A_KSTEP = A_MN ? 2048 : UMMA_K * 2;
+            constexpr uint32_t B_LBO = B_MN ? 64 * BK * 2 : 0, B_KSTEP = B_MN ? 2048 : UMMA_K * 2;
+            const uint32_t peer = rank ^ 1u;
+            PipeState st;
+            bool ok = true;
+            int64_t it = 0;
+            while (ok && walk.take(w)) {
+                if (w.kb0 == w.kb1) continue;                    // nothing to contract: the epilogue stores zeros
+                const int acc = (int)(it & 1);
+                if (!mbar_wait_cluster(smem_u32(&bar_tmem_empty[acc]), (uint32_t)((it >> 1) & 1) ^ 1, abortp)) {
+                    raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_MMA);
+                    break;
+                }
+                tc_fence_after_sync();
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    if (!mbar_wait_cluster(smem_u32(&bar_full[st.idx]), st.phase, abortp)) {
+                        raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_MMA);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t sa = smem_base + st.idx * CE_STAGE;
+                    const uint32_t a_lo = smem_desc_lo(sa, A_LBO), b_lo = smem_desc_lo(sa + SUB_BYTES, B_LBO);
+#pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; ++k)
+                        umma_bf16_pair(tmem_base + acc * CE_TILE, pack_desc(a_lo + ((k * A_KSTEP) >> 4), desc_hi),
+                                       pack_desc(b_lo + ((k * B_KSTEP) >> 4), desc_hi), idesc, ((kb - w.kb0) | k) != 0 ? 1u : 0u);
+                    umma_commit_pair(smem_u32(&bar_free[st.idx]));
+                    umma_commit_pair(mapa(smem_u32(&bar_free[st.idx]), peer));
+                    st.advance<CE_STAGES>();
+                }
+                if (ok) {
+                    umma_commit_pair(smem_u32(&bar_tmem_full[acc]));
+                    umma_commit_pair(mapa(smem_u32(&bar_tmem_full[acc]), peer));
+                }
+                ++it;
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue: 8 warps, this CTA's 128 rows
+        const int ew = warp - 2;
+        const int q = warp & 3;                      // TMEM lane quarter this warp may read
+        const int cg = ew >> 2;                      // which 128 of the 256 columns
+        const uint32_t leader_rank = rank & ~1u;
+        const uint32_t stag = smem_base + CE_STAGES * CE_STAGE + (uint32_t)ew * 4096u;
+        const uint32_t rowaddr = stag + (uint32_t)lane * 128u;
+        int64_t it = 0;
+        bool ok = true;
+        while (ok && walk.take(w)) {
+            const int64_t row_w = w.m * CE_TILE + half * BM + q * 32;
+            const int64_t n0 = w.n * CE_TILE + cg * 128;
+            const int acc = (int)(it & 1);
+            const bool empty = w.kb0 == w.kb1;
+            float off = 0.0f, scale = 0.0f, tval = 0.0f, sum = 0.0f;
+            int t_rel = -1;
+            if (EPI <= EPI_PROB) {                   // the rows' numbers are fetched while the tile is being multiplied
+                off = args.off2[row_w + lane];
+                t_rel = args.tcol[row_w + lane] - args.v0 - (int)n0;
+                if (EPI == EPI_PROB) { scale = args.scale[row_w + lane]; tval = args.tval[row_w + lane]; }
+            }
+            if (!empty) {
+                if (!mbar_wait_warp<true>(smem_u32(&bar_tmem_full[acc]), (uint32_t)((it >> 1) & 1), abortp)) {
+                    raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_EPILOGUE);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+            }
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * CE_TILE + cg * 128);
+            auto hand_back = [&]() {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(mapa(smem_u32(&bar_tmem_empty[acc]), leader_rank));
+            };
+            auto box_free = [&]() {                  // the last store from the staging box has read it
+                if (lane == 0) bulk_wait_group_read0();
+                __syncwarp();
+            };
+            if (EPI <= EPI_PROB) {
+#pragma unroll 1
+                for (int hb = 0; hb < 2; ++hb) {
+                    uint32_t r0[32], r1[32];
+                    tmem_ld_32x32(taddr + hb * 64, r0);
+                    tmem_ld_32x32(taddr + hb * 64 + 32, r1);
+                    tmem_ld_wait();
+                    if (hb == 1) hand_back();
+                    const int c0 = (int)n0 + hb * 64, tr = t_rel - hb * 64;
+                    float e[64];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        e[j] = ex2(__fmaf_rn(__uint_as_float(r0[j]), LOG2E, -off));
+                        e[32 + j] = ex2(__fmaf_rn(__uint_as_float(r1[j]), LOG2E, -off));
+                    }
+                    if (c0 + 64 > args.ncols) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) e[j] = c0 + j < args.ncols ? e[j] : 0.0f;
+                    }
+                    if (EPI == EPI_PROB) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) e[j] *= scale;
+                    }
+                    if (__any_sync(0xffffffffu, (unsigned)tr < 64u)) {      // a target among these columns: left out of the sum
+                        const float tv = EPI == EPI_PROB ? tval : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) e[j] = j == tr ? tv : e[j];
+                    }
+                    if (EPI != EPI_PROB) {
+                        float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 64; j += 4) { a0 += e[j]; a1 += e[j + 1]; a2 += e[j + 2]; a3 += e[j + 3]; }
+                        sum += (a0 + a1) + (a2 + a3);
+                    }
+                    if (EPI != EPI_SUM) {
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            box_free();
+#pragma unroll
+                            for (int ch = 0; ch < 8; ++ch) {
+                                uint32_t pk[4];
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    const int j = ch * 8 + 2 * x;
+                                    __nv_bfloat162 h = __floats2bfloat162_rn(e[j], e[j + 1]);
+                                    pk[x] = *reinterpret_cast<uint32_t *>(&h);
+                                    if (p + 1 < PARTS) {
+                                        e[j] -= __low2float(h);
+                                        e[j + 1] -= __high2float(h);
+                                    }
+                                }
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((ch ^ (lane & 7)) << 4)),
+                                             "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]) : "memory");
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                tma_store_2d(&tmap_d, stag, p * args.part_cols + c0, (int32_t)row_w);
+                                bulk_commit_group();
+                            }
+                        }
+                    }
+                }
+                if (EPI != EPI_PROB) args.partial[(w.n * 2 + cg) * args.ld_partial + row_w + lane] = sum;
+            } else if (EPI == EPI_BF16) {
+#pragma unroll 1
+                for (int hb = 0; hb < 2; ++hb) {
+                    uint32_t r0[32], r1[32];
+                    if (!empty) {
+                        tmem_ld_32x32(taddr + hb * 64, r0);
+                        tmem_ld_32x32(taddr + hb * 64 + 32, r1);
+                        tmem_ld_wait();
+                        if (hb == 1) hand_back();
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r0[j] = r1[j] = 0u;
+                    }
+                    box_free();
+#pragma unroll
+                    for (int ch = 0; ch < 8; ++ch) {
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int j = (ch & 3) * 8 + 2 * x;
+                            __nv_bfloat162 h = ch < 4 ? __floats2bfloat162_rn(__uint_as_float(r0[j]), __uint_as_float(r0[j + 1]))
+                                                      : __floats2bfloat162_rn(__uint_as_float(r1[j]), __uint_as_float(r1[j + 1]));
+                            pk[x] = *reinterpret_cast<uint32_t *>(&h);
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((ch ^ (lane & 7)) << 4)),
+                                     "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]) : "memory");
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int64_t c0 = n0 + hb * 64;
+                        if (row_w < rows && c0 < args.N) {
+                            tma_store_2d(&tmap_d, stag, (int32_t)c0, (int32_t)row_w);
+                            bulk_commit_group();
+                        }
+                    }
+                }
+            } else {
+                // float32: [32 rows x 32 columns] boxes
+#pragma unroll 1
+                for (int cb = 0; cb < 4; ++cb) {
+                    uint32_t r[32];
+                    if (!empty) {
+                        tmem_ld_32x32(taddr + cb * 32, r);
+                        tmem_ld_wait();
+                        if (cb == 3) hand_back();
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = 0u;
+                    }
+                    box_free();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((j ^ (lane & 7)) << 4)),
+                                     "r"(r[4 * j]), "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3]) : "memory");
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int64_t c0 = n0 + cb * 32;
+                        if (EPI == EPI_SLOT) {
+                            const int32_t x = cg * 128 + cb * 32, y = (int32_t)(w.slot * CE_TILE + half * BM + q * 32);
+                            if (args.accumulate) tma_reduce_add_2d(&tmap_d, stag, x, y);
+                            else tma_store_2d(&tmap_d, stag, x, y);
+                            bulk_commit_group();
+                        } else if (c0 < args.N && row_w < rows) {
+                            tma_store_2d(&tmap_d, stag, (int32_t)c0, (int32_t)row_w);
+                            bulk_commit_group();
+                        }
+                    }
+                }
+            }
+            if (!empty) ++it;
+        }
+        if (EPI != EPI_SUM && lane == 0) bulk_wait_group0();     // all output written before the CTA retires
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();   // no CTA retires (or frees TMEM) while its peer may still use it
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    }
+}
+
+// ================================================================================================
+// rows
+// ================================================================================================
+// Positions of the rows that count, in order: idx[compact] = row, map[row] = compact or -1.  One block; `zero` (losses, may be
+// null) is cleared at ignored rows.
+__global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict__ target, int64_t T, int64_t ignore, int use_ignore,
+                                                       int32_t *__restrict__ idx, int32_t *__restrict__ map, int32_t *__restrict__ count,
+                                                       float *__restrict__ zero_a, float *__restrict__ zero_b, float *__restrict__ count_f) {
+    __shared__ int warp_sum[32];
+    __shared__ int base;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) base = 0;
+    for (int64_t b = 0; b < T; b += 4096) {
+        const int64_t i0 = b + threadIdx.x * 4;
+        int keep[4], n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            keep[k] = i0 + k < T && !(use_ignore && target[i0 + k] == ignore);
+            n += keep[k];
+        }
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        int before = base, all = 0;
+        for (int k = 0; k < 32; ++k) {
+            const int s = warp_sum[k];
+            before += k < warp ? s : 0;
+            all += s;
+        }
+        int at = before + incl - n;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i0 + k < T) {
+                map[i0 + k] = keep[k] ? at : -1;
+                if (keep[k]) idx[at++] = (int32_t)(i0 + k);
+                else {
+                    if (zero_a) zero_a[i0 + k] = 0.0f;
+                    if (zero_b) zero_b[i0 + k] = 0.0f;
+                }
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) base += all;
+        __syncthreads();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *count = base;
+        if (count_f) *count_f = (float)base;
+    }
+}
+
+// The matrix a row's target selects: stored, or noise.
+struct Vocab {
+    const void *w;        // null: noise
+    int64_t ldw;
+    uint32_t seed, row0;
+};
+
+template <typename T> __device__ __forceinline__ float vocab_at(const Vocab &v, int64_t row, int64_t col) {
+    if (v.w) return to_f32<T>(reinterpret_cast<const T *>(v.w)[row * v.ldw + col]);
+    return to_f32<T>(from_f32<T>(sq5_to_float(sq5_bits(v.row0 + (uint32_t)row, (uint32_t)col, v.seed))));
+}
+
+template <int PARTS> __device__ __forceinline__ void split_store(__nv_bfloat16 *dst, int64_t part_cols, int64_t c, float v) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        const __nv_bfloat16 h = __float2bfloat16_rn(v);
+        dst[p * part_cols + c] = h;
+        v -= __bfloat162float(h);
+    }
+}
+
+struct CeRowArgs {
+    const void *x;
+    int64_t ldx, T, R, V;
+    const int64_t *target;
+    const int32_t *idx, *count;
+    __nv_bfloat16 *a;             // gathered rows [rows, PARTS * part_cols]
+    int64_t lda, part_cols;
+    float *off2, *lt, *scale, *tval;
+    int32_t *tcol;
+    // backward
+    const float *dloss;           // null: forward
+    const float *lse, *loss;
+    int reduction;
+};
+
+// One warp per gathered row: the row in bf16 parts, its target's logit (forward), or exponent offset, factor and target value of
+// the probabilities (backward).  Rows up to the next multiple of 256 are zeros that contribute nothing anywhere.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t j = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t n = *a.count;
+    if (j >= (n + CE_TILE - 1) / CE_TILE * CE_TILE) return;
+    __nv_bfloat16 *dst = a.a + j * a.lda;
+    if (j >= n) {
+        for (int64_t c = lane; c < a.lda; c += 32) dst[c] = __float2bfloat16_rn(0.0f);
+        if (lane == 0) {
+            a.off2[j] = INFINITY;
+            a.tcol[j] = -1;
+            if (a.dloss) { a.scale[j] = 0.0f; a.tval[j] = 0.0f; }
+        }
+        return;
+    }
+    const int64_t row = a.idx[j];
+    const int64_t t = a.target[row];
+    const bool known = t >= 0 && t < a.V;
+    const T *src = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    float dot = 0.0f;
+    for (int64_t c = lane; c < a.part_cols; c += 32) {
+        const float v = c < a.R ? to_f32<T>(src[c]) : 0.0f;
+        split_store<PARTS>(dst, a.part_cols, c, v);
+        if (!a.dloss && known && c < a.R) dot = fmaf(v, vocab_at<T>(voc, t, c), dot);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (lane == 0) {
+        a.tcol[j] = known ? (int32_t)t : -1;
+        if (!a.dloss) {
+            if (!known) dot = NAN;                    // a target outside the vocabulary: the row's loss says so
+            a.lt[j] = dot;
+            a.off2[j] = dot * LOG2E;
+        } else {
+            const float g = a.reduction == RDB_CE_NONE ? a.dloss[row] : a.reduction == RDB_CE_MEAN ? a.dloss[0] / (float)n : a.dloss[0];
+            a.off2[j] = a.lse[row] * LOG2E;
+            a.scale[j] = g;
+            a.tval[j] = g * expm1f(-a.loss[row]);     // softmax - 1 at the target, without a difference
+        }
+    }
+}
+
+// rows of the matrix in bf16 parts, zero between R and part_cols
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) ce_split_kernel(__nv_bfloat16 *__restrict__ dst, int64_t ldd, int64_t part_cols, int64_t rows, int64_t R,
+                                                       int64_t v0, Vocab voc) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t total = rows * part_cols;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / part_cols, c = i - r * part_cols;
+        split_store<PARTS>(dst + r * ldd, part_cols, c, c < R ? vocab_at<T>(voc, v0 + r, c) : 0.0f);
+    }
+}
+
+// ================================================================================================
+// finishing
+// ================================================================================================
+// s of 32 rows per block: eight threads per row add every eighth partial sum, then the eight are added in order.
+__global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ partial, int64_t ld, int nparts, const int32_t *__restrict__ idx,
+                                                     const int32_t *__restrict__ count, const float *__restrict__ lt, float *__restrict__ s_out,
+                                                     float *__restrict__ lse, float *__restrict__ loss) {
+    __shared__ float sh[8][33];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int64_t j = (int64_t)blockIdx.x * 32 + r, n = *count;
+    if ((int64_t)blockIdx.x * 32 >= n) return;
+    float a = 0.0f;
+    if (j < n)
+        for (int p = g; p < nparts; p += 8) a += partial[(int64_t)p * ld + j];
+    sh[g][r] = a;
+    __syncthreads();
+    if (g == 0 && j < n) {
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += sh[k][r];
+        const float l = log1pf(s);
+        s_out[j] = s;
+        loss[idx[j]] = l;
+        lse[idx[j]] = lt[j] + l;
+    }
+}
+
+// The parts of row j of the x-gradient: at(c, k) is column c in the k-th part, k = 0 .. last(c).
+struct SlotView {
+    float *base;
+    int64_t tiles_n, total, pairs, j;
+    int KB;
+    __device__ __forceinline__ SlotView(float *slots, int64_t count, int64_t R, int KB_, int64_t pairs_, int64_t j_)
+        : base(slots), tiles_n((R + CE_TILE - 1) / CE_TILE), j(j_), KB(KB_) {
+        total = (count + CE_TILE - 1) / CE_TILE * tiles_n * KB;
+        pairs = cut_pairs(total, pairs_);
+    }
+    __device__ __forceinline__ int64_t tile(int64_t c) const { return (j / CE_TILE) * tiles_n + c / CE_TILE; }
+    __device__ __forceinline__ int64_t first(int64_t c) const { return cut_owner(total, pairs, tile(c) * KB); }
+    __device__ __forceinline__ int64_t last(int64_t c) const { return cut_owner(total, pairs, (tile(c) + 1) * KB - 1) - first(c); }
+    __device__ __forceinline__ float *at(int64_t c, int64_t k) const {
+        return base + (slot_of(tile(c), first(c) + k) * CE_TILE + j % CE_TILE) * CE_TILE + c % CE_TILE;
+    }
+};
+
+// Rows whose sum left float32's range: logits once more on CUDA cores, first the maximum and the sum relative to it, then (grad)
+// the gradient itself.  One row per block at a time; the row of slot 0 receives the finished gradient and s becomes -1.
+template <typename T>
+__global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, float *__restrict__ s_io, float *__restrict__ lse,
+                                                        float *__restrict__ loss, float *__restrict__ slots, int KB, int64_t pairs) {
+    __shared__ float sh_m[16], sh_s[16], sh_p[16];
+    __shared__ int sh_v;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t n = *a.count;
+    for (int64_t j = blockIdx.x; j < n; j += gridDim.x) {
+        if (!(s_io[j] >= S_LIMIT)) continue;           // not-a-number is the answer already
+        const int64_t row = a.idx[j], t = a.target[row];
+        const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+        const float lt = a.lt[j];
+        auto logit = [&](int64_t v) {
+            float d = 0.0f;
+            for (int64_t c = lane; c < a.R; c += 32) d = fmaf(to_f32<T>(x[c]), vocab_at<T>(voc, v, c), d);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+            return d;
+        };
+        float m = lt, s = 0.0f;                        // sum of exp(l - m) over the columns other than t, m the maximum so far
+        for (int64_t v = warp; v < a.V; v += 16) {
+            if (v == t) continue;
+            const float l = logit(v);
+            if (l > m) { s = s * expf(m - l) + 1.0f; m = l; }
+            else s += expf(l - m);
+        }
+        if (lane == 0) { sh_m[warp] = m; sh_s[warp] = s; }
+        __syncthreads();
+        float mm = sh_m[0], ss = 0.0f;
+        for (int k = 1; k < 16; ++k) mm = fmaxf(mm, sh_m[k]);
+        for (int k = 0; k < 16; ++k) ss += sh_s[k] * expf(sh_m[k] - mm);
+        const float full = mm + logf(ss + expf(lt - mm));
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            loss[row] = full - lt;
+            lse[row] = full;
+            s_io[j] = -1.0f;
+        }
+        if (slots) {
+            const SlotView o(slots, n, a.R, KB, pairs, j);
+            const float pt = expf(lt - full);
+            for (int64_t c = threadIdx.x; c < a.R; c += blockDim.x) *o.at(c, 0) = (pt - 1.0f) * vocab_at<T>(voc, t, c);
+            __syncthreads();
+            for (int64_t v0 = 0; v0 < a.V; v0 += 16) {
+                const int64_t v = v0 + warp;
+                float p = 0.0f;
+                if (v < a.V && v != t) p = expf(logit(v) - full);
+                if (lane == 0) sh_p[warp] = p;
+                if (threadIdx.x == 0) sh_v = 0;
+                __syncthreads();
+                if (lane == 0 && p > 0.0f) sh_v = 1;
+                __syncthreads();
+                if (sh_v) {
+                    for (int64_t c = threadIdx.x; c < a.R; c += blockDim.x) {
+                        float acc = *o.at(c, 0);
+                        for (int k = 0; k < 16; ++k)
+                            if (sh_p[k] > 0.0f) acc = fmaf(sh_p[k], vocab_at<T>(voc, v0 + k, c), acc);
+                        *o.at(c, 0) = acc;
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+    }
+}
+
+__global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__ loss_rows, const int32_t *__restrict__ idx,
+                                                       const int32_t *__restrict__ count, float *__restrict__ loss, int mean) {
+    __shared__ double sh[1024];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int n = *count;
+    double a = 0.0;
+    for (int j = threadIdx.x; j < n; j += 1024) a += (double)loss_rows[idx[j]];
+    sh[threadIdx.x] = a;
+    __syncthreads();
+    for (int o = 512; o; o >>= 1) {
+        if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *loss = (float)(mean ? sh[0] / (double)n : sh[0]);
+}
+
+// x's gradient from the slots: their sum, finished with s and the target's row (noise: voc.w null and s given), written to the
+// rows' own places; zeros at ignored rows.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int32_t *__restrict__ map,
+                                                    const int32_t *__restrict__ count, const float *__restrict__ s, const int32_t *__restrict__ tcol,
+                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int64_t pairs) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t n = *count;
+    for (int64_t i = blockIdx.x; i < T_rows; i += gridDim.x) {
+        const int64_t j = map[i];
+        if (j < 0) {
+            for (int64_t c = threadIdx.x; c < R; c += blockDim.x) dx[i * R + c] = from_f32<T>(0.0f);
+            continue;
+        }
+        const SlotView o(slots, n, R, KB, pairs, j);
+        const float sj = s ? s[j] : 0.0f;
+        const int64_t t = s ? tcol[j] : 0;
+        for (int64_t c = threadIdx.x; c < R; c += blockDim.x) {
+            float v = *o.at(c, 0);
+            if (!(sj < 0.0f)) {                       // -1: the row was finished by ce_rescue_kernel
+                const int64_t last = o.last(c);
+                for (int64_t k = 1; k <= last; ++k) v += *o.at(c, k);
+                if (s) v = t >= 0 ? (v - sj * vocab_at<T>(voc, t, c)) / (1.0f + sj) : NAN;
+            }
+            dx[i * R + c] = from_f32<T>(v);
+        }
+    }
+}
+
+// dz = unit gradient times what the loss's own gradient (and the mean's 1 / count) say
+template <typename T>
+__global__ void __launch_bounds__(256) ce_scale_kernel(T *__restrict__ dz, const T *__restrict__ unit, const float *__restrict__ dloss,
+                                                       const float *__restrict__ count, int64_t rows, int64_t R, int reduction) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t total = rows * R;
+    const float g0 = reduction == RDB_CE_NONE ? 0.0f : reduction == RDB_CE_MEAN ? dloss[0] / *count : dloss[0];
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const float u = to_f32<T>(unit[i]);
+        const float g = reduction == RDB_CE_NONE ? dloss[i / R] : g0;
+        dz[i] = from_f32<T>(u == 0.0f ? 0.0f : u * g);       // ignored rows stay zero whatever the factor (0 rows: 1 / 0)
+    }
+}
+
+// ================================================================================================
+// host side
+// ================================================================================================
+struct CePlan {
+    int parts, nterm;
+    int64_t Mpad, Rp, lda;           // rows rounded to tiles; columns of one part, of all parts
+    int64_t piece, npieces;          // vocabulary columns per piece (a multiple of 256), pieces
+    bool stage_b;                    // the matrix goes through the workspace in bf16 parts
+    int pairs;
+    int64_t slot_rows;               // rows of 256 float32 that the parts of the x-gradient take
+    bool dw_direct;
+    int64_t ld_dw;
+    // workspace
+    size_t idx, map, count, off2, lt, scale, tval, tcol, s, a, b, e, partial, slots, dw, total;
+};
+
+constexpr size_t E_BUDGET = 512ull << 20;
+constexpr size_t B_BUDGET = 256ull << 20;
+
+static int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+// op 0: loss; 1: loss and unit gradient of x (noise); 2: gradients of a stored matrix
+static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw, const void *dw, int want_dx, int want_dw) {
+    CePlan p{};
+    p.parts = dtype == RDB_F32 ? 3 : 1;
+    p.nterm = dtype == RDB_F32 ? 6 : 1;
+    p.Mpad = round_up(T, CE_TILE);
+    p.Rp = round_up(R, p.parts == 3 ? 64 : 8);
+    p.lda = p.Rp * p.parts;
+    p.pairs = max_resident_pairs();
+    // a stored bf16 matrix whose rows start on 16-byte boundaries is read where it is
+    p.stage_b = !(w && dtype == RDB_BF16 && (ldw % 8) == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0);
+    const int64_t vtiles = cdiv64(V, CE_TILE);
+    int64_t most = vtiles;
+    if (op != 0) {
+        const int64_t m = (int64_t)(E_BUDGET / ((size_t)p.Mpad * p.parts * 2 * CE_TILE + 1));
+        most = m < most ? m : most;
+    }
+    if (p.stage_b) {
+        const int64_t m = (int64_t)(B_BUDGET / ((size_t)p.lda * 2 * CE_TILE));
+        most = m < most ? m : most;
+    }
+    if (most < 1) most = 1;
+    p.npieces = cdiv64(vtiles, most);
+    const int64_t per = cdiv64(vtiles, p.npieces);
+    p.npieces = cdiv64(vtiles, per);
+    p.piece = per * CE_TILE;
+    p.slot_rows = ((p.Mpad / CE_TILE) * cdiv64(R, CE_TILE) + p.pairs) * CE_TILE;
+    const size_t es = dtype_size(dtype);
+    p.dw_direct = dw && (reinterpret_cast<uintptr_t>(dw) & 15) == 0 && (R * es) % 16 == 0;
+    p.ld_dw = round_up(R, 8);
+    size_t o = 0;
+    auto take = [&](size_t bytes) { const size_t at = o; o += align_up(bytes, 1024); return at; };
+    p.idx = take((size_t)p.Mpad * 4);
+    p.map = take((size_t)T * 4);
+    p.count = take(16);
+    p.off2 = take((size_t)p.Mpad * 4);
+    p.tcol = take((size_t)p.Mpad * 4);
+    p.lt = take((size_t)p.Mpad * 4);
+    p.s = take((size_t)p.Mpad * 4);
+    p.scale = take(op == 2 ? (size_t)p.Mpad * 4 : 0);
+    p.tval = take(op == 2 ? (size_t)p.Mpad * 4 : 0);
+    p.a = take((size_t)p.Mpad * p.lda * 2);
+    p.b = take(p.stage_b ? (size_t)p.piece * p.lda * 2 : 0);
+    p.e = take(op != 0 ? (size_t)p.Mpad * p.piece * p.parts * 2 : 0);
+    p.partial = take(op != 2 ? (size_t)p.npieces * (p.piece / CE_TILE) * 2 * p.Mpad * 4 : 0);
+    p.slots = take(op == 1 || (op == 2 && want_dx) ? (size_t)p.slot_rows * CE_TILE * 4 : 0);
+    p.dw = take(op == 2 && want_dw && !p.dw_direct ? (size_t)p.piece * p.ld_dw * es : 0);
+    p.total = o;
+    return p;
+}
+
+static void ce_terms(CeArgs *a, int nterm, int64_t a_cols, int64_t b_cols) {
+    a->nterm = nterm;
+    static const int pa[6] = {0, 1, 2, 0, 1, 0}, pb[6] = {2, 1, 0, 1, 0, 0};    // smallest first
+    for (int i = 0; i < nterm; ++i) {
+        a->a_off[i] = nterm == 1 ? 0 : (int)(pa[i] * a_cols);
+        a->b_off[i] = nterm == 1 ? 0 : (int)(pb[i] * b_cols);
+    }
+}
+
+template <int A_MN, int B_MN, int EPI, int PARTS>
+static int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &td, const CeArgs &args, int64_t max_items, int pairs,
+                       cudaStream_t st) {
+    auto kern = ce_pair_kernel<A_MN, B_MN, EPI, PARTS>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CE_SMEM);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(CE_THREADS);
+    cfg.dynamicSmemBytes = CE_SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const int64_t n = max_items < pairs ? max_items : pairs;
+    cfg.gridDim = dim3((unsigned)(2 * (n < 1 ? 1 : n)));
+    e = cudaLaunchKernelEx(&cfg, kern, ta, tb, td, args);
+    if (e != cudaSuccess) return (int)e;
+    return launch_status();
+}
+
+struct CeCall {
+    CePlan p;
+    uint8_t *ws;
+    const void *x;
+    int64_t ldx, T, R, V;
+    Vocab voc;
+    const int64_t *target;
+    int dtype;
+    int32_t *status;
+    cudaStream_t st;
+    template <typename P> P *at(size_t off) const { return reinterpret_cast<P *>(ws + off); }
+};
+
+static int ce_find_rows(const CeCall &c, int64_t ignore, int use_ignore, float *zero_a, float *zero_b, float *count_f) {
+    return launch_pdl(ce_rows_kernel, dim3(1), 1024, 0, c.st, c.target, c.T, ignore, use_ignore, c.at<int32_t>(c.p.idx), c.at<int32_t>(c.p.map),
+                      c.at<int32_t>(c.p.count), zero_a, zero_b, count_f);
+}
+
+static CeRowArgs ce_row_args(const CeCall &c) {
+    CeRowArgs a{};
+    a.x = c.x; a.ldx = c.ldx; a.T = c.T; a.R = c.R; a.V = c.V;
+    a.target = c.target;
+    a.idx = c.at<int32_t>(c.p.idx);
+    a.count = c.at<int32_t>(c.p.count);
+    a.a = c.at<__nv_bfloat16>(c.p.a);
+    a.lda = c.p.lda; a.part_cols = c.p.Rp;
+    a.off2 = c.at<float>(c.p.off2);
+    a.lt = c.at<float>(c.p.lt);
+    a.scale = c.at<float>(c.p.scale);
+    a.tval = c.at<float>(c.p.tval);
+    a.tcol = c.at<int32_t>(c.p.tcol);
+    return a;
+}
+
+static int ce_gather(const CeCall &c, const CeRowArgs &a) {
+    const dim3 grid((unsigned)(c.p.Mpad / 8));
+    if (c.dtype == RDB_F32) return launch_pdl(ce_gather_kernel<float, 3>, grid, 256, 0, c.st, a, c.voc);
+    return launch_pdl(ce_gather_kernel<__nv_bfloat16, 1>, grid, 256, 0, c.st, a, c.voc);
+}
+
+// The matrix's rows [v0, v0 + n) as a bf16 operand: where it starts and its pitch.
+static int ce_stage(const CeCall &c, int64_t v0, int64_t n, const void **base, int64_t *ld) {
+    if (!c.p.stage_b) {
+        *base = reinterpret_cast<const __nv_bfloat16 *>(c.voc.w) + v0 * c.voc.ldw;
+        *ld = c.voc.ldw;
+        return RDB_OK;
+    }
+    __nv_bfloat16 *b = c.at<__nv_bfloat16>(c.p.b);
+    *base = b;
+    *ld = c.p.lda;
+    if (!c.voc.w && c.dtype == RDB_BF16)
+        return rdb_noise(b, RDB_BF16, n, c.R, c.p.lda, (int64_t)c.voc.row0 + v0, 0, c.voc.seed, c.st);
+    const int64_t want = cdiv64(n * c.p.Rp, 256 * 4);
+    const dim3 grid((unsigned)(want < 148 * 8 ? (want < 1 ? 1 : want) : 148 * 8));
+    if (c.dtype == RDB_F32) return launch_pdl(ce_split_kernel<float, 3>, grid, 256, 0, c.st, b, c.p.lda, c.p.Rp, n, c.R, v0, c.voc);
+    return launch_pdl(ce_split_kernel<__nv_bfloat16, 1>, grid, 256, 0, c.st, b, c.p.lda, c.p.Rp, n, c.R, v0, c.voc);
+}
+
+// logits of one piece through the epilogue EPI
+template <int EPI>
+static int ce_logits(const CeCall &c, const void *b, int64_t ldb, int64_t v0, int64_t n, int64_t piece_index) {
+    const CePlan &p = c.p;
+    const int64_t width = p.parts == 1 ? c.R : p.lda;              // columns beyond read as zero
+    CUtensorMap ta, tb, td;
+    int rc = make_tmap(&ta, c.at<void>(p.a), width, p.Mpad, p.lda, BK, BM);
+    if (rc) return rc;
+    rc = make_tmap(&tb, b, width, n, ldb, BK, BM);
+    if (rc) return rc;
+    td = ta;
+    CeArgs a{};
+    if (EPI != EPI_SUM) {
+        rc = make_tmap(&td, c.at<void>(p.e), p.piece * p.parts, p.Mpad, p.piece * p.parts, 64, 32);
+        if (rc) return rc;
+    }
+    a.count = c.at<int32_t>(p.count);
+    a.m_counted = 1;
+    a.N = p.piece;                    // columns past the vocabulary's end come out as zeros
+    if (EPI == EPI_SUM) a.N = n;
+    a.kbs = (int)cdiv64(p.parts == 1 ? c.R : p.Rp, BK);
+    ce_terms(&a, p.nterm, p.Rp, p.Rp);
+    a.m_fast = 1;
+    a.off2 = c.at<float>(p.off2);
+    a.scale = c.at<float>(p.scale);
+    a.tval = c.at<float>(p.tval);
+    a.tcol = c.at<int32_t>(p.tcol);
+    a.v0 = (int32_t)v0;
+    a.ncols = (int32_t)n;
+    a.partial = c.at<float>(p.partial) + piece_index * (p.piece / CE_TILE) * 2 * p.Mpad;
+    a.ld_partial = p.Mpad;
+    a.part_cols = (int)p.piece;
+    a.status = c.status;
+    const int64_t items = (p.Mpad / CE_TILE) * cdiv64(a.N, CE_TILE);
+    if (p.parts == 3) return launch_pair<0, 0, EPI, 3>(ta, tb, td, a, items, p.pairs, c.st);
+    return launch_pair<0, 0, EPI, 1>(ta, tb, td, a, items, p.pairs, c.st);
+}
+
+// slots (+)= E W_piece
+static int ce_accumulate(const CeCall &c, const void *b, int64_t ldb, int64_t n, bool add) {
+    const CePlan &p = c.p;
+    CUtensorMap ta, tb, td;
+    int rc = make_tmap(&ta, c.at<void>(p.e), p.piece * p.parts, p.Mpad, p.piece * p.parts, BK, BM);
+    if (rc) return rc;
+    rc = make_tmap(&tb, b, p.parts == 1 ? c.R : p.lda, n, ldb, 64, BK);
+    if (rc) return rc;
+    rc = make_tmap(&td, c.at<void>(p.slots), CE_TILE, p.slot_rows, CE_TILE, 32, 32, true);
+    if (rc) return rc;
+    CeArgs a{};
+    a.count = c.at<int32_t>(p.count);
+    a.m_counted = 1;
+    a.N = c.R;
+    a.kbs = (int)cdiv64(p.piece, BK);
+    ce_terms(&a, p.nterm, p.piece, p.Rp);
+    a.m_fast = 0;
+    a.accumulate = add ? 1 : 0;
+    a.status = c.status;
+    return launch_pair<0, 1, EPI_SLOT, 1>(ta, tb, td, a, p.pairs, p.pairs, c.st);
+}
+
+// dW rows [v0, v0 + n) = P^T x
+static int ce_dw(const CeCall &c, void *dw, int64_t v0, int64_t n) {
+    const CePlan &p = c.p;
+    const size_t es = dtype_size(c.dtype);
+    const int64_t ldd = p.dw_direct ? c.R : p.ld_dw;
+    void *out = p.dw_direct ? static_cast<void *>(static_cast<uint8_t *>(dw) + (size_t)v0 * c.R * es) : c.at<void>(p.dw);
+    CUtensorMap ta, tb, td;
+    int rc = make_tmap(&ta, c.at<void>(p.e), p.piece * p.parts, p.Mpad, p.piece * p.parts, 64, BK);
+    if (rc) return rc;
+    rc = make_tmap(&tb, c.at<void>(p.a), p.parts == 1 ? c.R : p.lda, p.Mpad, p.lda, 64, BK);
+    if (rc) return rc;
+    rc = c.dtype == RDB_F32 ? make_tmap(&td, out, c.R, n, ldd, 32, 32, true) : make_tmap(&td, out, c.R, n, ldd, 64, 32);
+    if (rc) return rc;
+    CeArgs a{};
+    a.count = c.at<int32_t>(p.count);
+    a.k_counted = 1;
+    a.M = n;
+    a.N = c.R;
+    ce_terms(&a, p.nterm, p.piece, p.Rp);
+    a.m_fast = 0;
+    a.status = c.status;
+    const int64_t items = cdiv64(n, CE_TILE) * cdiv64(c.R, CE_TILE);
+    rc = c.dtype == RDB_F32 ? launch_pair<1, 1, EPI_F32, 1>(ta, tb, td, a, items, p.pairs, c.st)
+                            : launch_pair<1, 1, EPI_BF16, 1>(ta, tb, td, a, items, p.pairs, c.st);
+    if (rc || p.dw_direct) return rc;
+    cudaError_t e = cudaMemcpy2DAsync(static_cast<uint8_t *>(dw) + (size_t)v0 * c.R * es, c.R * es, out, ldd * es, c.R * es, n, cudaMemcpyDeviceToDevice, c.st);
+    return e == cudaSuccess ? RDB_OK : (int)e;
+}
+
+static int ce_kb(const CePlan &p) { return p.nterm * (int)cdiv64(p.piece, BK); }
+
+static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
+    const CePlan &p = c.p;
+    const dim3 grid((unsigned)(c.T < 148 * 16 ? c.T : 148 * 16));
+    const float *s = unit ? c.at<float>(p.s) : nullptr;
+    const int32_t *map = c.at<int32_t>(p.map), *count = c.at<int32_t>(p.count), *tcol = c.at<int32_t>(p.tcol);
+    float *slots = c.at<float>(p.slots);
+    if (c.dtype == RDB_F32)
+        return launch_pdl(ce_dx_kernel<float>, grid, 256, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), (int64_t)p.pairs);
+    return launch_pdl(ce_dx_kernel<__nv_bfloat16>, grid, 256, 0, c.st, (__nv_bfloat16 *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p),
+                      (int64_t)p.pairs);
+}
+
+static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w, int64_t ldw, int dtype, int reduction) {
+    if (T < 0 || R < 1 || V < 1 || ldx < R || (w && ldw < R)) return RDB_ERR_SHAPE;
+    if (dtype != RDB_F32 && dtype != RDB_BF16) return RDB_ERR_DTYPE;
+    if (reduction != RDB_CE_NONE && reduction != RDB_CE_MEAN && reduction != RDB_CE_SUM) return RDB_ERR_UNSUPPORTED;
+    // coordinates of the tiled copies are 32-bit
+    if (T > (1LL << 28) || V > (1LL << 30) || R > (1LL << 24)) return RDB_ERR_TOO_LARGE;
+    return RDB_OK;
+}
+
+}  // namespace rdb
+
+using namespace rdb;
+
+extern "C" size_t rdb_ce_workspace_bytes(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw) {
+    if (op < RDB_CE_LOSS || op > RDB_CE_GRADS || ce_check(T, R, V, R, w, ldw, dtype, RDB_CE_SUM) != RDB_OK || T == 0) return 1024;
+    return ce_plan(op, T, R, V, dtype, w, ldw, nullptr, 1, 1).total;
+}
+
+extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
+                          void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t V, int64_t row0, uint32_t seed,
+                          int64_t ignore_index, int use_ignore, int dtype, int reduction, int32_t *status, void *stream) {
+    int rc = ce_check(T, R, V, ldx, w, ldw, dtype, reduction);
+    if (rc) return rc;
+    if (dx_unit && w) return RDB_ERR_UNSUPPORTED;        // a stored matrix takes its gradients in rdb_ce_bwd
+    if (!aux || (!loss && reduction != RDB_CE_NONE)) return RDB_ERR_NULL;
+    if (T > 0 && (!x || !target)) return RDB_ERR_NULL;
+    const size_t es = dtype_size(dtype);
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(dx_unit)) & (es - 1)) || (reinterpret_cast<uintptr_t>(target) & 7))
+        return RDB_ERR_ALIGN;
+    CeCall c{};
+    c.p = ce_plan(dx_unit ? 1 : 0, T, R, V, dtype, w, ldw, nullptr, 1, 0);
+    if (!workspace || workspace_bytes < (T ? c.p.total : 1024) || (reinterpret_cast<uintptr_t>(workspace) & 255)) return RDB_ERR_WORKSPACE;
+    c.ws = reinterpret_cast<uint8_t *>(workspace);
+    c.x = x; c.ldx = ldx; c.T = T; c.R = R; c.V = V;
+    c.voc = Vocab{w, ldw, seed, (uint32_t)row0};
+    c.target = target;
+    c.dtype = dtype;
+    c.status = status;
+    c.st = (cudaStream_t)stream;
+    float *lse = aux, *rows = aux + T, *count_f = aux + 2 * T;
+    if ((rc = ce_find_rows(c, ignore_index, use_ignore, lse, rows, count_f))) return rc;
+    if (T > 0) {
+        const CeRowArgs ra = ce_row_args(c);
+        if ((rc = ce_gather(c, ra))) return rc;
+        for (int64_t i = 0; i < c.p.npieces; ++i) {
+            const int64_t v0 = i * c.p.piece, n = V - v0 < c.p.piece ? V - v0 : c.p.piece;
+            const void *b;
+            int64_t ldb;
+            if ((rc = ce_stage(c, v0, n, &b, &ldb))) return rc;
+            if (dx_unit) {
+                if ((rc = ce_logits<EPI_EXP>(c, b, ldb, v0, n, i))) return rc;
+                if ((rc = ce_accumulate(c, b, ldb, n, i > 0))) return rc;
+            } else if ((rc = ce_logits<EPI_SUM>(c, b, ldb, v0, n, i))) return rc;
+        }
+        // row sums: a full piece leaves two per column tile; without the gradient the last piece has only the tiles that exist
+        const int64_t last = V - (c.p.npieces - 1) * c.p.piece;
+        const int nparts = (int)((c.p.npieces - 1) * (c.p.piece / CE_TILE) * 2 + (dx_unit ? c.p.piece / CE_TILE : cdiv64(last, CE_TILE)) * 2);
+        rc = launch_pdl(ce_sum_kernel, dim3((unsigned)(c.p.Mpad / 32)), 256, 0, c.st, (const float *)c.at<float>(c.p.partial), c.p.Mpad, nparts, ra.idx,
+                        ra.count, (const float *)ra.lt, c.at<float>(c.p.s), lse, rows);
+        if (rc) return rc;
+        float *slots = dx_unit ? c.at<float>(c.p.slots) : nullptr, *sums = c.at<float>(c.p.s);
+        const int64_t pairs = c.p.pairs;
+        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs)
+                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs);
+        if (rc) return rc;
+        if (dx_unit && (rc = ce_finish_dx(c, dx_unit, true))) return rc;
+    }
+    if (reduction == RDB_CE_NONE) return RDB_OK;
+    return launch_pdl(ce_loss_kernel, dim3(1), 1024, 0, c.st, (const float *)rows, (const int32_t *)c.at<int32_t>(c.p.idx),
+                      (const int32_t *)c.at<int32_t>(c.p.count), loss, reduction == RDB_CE_MEAN ? 1 : 0);
+}
+
+extern "C" int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
+                          const float *aux, void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t V, int64_t ignore_index,
+                          int use_ignore, int dtype, int reduction, int32_t *status, void *stream) {
+    int rc = ce_check(T, R, V, ldx, w, ldw, dtype, reduction);
+    if (rc) return rc;
+    if (!dx && !dw) return RDB_OK;
+    if (T > 0 && (!w || !dloss || !aux || !x || !target)) return RDB_ERR_NULL;
+    const size_t es = dtype_size(dtype);
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & (es - 1)) ||
+        (reinterpret_cast<uintptr_t>(target) & 7))
+        return RDB_ERR_ALIGN;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T == 0) {
+        if (!dw) return RDB_OK;
+        cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)V * R * es, st);
+        return e == cudaSuccess ? RDB_OK : (int)e;
+    }
+    CeCall c{};
+    c.p = ce_plan(2, T, R, V, dtype, w, ldw, dw, dx ? 1 : 0, dw ? 1 : 0);
+    if (!workspace || workspace_bytes < c.p.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return RDB_ERR_WORKSPACE;
+    c.ws = reinterpret_cast<uint8_t *>(workspace);
+    c.x = x; c.ldx = ldx; c.T = T; c.R = R; c.V = V;
+    c.voc = Vocab{w, ldw, 0, 0};
+    c.target = target;
+    c.dtype = dtype;
+    c.status = status;
+    c.st = st;
+    if ((rc = ce_find_rows(c, ignore_index, use_ignore, nullptr, nullptr, nullptr))) return rc;
+    CeRowArgs ra = ce_row_args(c);
+    ra.dloss = dloss;
+    ra.lse = aux;
+    ra.loss = aux + T;
+    ra.reduction = reduction;
+    if ((rc = ce_gather(c, ra))) return rc;
+    for (int64_t i = 0; i < c.p.npieces; ++i) {
+        const int64_t v0 = i * c.p.piece, n = V - v0 < c.p.piece ? V - v0 : c.p.piece;
+        const void *b;
+        int64_t ldb;
+        if ((rc = ce_stage(c, v0, n, &b, &ldb))) return rc;
+        if ((rc = ce_logits<EPI_PROB>(c, b, ldb, v0, n, i))) return rc;
+        if (dx && (rc = ce_accumulate(c, b, ldb, n, i > 0))) return rc;
+        if (dw && (rc = ce_dw(c, dw, v0, n))) return rc;
+    }
+    if (dx) return ce_finish_dx(c, dx, false);
+    return RDB_OK;
+}
+
+extern "C" int rdb_ce_scale(void *dz, const void *unit, const float *dloss, const float *aux, int64_t T, int64_t R, int dtype, int reduction,
+                            void *stream) {
+    int rc = ce_check(T, R, 1, R, nullptr, 0, dtype, reduction);
+    if (rc) return rc;
+    if (T == 0) return RDB_OK;
+    if (!dz || !unit || !dloss || !aux) return RDB_ERR_NULL;
+    cudaStream_t st = (cudaStream_t)stream;
+    const int64_t want = cdiv64(T * R, 256 * 8);
+    const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8));
+    if (dtype == RDB_F32)
+        return launch_pdl(ce_scale_kernel<float>, grid, 256, 0, st, (float *)dz, (const float *)unit, dloss, aux + 2 * T, T, R, reduction);
+    return launch_pdl(ce_scale_kernel<__nv_bfloat16>, grid, 256, 0, st, (__nv_bfloat16 *)dz, (const __nv_bfloat16 *)unit, dloss, aux + 2 * T, T, R, reduction);
+}

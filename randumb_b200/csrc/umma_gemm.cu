@@ -31,16 +31,11 @@
 
 #include "common.cuh"
 #include "umma.cuh"
+#include "umma_pipe.cuh"
 
 namespace rdb {
 
 using namespace ptx;
-
-constexpr int BM = 128;            // rows of one MMA (TMEM lanes)
-constexpr int BK = 64;             // bf16 elements per 128-byte swizzle row
-constexpr int UMMA_K = 16;         // K extent of one tcgen05.mma for 16-bit inputs
-constexpr int SUB_BYTES = BM * BK * 2;  // one [128 x 64] bf16 sub-tile
-constexpr int TMEM_COLS = 512;
 
 // ------------------------------------------------------------------------------------------------
 // epilogue helpers: one thread owns one accumulator row, 32 consecutive columns in registers
@@ -91,18 +86,6 @@ __device__ __forceinline__ void store_row32_bf16(__nv_bfloat16 *dst, const uint3
         for (int v = 0; v < 4; ++v)
             if (v * 8 < ncols) *reinterpret_cast<uint4 *>(dst + v * 8) = make_uint4(p[4 * v], p[4 * v + 1], p[4 * v + 2], p[4 * v + 3]);
     }
-}
-
-struct PipeState {
-    uint32_t idx = 0, phase = 0;
-    template <int STAGES> __device__ __forceinline__ void advance() {
-        if (++idx == STAGES) { idx = 0; phase ^= 1; }
-    }
-};
-
-__device__ __forceinline__ void raise_abort(volatile int *abort_flag, int32_t *status, int code) {
-    *abort_flag = 1;
-    if (status) atomicCAS(status, 0, code);
 }
 
 // ================================================================================================
@@ -1489,8 +1472,8 @@ static void ensure_context() {
 }
 
 // bf16 matrix with `inner` contiguous elements per row, `outer` rows, row pitch ld elements.
-static int make_tmap(CUtensorMap *m, const void *base, int64_t inner, int64_t outer, int64_t ld, uint32_t box_inner,
-                     uint32_t box_outer, bool f32 = false) {
+int make_tmap(CUtensorMap *m, const void *base, int64_t inner, int64_t outer, int64_t ld, uint32_t box_inner,
+                     uint32_t box_outer, bool f32) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return RDB_ERR_DRIVER;
     ensure_context();
@@ -1510,7 +1493,7 @@ static int make_tmap(CUtensorMap *m, const void *base, int64_t inner, int64_t ou
     return RDB_OK;
 }
 
-static int sm_count() {
+int sm_count() {
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 148;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
@@ -1728,7 +1711,7 @@ static int launch_dense_pair(void *const *dsts, int64_t rows_per_dst, const void
 }
 
 // how many CTA pairs can be resident at once (one CTA per SM)
-static int max_resident_pairs() {
+int max_resident_pairs() {
     static thread_local int cached_dev = -1, cached = 0;
     int dev = 0;
     (void)cudaGetDevice(&dev);

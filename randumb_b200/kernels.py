@@ -410,6 +410,83 @@ def embed_bwd(idx: torch.Tensor, dout: torch.Tensor, dcoefs_size: int, rowsize: 
     return dcoef
 
 
+# ------------------------------------------------------------------------------------------ cross entropy over a vocabulary
+def _ce_args(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor, V: int, reduction: str):
+    dev = _need_cuda(x, weight, target)
+    if x.dim() != 2 or target.dim() != 1 or target.shape[0] != x.shape[0]:
+        raise RuntimeError(f"cross entropy: x {tuple(x.shape)} and target {tuple(target.shape)} do not match [T, R] / [T]")
+    if target.dtype != torch.int64:
+        raise RuntimeError(f"cross entropy: target must be int64, got {target.dtype}")
+    if weight is not None and (weight.dim() != 2 or weight.shape[1] != x.shape[1] or weight.dtype != x.dtype):
+        raise RuntimeError(f"cross entropy: weight {tuple(weight.shape)} {weight.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    if x.shape[1] < 1 or V < 1:
+        raise RuntimeError("cross entropy: needs at least one column and one vocabulary row")
+    if reduction not in _lib.CE_REDUCTIONS:
+        raise RuntimeError(f"cross entropy: reduction must be one of {sorted(_lib.CE_REDUCTIONS)}, got {reduction!r}")
+    return dev, _dt(x.dtype), _lib.CE_REDUCTIONS[reduction]
+
+
+def _ce_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or _rows_ok(t) else t.contiguous()
+
+
+def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor, ignore_index: Optional[int] = -100, reduction: str = "mean",
+           seed: int = 0, vocab: int = 0, row0: int = 0, need_unit: bool = False
+           ) -> Tuple[Optional[torch.Tensor], torch.Tensor, Optional[torch.Tensor]]:
+    """(loss, aux, unit): cross entropy of ``x @ W.T`` against ``target`` (see rdb_ce_fwd).  ``weight`` None: ``vocab`` noise rows
+    from ``row0`` on.  loss: 0-d float32 (None for reduction "none": the rows' losses are ``aux[T:2T]``); unit: the rows' own
+    gradients in x, with ``need_unit``."""
+    V = int(vocab) if weight is None else weight.shape[0]
+    dev, dt, red = _ce_args(x, weight, target, V, reduction)
+    x, weight, target = _ce_rows(x), _ce_rows(weight), target.contiguous()
+    T, R = x.shape
+    L = _lib.lib()
+    aux = torch.empty((2 * T + 1,), dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
+    unit = torch.empty((T, R), dtype=x.dtype, device=dev) if need_unit else None
+    with torch.cuda.device(dev):
+        ldw = _pitch(weight) if weight is not None else 0
+        ws = _workspace(L.rdb_ce_workspace_bytes(_lib.CE_LOSS_GRAD if need_unit else _lib.CE_LOSS, T, R, V, dt, _ptr(weight), ldw), dev)
+        rc = L.rdb_ce_fwd(_ptr(loss), _ptr(aux), _ptr(unit), _ptr(x), _pitch(x), _ptr(weight), ldw, _ptr(target), _ptr(ws), ws.numel(), T, R, V, row0,
+                          _seed(seed), 0 if ignore_index is None else int(ignore_index), 0 if ignore_index is None else 1, dt, red,
+                          _ptr(status_buffer(dev)), _stream(dev))
+    _lib.check(rc, "rdb_ce_fwd")
+    return loss, aux, unit
+
+
+def ce_scale(unit: torch.Tensor, dloss: torch.Tensor, aux: torch.Tensor, reduction: str) -> torch.Tensor:
+    dev = _need_cuda(unit, dloss, aux)
+    assert unit.is_contiguous() and aux.is_contiguous() and dloss.dtype == torch.float32
+    dloss = dloss.contiguous()
+    T, R = unit.shape
+    dz = torch.empty_like(unit)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().rdb_ce_scale(_ptr(dz), _ptr(unit), _ptr(dloss), _ptr(aux), T, R, _dt(unit.dtype), _lib.CE_REDUCTIONS[reduction], _stream(dev))
+    _lib.check(rc, "rdb_ce_scale")
+    return dz
+
+
+def ce_bwd(dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, aux: torch.Tensor, ignore_index: Optional[int] = -100,
+           reduction: str = "mean", need_dx: bool = True, need_dw: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dweight) of a stored matrix, contiguous, from the forward's ``aux``; either may be skipped."""
+    V = weight.shape[0]
+    dev, dt, red = _ce_args(x, weight, target, V, reduction)
+    x, weight, target, dloss = _ce_rows(x), _ce_rows(weight), target.contiguous(), dloss.contiguous()
+    assert dloss.dtype == torch.float32 and dloss.device == dev and dloss.numel() == (x.shape[0] if reduction == "none" else 1)
+    assert aux.dtype == torch.float32 and aux.device == dev and aux.is_contiguous() and aux.numel() == 2 * x.shape[0] + 1
+    T, R = x.shape
+    L = _lib.lib()
+    dx = torch.empty((T, R), dtype=x.dtype, device=dev) if need_dx else None
+    dw = torch.empty((V, R), dtype=x.dtype, device=dev) if need_dw else None
+    with torch.cuda.device(dev):
+        ws = _workspace(L.rdb_ce_workspace_bytes(_lib.CE_GRADS, T, R, V, dt, _ptr(weight), _pitch(weight)), dev)
+        rc = L.rdb_ce_bwd(_ptr(dx), _ptr(dw), _ptr(dloss), _ptr(x), _pitch(x), _ptr(weight), _pitch(weight), _ptr(target), _ptr(aux), _ptr(ws),
+                          ws.numel(), T, R, V, 0 if ignore_index is None else int(ignore_index), 0 if ignore_index is None else 1, dt, red,
+                          _ptr(status_buffer(dev)), _stream(dev))
+    _lib.check(rc, "rdb_ce_bwd")
+    return dx, dw
+
+
 # ------------------------------------------------------------------------------------------ exchange over peer memory
 def _ptr_array(ptrs):
     arr = (ctypes.c_void_p * len(ptrs))(*[int(p) for p in ptrs])

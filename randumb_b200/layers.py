@@ -151,6 +151,14 @@ class RandumbLinear(RandumbModuleMixin, nn.Module):
         coef = self.weight_coef if self.weight_coef.dtype == input.dtype else self.weight_coef.to(input.dtype)
         return ops.rlinear(input, coef, self.seed, self.out_features, self.row0, self.bias)
 
+    def cross_entropy(self, input: torch.Tensor, target: torch.Tensor, ignore_index: Optional[int] = -100, reduction: str = "mean") -> torch.Tensor:
+        """``F.cross_entropy(self(input), target)`` over this layer's outputs without forming them (see
+        ``ops.rlinear_cross_entropy``): the loss of a model whose last layer this is.  A layer with a bias is refused."""
+        if self.bias is not None:
+            raise RuntimeError("cross_entropy: the layer has a bias, which the fused loss does not add")
+        coef = self.weight_coef if self.weight_coef.dtype == input.dtype else self.weight_coef.to(input.dtype)
+        return ops.rlinear_cross_entropy(input, coef, self.seed, self.out_features, target, self.row0, ignore_index, reduction)
+
     def get_extra_state(self):
         return {"seed": self.seed, "d_c": self.d_c, "out_features": self.out_features, "row0": self.row0}
 

@@ -14,6 +14,13 @@ reference left to ``fakeMM`` (RandumbTensor.py:771-791, 942-946):
   rten::rlinear_bwd(dy, x, coef, seed, row0, need_dx, need_dc) -> (dx, dc)
   rten::noise(rows, cols, seed, row0, dtype, device) -> S
 
+and the loss over a large vocabulary, which keeps no logits (the reference ends in F.cross_entropy on all of them,
+modded-nanogpt/train_gpt2.py:236-240):
+
+  rten::noise_ce_fwd / rten::noise_ce_bwd     logits z S^T over regenerated noise rows
+  rten::linear_ce_fwd / rten::linear_ce_bwd   logits x W^T over a stored matrix
+  noise_cross_entropy, rlinear_cross_entropy, linear_cross_entropy   the differentiable functions on top of them
+
 Every operator is functional (fresh outputs, current stream), has a fake (meta) kernel so
 FakeTensor / torch.compile tracing works, and -- like the reference (RandumbTensor.py:438-448) --
 a CPU registration that raises ``NotImplementedError``: there is no CPU implementation.
@@ -108,6 +115,158 @@ def noise(rows: int, cols: int, seed: int, row0: int, dtype: torch.dtype, device
 @noise.register_fake
 def _(rows, cols, seed, row0, dtype, device):
     return torch.empty((rows, cols), dtype=dtype, device=device)
+
+
+# ------------------------------------------------------------------------------------------------
+# cross entropy over a large vocabulary
+# ------------------------------------------------------------------------------------------------
+@custom_op("rten::noise_ce_fwd", mutates_args=(), device_types="cuda")
+def noise_ce_fwd(z: torch.Tensor, target: torch.Tensor, seed: int, out_features: int, row0: int, ignore_index: Optional[int], reduction: str,
+                 need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    loss, aux, unit = K.ce_fwd(z, None, target, ignore_index, reduction, seed, out_features, row0, need_grad)
+    T = z.shape[0]
+    return aux[T:2 * T].clone() if loss is None else loss, aux, unit if unit is not None else z.new_empty((0,))
+
+
+@noise_ce_fwd.register_fake
+def _(z, target, seed, out_features, row0, ignore_index, reduction, need_grad):
+    T = z.shape[0]
+    return (z.new_empty((T,) if reduction == "none" else (), dtype=torch.float32), z.new_empty((2 * T + 1,), dtype=torch.float32),
+            z.new_empty(z.shape if need_grad else (0,)))
+
+
+noise_ce_fwd.register_kernel("cpu")(_cpu_raises("noise_ce_fwd"))
+
+
+@custom_op("rten::noise_ce_bwd", mutates_args=(), device_types="cuda")
+def noise_ce_bwd(dloss: torch.Tensor, unit: torch.Tensor, aux: torch.Tensor, reduction: str) -> torch.Tensor:
+    return K.ce_scale(unit, dloss, aux, reduction)
+
+
+@noise_ce_bwd.register_fake
+def _(dloss, unit, aux, reduction):
+    return torch.empty_like(unit)
+
+
+noise_ce_bwd.register_kernel("cpu")(_cpu_raises("noise_ce_bwd"))
+
+
+def _noise_ce_setup(ctx, inputs, output):
+    _, aux, unit = output
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(aux, unit)
+    ctx.save_for_backward(aux, unit)
+    ctx.reduction, ctx.has_unit = inputs[6], inputs[7]
+
+
+def _noise_ce_backward(ctx, dloss, daux, dunit):
+    aux, unit = ctx.saved_tensors
+    if dloss is None or not ctx.needs_input_grad[0]:
+        return (None,) * 8
+    if not ctx.has_unit:
+        raise RuntimeError("noise_ce_fwd was called with need_grad=False: it kept nothing for a backward pass")
+    return (noise_ce_bwd(dloss, unit, aux, ctx.reduction),) + (None,) * 7
+
+
+noise_ce_fwd.register_autograd(_noise_ce_backward, setup_context=_noise_ce_setup)
+
+
+@custom_op("rten::linear_ce_fwd", mutates_args=(), device_types="cuda")
+def linear_ce_fwd(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: Optional[int], reduction: str
+                  ) -> Tuple[torch.Tensor, torch.Tensor]:
+    loss, aux, _ = K.ce_fwd(x, weight, target, ignore_index, reduction)
+    T = x.shape[0]
+    return aux[T:2 * T].clone() if loss is None else loss, aux
+
+
+@linear_ce_fwd.register_fake
+def _(x, weight, target, ignore_index, reduction):
+    T = x.shape[0]
+    return x.new_empty((T,) if reduction == "none" else (), dtype=torch.float32), x.new_empty((2 * T + 1,), dtype=torch.float32)
+
+
+linear_ce_fwd.register_kernel("cpu")(_cpu_raises("linear_ce_fwd"))
+
+
+@custom_op("rten::linear_ce_bwd", mutates_args=(), device_types="cuda")
+def linear_ce_bwd(dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, aux: torch.Tensor, ignore_index: Optional[int],
+                  reduction: str, need_dx: bool, need_dw: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    dx, dw = K.ce_bwd(dloss, x, weight, target, aux, ignore_index, reduction, need_dx, need_dw)
+    return dx if dx is not None else x.new_empty((0,)), dw if dw is not None else weight.new_empty((0,))
+
+
+@linear_ce_bwd.register_fake
+def _(dloss, x, weight, target, aux, ignore_index, reduction, need_dx, need_dw):
+    return x.new_empty(x.shape if need_dx else (0,)), weight.new_empty(weight.shape if need_dw else (0,))
+
+
+linear_ce_bwd.register_kernel("cpu")(_cpu_raises("linear_ce_bwd"))
+
+
+def _linear_ce_setup(ctx, inputs, output):
+    x, weight, target, ctx.ignore_index, ctx.reduction = inputs
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, weight, target, output[1])
+
+
+def _linear_ce_backward(ctx, dloss, daux):
+    x, weight, target, aux = ctx.saved_tensors
+    need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+    if dloss is None or not (need_dx or need_dw):
+        return (None,) * 5
+    dx, dw = linear_ce_bwd(dloss, x, weight, target, aux, ctx.ignore_index, ctx.reduction, need_dx, need_dw)
+    return dx if need_dx else None, dw if need_dw else None, None, None, None
+
+
+linear_ce_fwd.register_autograd(_linear_ce_backward, setup_context=_linear_ce_setup)
+
+
+def noise_cross_entropy(z: torch.Tensor, seed: int, out_features: int, target: torch.Tensor, row0: int = 0, ignore_index: Optional[int] = -100,
+                        reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of the logits ``z @ S[row0:row0 + out_features].T`` (noise of ``seed`` in z's type) against ``target``,
+    for z of shape [..., R] and int64 target of shape [...]; differentiable in z.
+
+    The logits are never kept: the loss and, when z takes part in autograd, its gradient come out of one pass over the noise in
+    pieces.  Rows whose target is ``ignore_index`` (None: no such value) count for nothing, whatever they contain; any other
+    target outside [0, out_features) makes its row's loss and gradient NaN.  Returns float32: a scalar for reduction "mean" (over
+    the rows that count; NaN when there are none) and "sum", the rows' losses in target's shape for "none"."""
+    lead = z.shape[:-1]
+    if tuple(target.shape) != tuple(lead):
+        raise RuntimeError(f"noise_cross_entropy: target {tuple(target.shape)} does not match z {tuple(z.shape)}")
+    need = torch.is_grad_enabled() and z.requires_grad
+    loss = noise_ce_fwd(z.reshape(-1, z.shape[-1]), target.reshape(-1), seed, out_features, row0, ignore_index, reduction, need)[0]
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: Optional[int] = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of the logits ``x @ weight.T`` against ``target``, for x of shape [..., K], weight [V, K] of the same
+    type and int64 target of shape [...]; differentiable in x and weight.  The logits are never kept: the backward recomputes
+    them in pieces of the vocabulary.  ignore_index, other targets, reduction and result as ``noise_cross_entropy``."""
+    lead = x.shape[:-1]
+    if tuple(target.shape) != tuple(lead):
+        raise RuntimeError(f"linear_cross_entropy: target {tuple(target.shape)} does not match x {tuple(x.shape)}")
+    loss = linear_ce_fwd(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1), ignore_index, reduction)[0]
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
+def rlinear_cross_entropy(x: torch.Tensor, coef: torch.Tensor, seed: int, out_features: int, target: torch.Tensor, row0: int = 0,
+                          ignore_index: Optional[int] = -100, reduction: str = "mean") -> torch.Tensor:
+    """``cross_entropy(rlinear(x, coef, seed, out_features, row0), target)`` without the logits: z = x C^T (rounded to x's type, as
+    the layer's forward keeps it), then ``noise_cross_entropy``; differentiable in x and coef.  Rows of x whose target is ignored
+    are taken as zeros, so whatever they hold reaches neither the loss nor a gradient."""
+    lead = x.shape[:-1]
+    if tuple(target.shape) != tuple(lead):
+        raise RuntimeError(f"rlinear_cross_entropy: target {tuple(target.shape)} does not match x {tuple(x.shape)}")
+    if coef.dim() != 2 or coef.shape[1] != x.shape[-1] or coef.dtype != x.dtype:
+        raise RuntimeError(f"rlinear_cross_entropy: coef {tuple(coef.shape)} {coef.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    x2 = x.reshape(-1, x.shape[-1])
+    if ignore_index is not None:
+        x2 = x2.masked_fill((target.reshape(-1) == ignore_index).unsqueeze(1), 0.0)
+    z = _DenseMMT.apply(x2, coef)
+    loss = noise_cross_entropy(z, seed, out_features, target.reshape(-1), row0, ignore_index, reduction)
+    return loss.reshape(lead) if reduction == "none" else loss
 
 
 # ------------------------------------------------------------------------------------------------
@@ -275,6 +434,23 @@ class _DenseMM(torch.autograd.Function):
         grad = grad.contiguous()
         da = K.gemm_dense(grad, b.contiguous(), True, True) if ctx.needs_input_grad[0] else None      # grad @ b^T
         db = K.gemm_dense(a.contiguous(), grad, False, False) if ctx.needs_input_grad[1] else None   # a^T @ grad
+        return da, db
+
+
+class _DenseMMT(torch.autograd.Function):
+    """a[L, P] @ b[Q, P].T on the library's product kernels."""
+
+    @staticmethod
+    def forward(ctx, a, b):
+        ctx.save_for_backward(a, b)
+        return K.gemm_dense(a.contiguous(), b.contiguous(), True, True)
+
+    @staticmethod
+    def backward(ctx, grad):
+        a, b = ctx.saved_tensors
+        grad = grad.contiguous()
+        da = K.gemm_dense(grad, b.contiguous(), True, False) if ctx.needs_input_grad[0] else None     # grad @ b
+        db = K.gemm_dense(grad, a.contiguous(), False, False) if ctx.needs_input_grad[1] else None    # grad^T @ a
         return da, db
 
 

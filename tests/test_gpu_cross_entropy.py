@@ -1,0 +1,401 @@
+"""Cross entropy over a vocabulary matrix (stored, or noise) on the GPU against a plain 64-bit implementation.
+
+Tolerances.  bf16: the inputs' products are exact in float32, so a logit is off by float32 accumulation only: at most
+2^-23 (R / 16 + 16) sum |x_i w_i| (the tensor core adds 16 products at a time, each addition may cut instead of round); the same
+goes for the sum of exponentials.  A loss (or log-sum-exp) moves by at most the largest logit's error plus 2^-20 for the exponential and
+the row's sum.  Gradients in bf16 carry two roundings, of the probability (2^-9 relative after averaging, 2^-8 at most) and of the
+result (2^-8): 2^-7 of sum |p w| bounds the worst element; elements are compared with 2^-7 of that sum.
+"""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from oracle import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def rb():
+    import randumb_b200
+    assert torch.cuda.is_available()
+    return randumb_b200
+
+
+def noise_matrix(V, R, seed, row0, dtype):
+    return torch.from_numpy(O.noise_f32(V, R, seed, row0)).to(dtype)
+
+
+def plain(x, w, target, ignore, reduction, gout):
+    """Loss, dx, dw, logit and gradient error scales, in 64 bits on the GPU, from the definition; ignored rows are left out before anything is computed."""
+    keep = torch.ones_like(target, dtype=torch.bool) if ignore is None else target != ignore
+    rows = torch.nonzero(keep)[:, 0]
+    xd, wd, t = x.double()[rows], w.double(), target[rows]
+    logits = xd @ wd.t()
+    lse = torch.logsumexp(logits, 1)
+    l = lse - logits.gather(1, t[:, None])[:, 0]
+    losses = torch.zeros(x.shape[0], dtype=torch.float64, device=x.device)
+    losses[rows] = l
+    n = rows.numel()
+    if reduction == "none":
+        loss, g = losses, gout.double()[rows]
+    else:
+        loss = losses.sum() / (1 if reduction == "sum" else n) if n else torch.tensor(0.0 if reduction == "sum" else float("nan"), dtype=torch.float64)
+        g = torch.full((n,), float(gout) / (1 if reduction == "sum" else max(n, 1)), dtype=torch.float64, device=x.device)
+    p = torch.softmax(logits, 1)
+    # p - 1 at the target as the sum of the others: 1 - p itself is lost in 64 bits where p is nearly 1
+    at = torch.arange(n, device=x.device)
+    p[at, t] = 0
+    p[at, t] = -p.sum(1)
+    pa = p.abs()
+    dx = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    dx[rows] = (p * g[:, None]) @ wd
+    dxa = torch.zeros_like(dx)
+    dxa[rows] = (pa * g.abs()[:, None]) @ wd.abs()
+    dw = (p * g[:, None]).t() @ xd
+    dwa = (pa * g.abs()[:, None]).t() @ xd.abs()
+    terms = (xd.abs() @ wd.abs().t()).amax().item() if n else 0.0
+    return loss, losses, dx, dxa, dw, dwa, terms
+
+
+def tolerances(dtype, R, V, terms):
+    """(absolute error of a logit and a loss, relative factor of a gradient on the sum of its terms' magnitudes)."""
+    steps = (R / 16 + 16) * (1 if dtype == torch.bfloat16 else 6)
+    logit = 2.0 ** -23 * steps * terms + 2.0 ** -19
+    # exponent offset and argument in powers of two: 2 u of up to `terms` * log2(e), twice
+    logit += 4 * 2.0 ** -24 * 1.5 * terms
+    acc = 2.0 ** -23 * (V / 16 + 64) * (1 if dtype == torch.bfloat16 else 6)
+    return logit, (2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -22) + 3 * logit + acc
+
+
+def inputs(kind, T, R, V, dtype, seed, std=2.0):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "noise":
+        w = noise_matrix(V, R, 1000 + seed, 5, dtype).cuda()
+        x = (torch.randn(T, R, generator=g) * std * (3.0 / R) ** 0.5).to(dtype).cuda()
+    else:
+        w = (torch.randn(V, R, generator=g) * std / R ** 0.5).to(dtype).cuda()
+        x = torch.randn(T, R, generator=g).to(dtype).cuda()
+    target = torch.randint(0, V, (T,), generator=g).cuda()
+    return x, w, target
+
+
+def call(rb, kind, x, w, target, seed, ignore=-100, reduction="mean"):
+    if kind == "noise":
+        return rb.ops.noise_cross_entropy(x, 1000 + seed, w.shape[0], target, row0=5, ignore_index=ignore, reduction=reduction)
+    return rb.ops.linear_cross_entropy(x, w, target, ignore_index=ignore, reduction=reduction)
+
+
+def check(rb, kind, x, w, target, seed, ignore, reduction, gout=None):
+    T, R = x.shape
+    V = w.shape[0]
+    if gout is None:
+        gout = torch.rand(T, device="cuda") - 0.3 if reduction == "none" else torch.tensor(1.7, device="cuda")
+    loss_w, losses, dx_w, dxa, dw_w, dwa, terms = plain(x, w, target, ignore, reduction, gout)
+    xl = x.detach().clone().requires_grad_()
+    wl = w.detach().clone().requires_grad_()
+    loss = call(rb, kind, xl, wl, target, seed, ignore, reduction)
+    assert loss.dtype == torch.float32 and loss.shape == ((T,) if reduction == "none" else ())
+    grads = torch.autograd.grad(loss, [xl] if kind == "noise" else [xl, wl], gout)
+    rb.kernels.check_status()
+    logit, fac = tolerances(x.dtype, R, V, terms)
+    scale = 1 if reduction != "sum" else max(1, int((target != ignore).sum()))
+    assert torch.allclose(loss.double(), loss_w.to(loss.device), rtol=2.0 ** -21, atol=logit * scale, equal_nan=True), (loss, loss_w)
+    assert ((grads[0].double() - dx_w).abs() <= fac * dxa + 1e-30).all(), ((grads[0].double() - dx_w).abs() / (dxa + 1e-30)).max()
+    if kind == "linear":
+        accT = 2.0 ** -23 * (T / 16 + 64) * 6
+        assert ((grads[1].double() - dw_w).abs() <= (fac + accT) * dwa + 1e-30).all(), ((grads[1].double() - dw_w).abs() / (dwa + 1e-30)).max()
+    # the loss alone, without autograd, is the same number
+    with torch.no_grad():
+        alone = call(rb, kind, x, w, target, seed, ignore, reduction)
+    assert torch.allclose(alone, loss.detach(), rtol=2.0 ** -20, atol=2 * logit * scale, equal_nan=True)
+    return loss, grads
+
+
+SHAPES = [(1, 8, 1), (1, 128, 50257), (2, 1, 3), (3, 5, 300), (31, 64, 256), (128, 72, 257), (129, 256, 1000), (255, 250, 511), (257, 264, 513),
+          (600, 40, 2049), (1000, 513, 777), (2048, 128, 4096)]
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_loss_and_gradients(rb, kind, dtype, shape):
+    T, R, V = shape
+    x, w, target = inputs(kind, T, R, V, dtype, T + R)
+    check(rb, kind, x, w, target, T + R, -100, "mean")
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_ignored_rows_may_hold_anything(rb, kind, dtype, reduction):
+    T, R, V, seed = 700, 96, 1111, 3
+    x, w, target = inputs(kind, T, R, V, dtype, seed)
+    skip = torch.rand(T, generator=torch.Generator().manual_seed(1)).cuda() < 0.45
+    target[skip] = -7
+    want, _ = check(rb, kind, x, w, target, seed, -7, reduction, torch.linspace(-1, 2, T, device="cuda") if reduction == "none" else None)
+    dirty = x.clone()
+    dirty[skip] = torch.tensor([float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).max], device="cuda").to(dtype).repeat(R // 4)
+    g = torch.linspace(-1, 2, T, device="cuda") if reduction == "none" else torch.tensor(1.7, device="cuda")
+    both = []
+    for xx in (x, dirty):
+        leaves = [xx.clone().requires_grad_()] + ([w.clone().requires_grad_()] if kind == "linear" else [])
+        loss = call(rb, kind, leaves[0], leaves[-1] if kind == "linear" else w, target, seed, -7, reduction)
+        both.append([loss.detach()] + list(torch.autograd.grad(loss, leaves, g)))
+    for a, b in zip(*both):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+    assert (both[1][1][skip] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+def test_no_row_counts(rb, kind):
+    x, w, target = inputs(kind, 300, 64, 500, torch.bfloat16, 2)
+    target[:] = -100
+    for reduction in ("mean", "sum", "none"):
+        leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+        loss = call(rb, kind, *leaves, target, 2, -100, reduction)
+        assert torch.isnan(loss) if reduction == "mean" else (loss == 0).all()
+        for g in torch.autograd.grad(loss.sum(), leaves[:1 if kind == "noise" else 2]):
+            assert (g == 0).all()
+    # no rows at all
+    for reduction in ("mean", "sum", "none"):
+        leaves = [x[:0].clone().requires_grad_(), w.clone().requires_grad_()]
+        loss = call(rb, kind, *leaves, target[:0], 2, -100, reduction)
+        assert torch.isnan(loss) if reduction == "mean" else loss.sum() == 0
+        grads = torch.autograd.grad(loss.sum(), leaves[:1 if kind == "noise" else 2])
+        assert grads[0].shape == (0, 64) and all((g == 0).all() for g in grads)
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_far_above_the_target(rb, kind, dtype):
+    """Rows whose sum relative to the target's logit leaves float32 (other logits hundreds above it), beside ordinary rows and rows
+    that the model knows almost for sure."""
+    T, R, V, seed = 300, 128, 900, 8
+    x, w, target = inputs(kind, T, R, V, dtype, seed)
+    far = torch.arange(0, T, 7, device="cuda")
+    sure = torch.arange(3, T, 7, device="cuda")
+    norm = (w.float() ** 2).sum(1, keepdim=True)
+    x[far] = (w[(target[far] + 1) % V].float() / norm[(target[far] + 1) % V] * torch.linspace(60, 900, far.numel(), device="cuda")[:, None]).to(dtype)
+    x[sure] = (w[target[sure]].float() / norm[target[sure]] * torch.linspace(15, 300, sure.numel(), device="cuda")[:, None]).to(dtype)
+    loss, grads = check(rb, kind, x, w, target, seed, -100, "none", torch.ones(T, device="cuda"))
+    assert loss[far].max() > 300 and loss[sure].min() < 1e-6
+
+
+def test_target_outside_the_vocabulary(rb):
+    for kind in ("noise", "linear"):
+        x, w, target = inputs(kind, 40, 32, 100, torch.bfloat16, 4)
+        for bad in (100, -1, 2 ** 40, -2 ** 40):
+            t = target.clone()
+            t[17] = bad
+            leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+            loss = call(rb, kind, *leaves, t, 4, -100, "none")
+            ok = torch.arange(40, device="cuda") != 17
+            assert torch.isnan(loss[17]) and torch.isfinite(loss[ok]).all()
+            dx = torch.autograd.grad(loss, leaves[0], torch.ones_like(loss))[0]
+            assert torch.isnan(dx[17]).all() and torch.isfinite(dx[ok]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strided_and_misaligned_operands(rb, dtype):
+    T, R, V, seed = 200, 100, 333, 6
+    x, w, target = inputs("linear", T, R, V, dtype, seed)
+    want = [t.clone() for t in _value(rb, x, w, target)]
+    bx = torch.zeros(T, R + 13, device="cuda", dtype=dtype)
+    bw = torch.zeros(V, R + 24, device="cuda", dtype=dtype)
+    bx[:, 3:3 + R], bw[:, 8:8 + R] = x, w
+    odd = torch.zeros(V * R + 1, device="cuda", dtype=dtype)[1:].view(V, R).copy_(w)
+    for xx, ww in ((bx[:, 3:3 + R], w), (x, bw[:, 8:8 + R]), (x, odd), (x.t().contiguous().t(), w.t().contiguous().t())):
+        for a, b in zip(_value(rb, xx, ww, target), want):
+            assert torch.equal(a, b)
+    # a target that is a slice of a wider matrix; leading dimensions
+    wide = torch.zeros(T, 3, dtype=torch.int64, device="cuda")
+    wide[:, 1] = target
+    assert torch.equal(rb.linear_cross_entropy(x, w, wide[:, 1]), want[0])
+    l3 = rb.linear_cross_entropy(x.view(4, 50, R), w, target.view(4, 50), reduction="none")
+    assert l3.shape == (4, 50) and torch.equal(l3.reshape(-1), rb.linear_cross_entropy(x, w, target, reduction="none"))
+
+
+def _value(rb, x, w, target):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = rb.linear_cross_entropy(x, w, target)
+    return [loss.detach()] + list(torch.autograd.grad(loss, [x, w]))
+
+
+def test_only_what_is_asked_for(rb):
+    x, w, target = inputs("linear", 150, 64, 400, torch.bfloat16, 5)
+    both = _value(rb, x, w, target)
+    xl = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(rb.linear_cross_entropy(xl, w, target), xl)[0], both[1])
+    wl = w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(rb.linear_cross_entropy(x, wl, target), wl)[0], both[2])
+    # twice through the same graph: the second gradient is the first
+    xl = x.clone().requires_grad_()
+    loss = call(rb, "noise", xl, w, target, 5)
+    a = torch.autograd.grad(loss, xl, torch.tensor(3.0, device="cuda"), retain_graph=True)[0]
+    b = torch.autograd.grad(loss, xl, torch.tensor(3.0, device="cuda"))[0]
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+def test_several_pieces_and_repeatability(rb, kind):
+    """Enough rows that the vocabulary is taken in several pieces; the same call gives the same bits."""
+    T, R, V, seed = 40000, 64, 20000, 11
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = (torch.randn(T, R, device="cuda", generator=g) * (3.0 / R) ** 0.5 * 2).bfloat16()
+    w = (noise_matrix(V, R, 1000 + seed, 5, torch.bfloat16).cuda() if kind == "noise" else (torch.randn(V, R, device="cuda", generator=g) * 2 / R ** 0.5).bfloat16())
+    target = torch.randint(0, V, (T,), device="cuda", generator=g)
+    target[torch.rand(T, device="cuda", generator=g) < 0.2] = -100
+    out = []
+    for _ in range(2):
+        leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+        loss = call(rb, kind, *leaves, target, seed)
+        out.append([loss.detach()] + list(torch.autograd.grad(loss, leaves[:1 if kind == "noise" else 2])))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    xs, ws = x.float().requires_grad_(), w.float().requires_grad_()
+    want = F.cross_entropy(xs @ ws.t(), target)
+    gx, gw = torch.autograd.grad(want, [xs, ws])
+    # norms: rounding errors of single elements average out; 2^-8 covers the two bf16 roundings
+    assert abs(out[0][0].item() / want.item() - 1) < 1e-5
+    assert O.rel_fro(out[0][1].float().cpu(), gx.cpu()) < 2.0 ** -8
+    if kind == "linear":
+        assert O.rel_fro(out[0][2].float().cpu(), gw.cpu()) < 2.0 ** -8
+
+
+def test_gradient_is_the_slope(rb):
+    """float32: the loss along a direction, by differences, against the gradient."""
+    for kind in ("noise", "linear"):
+        x, w, target = inputs(kind, 64, 40, 200, torch.float32, 9)
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        leaves = [xl] if kind == "noise" else [xl, wl]
+        grads = torch.autograd.grad(call(rb, kind, xl, wl, target, 9, reduction="sum"), leaves)
+        for i, (leaf, gr) in enumerate(zip(leaves, grads)):
+            d = gr / gr.norm()
+            h = 0.05
+            with torch.no_grad():
+                f = [call(rb, kind, x + s * h * d if i == 0 else x, w + s * h * d if i == 1 else w, target, 9, reduction="sum").double().item() for s in (-1, 1)]
+            # third derivatives of the sum along a unit direction stay below its second's scale: h^2 / 6 of them is under 1 %; losses of 64 rows
+            # are off by 64 * 2e-6 each: 64 * 4e-6 / (2 h) / |g|
+            assert abs((f[1] - f[0]) / (2 * h) / gr.norm().item() - 1) < 0.01 + 64 * 4e-6 / (2 * h) / gr.norm().item()
+
+
+def test_captured_and_on_a_side_stream(rb):
+    for kind in ("noise", "linear"):
+        x, w, target = inputs(kind, 500, 128, 3001, torch.bfloat16, 7)
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        leaves = [xl] if kind == "noise" else [xl, wl]
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            loss = call(rb, kind, xl, wl, target, 7)
+            eager = [loss.detach()] + list(torch.autograd.grad(loss, leaves))
+        torch.cuda.synchronize()
+        del loss
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            loss = call(rb, kind, xl, wl, target, 7)
+            out = [loss.detach()] + list(torch.autograd.grad(loss, leaves))
+        del loss
+        x2, _, target2 = inputs(kind, 500, 128, 3001, torch.bfloat16, 70)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+        with torch.no_grad():
+            xl.copy_(x2)
+        target2[100:300] = -100
+        target.copy_(target2)
+        graph.replay()
+        torch.cuda.synchronize()
+        xn = x2.clone().requires_grad_()
+        wn = w.clone().requires_grad_()
+        fresh = call(rb, kind, xn, wn, target2, 7)
+        want = [fresh.detach()] + list(torch.autograd.grad(fresh, [xn] if kind == "noise" else [xn, wn]))
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.bfloat16, 2e-2), (torch.float32, 2e-5)])
+def test_layer_loss(rb, dtype, tol):
+    """RandumbLinear.cross_entropy against the layer's weight in 64 bits.  bf16: z and dz are rounded to bf16 on the way, as the
+    layer's forward and backward round them (the tolerance of the layer's own tests); float32: the CUDA-core products' 1e-5 and the loss's."""
+    torch.manual_seed(0)
+    head = rb.RandumbLinear(96, 1234, 64, seed=21, device="cuda", dtype=dtype)
+    x = torch.randn(3, 100, 96, device="cuda", dtype=dtype)
+    target = torch.randint(0, 1234, (3, 100), device="cuda")
+    target[1, 20:70] = -100
+    xl = x.clone()
+    xl[1, 20:70] = float("nan")
+    xl.requires_grad_()
+    loss = head.cross_entropy(xl, target)
+    dx, dc = torch.autograd.grad(loss, [xl, head.weight_coef])
+    S = noise_matrix(1234, 64, 21, 0, dtype).double().cuda()
+    C = head.weight_coef.detach().double().requires_grad_()
+    xd = x.double().requires_grad_()
+    want = F.cross_entropy(((xd @ C.t()) @ S.t()).reshape(-1, 1234), target.reshape(-1))
+    wx, wc = torch.autograd.grad(want, [xd, C])
+    assert abs(loss.item() - want.item()) < tol * want.item()
+    assert (dx[1, 20:70] == 0).all()
+    assert O.rel_fro(dx.double().cpu(), wx.cpu()) < tol and O.rel_fro(dc.double().cpu(), wc.cpu()) < tol
+    with pytest.raises(RuntimeError, match="bias"):
+        rb.RandumbLinear(96, 12, 8, seed=1, bias=True, device="cuda", dtype=dtype).cross_entropy(x, target)
+
+
+def test_training_steps_with_all_operators(rb):
+    """A pseudorandom layer and head, the fused loss, clipping and AdamW together: gradients of a step against autograd on dense weights,
+    the update against torch's AdamW on the same gradients."""
+    torch.manual_seed(1)
+    dev = "cuda"
+    body = rb.RandumbLinear(64, 96, 32, seed=3, device=dev)
+    head = rb.RandumbLinear(96, 517, 48, seed=10, device=dev)
+    params = [body.weight_coef, head.weight_coef]
+    opt = rb.optim.AdamW(params, lr=1e-2, weight_decay=0.05, max_grad_norm=0.5)
+    ref = [p.detach().clone().requires_grad_() for p in params]
+    topt = torch.optim.AdamW(ref, lr=1e-2, weight_decay=0.05)
+    S1, S2 = (torch.from_numpy(O.noise_f32(n, r, s)).cuda() for n, r, s in ((96, 32, 3), (517, 48, 10)))
+    for k in range(3):
+        x = torch.randn(200, 64, device=dev)
+        target = torch.randint(0, 517, (200,), device=dev)
+        target[::9] = -100
+        loss = head.cross_entropy(torch.tanh(body(x)), target)
+        opt.zero_grad()
+        loss.backward()
+        topt.zero_grad()
+        want = F.cross_entropy(torch.tanh(x @ (S1 @ ref[0]).t()) @ (S2 @ ref[1]).t(), target)
+        want.backward()
+        assert abs(loss.item() / want.item() - 1) < 1e-4
+        for p, r in zip(params, ref):
+            assert O.rel_fro(p.grad.cpu(), r.grad.cpu()) < 1e-4
+        norm = torch.nn.utils.clip_grad_norm_(ref, 0.5)
+        opt.step()
+        topt.step()
+        assert abs(opt.last_grad_norm.item() / norm.item() - 1) < 1e-4
+        with torch.no_grad():
+            for p, r in zip(params, ref):
+                # m / sqrt(v) of the first steps is near the gradient's sign: elements whose gradient is all rounding may go either way
+                assert (p - r).abs().mean() < 1e-5
+                r.copy_(p)
+
+
+def test_refusals(rb):
+    x, w, target = inputs("linear", 8, 16, 20, torch.bfloat16, 1)
+    ce, nce = rb.linear_cross_entropy, rb.noise_cross_entropy
+    with pytest.raises(RuntimeError, match="does not match"):
+        ce(x, w, target[:7])
+    with pytest.raises(RuntimeError, match="does not match"):
+        ce(x, w[:, :8], target)
+    with pytest.raises(RuntimeError, match="does not match"):
+        ce(x, w.float(), target)
+    with pytest.raises(RuntimeError, match="int64"):
+        ce(x, w, target.int())
+    with pytest.raises(RuntimeError, match="reduction"):
+        ce(x, w, target, reduction="average")
+    with pytest.raises(RuntimeError, match="float32 and bfloat16"):
+        nce(x.half(), 1, 20, target)
+    with pytest.raises(RuntimeError, match="at least one"):
+        nce(x, 1, 0, target)
+    with pytest.raises(RuntimeError, match="does not match"):
+        rb.rlinear_cross_entropy(x, torch.zeros(4, 15, device="cuda", dtype=torch.bfloat16), 1, 20, target)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ce(x, w, target.cpu())
