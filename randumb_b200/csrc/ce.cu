@@ -76,21 +76,34 @@ __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *m, uint32_t
                  ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_src), "r"(x), "r"(y) : "memory");
 }
 
-// ---- the equal cut of `total` k-blocks over `pairs`: pair p owns [total p / pairs, total (p + 1) / pairs) ----------------
-// As many pairs take part as get four k-blocks each (a part of a tile costs a 256 x 256 float32 slot, written and read back).
-__host__ __device__ __forceinline__ int64_t cut_pairs(int64_t total, int64_t pairs) {
-    const int64_t p = total / 4;
-    return p < 1 ? 1 : (p < pairs ? p : pairs);
-}
-__host__ __device__ __forceinline__ int64_t cut_begin(int64_t total, int64_t pairs, int64_t p) { return total * p / pairs; }
-__host__ __device__ __forceinline__ int64_t cut_owner(int64_t total, int64_t pairs, int64_t g) {
-    int64_t p = ((g + 1) * pairs + total - 1) / total - 1;
-    return p;
-}
-
-// Part of tile `tile` computed by pair `p`: one 256 x 256 float32 slot.  tile + p grows from each part to the next, so the parts
-// need (tiles + pairs) slots whatever the cut.
-__host__ __device__ __forceinline__ int64_t slot_of(int64_t tile, int64_t p) { return tile + p; }
+// ---- how the x-gradient's work is cut ---------------------------------------------------------------------------------------
+// The row tiles of one 256-column tile each read the same rows of E, which is too large for L2: the `size` pairs of a group work
+// on neighbouring column tiles of one row tile over the same run of k-blocks, so E crosses from memory once (R = 1024, 8192 rows,
+// 25344 columns: 441 us when each pair had a run of its own).  Groups own equal runs of the (panel, k-block) sequence, a panel being
+// a row tile and `size` column tiles.  Group g leaves its part of a panel in slot panel + g, which grows from each part to the next:
+// (panels + groups) * size slots of 256 x 256 float32 hold them all, whatever the number of rows turns out to be.
+struct Cut {
+    int64_t total;                // k-blocks of all panels
+    int64_t groups;               // groups that take part: as many as get four k-blocks each
+    int size, per_row, tiles_n;   // pairs per group, panels per row tile
+    int KB;
+    __host__ __device__ __forceinline__ Cut(int64_t rows, int64_t cols, int KB_, int pairs) : KB(KB_) {
+        tiles_n = (int)((cols + CE_TILE - 1) / CE_TILE);
+        per_row = (tiles_n + 7) / 8;
+        size = (tiles_n + per_row - 1) / per_row;
+        if (size > pairs) {
+            size = pairs;
+            per_row = (tiles_n + size - 1) / size;
+        }
+        total = (rows + CE_TILE - 1) / CE_TILE * per_row * KB;
+        groups = pairs / size;
+        if (groups > total / 4) groups = total / 4 < 1 ? 1 : total / 4;
+    }
+    __host__ __device__ __forceinline__ int64_t begin(int64_t g) const { return total * g / groups; }
+    __host__ __device__ __forceinline__ int64_t owner(int64_t at) const { return ((at + 1) * groups + total - 1) / total - 1; }
+    __host__ __device__ __forceinline__ int64_t slot(int64_t panel, int64_t g, int member) const { return (panel + g) * size + member; }
+    __host__ __device__ __forceinline__ int64_t slots(int pairs) const { return (total / (KB ? KB : 1) + pairs / size) * size; }
+};
 
 struct WorkItem {
     int64_t m, n, slot;
@@ -99,48 +112,48 @@ struct WorkItem {
 
 // The sequence of work items of one pair; every role walks it by itself.
 struct Walk {
-    int64_t tiles_m, tiles_n, total, next, end, pairs, pair;
-    int KB, m_fast;
-    bool cut;
-    __device__ __forceinline__ void start(const CeArgs &a, bool cut_, int64_t rows, int kb_total, int64_t pair_, int64_t pairs_) {
+    Cut cut;
+    int64_t tiles_m, tiles_n, next, end, group, step;
+    int KB, m_fast, member;
+    bool by_cut;
+    __device__ __forceinline__ Walk(const CeArgs &a, bool by_cut_, int64_t rows, int kb_total, int pair, int pairs)
+        : cut(rows, a.N, kb_total, pairs), KB(kb_total), m_fast(a.m_fast), by_cut(by_cut_) {
         tiles_m = (rows + CE_TILE - 1) / CE_TILE;
-        tiles_n = (a.N + CE_TILE - 1) / CE_TILE;
-        KB = kb_total;
-        m_fast = a.m_fast;
-        cut = cut_;
-        pairs = pairs_;
-        pair = pair_;
-        if (cut) {
-            total = tiles_m * tiles_n * KB;
-            pairs = cut_pairs(total, pairs_);
-            next = pair < pairs ? cut_begin(total, pairs, pair) : total;
-            end = pair < pairs ? cut_begin(total, pairs, pair + 1) : total;
+        tiles_n = cut.tiles_n;
+        step = pairs;
+        if (by_cut) {
+            group = pair / cut.size;
+            member = pair % cut.size;
+            const bool in = group < cut.groups;
+            next = in ? cut.begin(group) : 0;
+            end = in ? cut.begin(group + 1) : 0;
         } else {
-            total = tiles_m * tiles_n;
             next = pair;
-            end = total;
+            end = tiles_m * tiles_n;
         }
     }
     __device__ __forceinline__ bool take(WorkItem &w) {
-        if (next >= end) return false;
-        int64_t tile;
-        if (cut) {
-            tile = next / KB;
-            w.kb0 = (int)(next - tile * KB);
+        while (next < end) {
+            if (!by_cut) {
+                w.kb0 = 0;
+                w.kb1 = KB;
+                w.slot = 0;
+                w.m = m_fast ? next % tiles_m : next / tiles_n;
+                w.n = m_fast ? next / tiles_m : next % tiles_n;
+                next += step;
+                return true;
+            }
+            const int64_t panel = next / KB;
+            w.kb0 = (int)(next - panel * KB);
             const int64_t left = end - next;
             w.kb1 = left < KB - w.kb0 ? w.kb0 + (int)left : KB;
-            w.slot = slot_of(tile, pair);
             next += w.kb1 - w.kb0;
-        } else {
-            tile = next;
-            w.kb0 = 0;
-            w.kb1 = KB;
-            w.slot = 0;
-            next += pairs;
+            w.m = panel / cut.per_row;
+            w.n = (panel % cut.per_row) * cut.size + member;
+            w.slot = cut.slot(panel, group, member);
+            if (w.n < tiles_n) return true;
         }
-        w.m = m_fast ? tile % tiles_m : tile / tiles_n;
-        w.n = m_fast ? tile / tiles_m : tile % tiles_n;
-        return true;
+        return false;
     }
 };
 
@@ -189,8 +202,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     const int64_t rows = args.m_counted ? counted : args.M;
     const int kbs = args.k_counted ? (int)((counted + BK - 1) / BK) : args.kbs;
     const int KB = kbs * args.nterm;
-    Walk walk;
-    walk.start(args, CUT, rows, KB, blockIdx.x >> 1, gridDim.x >> 1);
+    Walk walk(args, CUT, rows, KB, (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1));
     WorkItem w;
 
     if (warp == 0) {
@@ -473,10 +485,10 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 // rows
 // ================================================================================================
 // Positions of the rows that count, in order: idx[compact] = row, map[row] = compact or -1.  One block; `zero` (losses, may be
-// null) is cleared at ignored rows.
+// null) is cleared at ignored rows; so is the list of far rows.
 __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict__ target, int64_t T, int64_t ignore, int use_ignore,
                                                        int32_t *__restrict__ idx, int32_t *__restrict__ map, int32_t *__restrict__ count,
-                                                       float *__restrict__ zero_a, float *__restrict__ zero_b, float *__restrict__ count_f) {
+                                                       float *__restrict__ zero_a, float *__restrict__ zero_b, float *__restrict__ count_f, int32_t *__restrict__ far) {
     __shared__ int warp_sum[32];
     __shared__ int base;
     pdl_launch_dependents();
@@ -524,6 +536,7 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict
     __syncthreads();
     if (threadIdx.x == 0) {
         *count = base;
+        *far = 0;
         if (count_f) *count_f = (float)base;
     }
 }
@@ -630,7 +643,7 @@ __global__ void __launch_bounds__(256) ce_split_kernel(__nv_bfloat16 *__restrict
 // s of 32 rows per block: eight threads per row add every eighth partial sum, then the eight are added in order.
 __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ partial, int64_t ld, int nparts, const int32_t *__restrict__ idx,
                                                      const int32_t *__restrict__ count, const float *__restrict__ lt, float *__restrict__ s_out,
-                                                     float *__restrict__ lse, float *__restrict__ loss) {
+                                                     float *__restrict__ lse, float *__restrict__ loss, int32_t *__restrict__ far) {
     __shared__ float sh[8][33];
     pdl_launch_dependents();
     pdl_wait();
@@ -650,40 +663,41 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ p
         s_out[j] = s;
         loss[idx[j]] = l;
         lse[idx[j]] = lt[j] + l;
+        if (s >= S_LIMIT) far[1 + atomicAdd(far, 1)] = (int32_t)j;    // in any order: each row is redone by itself
     }
 }
 
-// The parts of row j of the x-gradient: at(c, k) is column c in the k-th part, k = 0 .. last(c).
+// The parts of a row tile's column tile n of the x-gradient: first() .. last() groups, row r and column c of the k-th at at(..).
 struct SlotView {
     float *base;
-    int64_t tiles_n, total, pairs, j;
-    int KB;
-    __device__ __forceinline__ SlotView(float *slots, int64_t count, int64_t R, int KB_, int64_t pairs_, int64_t j_)
-        : base(slots), tiles_n((R + CE_TILE - 1) / CE_TILE), j(j_), KB(KB_) {
-        total = (count + CE_TILE - 1) / CE_TILE * tiles_n * KB;
-        pairs = cut_pairs(total, pairs_);
+    Cut cut;
+    int64_t panel, lo, hi;
+    int member;
+    __device__ __forceinline__ SlotView(float *slots, int64_t count, int64_t R, int KB, int pairs) : base(slots), cut(count, R, KB, pairs) {}
+    __device__ __forceinline__ void tile(int64_t m, int n) {
+        panel = m * cut.per_row + n / cut.size;
+        member = n % cut.size;
+        lo = cut.owner(panel * cut.KB);
+        hi = cut.owner((panel + 1) * cut.KB - 1);
     }
-    __device__ __forceinline__ int64_t tile(int64_t c) const { return (j / CE_TILE) * tiles_n + c / CE_TILE; }
-    __device__ __forceinline__ int64_t first(int64_t c) const { return cut_owner(total, pairs, tile(c) * KB); }
-    __device__ __forceinline__ int64_t last(int64_t c) const { return cut_owner(total, pairs, (tile(c) + 1) * KB - 1) - first(c); }
-    __device__ __forceinline__ float *at(int64_t c, int64_t k) const {
-        return base + (slot_of(tile(c), first(c) + k) * CE_TILE + j % CE_TILE) * CE_TILE + c % CE_TILE;
-    }
+    __device__ __forceinline__ float *at(int64_t g, int r, int c) const { return base + (cut.slot(panel, g, member) * CE_TILE + r) * CE_TILE + c; }
 };
 
 // Rows whose sum left float32's range: logits once more on CUDA cores, first the maximum and the sum relative to it, then (grad)
-// the gradient itself.  One row per block at a time; the row of slot 0 receives the finished gradient and s becomes -1.
+// the gradient itself.  One row per block at a time; the row's first slot receives the finished gradient and s becomes -1.
+// far[0] rows, listed behind it.
 template <typename T>
 __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, float *__restrict__ s_io, float *__restrict__ lse,
-                                                        float *__restrict__ loss, float *__restrict__ slots, int KB, int64_t pairs) {
+                                                        float *__restrict__ loss, float *__restrict__ slots, int KB, int pairs,
+                                                        const int32_t *__restrict__ far) {
     __shared__ float sh_m[16], sh_s[16], sh_p[16];
-    __shared__ int sh_v;
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t n = *a.count;
-    for (int64_t j = blockIdx.x; j < n; j += gridDim.x) {
-        if (!(s_io[j] >= S_LIMIT)) continue;           // not-a-number is the answer already
+    const int nfar = far[0];
+    for (int i = blockIdx.x; i < nfar; i += gridDim.x) {
+        const int64_t j = far[1 + i];
         const int64_t row = a.idx[j], t = a.target[row];
         const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
         const float lt = a.lt[j];
@@ -714,78 +728,93 @@ __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, 
             s_io[j] = -1.0f;
         }
         if (slots) {
-            const SlotView o(slots, n, a.R, KB, pairs, j);
+            SlotView o(slots, n, a.R, KB, pairs);
+            const int r = (int)(j % CE_TILE);
             const float pt = expf(lt - full);
-            for (int64_t c = threadIdx.x; c < a.R; c += blockDim.x) *o.at(c, 0) = (pt - 1.0f) * vocab_at<T>(voc, t, c);
-            __syncthreads();
-            for (int64_t v0 = 0; v0 < a.V; v0 += 16) {
-                const int64_t v = v0 + warp;
-                float p = 0.0f;
-                if (v < a.V && v != t) p = expf(logit(v) - full);
-                if (lane == 0) sh_p[warp] = p;
-                if (threadIdx.x == 0) sh_v = 0;
-                __syncthreads();
-                if (lane == 0 && p > 0.0f) sh_v = 1;
-                __syncthreads();
-                if (sh_v) {
-                    for (int64_t c = threadIdx.x; c < a.R; c += blockDim.x) {
-                        float acc = *o.at(c, 0);
+            for (int nt = 0; nt < o.cut.tiles_n; ++nt) {          // columns of one tile at a time
+                o.tile(j / CE_TILE, nt);
+                const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
+                const bool mine = threadIdx.x < CE_TILE && c < a.R;
+                float acc = mine ? (pt - 1.0f) * vocab_at<T>(voc, t, c) : 0.0f;
+                for (int64_t v0 = 0; v0 < a.V; v0 += 16) {
+                    const int64_t v = v0 + warp;
+                    float p = 0.0f;
+                    if (v < a.V && v != t) p = expf(logit(v) - full);
+                    if (lane == 0) sh_p[warp] = p;
+                    __syncthreads();
+                    if (mine) {
+#pragma unroll 1
                         for (int k = 0; k < 16; ++k)
-                            if (sh_p[k] > 0.0f) acc = fmaf(sh_p[k], vocab_at<T>(voc, v0 + k, c), acc);
-                        *o.at(c, 0) = acc;
+                            if (sh_p[k] != 0.0f) acc = fmaf(sh_p[k], vocab_at<T>(voc, v0 + k, c), acc);
                     }
+                    __syncthreads();
                 }
-                __syncthreads();
+                if (mine) *o.at(o.lo, r, threadIdx.x) = acc;
             }
         }
         __syncthreads();
     }
 }
 
-__global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__ loss_rows, const int32_t *__restrict__ idx,
-                                                       const int32_t *__restrict__ count, float *__restrict__ loss, int mean) {
-    __shared__ double sh[1024];
+// ignored rows hold 0: all T are added, in one fixed order
+__global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__ loss_rows, int64_t T, const int32_t *__restrict__ count,
+                                                       float *__restrict__ loss, int mean) {
+    __shared__ double sh[32];
     pdl_launch_dependents();
     pdl_wait();
-    const int n = *count;
     double a = 0.0;
-    for (int j = threadIdx.x; j < n; j += 1024) a += (double)loss_rows[idx[j]];
-    sh[threadIdx.x] = a;
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < T; i += 1024) a += (double)loss_rows[i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
     __syncthreads();
-    for (int o = 512; o; o >>= 1) {
-        if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
-        __syncthreads();
+    if (threadIdx.x < 32) {
+        a = sh[threadIdx.x];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (threadIdx.x == 0) *loss = (float)(mean ? a / (double)*count : a);
     }
-    if (threadIdx.x == 0) *loss = (float)(mean ? sh[0] / (double)n : sh[0]);
 }
 
 // x's gradient from the slots: their sum, finished with s and the target's row (noise: voc.w null and s given), written to the
 // rows' own places; zeros at ignored rows.
+// A block takes DX_ROWS rows of one column tile, a thread one column.
+constexpr int DX_ROWS = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int32_t *__restrict__ map,
+__global__ void __launch_bounds__(CE_TILE) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int32_t *__restrict__ map,
                                                     const int32_t *__restrict__ count, const float *__restrict__ s, const int32_t *__restrict__ tcol,
-                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int64_t pairs) {
+                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int pairs) {
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t n = *count;
-    for (int64_t i = blockIdx.x; i < T_rows; i += gridDim.x) {
+    SlotView o(slots, *count, R, KB, pairs);
+    const int nt = (int)(blockIdx.x % o.cut.tiles_n);
+    const int64_t i0 = (int64_t)(blockIdx.x / o.cut.tiles_n) * DX_ROWS;
+    const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
+    int64_t m = -1;
+#pragma unroll 4
+    for (int k = 0; k < DX_ROWS; ++k) {
+        const int64_t i = i0 + k;
+        if (i >= T_rows) break;
         const int64_t j = map[i];
-        if (j < 0) {
-            for (int64_t c = threadIdx.x; c < R; c += blockDim.x) dx[i * R + c] = from_f32<T>(0.0f);
-            continue;
-        }
-        const SlotView o(slots, n, R, KB, pairs, j);
-        const float sj = s ? s[j] : 0.0f;
-        const int64_t t = s ? tcol[j] : 0;
-        for (int64_t c = threadIdx.x; c < R; c += blockDim.x) {
-            float v = *o.at(c, 0);
-            if (!(sj < 0.0f)) {                       // -1: the row was finished by ce_rescue_kernel
-                const int64_t last = o.last(c);
-                for (int64_t k = 1; k <= last; ++k) v += *o.at(c, k);
-                if (s) v = t >= 0 ? (v - sj * vocab_at<T>(voc, t, c)) / (1.0f + sj) : NAN;
+        float v = 0.0f;
+        if (j >= 0 && c < R) {
+            if (j / CE_TILE != m) {
+                m = j / CE_TILE;
+                o.tile(m, nt);
             }
-            dx[i * R + c] = from_f32<T>(v);
+            const int r = (int)(j % CE_TILE);
+            const float sj = s ? s[j] : 0.0f;
+            v = *o.at(o.lo, r, threadIdx.x);
+            if (!(sj < 0.0f)) {                       // -1: the row was finished by ce_rescue_kernel
+                for (int64_t g = o.lo + 1; g <= o.hi; ++g) v += *o.at(g, r, threadIdx.x);
+                if (s) {
+                    const int64_t t = tcol[j];
+                    v = t >= 0 ? (v - sj * vocab_at<T>(voc, t, c)) / (1.0f + sj) : NAN;
+                }
+            }
         }
+        if (c < R) dx[i * R + c] = from_f32<T>(v);
     }
 }
 
@@ -817,13 +846,15 @@ struct CePlan {
     bool dw_direct;
     int64_t ld_dw;
     // workspace
-    size_t idx, map, count, off2, lt, scale, tval, tcol, s, a, b, e, partial, slots, dw, total;
+    size_t idx, map, count, off2, lt, scale, tval, tcol, s, far, a, b, e, partial, slots, dw, total;
 };
 
 constexpr size_t E_BUDGET = 512ull << 20;
 constexpr size_t B_BUDGET = 256ull << 20;
 
 static int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+static int ce_kb(const CePlan &p) { return p.nterm * (int)cdiv64(p.piece, BK); }     // k-blocks of the x-gradient's product
 
 // op 0: loss; 1: loss and unit gradient of x (noise); 2: gradients of a stored matrix
 static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw, const void *dw, int want_dx, int want_dw) {
@@ -851,7 +882,7 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     const int64_t per = cdiv64(vtiles, p.npieces);
     p.npieces = cdiv64(vtiles, per);
     p.piece = per * CE_TILE;
-    p.slot_rows = ((p.Mpad / CE_TILE) * cdiv64(R, CE_TILE) + p.pairs) * CE_TILE;
+    p.slot_rows = Cut(T, R, ce_kb(p), p.pairs).slots(p.pairs) * CE_TILE;
     const size_t es = dtype_size(dtype);
     p.dw_direct = dw && (reinterpret_cast<uintptr_t>(dw) & 15) == 0 && (R * es) % 16 == 0;
     p.ld_dw = round_up(R, 8);
@@ -864,6 +895,7 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     p.tcol = take((size_t)p.Mpad * 4);
     p.lt = take((size_t)p.Mpad * 4);
     p.s = take((size_t)p.Mpad * 4);
+    p.far = take((size_t)p.Mpad * 4 + 4);
     p.scale = take(op == 2 ? (size_t)p.Mpad * 4 : 0);
     p.tval = take(op == 2 ? (size_t)p.Mpad * 4 : 0);
     p.a = take((size_t)p.Mpad * p.lda * 2);
@@ -926,7 +958,7 @@ struct CeCall {
 
 static int ce_find_rows(const CeCall &c, int64_t ignore, int use_ignore, float *zero_a, float *zero_b, float *count_f) {
     return launch_pdl(ce_rows_kernel, dim3(1), 1024, 0, c.st, c.target, c.T, ignore, use_ignore, c.at<int32_t>(c.p.idx), c.at<int32_t>(c.p.map),
-                      c.at<int32_t>(c.p.count), zero_a, zero_b, count_f);
+                      c.at<int32_t>(c.p.count), zero_a, zero_b, count_f, c.at<int32_t>(c.p.far));
 }
 
 static CeRowArgs ce_row_args(const CeCall &c) {
@@ -1058,18 +1090,16 @@ static int ce_dw(const CeCall &c, void *dw, int64_t v0, int64_t n) {
     return e == cudaSuccess ? RDB_OK : (int)e;
 }
 
-static int ce_kb(const CePlan &p) { return p.nterm * (int)cdiv64(p.piece, BK); }
-
 static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
     const CePlan &p = c.p;
-    const dim3 grid((unsigned)(c.T < 148 * 16 ? c.T : 148 * 16));
+    const dim3 grid((unsigned)(cdiv64(c.T, DX_ROWS) * cdiv64(c.R, CE_TILE)));
     const float *s = unit ? c.at<float>(p.s) : nullptr;
     const int32_t *map = c.at<int32_t>(p.map), *count = c.at<int32_t>(p.count), *tcol = c.at<int32_t>(p.tcol);
     float *slots = c.at<float>(p.slots);
     if (c.dtype == RDB_F32)
-        return launch_pdl(ce_dx_kernel<float>, grid, 256, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), (int64_t)p.pairs);
-    return launch_pdl(ce_dx_kernel<__nv_bfloat16>, grid, 256, 0, c.st, (__nv_bfloat16 *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p),
-                      (int64_t)p.pairs);
+        return launch_pdl(ce_dx_kernel<float>, grid, CE_TILE, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs);
+    return launch_pdl(ce_dx_kernel<__nv_bfloat16>, grid, CE_TILE, 0, c.st, (__nv_bfloat16 *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p),
+                      p.pairs);
 }
 
 static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w, int64_t ldw, int dtype, int reduction) {
@@ -1128,20 +1158,20 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x,
         }
         // row sums: a full piece leaves two per column tile; without the gradient the last piece has only the tiles that exist
         const int64_t last = V - (c.p.npieces - 1) * c.p.piece;
+        int32_t *far = c.at<int32_t>(c.p.far);
         const int nparts = (int)((c.p.npieces - 1) * (c.p.piece / CE_TILE) * 2 + (dx_unit ? c.p.piece / CE_TILE : cdiv64(last, CE_TILE)) * 2);
         rc = launch_pdl(ce_sum_kernel, dim3((unsigned)(c.p.Mpad / 32)), 256, 0, c.st, (const float *)c.at<float>(c.p.partial), c.p.Mpad, nparts, ra.idx,
-                        ra.count, (const float *)ra.lt, c.at<float>(c.p.s), lse, rows);
+                        ra.count, (const float *)ra.lt, c.at<float>(c.p.s), lse, rows, far);
         if (rc) return rc;
         float *slots = dx_unit ? c.at<float>(c.p.slots) : nullptr, *sums = c.at<float>(c.p.s);
-        const int64_t pairs = c.p.pairs;
-        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs)
-                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs);
+        const int pairs = c.p.pairs;
+        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs, (const int32_t *)far)
+                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs, (const int32_t *)far);
         if (rc) return rc;
         if (dx_unit && (rc = ce_finish_dx(c, dx_unit, true))) return rc;
     }
     if (reduction == RDB_CE_NONE) return RDB_OK;
-    return launch_pdl(ce_loss_kernel, dim3(1), 1024, 0, c.st, (const float *)rows, (const int32_t *)c.at<int32_t>(c.p.idx),
-                      (const int32_t *)c.at<int32_t>(c.p.count), loss, reduction == RDB_CE_MEAN ? 1 : 0);
+    return launch_pdl(ce_loss_kernel, dim3(1), 1024, 0, c.st, (const float *)rows, T, (const int32_t *)c.at<int32_t>(c.p.count), loss, reduction == RDB_CE_MEAN ? 1 : 0);
 }
 
 extern "C" int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
