@@ -481,8 +481,8 @@ int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int6
  * the row's loss and gradient NaN.  reduction RDB_CE_NONE: loss per row; RDB_CE_SUM; RDB_CE_MEAN: over the rows that count (NaN
  * when none does).  x, w and the gradients are of type dtype, losses float32.
  *
- * rdb_ce_fwd   loss (one float32; ignored for RDB_CE_NONE) and aux, float32 [2T + 1]: log-sum-exp per row, loss per row, number
- *              of rows that count.  dx_unit (may be null, only with w null): d(row's loss)/dx, contiguous [T, R].
+ * rdb_ce_fwd   loss (one float32, or T of them for RDB_CE_NONE) and aux, float32 [2T + 1]: log-sum-exp per row, loss per row,
+ *              number of rows that count.  dx_unit (may be null, only with w null): d(row's loss)/dx, contiguous [T, R].
  * rdb_ce_scale dz = dx_unit times the gradient of the loss: *dloss (RDB_CE_SUM), *dloss / count (RDB_CE_MEAN), dloss[row] (NONE).
  * rdb_ce_bwd   gradients for a stored matrix from the forward's aux: dx [T, R] and dw [V, R], contiguous, either may be null.
  * workspace: 256-byte aligned, rdb_ce_workspace_bytes(op, ...) bytes with op RDB_CE_LOSS (fwd), RDB_CE_LOSS_GRAD (fwd with

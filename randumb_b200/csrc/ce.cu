@@ -484,24 +484,30 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 // ================================================================================================
 // rows
 // ================================================================================================
-// Positions of the rows that count, in order: idx[compact] = row, map[row] = compact or -1.  One block; `zero` (losses, may be
-// null) is cleared at ignored rows; so is the list of far rows.
+// Positions of the rows that count, in order: idx[compact] = row, map[row] = compact or -1.  One block; the losses (zero_*, may be
+// null) are cleared at ignored rows, the list of far rows is emptied.
 __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict__ target, int64_t T, int64_t ignore, int use_ignore,
                                                        int32_t *__restrict__ idx, int32_t *__restrict__ map, int32_t *__restrict__ count,
-                                                       float *__restrict__ zero_a, float *__restrict__ zero_b, float *__restrict__ count_f, int32_t *__restrict__ far) {
-    __shared__ int warp_sum[32];
-    __shared__ int base;
+                                                       float *__restrict__ zero_a, float *__restrict__ zero_b, float *__restrict__ zero_c,
+                                                       float *__restrict__ count_f, int32_t *__restrict__ far) {
+    constexpr int PER = 8;
+    __shared__ int warp_sum[2][32];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) base = 0;
-    for (int64_t b = 0; b < T; b += 4096) {
-        const int64_t i0 = b + threadIdx.x * 4;
-        int keep[4], n = 0;
+    int base = 0, turn = 0;
+    for (int64_t b = 0; b < T; b += 1024 * PER, turn ^= 1) {
+        const int64_t i0 = b + threadIdx.x * PER;
+        int64_t t[PER];
+        int n = 0;
+        unsigned keep = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            keep[k] = i0 + k < T && !(use_ignore && target[i0 + k] == ignore);
-            n += keep[k];
+        for (int k = 0; k < PER; ++k) t[k] = i0 + k < T ? target[i0 + k] : 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const bool ok = i0 + k < T && !(use_ignore && t[k] == ignore);
+            keep |= (unsigned)ok << k;
+            n += ok;
         }
         int incl = n;
 #pragma unroll
@@ -509,31 +515,30 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict
             const int y = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += y;
         }
-        if (lane == 31) warp_sum[warp] = incl;
+        if (lane == 31) warp_sum[turn][warp] = incl;
         __syncthreads();
-        int before = base, all = 0;
-        for (int k = 0; k < 32; ++k) {
-            const int s = warp_sum[k];
-            before += k < warp ? s : 0;
-            all += s;
-        }
-        int at = before + incl - n;
+        int ws = warp_sum[turn][lane];               // every warp scans the warps' sums itself
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (i0 + k < T) {
-                map[i0 + k] = keep[k] ? at : -1;
-                if (keep[k]) idx[at++] = (int32_t)(i0 + k);
-                else {
-                    if (zero_a) zero_a[i0 + k] = 0.0f;
-                    if (zero_b) zero_b[i0 + k] = 0.0f;
-                }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, ws, o);
+            if (lane >= o) ws += y;
+        }
+        const int before = warp ? __shfl_sync(0xffffffffu, ws, warp - 1) : 0;
+        int at = base + before + incl - n;
+        base += __shfl_sync(0xffffffffu, ws, 31);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            if (i0 + k >= T) break;
+            const bool ok = (keep >> k) & 1u;
+            map[i0 + k] = ok ? at : -1;
+            if (ok) idx[at++] = (int32_t)(i0 + k);
+            else {
+                if (zero_a) zero_a[i0 + k] = 0.0f;
+                if (zero_b) zero_b[i0 + k] = 0.0f;
+                if (zero_c) zero_c[i0 + k] = 0.0f;
             }
         }
-        __syncthreads();
-        if (threadIdx.x == 0) base += all;
-        __syncthreads();
     }
-    __syncthreads();
     if (threadIdx.x == 0) {
         *count = base;
         *far = 0;
@@ -577,6 +582,44 @@ struct CeRowArgs {
     int reduction;
 };
 
+// eight consecutive elements, 16-byte aligned for bf16 and 32-byte for float32
+__device__ __forceinline__ void load_f8(float (&f)[8], const __nv_bfloat16 *p) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { f[2 * k] = __low2float(h[k]); f[2 * k + 1] = __high2float(h[k]); }
+}
+__device__ __forceinline__ void load_f8(float (&f)[8], const float *p) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ uint4 pack_f8(const float (&f)[8]) {
+    uint4 v;
+    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return v;
+}
+template <int PARTS> __device__ __forceinline__ void split_store8(__nv_bfloat16 *dst, int64_t part_cols, float (&f)[8]) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        const uint4 v = pack_f8(f);
+        *reinterpret_cast<uint4 *>(dst + p * part_cols) = v;
+        if (p + 1 < PARTS) {
+            float g[8];
+            load_f8(g, reinterpret_cast<const __nv_bfloat16 *>(&v));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] -= g[k];
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ bool rows_aligned(const void *base, int64_t ld) {
+    return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
+}
+
 // One warp per gathered row: the row in bf16 parts, its target's logit (forward), or exponent offset, factor and target value of
 // the probabilities (backward).  Rows up to the next multiple of 256 are zeros that contribute nothing anywhere.
 template <typename T, int PARTS>
@@ -589,7 +632,7 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) 
     if (j >= (n + CE_TILE - 1) / CE_TILE * CE_TILE) return;
     __nv_bfloat16 *dst = a.a + j * a.lda;
     if (j >= n) {
-        for (int64_t c = lane; c < a.lda; c += 32) dst[c] = __float2bfloat16_rn(0.0f);
+        for (int64_t c = lane * 8; c < a.lda; c += 256) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
         if (lane == 0) {
             a.off2[j] = INFINITY;
             a.tcol[j] = -1;
@@ -600,12 +643,38 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) 
     const int64_t row = a.idx[j];
     const int64_t t = a.target[row];
     const bool known = t >= 0 && t < a.V;
+    const bool dot_it = !a.dloss && known;
     const T *src = reinterpret_cast<const T *>(a.x) + row * a.ldx;
     float dot = 0.0f;
-    for (int64_t c = lane; c < a.part_cols; c += 32) {
+    // the same order of additions whether or not the operands start on vector boundaries
+    const bool vx = rows_aligned<T>(a.x, a.ldx), vw = voc.w && rows_aligned<T>(voc.w, voc.ldw);
+    const T *wrow = reinterpret_cast<const T *>(voc.w) + (voc.w && dot_it ? t * voc.ldw : 0);
+    const Sq5Lin lin = sq5_lin_rows(voc.seed, voc.row0 + (uint32_t)t, 0u);
+    const int64_t done = a.R / 8 * 8;
+#pragma unroll 4
+    for (int64_t c = lane * 8; c < done; c += 256) {
+        float f[8], w[8];
+        if (vx) load_f8(f, src + c);
+        else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = to_f32<T>(src[c + k]);
+        }
+        if (dot_it) {
+            if (vw) load_f8(w, wrow + c);
+            else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    w[k] = voc.w ? to_f32<T>(wrow[c + k]) : to_f32<T>(from_f32<T>(sq5_to_float(sq5_tail(lin.base + ((uint32_t)c + k) * lin.sk))));
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) dot = fmaf(f[k], w[k], dot);
+        }
+        split_store8<PARTS>(dst + c, a.part_cols, f);
+    }
+    for (int64_t c = done + lane; c < a.part_cols; c += 32) {
         const float v = c < a.R ? to_f32<T>(src[c]) : 0.0f;
         split_store<PARTS>(dst, a.part_cols, c, v);
-        if (!a.dloss && known && c < a.R) dot = fmaf(v, vocab_at<T>(voc, t, c), dot);
+        if (dot_it && c < a.R) dot = fmaf(v, vocab_at<T>(voc, t, c), dot);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
@@ -643,7 +712,8 @@ __global__ void __launch_bounds__(256) ce_split_kernel(__nv_bfloat16 *__restrict
 // s of 32 rows per block: eight threads per row add every eighth partial sum, then the eight are added in order.
 __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ partial, int64_t ld, int nparts, const int32_t *__restrict__ idx,
                                                      const int32_t *__restrict__ count, const float *__restrict__ lt, float *__restrict__ s_out,
-                                                     float *__restrict__ lse, float *__restrict__ loss, int32_t *__restrict__ far) {
+                                                     float *__restrict__ lse, float *__restrict__ loss, float *__restrict__ loss2,
+                                                     int32_t *__restrict__ far) {
     __shared__ float sh[8][33];
     pdl_launch_dependents();
     pdl_wait();
@@ -651,8 +721,10 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ p
     const int64_t j = (int64_t)blockIdx.x * 32 + r, n = *count;
     if ((int64_t)blockIdx.x * 32 >= n) return;
     float a = 0.0f;
-    if (j < n)
+    if (j < n) {
+#pragma unroll 8
         for (int p = g; p < nparts; p += 8) a += partial[(int64_t)p * ld + j];
+    }
     sh[g][r] = a;
     __syncthreads();
     if (g == 0 && j < n) {
@@ -661,8 +733,10 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ p
         for (int k = 0; k < 8; ++k) s += sh[k][r];
         const float l = log1pf(s);
         s_out[j] = s;
-        loss[idx[j]] = l;
-        lse[idx[j]] = lt[j] + l;
+        const int32_t row = idx[j];
+        loss[row] = l;
+        if (loss2) loss2[row] = l;
+        lse[row] = lt[j] + l;
         if (s >= S_LIMIT) far[1 + atomicAdd(far, 1)] = (int32_t)j;    // in any order: each row is redone by itself
     }
 }
@@ -688,7 +762,7 @@ struct SlotView {
 // far[0] rows, listed behind it.
 template <typename T>
 __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, float *__restrict__ s_io, float *__restrict__ lse,
-                                                        float *__restrict__ loss, float *__restrict__ slots, int KB, int pairs,
+                                                        float *__restrict__ loss, float *__restrict__ loss2, float *__restrict__ slots, int KB, int pairs,
                                                         const int32_t *__restrict__ far) {
     __shared__ float sh_m[16], sh_s[16], sh_p[16];
     pdl_launch_dependents();
@@ -724,6 +798,7 @@ __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, 
         __syncthreads();
         if (threadIdx.x == 0) {
             loss[row] = full - lt;
+            if (loss2) loss2[row] = full - lt;
             lse[row] = full;
             s_io[j] = -1.0f;
         }
@@ -779,46 +854,68 @@ __global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__
 
 // x's gradient from the slots: their sum, finished with s and the target's row (noise: voc.w null and s given), written to the
 // rows' own places; zeros at ignored rows.
-// A block takes DX_ROWS rows of one column tile, a thread one column.
-constexpr int DX_ROWS = 16;
+// A block takes DX_ROWS rows of one column tile, a thread one column; what concerns a row is worked out once, by one thread.
+constexpr int DX_ROWS = 8;
 template <typename T>
 __global__ void __launch_bounds__(CE_TILE) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int32_t *__restrict__ map,
                                                     const int32_t *__restrict__ count, const float *__restrict__ s, const int32_t *__restrict__ tcol,
-                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int pairs) {
+                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int pairs, int tiles_n) {
+    __shared__ const float *sh_at[DX_ROWS];
+    __shared__ int sh_parts[DX_ROWS], sh_t[DX_ROWS];
+    __shared__ float sh_s[DX_ROWS];
+    __shared__ int64_t sh_step;
     pdl_launch_dependents();
     pdl_wait();
-    SlotView o(slots, *count, R, KB, pairs);
-    const int nt = (int)(blockIdx.x % o.cut.tiles_n);
-    const int64_t i0 = (int64_t)(blockIdx.x / o.cut.tiles_n) * DX_ROWS;
+    const int nt = (int)(blockIdx.x % (unsigned)tiles_n);
+    const int64_t i0 = (int64_t)(blockIdx.x / (unsigned)tiles_n) * DX_ROWS;
     const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
-    int64_t m = -1;
-#pragma unroll 4
-    for (int k = 0; k < DX_ROWS; ++k) {
-        const int64_t i = i0 + k;
-        if (i >= T_rows) break;
-        const int64_t j = map[i];
-        float v = 0.0f;
-        if (j >= 0 && c < R) {
-            if (j / CE_TILE != m) {
-                m = j / CE_TILE;
-                o.tile(m, nt);
-            }
-            const int r = (int)(j % CE_TILE);
-            const float sj = s ? s[j] : 0.0f;
-            v = *o.at(o.lo, r, threadIdx.x);
-            if (!(sj < 0.0f)) {                       // -1: the row was finished by ce_rescue_kernel
-                for (int64_t g = o.lo + 1; g <= o.hi; ++g) v += *o.at(g, r, threadIdx.x);
-                if (s) {
-                    const int64_t t = tcol[j];
-                    v = t >= 0 ? (v - sj * vocab_at<T>(voc, t, c)) / (1.0f + sj) : NAN;
-                }
+    if (threadIdx.x < DX_ROWS) {
+        const int64_t i = i0 + threadIdx.x;
+        const int64_t j = i < T_rows ? map[i] : -1;
+        int parts = 0;
+        if (j >= 0) {
+            SlotView o(slots, *count, R, KB, pairs);
+            o.tile(j / CE_TILE, nt);
+            sh_at[threadIdx.x] = o.at(o.lo, (int)(j % CE_TILE), 0);
+            sh_step = (int64_t)o.cut.size * CE_TILE * CE_TILE;       // the same for every row
+            parts = (int)(o.hi - o.lo) + 1;
+            if (s) {
+                sh_s[threadIdx.x] = s[j];
+                sh_t[threadIdx.x] = tcol[j];
+                if (s[j] < 0.0f) parts = -1;          // the row was finished by ce_rescue_kernel
             }
         }
-        if (c < R) dx[i * R + c] = from_f32<T>(v);
+        sh_parts[threadIdx.x] = parts;
+    }
+    __syncthreads();
+    if (c >= R) return;
+#pragma unroll
+    for (int k = 0; k < DX_ROWS; ++k) {
+        const int64_t i = i0 + k;
+        if (i >= T_rows) return;
+        const int parts = sh_parts[k];
+        float v = 0.0f;
+        if (parts != 0) {
+            const float *at = sh_at[k] + threadIdx.x;
+            v = *at;
+            for (int g = 1; g < parts; ++g) v += at[g * sh_step];
+            if (s && parts > 0) {
+                const float sj = sh_s[k];
+                v = sh_t[k] >= 0 ? (v - sj * vocab_at<T>(voc, sh_t[k], c)) / (1.0f + sj) : NAN;
+            }
+        }
+        dx[i * R + c] = from_f32<T>(v);
     }
 }
 
 // dz = unit gradient times what the loss's own gradient (and the mean's 1 / count) say
+__device__ __forceinline__ void store_f8(__nv_bfloat16 *p, const float (&f)[8]) { *reinterpret_cast<uint4 *>(p) = pack_f8(f); }
+__device__ __forceinline__ void store_f8(float *p, const float (&f)[8]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+// ignored rows stay zero whatever the factor (no row counts: 1 / 0)
+__device__ __forceinline__ float scaled(float u, float g) { return u == 0.0f ? 0.0f : u * g; }
 template <typename T>
 __global__ void __launch_bounds__(256) ce_scale_kernel(T *__restrict__ dz, const T *__restrict__ unit, const float *__restrict__ dloss,
                                                        const float *__restrict__ count, int64_t rows, int64_t R, int reduction) {
@@ -826,11 +923,21 @@ __global__ void __launch_bounds__(256) ce_scale_kernel(T *__restrict__ dz, const
     pdl_wait();
     const int64_t total = rows * R;
     const float g0 = reduction == RDB_CE_NONE ? 0.0f : reduction == RDB_CE_MEAN ? dloss[0] / *count : dloss[0];
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const float u = to_f32<T>(unit[i]);
-        const float g = reduction == RDB_CE_NONE ? dloss[i / R] : g0;
-        dz[i] = from_f32<T>(u == 0.0f ? 0.0f : u * g);       // ignored rows stay zero whatever the factor (0 rows: 1 / 0)
+    const bool vec = R % 8 == 0 && ((reinterpret_cast<uintptr_t>(dz) | reinterpret_cast<uintptr_t>(unit)) & 15) == 0;
+    if (vec) {
+        const int64_t groups = total / 8, per = R / 8;
+        for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < groups; i += (int64_t)gridDim.x * blockDim.x) {
+            const float g = reduction == RDB_CE_NONE ? dloss[i / per] : g0;
+            float f[8];
+            load_f8(f, unit + i * 8);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = scaled(f[k], g);
+            store_f8(dz + i * 8, f);
+        }
+        return;
     }
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x)
+        dz[i] = from_f32<T>(scaled(to_f32<T>(unit[i]), reduction == RDB_CE_NONE ? dloss[i / R] : g0));
 }
 
 // ================================================================================================
@@ -956,9 +1063,9 @@ struct CeCall {
     template <typename P> P *at(size_t off) const { return reinterpret_cast<P *>(ws + off); }
 };
 
-static int ce_find_rows(const CeCall &c, int64_t ignore, int use_ignore, float *zero_a, float *zero_b, float *count_f) {
+static int ce_find_rows(const CeCall &c, int64_t ignore, int use_ignore, float *zero_a, float *zero_b, float *zero_c, float *count_f) {
     return launch_pdl(ce_rows_kernel, dim3(1), 1024, 0, c.st, c.target, c.T, ignore, use_ignore, c.at<int32_t>(c.p.idx), c.at<int32_t>(c.p.map),
-                      c.at<int32_t>(c.p.count), zero_a, zero_b, count_f, c.at<int32_t>(c.p.far));
+                      c.at<int32_t>(c.p.count), zero_a, zero_b, zero_c, count_f, c.at<int32_t>(c.p.far));
 }
 
 static CeRowArgs ce_row_args(const CeCall &c) {
@@ -1097,9 +1204,9 @@ static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
     const int32_t *map = c.at<int32_t>(p.map), *count = c.at<int32_t>(p.count), *tcol = c.at<int32_t>(p.tcol);
     float *slots = c.at<float>(p.slots);
     if (c.dtype == RDB_F32)
-        return launch_pdl(ce_dx_kernel<float>, grid, CE_TILE, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs);
-    return launch_pdl(ce_dx_kernel<__nv_bfloat16>, grid, CE_TILE, 0, c.st, (__nv_bfloat16 *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p),
-                      p.pairs);
+        return launch_pdl(ce_dx_kernel<float>, grid, CE_TILE, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs, (int)cdiv64(c.R, CE_TILE));
+    return launch_pdl(ce_dx_kernel<__nv_bfloat16>, grid, CE_TILE, 0, c.st, (__nv_bfloat16 *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs,
+                      (int)cdiv64(c.R, CE_TILE));
 }
 
 static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w, int64_t ldw, int dtype, int reduction) {
@@ -1126,7 +1233,7 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x,
     int rc = ce_check(T, R, V, ldx, w, ldw, dtype, reduction);
     if (rc) return rc;
     if (dx_unit && w) return RDB_ERR_UNSUPPORTED;        // a stored matrix takes its gradients in rdb_ce_bwd
-    if (!aux || (!loss && reduction != RDB_CE_NONE)) return RDB_ERR_NULL;
+    if (!aux || (!loss && (T > 0 || reduction != RDB_CE_NONE))) return RDB_ERR_NULL;
     if (T > 0 && (!x || !target)) return RDB_ERR_NULL;
     const size_t es = dtype_size(dtype);
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(dx_unit)) & (es - 1)) || (reinterpret_cast<uintptr_t>(target) & 7))
@@ -1142,7 +1249,8 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x,
     c.status = status;
     c.st = (cudaStream_t)stream;
     float *lse = aux, *rows = aux + T, *count_f = aux + 2 * T;
-    if ((rc = ce_find_rows(c, ignore_index, use_ignore, lse, rows, count_f))) return rc;
+    float *rows2 = reduction == RDB_CE_NONE ? loss : nullptr;       // the caller's own copy of the rows' losses
+    if ((rc = ce_find_rows(c, ignore_index, use_ignore, lse, rows, rows2, count_f))) return rc;
     if (T > 0) {
         const CeRowArgs ra = ce_row_args(c);
         if ((rc = ce_gather(c, ra))) return rc;
@@ -1161,12 +1269,12 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x,
         int32_t *far = c.at<int32_t>(c.p.far);
         const int nparts = (int)((c.p.npieces - 1) * (c.p.piece / CE_TILE) * 2 + (dx_unit ? c.p.piece / CE_TILE : cdiv64(last, CE_TILE)) * 2);
         rc = launch_pdl(ce_sum_kernel, dim3((unsigned)(c.p.Mpad / 32)), 256, 0, c.st, (const float *)c.at<float>(c.p.partial), c.p.Mpad, nparts, ra.idx,
-                        ra.count, (const float *)ra.lt, c.at<float>(c.p.s), lse, rows, far);
+                        ra.count, (const float *)ra.lt, c.at<float>(c.p.s), lse, rows, rows2, far);
         if (rc) return rc;
         float *slots = dx_unit ? c.at<float>(c.p.slots) : nullptr, *sums = c.at<float>(c.p.s);
         const int pairs = c.p.pairs;
-        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs, (const int32_t *)far)
-                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, slots, ce_kb(c.p), pairs, (const int32_t *)far);
+        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, ce_kb(c.p), pairs, (const int32_t *)far)
+                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, ce_kb(c.p), pairs, (const int32_t *)far);
         if (rc) return rc;
         if (dx_unit && (rc = ce_finish_dx(c, dx_unit, true))) return rc;
     }
@@ -1201,7 +1309,7 @@ extern "C" int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x,
     c.dtype = dtype;
     c.status = status;
     c.st = st;
-    if ((rc = ce_find_rows(c, ignore_index, use_ignore, nullptr, nullptr, nullptr))) return rc;
+    if ((rc = ce_find_rows(c, ignore_index, use_ignore, nullptr, nullptr, nullptr, nullptr))) return rc;
     CeRowArgs ra = ce_row_args(c);
     ra.dloss = dloss;
     ra.lse = aux;

@@ -432,17 +432,16 @@ def _ce_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor, ignore_index: Optional[int] = -100, reduction: str = "mean",
            seed: int = 0, vocab: int = 0, row0: int = 0, need_unit: bool = False
-           ) -> Tuple[Optional[torch.Tensor], torch.Tensor, Optional[torch.Tensor]]:
+           ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """(loss, aux, unit): cross entropy of ``x @ W.T`` against ``target`` (see rdb_ce_fwd).  ``weight`` None: ``vocab`` noise rows
-    from ``row0`` on.  loss: 0-d float32 (None for reduction "none": the rows' losses are ``aux[T:2T]``); unit: the rows' own
-    gradients in x, with ``need_unit``."""
+    from ``row0`` on.  loss: float32, 0-d or (reduction "none") [T]; unit: the rows' own gradients in x, with ``need_unit``."""
     V = int(vocab) if weight is None else weight.shape[0]
     dev, dt, red = _ce_args(x, weight, target, V, reduction)
     x, weight, target = _ce_rows(x), _ce_rows(weight), target.contiguous()
     T, R = x.shape
     L = _lib.lib()
     aux = torch.empty((2 * T + 1,), dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
+    loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
     unit = torch.empty((T, R), dtype=x.dtype, device=dev) if need_unit else None
     with torch.cuda.device(dev):
         ldw = _pitch(weight) if weight is not None else 0

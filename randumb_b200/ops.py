@@ -124,8 +124,7 @@ def _(rows, cols, seed, row0, dtype, device):
 def noise_ce_fwd(z: torch.Tensor, target: torch.Tensor, seed: int, out_features: int, row0: int, ignore_index: Optional[int], reduction: str,
                  need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     loss, aux, unit = K.ce_fwd(z, None, target, ignore_index, reduction, seed, out_features, row0, need_grad)
-    T = z.shape[0]
-    return aux[T:2 * T].clone() if loss is None else loss, aux, unit if unit is not None else z.new_empty((0,))
+    return loss, aux, unit if unit is not None else z.new_empty((0,))
 
 
 @noise_ce_fwd.register_fake
@@ -175,8 +174,7 @@ noise_ce_fwd.register_autograd(_noise_ce_backward, setup_context=_noise_ce_setup
 def linear_ce_fwd(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: Optional[int], reduction: str
                   ) -> Tuple[torch.Tensor, torch.Tensor]:
     loss, aux, _ = K.ce_fwd(x, weight, target, ignore_index, reduction)
-    T = x.shape[0]
-    return aux[T:2 * T].clone() if loss is None else loss, aux
+    return loss, aux
 
 
 @linear_ce_fwd.register_fake
@@ -222,6 +220,48 @@ def _linear_ce_backward(ctx, dloss, daux):
 linear_ce_fwd.register_autograd(_linear_ce_backward, setup_context=_linear_ce_setup)
 
 
+def _eager(*ts: torch.Tensor) -> bool:
+    """Plain CUDA tensors outside of any tracing: the kernels can be called without going through the dispatcher, which costs more
+    than they do on small problems."""
+    return not torch.compiler.is_compiling() and all([t.is_cuda and type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts]) \
+        and not torch._C._len_torch_dispatch_stack()
+
+
+class _NoiseCE(torch.autograd.Function):
+    """noise_ce_fwd / noise_ce_bwd for eager calls that take part in autograd."""
+
+    @staticmethod
+    def forward(ctx, z, target, seed, out_features, row0, ignore_index, reduction):
+        loss, aux, unit = K.ce_fwd(z, None, target, ignore_index, reduction, seed, out_features, row0, True)
+        ctx.save_for_backward(aux, unit)
+        ctx.reduction = reduction
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        aux, unit = ctx.saved_tensors
+        return K.ce_scale(unit, dloss, aux, ctx.reduction), None, None, None, None, None, None
+
+
+class _LinearCE(torch.autograd.Function):
+    """linear_ce_fwd / linear_ce_bwd for eager calls that take part in autograd."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, reduction):
+        loss, aux, _ = K.ce_fwd(x, weight, target, ignore_index, reduction)
+        ctx.save_for_backward(x, weight, target, aux)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, weight, target, aux = ctx.saved_tensors
+        dx, dw = K.ce_bwd(dloss, x, weight, target, aux, ctx.ignore_index, ctx.reduction, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
 def noise_cross_entropy(z: torch.Tensor, seed: int, out_features: int, target: torch.Tensor, row0: int = 0, ignore_index: Optional[int] = -100,
                         reduction: str = "mean") -> torch.Tensor:
     """Softmax cross entropy of the logits ``z @ S[row0:row0 + out_features].T`` (noise of ``seed`` in z's type) against ``target``,
@@ -234,8 +274,14 @@ def noise_cross_entropy(z: torch.Tensor, seed: int, out_features: int, target: t
     lead = z.shape[:-1]
     if tuple(target.shape) != tuple(lead):
         raise RuntimeError(f"noise_cross_entropy: target {tuple(target.shape)} does not match z {tuple(z.shape)}")
+    z2, t = z.reshape(-1, z.shape[-1]), target.reshape(-1)
     need = torch.is_grad_enabled() and z.requires_grad
-    loss = noise_ce_fwd(z.reshape(-1, z.shape[-1]), target.reshape(-1), seed, out_features, row0, ignore_index, reduction, need)[0]
+    if not _eager(z2, t):
+        loss = noise_ce_fwd(z2, t, seed, out_features, row0, ignore_index, reduction, need)[0]
+    elif need:
+        loss = _NoiseCE.apply(z2, t, seed, out_features, row0, ignore_index, reduction)
+    else:
+        loss = K.ce_fwd(z2, None, t, ignore_index, reduction, seed, out_features, row0)[0]
     return loss.reshape(lead) if reduction == "none" else loss
 
 
@@ -247,7 +293,13 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     lead = x.shape[:-1]
     if tuple(target.shape) != tuple(lead):
         raise RuntimeError(f"linear_cross_entropy: target {tuple(target.shape)} does not match x {tuple(x.shape)}")
-    loss = linear_ce_fwd(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1), ignore_index, reduction)[0]
+    x2, t = x.reshape(-1, x.shape[-1]), target.reshape(-1)
+    if not _eager(x2, weight, t):
+        loss = linear_ce_fwd(x2, weight, t, ignore_index, reduction)[0]
+    elif torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        loss = _LinearCE.apply(x2, weight, t, ignore_index, reduction)
+    else:
+        loss = K.ce_fwd(x2, weight, t, ignore_index, reduction)[0]
     return loss.reshape(lead) if reduction == "none" else loss
 
 
