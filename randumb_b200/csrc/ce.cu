@@ -23,10 +23,12 @@
 // parts whose orders add up to at most two, accumulated in the same float32 accumulator: exact products, terms below 2^-24
 // left out.
 //
-// The products run on CTA pairs (cta_group::2), 256 x 256 tiles, six 32 KB stages of TMA-fed operands, two accumulators in TMEM
-// so that the exponentials of one tile run under the next tile's MMAs.  The x-gradient product is cut by k-blocks: every pair
-// takes an equal run of the (tile, k-block) sequence and leaves its part of a tile in a slot of its own; the slots are added in
-// order, so results repeat run to run whatever the number of tiles.
+// The products run on CTA pairs (cta_group::2).  bf16: 512 x 256 tiles, two 256 x 256 accumulators that fill TMEM and take MMAs in
+// turn, four 48 KB stages of TMA-fed operands; an epilogue warp takes its 32 rows x 128 columns of an accumulator into registers,
+// hands the accumulator back and computes from the registers, and the MMA thread runs ahead on the first accumulator while the
+// second is still being read.  (256 x 256 tiles, whose MMAs all go to one accumulator, kept the tensor pipe 62 % busy.)  At most 256
+// rows: 256 x 256 tiles, six 32 KB stages.  float32: the same, and the accumulators, whose additions cut instead of rounding (about
+// 2^-26 of the sum per 16 products, all in one direction), are added up in the epilogue's registers every eight k-blocks.
 #include <cmath>
 
 #include "umma.cuh"
@@ -39,12 +41,23 @@ using namespace ptx;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float S_LIMIT = 1.2676506e30f;       // 2^100: rows above are redone with their maximum
 constexpr int CE_TILE = 256;
-constexpr int CE_STAGES = 6;
-constexpr int CE_STAGE = 2 * SUB_BYTES;        // this CTA's 128 rows of A and its half (128 rows) of B
 constexpr int CE_EPI = 8;
-constexpr int CE_THREADS = (2 + CE_EPI) * 32;
-constexpr int CE_SMEM = CE_STAGES * CE_STAGE + CE_EPI * 4096 + 1024;
-static_assert(CE_SMEM <= 232448 - 512, "shared memory");
+constexpr int CE_THREADS = (4 + CE_EPI) * 32;   // a control warpgroup (TMA, MMA, two idle warps) and two epilogue warpgroups
+// An epilogue warp holds 128 accumulator columns: registers move from the control warpgroup to the epilogue's.  Launched with 168
+// each (12 warps): 4 x 72 + 8 x 216 = 12 x 168.
+constexpr int CE_REGS_CONTROL = 72, CE_REGS_EPI = 216;
+static_assert(4 * CE_REGS_CONTROL + CE_EPI * CE_REGS_EPI <= 12 * 168, "setmaxnreg draws on the launch's registers");
+constexpr int CE_CHUNK = 8;                    // float32: k-blocks between additions in registers
+
+// MT row sub-tiles of 256 per pair tile: a stage holds this CTA's 128 rows of each and its half (128 rows) of B
+template <int MT>
+struct CeCfg {
+    static constexpr int STAGES = MT == 2 ? 4 : 6;
+    static constexpr int STAGE = (MT + 1) * SUB_BYTES;
+    static constexpr int ROWS = MT * CE_TILE;
+    static constexpr int SMEM = STAGES * STAGE + CE_EPI * 4096 + 1024;
+    static_assert(SMEM <= 232448 - 512, "shared memory");
+};
 
 enum { EPI_SUM, EPI_EXP, EPI_PROB, EPI_SLOT, EPI_BF16, EPI_F32 };
 
@@ -57,6 +70,7 @@ struct CeArgs {
     int a_off[6], b_off[6];       // column offsets of the parts a term multiplies
     int m_fast;
     int accumulate;               // EPI_SLOT: add to the slots instead of storing
+    int tail, tail_parts;         // EPI_BF16 / EPI_F32: the last `tail` tiles are each cut into this many runs of k-blocks, stored in slots
     const float *off2, *scale, *tval;   // per row: exponent offset in powers of two; EPI_PROB: factor and the target's value
     const int32_t *tcol;          // per row: target column, -1 for none
     int32_t v0, ncols;            // first column of this piece, columns of it that exist
@@ -81,13 +95,14 @@ __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *m, uint32_t
 // on neighbouring column tiles of one row tile over the same run of k-blocks, so E crosses from memory once (R = 1024, 8192 rows,
 // 25344 columns: 441 us when each pair had a run of its own).  Groups own equal runs of the (panel, k-block) sequence, a panel being
 // a row tile and `size` column tiles.  Group g leaves its part of a panel in slot panel + g, which grows from each part to the next:
-// (panels + groups) * size slots of 256 x 256 float32 hold them all, whatever the number of rows turns out to be.
+// (panels + groups) * size slots of one tile in float32 hold them all, whatever the number of rows turns out to be.
+// Counts fit 32 bits (the entry points refuse more).
 struct Cut {
-    int64_t total;                // k-blocks of all panels
-    int64_t groups;               // groups that take part: as many as get four k-blocks each
+    int total;                    // k-blocks of all panels
+    int groups;                   // groups that take part: as many as get four k-blocks each
     int size, per_row, tiles_n;   // pairs per group, panels per row tile
     int KB;
-    __host__ __device__ __forceinline__ Cut(int64_t rows, int64_t cols, int KB_, int pairs) : KB(KB_) {
+    __host__ __device__ __forceinline__ Cut(int64_t rows, int64_t cols, int KB_, int pairs, int tile_rows) : KB(KB_) {
         tiles_n = (int)((cols + CE_TILE - 1) / CE_TILE);
         per_row = (tiles_n + 7) / 8;
         size = (tiles_n + per_row - 1) / per_row;
@@ -95,77 +110,120 @@ struct Cut {
             size = pairs;
             per_row = (tiles_n + size - 1) / size;
         }
-        total = (rows + CE_TILE - 1) / CE_TILE * per_row * KB;
+        total = (int)((rows + tile_rows - 1) / tile_rows) * per_row * KB;
         groups = pairs / size;
         if (groups > total / 4) groups = total / 4 < 1 ? 1 : total / 4;
     }
-    __host__ __device__ __forceinline__ int64_t begin(int64_t g) const { return total * g / groups; }
-    __host__ __device__ __forceinline__ int64_t owner(int64_t at) const { return ((at + 1) * groups + total - 1) / total - 1; }
-    __host__ __device__ __forceinline__ int64_t slot(int64_t panel, int64_t g, int member) const { return (panel + g) * size + member; }
-    __host__ __device__ __forceinline__ int64_t slots(int pairs) const { return (total / (KB ? KB : 1) + pairs / size) * size; }
+    __host__ __device__ __forceinline__ int begin(int g) const { return (int)((int64_t)total * g / groups); }
+    __host__ __device__ __forceinline__ int owner(int at) const { return (int)((((int64_t)at + 1) * groups + total - 1) / total - 1); }
+    __host__ __device__ __forceinline__ int slot(int panel, int g, int member) const { return (panel + g) * size + member; }
+    __host__ __device__ __forceinline__ int slots(int pairs) const { return (total / (KB ? KB : 1) + pairs / size) * size; }
 };
 
 struct WorkItem {
-    int64_t m, n, slot;
+    int m, n, slot;               // slot < 0: the tile goes to the output itself
     int kb0, kb1;
 };
 
 // The sequence of work items of one pair; every role walks it by itself.
 struct Walk {
-    Cut cut;
-    int64_t tiles_m, tiles_n, next, end, group, step;
-    int KB, m_fast, member;
+    int tiles_m, tiles_n, next, end, step, whole, KB, parts, m_fast;
+    int group, member, size, per_row;
     bool by_cut;
-    __device__ __forceinline__ Walk(const CeArgs &a, bool by_cut_, int64_t rows, int kb_total, int pair, int pairs)
-        : cut(rows, a.N, kb_total, pairs), KB(kb_total), m_fast(a.m_fast), by_cut(by_cut_) {
-        tiles_m = (rows + CE_TILE - 1) / CE_TILE;
-        tiles_n = cut.tiles_n;
-        step = pairs;
+    __device__ __forceinline__ Walk(const CeArgs &a, bool by_cut_, int64_t rows, int kb_total, int pair, int pairs, int tile_rows)
+        : KB(kb_total), m_fast(a.m_fast), by_cut(by_cut_) {
+        tiles_m = (int)((rows + tile_rows - 1) / tile_rows);
         if (by_cut) {
-            group = pair / cut.size;
-            member = pair % cut.size;
+            const Cut cut(rows, a.N, kb_total, pairs, tile_rows);
+            tiles_n = cut.tiles_n;
+            size = cut.size;
+            per_row = cut.per_row;
+            group = pair / size;
+            member = pair % size;
             const bool in = group < cut.groups;
             next = in ? cut.begin(group) : 0;
             end = in ? cut.begin(group + 1) : 0;
         } else {
+            tiles_n = (int)((a.N + CE_TILE - 1) / CE_TILE);
+            step = pairs;
+            parts = a.tail_parts;
             next = pair;
-            end = tiles_m * tiles_n;
+            whole = tiles_m * tiles_n - a.tail;
+            end = whole + a.tail * parts;
         }
     }
     __device__ __forceinline__ bool take(WorkItem &w) {
         while (next < end) {
             if (!by_cut) {
+                int tile = next;
                 w.kb0 = 0;
                 w.kb1 = KB;
-                w.slot = 0;
-                w.m = m_fast ? next % tiles_m : next / tiles_n;
-                w.n = m_fast ? next / tiles_m : next % tiles_n;
+                w.slot = -1;
+                if (next >= whole) {
+                    const int piece = (next - whole) % parts;
+                    tile = whole + (next - whole) / parts;
+                    w.slot = next - whole;
+                    w.kb0 = KB * piece / parts;
+                    w.kb1 = KB * (piece + 1) / parts;
+                }
+                w.m = m_fast ? tile % tiles_m : tile / tiles_n;
+                w.n = m_fast ? tile / tiles_m : tile % tiles_n;
                 next += step;
                 return true;
             }
-            const int64_t panel = next / KB;
-            w.kb0 = (int)(next - panel * KB);
-            const int64_t left = end - next;
-            w.kb1 = left < KB - w.kb0 ? w.kb0 + (int)left : KB;
+            const int panel = next / KB;
+            w.kb0 = next - panel * KB;
+            w.kb1 = end - next < KB - w.kb0 ? w.kb0 + end - next : KB;
             next += w.kb1 - w.kb0;
-            w.m = panel / cut.per_row;
-            w.n = (panel % cut.per_row) * cut.size + member;
-            w.slot = cut.slot(panel, group, member);
+            w.m = panel / per_row;
+            w.n = (panel % per_row) * size + member;
+            w.slot = (panel + group) * size + member;
             if (w.n < tiles_n) return true;
         }
         return false;
     }
 };
 
-template <int A_MN, int B_MN, int EPI, int PARTS>
+// 32 rows x 64 bf16 columns of a warp, from registers through the swizzled staging box
+__device__ __forceinline__ void stage_bf16(uint32_t rowaddr, int lane, const float *v) {
+#pragma unroll
+    for (int ch = 0; ch < 8; ++ch) {
+        uint32_t pk[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[ch * 8 + 2 * x], v[ch * 8 + 2 * x + 1]);
+            pk[x] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((ch ^ (lane & 7)) << 4)), "r"(pk[0]), "r"(pk[1]),
+                     "r"(pk[2]), "r"(pk[3]) : "memory");
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+// 32 rows x 32 float32 columns
+__device__ __forceinline__ void stage_f32(uint32_t rowaddr, int lane, const float *v) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((j ^ (lane & 7)) << 4)), "r"(__float_as_uint(v[4 * j])),
+                     "r"(__float_as_uint(v[4 * j + 1])), "r"(__float_as_uint(v[4 * j + 2])), "r"(__float_as_uint(v[4 * j + 3])) : "memory");
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// PARTS 3: float32 operands (and MT 1, accumulators added up in registers).
+template <int A_MN, int B_MN, int EPI, int PARTS, int MT>
 __global__ void __launch_bounds__(CE_THREADS, 1)
 ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-               const __grid_constant__ CUtensorMap tmap_d, const __grid_constant__ CeArgs args) {
+               const __grid_constant__ CUtensorMap tmap_d, const __grid_constant__ CUtensorMap tmap_slot, const __grid_constant__ CeArgs args) {
+    using Cfg = CeCfg<MT>;
+    constexpr int STAGES = Cfg::STAGES;
+    constexpr bool ADD = PARTS == 3;              // chunks of CE_CHUNK k-blocks, added in registers
+    constexpr bool CUT = EPI == EPI_SLOT;
+    static_assert(!ADD || MT == 1, "the registers hold one sub-tile");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bar_full[CE_STAGES], bar_free[CE_STAGES], bar_tmem_full[2], bar_tmem_empty[2];
+    __shared__ uint64_t bar_full[STAGES], bar_free[STAGES], bar_tmem_full[2], bar_tmem_empty[2];
     __shared__ uint32_t tmem_holder;
     __shared__ int abort_flag;
-    constexpr bool CUT = EPI == EPI_SLOT;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -174,7 +232,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     const bool leader = half == 0;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < CE_STAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&bar_full[s]), 1);      // the even CTA's TMA thread; both CTAs' loads complete their bytes here
             mbar_init(smem_u32(&bar_free[s]), 1);      // one tcgen05.commit from the pair's MMA thread
         }
@@ -201,10 +259,11 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     const int64_t counted = (args.m_counted || args.k_counted) ? (int64_t)*args.count : 0;
     const int64_t rows = args.m_counted ? counted : args.M;
     const int kbs = args.k_counted ? (int)((counted + BK - 1) / BK) : args.kbs;
-    const int KB = kbs * args.nterm;
-    Walk walk(args, CUT, rows, KB, (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1));
+    Walk walk(args, CUT, rows, kbs * args.nterm, (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1), Cfg::ROWS);
     WorkItem w;
 
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CE_REGS_CONTROL));
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
         if (lane == 0) {
@@ -213,7 +272,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             PipeState st;
             bool ok = true;
             while (ok && walk.take(w)) {
-                const int32_t m0 = (int32_t)(w.m * CE_TILE + half * BM);
+                const int32_t m0 = (int32_t)(w.m * Cfg::ROWS + half * BM);
                 const int32_t n0 = (int32_t)(w.n * CE_TILE + half * BM);
                 int term = kbs ? w.kb0 / kbs : 0, kk = w.kb0 - term * kbs;
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
@@ -223,14 +282,18 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                         break;
                     }
                     const uint32_t fb = mapa(smem_u32(&bar_full[st.idx]), rank & ~1u);
-                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[st.idx]), 2 * CE_STAGE);
-                    const uint32_t sa = smem_base + st.idx * CE_STAGE, sb = sa + SUB_BYTES;
+                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[st.idx]), 2 * Cfg::STAGE);
+                    const uint32_t sa = smem_base + st.idx * Cfg::STAGE, sb = sa + MT * SUB_BYTES;
                     const int32_t ax = args.a_off[term], bx = args.b_off[term], k0 = kk * BK;
-                    if (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < BM / 64; ++i) tma_load_2d_pair(sa + i * (64 * BK * 2), &tmap_a, fb, ax + m0 + i * 64, k0);
-                    } else {
-                        tma_load_2d_pair(sa, &tmap_a, fb, ax + k0, m0);
+                    for (int s = 0; s < MT; ++s) {
+                        if (A_MN) {
+#pragma unroll
+                            for (int i = 0; i < BM / 64; ++i)
+                                tma_load_2d_pair(sa + s * SUB_BYTES + i * (64 * BK * 2), &tmap_a, fb, ax + m0 + s * CE_TILE + i * 64, k0);
+                        } else {
+                            tma_load_2d_pair(sa + s * SUB_BYTES, &tmap_a, fb, ax + k0, m0 + s * CE_TILE);
+                        }
                     }
                     if (B_MN) {
 #pragma unroll
@@ -238,7 +301,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                     } else {
                         tma_load_2d_pair(sb, &tmap_b, fb, bx + k0, n0);
                     }
-                    st.advance<CE_STAGES>();
+                    st.advance<STAGES>();
                     if (++kk == kbs) { kk = 0; ++term; }
                 }
             }
@@ -257,217 +320,245 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             constexpr uint32_t A_LBO = A_MN ? 64 * BK * 2 : 0, A_KSTEP = A_MN ? 2048 : UMMA_K * 2;
             constexpr uint32_t B_LBO = B_MN ? 64 * BK * 2 : 0, B_KSTEP = B_MN ? 2048 : UMMA_K * 2;
             const uint32_t peer = rank ^ 1u;
-            PipeState st;
             bool ok = true;
-            int64_t it = 0;
-            while (ok && walk.take(w)) {
-                if (w.kb0 == w.kb1) continue;                    // nothing to contract: the epilogue stores zeros
-                const int acc = (int)(it & 1);
-                if (!mbar_wait_cluster(smem_u32(&bar_tmem_empty[acc]), (uint32_t)((it >> 1) & 1) ^ 1, abortp)) {
+            auto issue = [&](uint32_t stage, int sub, int acc, int k, bool fresh) {
+                const uint32_t sa = smem_base + stage * Cfg::STAGE;
+                const uint32_t a_lo = smem_desc_lo(sa + sub * SUB_BYTES, A_LBO), b_lo = smem_desc_lo(sa + MT * SUB_BYTES, B_LBO);
+                umma_bf16_pair(tmem_base + acc * CE_TILE, pack_desc(a_lo + ((k * A_KSTEP) >> 4), desc_hi),
+                               pack_desc(b_lo + ((k * B_KSTEP) >> 4), desc_hi), idesc, fresh ? 0u : 1u);
+            };
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                if (!mbar_wait_cluster(bar, parity, abortp)) {
                     raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_MMA);
-                    break;
-                }
-                tc_fence_after_sync();
-                for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    if (!mbar_wait_cluster(smem_u32(&bar_full[st.idx]), st.phase, abortp)) {
-                        raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_MMA);
-                        ok = false;
-                        break;
-                    }
+                    ok = false;
+                } else {
                     tc_fence_after_sync();
-                    const uint32_t sa = smem_base + st.idx * CE_STAGE;
-                    const uint32_t a_lo = smem_desc_lo(sa, A_LBO), b_lo = smem_desc_lo(sa + SUB_BYTES, B_LBO);
+                }
+                return ok;
+            };
+            auto commit_both = [&](uint32_t bar) {          // to the barrier of both CTAs
+                umma_commit_pair(bar);
+                umma_commit_pair(mapa(bar, peer));
+            };
+            if (MT == 1) {
+                PipeState st;
+                uint32_t it = 0;
+                while (ok && walk.take(w)) {
+                    for (int c0 = w.kb0; c0 < w.kb1 && ok;) {
+                        const int c1 = ADD && c0 + CE_CHUNK < w.kb1 ? c0 + CE_CHUNK : w.kb1;
+                        const int acc = (int)(it & 1);
+                        if (!wait(smem_u32(&bar_tmem_empty[acc]), ((it >> 1) & 1) ^ 1)) break;
+                        for (int kb = c0; kb < c1; ++kb) {
+                            if (!wait(smem_u32(&bar_full[st.idx]), st.phase)) break;
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k)
-                        umma_bf16_pair(tmem_base + acc * CE_TILE, pack_desc(a_lo + ((k * A_KSTEP) >> 4), desc_hi),
-                                       pack_desc(b_lo + ((k * B_KSTEP) >> 4), desc_hi), idesc, ((kb - w.kb0) | k) != 0 ? 1u : 0u);
-                    umma_commit_pair(smem_u32(&bar_free[st.idx]));
-                    umma_commit_pair(mapa(smem_u32(&bar_free[st.idx]), peer));
-                    st.advance<CE_STAGES>();
+                            for (int k = 0; k < BK / UMMA_K; ++k) issue(st.idx, 0, acc, k, ((kb - c0) | k) == 0);
+                            commit_both(smem_u32(&bar_free[st.idx]));
+                            st.advance<STAGES>();
+                        }
+                        if (ok) commit_both(smem_u32(&bar_tmem_full[acc]));
+                        ++it;
+                        c0 = c1;
+                    }
                 }
-                if (ok) {
-                    umma_commit_pair(smem_u32(&bar_tmem_full[acc]));
-                    umma_commit_pair(mapa(smem_u32(&bar_tmem_full[acc]), peer));
+            } else {
+                // Two accumulators per tile.  While the epilogue still reads accumulator 1 of the tile before, the k-blocks that
+                // are staged already go to accumulator 0 alone (ahead of accumulator 1 by at most the ring); then both in turn:
+                // consecutive MMAs to one accumulator are a quarter slower.
+                PipeState st0, st1;
+                uint32_t it = 0;
+                while (ok && walk.take(w)) {
+                    const int n = w.kb1 - w.kb0;
+                    if (n == 0) continue;
+                    const uint32_t par = (it & 1) ^ 1;
+                    bool have1 = false;
+                    int i0 = 0, i1 = 0;
+                    while (i1 < n && ok) {
+                        if (!have1 && (i0 - i1 == STAGES || i0 == n || mbar_try_wait_cluster(smem_u32(&bar_tmem_empty[1]), par))) {
+                            if (!wait(smem_u32(&bar_tmem_empty[1]), par)) break;
+                            have1 = true;
+                        }
+                        if (have1 && i1 < i0) {
+#pragma unroll
+                            for (int k = 0; k < BK / UMMA_K; ++k) issue(st1.idx, 1, 1, k, (i1 | k) == 0);
+                            commit_both(smem_u32(&bar_free[st1.idx]));
+                            st1.advance<STAGES>();
+                            if (++i1 == n) commit_both(smem_u32(&bar_tmem_full[1]));
+                            continue;
+                        }
+                        if (i0 == 0 && !wait(smem_u32(&bar_tmem_empty[0]), par)) break;
+                        if (!wait(smem_u32(&bar_full[st0.idx]), st0.phase)) break;
+                        const bool last = i0 == n - 1;
+                        if (!have1 || last) {
+#pragma unroll
+                            for (int k = 0; k < BK / UMMA_K; ++k) issue(st0.idx, 0, 0, k, (i0 | k) == 0);
+                            if (last) commit_both(smem_u32(&bar_tmem_full[0]));     // drained while accumulator 1 finishes
+                            st0.advance<STAGES>();
+                            ++i0;
+                            continue;                                                // accumulator 1 catches up at the loop's top
+                        }
+#pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; ++k) {
+                            issue(st0.idx, 0, 0, k, (i0 | k) == 0);
+                            issue(st0.idx, 1, 1, k, (i0 | k) == 0);
+                        }
+                        commit_both(smem_u32(&bar_free[st0.idx]));
+                        st0.advance<STAGES>();
+                        st1.advance<STAGES>();
+                        ++i0;
+                        ++i1;
+                    }
+                    ++it;
                 }
-                ++it;
             }
         }
+    }
     } else {
-        // ------------------------------------------------------------------ epilogue: 8 warps, this CTA's 128 rows
-        const int ew = warp - 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CE_REGS_EPI));
+        // ------------------------------------------------------------------ epilogue: 8 warps, this CTA's 128 rows of a sub-tile
+        const int ew = warp - 4;
         const int q = warp & 3;                      // TMEM lane quarter this warp may read
         const int cg = ew >> 2;                      // which 128 of the 256 columns
         const uint32_t leader_rank = rank & ~1u;
-        const uint32_t stag = smem_base + CE_STAGES * CE_STAGE + (uint32_t)ew * 4096u;
+        const uint32_t stag = smem_base + STAGES * Cfg::STAGE + (uint32_t)ew * 4096u;
         const uint32_t rowaddr = stag + (uint32_t)lane * 128u;
-        int64_t it = 0;
+        auto box_free = [&]() {                      // the last store from the staging box has read it
+            if (lane == 0) bulk_wait_group_read0();
+            __syncwarp();
+        };
+        uint32_t it = 0;
         bool ok = true;
-        while (ok && walk.take(w)) {
-            const int64_t row_w = w.m * CE_TILE + half * BM + q * 32;
-            const int64_t n0 = w.n * CE_TILE + cg * 128;
-            const int acc = (int)(it & 1);
-            const bool empty = w.kb0 == w.kb1;
-            float off = 0.0f, scale = 0.0f, tval = 0.0f, sum = 0.0f;
-            int t_rel = -1;
-            if (EPI <= EPI_PROB) {                   // the rows' numbers are fetched while the tile is being multiplied
-                off = args.off2[row_w + lane];
-                t_rel = args.tcol[row_w + lane] - args.v0 - (int)n0;
-                if (EPI == EPI_PROB) { scale = args.scale[row_w + lane]; tval = args.tval[row_w + lane]; }
+        // this warp's 32 rows x 128 columns of the next accumulator, which goes back to the MMA thread
+        auto drain = [&](float (&r)[128], int acc, uint32_t parity, bool add) {
+            if (!mbar_wait_warp<true>(smem_u32(&bar_tmem_full[acc]), parity, abortp)) {
+                raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_EPILOGUE);
+                ok = false;
+                return;
             }
-            if (!empty) {
-                if (!mbar_wait_warp<true>(smem_u32(&bar_tmem_full[acc]), (uint32_t)((it >> 1) & 1), abortp)) {
-                    raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_EPILOGUE);
-                    ok = false;
-                    break;
-                }
-                tc_fence_after_sync();
-            }
+            tc_fence_after_sync();
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * CE_TILE + cg * 128);
-            auto hand_back = [&]() {
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_remote(mapa(smem_u32(&bar_tmem_empty[acc]), leader_rank));
-            };
-            auto box_free = [&]() {                  // the last store from the staging box has read it
-                if (lane == 0) bulk_wait_group_read0();
-                __syncwarp();
-            };
-            if (EPI <= EPI_PROB) {
-#pragma unroll 1
-                for (int hb = 0; hb < 2; ++hb) {
-                    uint32_t r0[32], r1[32];
-                    tmem_ld_32x32(taddr + hb * 64, r0);
-                    tmem_ld_32x32(taddr + hb * 64 + 32, r1);
+            if (add) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t t[32];
+                    tmem_ld_32x32(taddr + b * 32, t);
                     tmem_ld_wait();
-                    if (hb == 1) hand_back();
-                    const int c0 = (int)n0 + hb * 64, tr = t_rel - hb * 64;
-                    float e[64];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        e[j] = ex2(__fmaf_rn(__uint_as_float(r0[j]), LOG2E, -off));
-                        e[32 + j] = ex2(__fmaf_rn(__uint_as_float(r1[j]), LOG2E, -off));
-                    }
-                    if (c0 + 64 > args.ncols) {
+                    for (int j = 0; j < 32; ++j) r[b * 32 + j] += __uint_as_float(t[j]);
+                }
+            } else {
+                uint32_t(&t)[128] = reinterpret_cast<uint32_t(&)[128]>(r);
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) e[j] = c0 + j < args.ncols ? e[j] : 0.0f;
-                    }
-                    if (EPI == EPI_PROB) {
+                for (int b = 0; b < 4; ++b) tmem_ld_32x32(taddr + b * 32, reinterpret_cast<uint32_t(&)[32]>(t[b * 32]));
+                tmem_ld_wait();
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(mapa(smem_u32(&bar_tmem_empty[acc]), leader_rank));
+        };
+        while (ok && walk.take(w)) {
+            const int64_t n0 = (int64_t)w.n * CE_TILE + cg * 128;
+#pragma unroll 1
+            for (int s = 0; s < MT && ok; ++s) {
+                const int64_t row_w = (int64_t)w.m * Cfg::ROWS + s * CE_TILE + half * BM + q * 32;
+                float off = 0.0f, scale = 0.0f, tval = 0.0f;
+                int t_rel = -1;
+                if (EPI <= EPI_PROB) {               // the rows' numbers are fetched while the tile is being multiplied
+                    off = args.off2[row_w + lane];
+                    t_rel = args.tcol[row_w + lane] - args.v0 - (int)n0;
+                    if (EPI == EPI_PROB) { scale = args.scale[row_w + lane]; tval = args.tval[row_w + lane]; }
+                }
+                float r[128];
+                if (EPI >= EPI_BF16 && w.kb0 == w.kb1) {   // nothing to contract
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) e[j] *= scale;
-                    }
-                    if (__any_sync(0xffffffffu, (unsigned)tr < 64u)) {      // a target among these columns: left out of the sum
-                        const float tv = EPI == EPI_PROB ? tval : 0.0f;
+                    for (int j = 0; j < 128; ++j) r[j] = 0.0f;
+                } else if (MT == 2) {
+                    drain(r, s, it & 1, false);
+                } else if (!ADD) {
+                    drain(r, (int)(it & 1), (it >> 1) & 1, false);
+                    ++it;
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) e[j] = j == tr ? tv : e[j];
-                    }
-                    if (EPI != EPI_PROB) {
-                        float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+                    for (int j = 0; j < 128; ++j) r[j] = 0.0f;
+                    for (int c0 = w.kb0; c0 < w.kb1 && ok; c0 += CE_CHUNK, ++it) drain(r, (int)(it & 1), (it >> 1) & 1, true);
+                }
+                if (!ok) break;
+                if (EPI <= EPI_PROB) {
+                    float sum = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 64; j += 4) { a0 += e[j]; a1 += e[j + 1]; a2 += e[j + 2]; a3 += e[j + 3]; }
-                        sum += (a0 + a1) + (a2 + a3);
-                    }
-                    if (EPI != EPI_SUM) {
+                    for (int hb = 0; hb < 2; ++hb) {
+                        float *e = r + hb * 64;
+                        const int c0 = (int)n0 + hb * 64, tr = t_rel - hb * 64;
 #pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            box_free();
+                        for (int j = 0; j < 64; ++j) e[j] = ex2(__fmaf_rn(e[j], LOG2E, -off));
+                        if (c0 + 64 > args.ncols) {
 #pragma unroll
-                            for (int ch = 0; ch < 8; ++ch) {
-                                uint32_t pk[4];
+                            for (int j = 0; j < 64; ++j) e[j] = c0 + j < args.ncols ? e[j] : 0.0f;
+                        }
+                        if (EPI == EPI_PROB) {
 #pragma unroll
-                                for (int x = 0; x < 4; ++x) {
-                                    const int j = ch * 8 + 2 * x;
-                                    __nv_bfloat162 h = __floats2bfloat162_rn(e[j], e[j + 1]);
-                                    pk[x] = *reinterpret_cast<uint32_t *>(&h);
-                                    if (p + 1 < PARTS) {
-                                        e[j] -= __low2float(h);
-                                        e[j + 1] -= __high2float(h);
-                                    }
+                            for (int j = 0; j < 64; ++j) e[j] *= scale;
+                        }
+                        if (__any_sync(0xffffffffu, (unsigned)tr < 64u)) {      // a target among these columns: left out of the sum
+                            const float tv = EPI == EPI_PROB ? tval : 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 64; ++j) e[j] = j == tr ? tv : e[j];
+                        }
+                        if (EPI != EPI_PROB) {
+                            float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 64; j += 4) { a0 += e[j]; a1 += e[j + 1]; a2 += e[j + 2]; a3 += e[j + 3]; }
+                            sum += (a0 + a1) + (a2 + a3);
+                        }
+                        if (EPI != EPI_SUM) {
+#pragma unroll
+                            for (int p = 0; p < PARTS; ++p) {
+                                box_free();
+                                stage_bf16(rowaddr, lane, e);
+                                if (p + 1 < PARTS) {
+#pragma unroll
+                                    for (int j = 0; j < 64; ++j) e[j] -= __bfloat162float(__float2bfloat16_rn(e[j]));
                                 }
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((ch ^ (lane & 7)) << 4)),
-                                             "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]) : "memory");
+                                if (lane == 0) {
+                                    tma_store_2d(&tmap_d, stag, p * args.part_cols + c0, (int32_t)row_w);
+                                    bulk_commit_group();
+                                }
                             }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) {
-                                tma_store_2d(&tmap_d, stag, p * args.part_cols + c0, (int32_t)row_w);
+                        }
+                    }
+                    if (EPI != EPI_PROB) args.partial[(w.n * 2 + cg) * args.ld_partial + row_w + lane] = sum;
+                } else if (EPI == EPI_BF16 && w.slot < 0) {
+#pragma unroll
+                    for (int hb = 0; hb < 2; ++hb) {
+                        box_free();
+                        stage_bf16(rowaddr, lane, r + hb * 64);
+                        const int64_t c0 = n0 + hb * 64;
+                        if (lane == 0 && row_w < rows && c0 < args.N) {
+                            tma_store_2d(&tmap_d, stag, (int32_t)c0, (int32_t)row_w);
+                            bulk_commit_group();
+                        }
+                    }
+                } else {
+                    // float32 boxes, to the output or to a slot
+#pragma unroll
+                    for (int cb = 0; cb < 4; ++cb) {
+                        box_free();
+                        stage_f32(rowaddr, lane, r + cb * 32);
+                        if (lane == 0) {
+                            const int64_t c0 = n0 + cb * 32;
+                            if (w.slot >= 0) {
+                                const int32_t x = cg * 128 + cb * 32, y = (int32_t)(w.slot * Cfg::ROWS + s * CE_TILE + half * BM + q * 32);
+                                if (EPI == EPI_SLOT && args.accumulate) tma_reduce_add_2d(&tmap_slot, stag, x, y);
+                                else tma_store_2d(&tmap_slot, stag, x, y);
+                                bulk_commit_group();
+                            } else if (c0 < args.N && row_w < rows) {
+                                tma_store_2d(&tmap_d, stag, (int32_t)c0, (int32_t)row_w);
                                 bulk_commit_group();
                             }
                         }
                     }
                 }
-                if (EPI != EPI_PROB) args.partial[(w.n * 2 + cg) * args.ld_partial + row_w + lane] = sum;
-            } else if (EPI == EPI_BF16) {
-#pragma unroll 1
-                for (int hb = 0; hb < 2; ++hb) {
-                    uint32_t r0[32], r1[32];
-                    if (!empty) {
-                        tmem_ld_32x32(taddr + hb * 64, r0);
-                        tmem_ld_32x32(taddr + hb * 64 + 32, r1);
-                        tmem_ld_wait();
-                        if (hb == 1) hand_back();
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r0[j] = r1[j] = 0u;
-                    }
-                    box_free();
-#pragma unroll
-                    for (int ch = 0; ch < 8; ++ch) {
-                        uint32_t pk[4];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int j = (ch & 3) * 8 + 2 * x;
-                            __nv_bfloat162 h = ch < 4 ? __floats2bfloat162_rn(__uint_as_float(r0[j]), __uint_as_float(r0[j + 1]))
-                                                      : __floats2bfloat162_rn(__uint_as_float(r1[j]), __uint_as_float(r1[j + 1]));
-                            pk[x] = *reinterpret_cast<uint32_t *>(&h);
-                        }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((ch ^ (lane & 7)) << 4)),
-                                     "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]) : "memory");
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        const int64_t c0 = n0 + hb * 64;
-                        if (row_w < rows && c0 < args.N) {
-                            tma_store_2d(&tmap_d, stag, (int32_t)c0, (int32_t)row_w);
-                            bulk_commit_group();
-                        }
-                    }
-                }
-            } else {
-                // float32: [32 rows x 32 columns] boxes
-#pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
-                    uint32_t r[32];
-                    if (!empty) {
-                        tmem_ld_32x32(taddr + cb * 32, r);
-                        tmem_ld_wait();
-                        if (cb == 3) hand_back();
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = 0u;
-                    }
-                    box_free();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((j ^ (lane & 7)) << 4)),
-                                     "r"(r[4 * j]), "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3]) : "memory");
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        const int64_t c0 = n0 + cb * 32;
-                        if (EPI == EPI_SLOT) {
-                            const int32_t x = cg * 128 + cb * 32, y = (int32_t)(w.slot * CE_TILE + half * BM + q * 32);
-                            if (args.accumulate) tma_reduce_add_2d(&tmap_d, stag, x, y);
-                            else tma_store_2d(&tmap_d, stag, x, y);
-                            bulk_commit_group();
-                        } else if (c0 < args.N && row_w < rows) {
-                            tma_store_2d(&tmap_d, stag, (int32_t)c0, (int32_t)row_w);
-                            bulk_commit_group();
-                        }
-                    }
-                }
             }
-            if (!empty) ++it;
+            if (MT == 2 && w.kb0 != w.kb1) ++it;
         }
         if (EPI != EPI_SUM && lane == 0) bulk_wait_group0();     // all output written before the CTA retires
     }
@@ -479,6 +570,24 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         tc_fence_after_sync();
         tmem_dealloc_pair(tmem_base, TMEM_COLS);
     }
+}
+
+// Output rows of the tiles whose contraction was cut (CeArgs::tail): their parts, added in order.
+template <typename T>
+__global__ void __launch_bounds__(CE_TILE) ce_tail_kernel(T *__restrict__ out, int64_t ldo, const float *__restrict__ slots, int64_t M, int64_t N,
+                                                          int64_t first, int parts, int tile_rows) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t tiles_n = (N + CE_TILE - 1) / CE_TILE;
+    const int64_t i = blockIdx.x / tile_rows, r = blockIdx.x % tile_rows;
+    const int64_t tile = first + i;
+    const int64_t row = tile / tiles_n * tile_rows + r, col = tile % tiles_n * CE_TILE + threadIdx.x;
+    if (row >= M || col >= N) return;
+    const float *p = slots + (i * parts * tile_rows + r) * CE_TILE + threadIdx.x;
+    float v = *p;
+#pragma unroll 4
+    for (int k = 1; k < parts; ++k) v += p[(int64_t)k * tile_rows * CE_TILE];
+    out[row * ldo + col] = from_f32<T>(v);
 }
 
 // ================================================================================================
@@ -580,6 +689,7 @@ struct CeRowArgs {
     const float *dloss;           // null: forward
     const float *lse, *loss;
     int reduction;
+    int tile_rows;
 };
 
 // eight consecutive elements, 16-byte aligned for bf16 and 32-byte for float32
@@ -621,7 +731,7 @@ template <typename T> __device__ __forceinline__ bool rows_aligned(const void *b
 }
 
 // One warp per gathered row: the row in bf16 parts, its target's logit (forward), or exponent offset, factor and target value of
-// the probabilities (backward).  Rows up to the next multiple of 256 are zeros that contribute nothing anywhere.
+// the probabilities (backward).  Rows up to the tile's end are zeros that contribute nothing anywhere.
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) {
     pdl_launch_dependents();
@@ -629,7 +739,7 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) 
     const int lane = threadIdx.x & 31;
     const int64_t j = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int64_t n = *a.count;
-    if (j >= (n + CE_TILE - 1) / CE_TILE * CE_TILE) return;
+    if (j >= (n + a.tile_rows - 1) / a.tile_rows * a.tile_rows) return;
     __nv_bfloat16 *dst = a.a + j * a.lda;
     if (j >= n) {
         for (int64_t c = lane * 8; c < a.lda; c += 256) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
@@ -745,16 +855,16 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ p
 struct SlotView {
     float *base;
     Cut cut;
-    int64_t panel, lo, hi;
-    int member;
-    __device__ __forceinline__ SlotView(float *slots, int64_t count, int64_t R, int KB, int pairs) : base(slots), cut(count, R, KB, pairs) {}
+    int panel, lo, hi, member, tile_rows;
+    __device__ __forceinline__ SlotView(float *slots, int64_t count, int64_t R, int KB, int pairs, int tile_rows_)
+        : base(slots), cut(count, R, KB, pairs, tile_rows_), tile_rows(tile_rows_) {}
     __device__ __forceinline__ void tile(int64_t m, int n) {
-        panel = m * cut.per_row + n / cut.size;
+        panel = (int)m * cut.per_row + n / cut.size;
         member = n % cut.size;
         lo = cut.owner(panel * cut.KB);
         hi = cut.owner((panel + 1) * cut.KB - 1);
     }
-    __device__ __forceinline__ float *at(int64_t g, int r, int c) const { return base + (cut.slot(panel, g, member) * CE_TILE + r) * CE_TILE + c; }
+    __device__ __forceinline__ float *at(int64_t g, int r, int c) const { return base + ((int64_t)cut.slot(panel, (int)g, member) * tile_rows + r) * CE_TILE + c; }
 };
 
 // Rows whose sum left float32's range: logits once more on CUDA cores, first the maximum and the sum relative to it, then (grad)
@@ -803,11 +913,11 @@ __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, 
             s_io[j] = -1.0f;
         }
         if (slots) {
-            SlotView o(slots, n, a.R, KB, pairs);
-            const int r = (int)(j % CE_TILE);
+            SlotView o(slots, n, a.R, KB, pairs, a.tile_rows);
+            const int r = (int)(j % a.tile_rows);
             const float pt = expf(lt - full);
             for (int nt = 0; nt < o.cut.tiles_n; ++nt) {          // columns of one tile at a time
-                o.tile(j / CE_TILE, nt);
+                o.tile(j / a.tile_rows, nt);
                 const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
                 const bool mine = threadIdx.x < CE_TILE && c < a.R;
                 float acc = mine ? (pt - 1.0f) * vocab_at<T>(voc, t, c) : 0.0f;
@@ -859,7 +969,7 @@ constexpr int DX_ROWS = 8;
 template <typename T>
 __global__ void __launch_bounds__(CE_TILE) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int32_t *__restrict__ map,
                                                     const int32_t *__restrict__ count, const float *__restrict__ s, const int32_t *__restrict__ tcol,
-                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int pairs, int tiles_n) {
+                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int pairs, int tile_rows, int tiles_n) {
     __shared__ const float *sh_at[DX_ROWS];
     __shared__ int sh_parts[DX_ROWS], sh_t[DX_ROWS];
     __shared__ float sh_s[DX_ROWS];
@@ -874,10 +984,10 @@ __global__ void __launch_bounds__(CE_TILE) ce_dx_kernel(T *__restrict__ dx, floa
         const int64_t j = i < T_rows ? map[i] : -1;
         int parts = 0;
         if (j >= 0) {
-            SlotView o(slots, *count, R, KB, pairs);
-            o.tile(j / CE_TILE, nt);
-            sh_at[threadIdx.x] = o.at(o.lo, (int)(j % CE_TILE), 0);
-            sh_step = (int64_t)o.cut.size * CE_TILE * CE_TILE;       // the same for every row
+            SlotView o(slots, *count, R, KB, pairs, tile_rows);
+            o.tile(j / tile_rows, nt);
+            sh_at[threadIdx.x] = o.at(o.lo, (int)(j % tile_rows), 0);
+            sh_step = (int64_t)o.cut.size * tile_rows * CE_TILE;     // the same for every row
             parts = (int)(o.hi - o.lo) + 1;
             if (s) {
                 sh_s[threadIdx.x] = s[j];
@@ -948,12 +1058,12 @@ struct CePlan {
     int64_t Mpad, Rp, lda;           // rows rounded to tiles; columns of one part, of all parts
     int64_t piece, npieces;          // vocabulary columns per piece (a multiple of 256), pieces
     bool stage_b;                    // the matrix goes through the workspace in bf16 parts
-    int pairs;
+    int pairs, tile_rows;
     int64_t slot_rows;               // rows of 256 float32 that the parts of the x-gradient take
     bool dw_direct;
     int64_t ld_dw;
     // workspace
-    size_t idx, map, count, off2, lt, scale, tval, tcol, s, far, a, b, e, partial, slots, dw, total;
+    size_t idx, map, count, off2, lt, scale, tval, tcol, s, far, a, b, e, partial, slots, dw, tail, total;
 };
 
 constexpr size_t E_BUDGET = 512ull << 20;
@@ -968,7 +1078,9 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     CePlan p{};
     p.parts = dtype == RDB_F32 ? 3 : 1;
     p.nterm = dtype == RDB_F32 ? 6 : 1;
-    p.Mpad = round_up(T, CE_TILE);
+    // 512-row tiles unless all rows fit 256 or the numbers are float32 (see the top)
+    p.tile_rows = p.parts == 3 || T <= CE_TILE ? CE_TILE : 2 * CE_TILE;
+    p.Mpad = round_up(T, p.tile_rows);
     p.Rp = round_up(R, p.parts == 3 ? 64 : 8);
     p.lda = p.Rp * p.parts;
     p.pairs = max_resident_pairs();
@@ -989,7 +1101,7 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     const int64_t per = cdiv64(vtiles, p.npieces);
     p.npieces = cdiv64(vtiles, per);
     p.piece = per * CE_TILE;
-    p.slot_rows = Cut(T, R, ce_kb(p), p.pairs).slots(p.pairs) * CE_TILE;
+    p.slot_rows = (int64_t)Cut(T, R, ce_kb(p), p.pairs, p.tile_rows).slots(p.pairs) * p.tile_rows;
     const size_t es = dtype_size(dtype);
     p.dw_direct = dw && (reinterpret_cast<uintptr_t>(dw) & 15) == 0 && (R * es) % 16 == 0;
     p.ld_dw = round_up(R, 8);
@@ -1011,6 +1123,7 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     p.partial = take(op != 2 ? (size_t)p.npieces * (p.piece / CE_TILE) * 2 * p.Mpad * 4 : 0);
     p.slots = take(op == 1 || (op == 2 && want_dx) ? (size_t)p.slot_rows * CE_TILE * 4 : 0);
     p.dw = take(op == 2 && want_dw && !p.dw_direct ? (size_t)p.piece * p.ld_dw * es : 0);
+    p.tail = take(op == 2 && want_dw ? (size_t)p.pairs * p.tile_rows * CE_TILE * 4 : 0);
     p.total = o;
     return p;
 }
@@ -1024,15 +1137,15 @@ static void ce_terms(CeArgs *a, int nterm, int64_t a_cols, int64_t b_cols) {
     }
 }
 
-template <int A_MN, int B_MN, int EPI, int PARTS>
-static int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &td, const CeArgs &args, int64_t max_items, int pairs,
-                       cudaStream_t st) {
-    auto kern = ce_pair_kernel<A_MN, B_MN, EPI, PARTS>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CE_SMEM);
+template <int A_MN, int B_MN, int EPI, int PARTS, int MT>
+static int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &td, const CUtensorMap &ts, const CeArgs &args,
+                       int64_t max_items, int pairs, cudaStream_t st) {
+    auto kern = ce_pair_kernel<A_MN, B_MN, EPI, PARTS, MT>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CeCfg<MT>::SMEM);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(CE_THREADS);
-    cfg.dynamicSmemBytes = CE_SMEM;
+    cfg.dynamicSmemBytes = CeCfg<MT>::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1045,7 +1158,7 @@ static int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUten
     cfg.numAttrs = 2;
     const int64_t n = max_items < pairs ? max_items : pairs;
     cfg.gridDim = dim3((unsigned)(2 * (n < 1 ? 1 : n)));
-    e = cudaLaunchKernelEx(&cfg, kern, ta, tb, td, args);
+    e = cudaLaunchKernelEx(&cfg, kern, ta, tb, td, ts, args);
     if (e != cudaSuccess) return (int)e;
     return launch_status();
 }
@@ -1081,6 +1194,7 @@ static CeRowArgs ce_row_args(const CeCall &c) {
     a.scale = c.at<float>(c.p.scale);
     a.tval = c.at<float>(c.p.tval);
     a.tcol = c.at<int32_t>(c.p.tcol);
+    a.tile_rows = c.p.tile_rows;
     return a;
 }
 
@@ -1141,9 +1255,10 @@ static int ce_logits(const CeCall &c, const void *b, int64_t ldb, int64_t v0, in
     a.ld_partial = p.Mpad;
     a.part_cols = (int)p.piece;
     a.status = c.status;
-    const int64_t items = (p.Mpad / CE_TILE) * cdiv64(a.N, CE_TILE);
-    if (p.parts == 3) return launch_pair<0, 0, EPI, 3>(ta, tb, td, a, items, p.pairs, c.st);
-    return launch_pair<0, 0, EPI, 1>(ta, tb, td, a, items, p.pairs, c.st);
+    const int64_t items = (p.Mpad / p.tile_rows) * cdiv64(a.N, CE_TILE);
+    if (p.parts == 3) return launch_pair<0, 0, EPI, 3, 1>(ta, tb, td, td, a, items, p.pairs, c.st);
+    if (p.tile_rows == CE_TILE) return launch_pair<0, 0, EPI, 1, 1>(ta, tb, td, td, a, items, p.pairs, c.st);
+    return launch_pair<0, 0, EPI, 1, 2>(ta, tb, td, td, a, items, p.pairs, c.st);
 }
 
 // slots (+)= E W_piece
@@ -1165,7 +1280,9 @@ static int ce_accumulate(const CeCall &c, const void *b, int64_t ldb, int64_t n,
     a.m_fast = 0;
     a.accumulate = add ? 1 : 0;
     a.status = c.status;
-    return launch_pair<0, 1, EPI_SLOT, 1>(ta, tb, td, a, p.pairs, p.pairs, c.st);
+    if (p.parts == 3) return launch_pair<0, 1, EPI_SLOT, 3, 1>(ta, tb, td, td, a, p.pairs, p.pairs, c.st);
+    if (p.tile_rows == CE_TILE) return launch_pair<0, 1, EPI_SLOT, 1, 1>(ta, tb, td, td, a, p.pairs, p.pairs, c.st);
+    return launch_pair<0, 1, EPI_SLOT, 1, 2>(ta, tb, td, td, a, p.pairs, p.pairs, c.st);
 }
 
 // dW rows [v0, v0 + n) = P^T x
@@ -1189,9 +1306,32 @@ static int ce_dw(const CeCall &c, void *dw, int64_t v0, int64_t n) {
     ce_terms(&a, p.nterm, p.piece, p.Rp);
     a.m_fast = 0;
     a.status = c.status;
-    const int64_t items = cdiv64(n, CE_TILE) * cdiv64(c.R, CE_TILE);
-    rc = c.dtype == RDB_F32 ? launch_pair<1, 1, EPI_F32, 1>(ta, tb, td, a, items, p.pairs, c.st)
-                            : launch_pair<1, 1, EPI_BF16, 1>(ta, tb, td, a, items, p.pairs, c.st);
+    // Tiles that do not fill the last round of pairs are cut along the contraction when two or more pairs can share each; their
+    // parts go through slots of their own.
+    const int tile_rows = p.tile_rows;
+    const int64_t tiles = cdiv64(n, tile_rows) * cdiv64(c.R, CE_TILE);
+    const int left = (int)(tiles % p.pairs);
+    const int64_t kb = a.nterm * cdiv64(c.T, BK);
+    a.tail_parts = 1;
+    if (left > 0 && p.pairs / left >= 2 && kb >= 8) {
+        int64_t parts = p.pairs / left;
+        if (parts > kb / 4) parts = kb / 4;
+        a.tail = left;
+        a.tail_parts = (int)parts;
+    }
+    CUtensorMap ts = td;
+    float *tail = c.at<float>(p.tail);
+    if (a.tail && (rc = make_tmap(&ts, tail, CE_TILE, (int64_t)p.pairs * tile_rows, CE_TILE, 32, 32, true))) return rc;
+    const int64_t items = tiles - a.tail + (int64_t)a.tail * a.tail_parts;
+    rc = c.dtype == RDB_F32 ? launch_pair<1, 1, EPI_F32, 3, 1>(ta, tb, td, ts, a, items, p.pairs, c.st)
+         : tile_rows == CE_TILE ? launch_pair<1, 1, EPI_BF16, 1, 1>(ta, tb, td, ts, a, items, p.pairs, c.st)
+                                : launch_pair<1, 1, EPI_BF16, 1, 2>(ta, tb, td, ts, a, items, p.pairs, c.st);
+    if (rc) return rc;
+    if (a.tail) {
+        const dim3 grid((unsigned)(a.tail * tile_rows));
+        rc = c.dtype == RDB_F32 ? launch_pdl(ce_tail_kernel<float>, grid, CE_TILE, 0, c.st, (float *)out, ldd, (const float *)tail, n, c.R, tiles - a.tail, a.tail_parts, tile_rows)
+                                : launch_pdl(ce_tail_kernel<__nv_bfloat16>, grid, CE_TILE, 0, c.st, (__nv_bfloat16 *)out, ldd, (const float *)tail, n, c.R, tiles - a.tail, a.tail_parts, tile_rows);
+    }
     if (rc || p.dw_direct) return rc;
     cudaError_t e = cudaMemcpy2DAsync(static_cast<uint8_t *>(dw) + (size_t)v0 * c.R * es, c.R * es, out, ldd * es, c.R * es, n, cudaMemcpyDeviceToDevice, c.st);
     return e == cudaSuccess ? RDB_OK : (int)e;
@@ -1204,17 +1344,18 @@ static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
     const int32_t *map = c.at<int32_t>(p.map), *count = c.at<int32_t>(p.count), *tcol = c.at<int32_t>(p.tcol);
     float *slots = c.at<float>(p.slots);
     if (c.dtype == RDB_F32)
-        return launch_pdl(ce_dx_kernel<float>, grid, CE_TILE, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs, (int)cdiv64(c.R, CE_TILE));
+        return launch_pdl(ce_dx_kernel<float>, grid, CE_TILE, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs, p.tile_rows, (int)cdiv64(c.R, CE_TILE));
     return launch_pdl(ce_dx_kernel<__nv_bfloat16>, grid, CE_TILE, 0, c.st, (__nv_bfloat16 *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs,
-                      (int)cdiv64(c.R, CE_TILE));
+                      p.tile_rows, (int)cdiv64(c.R, CE_TILE));
 }
 
 static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w, int64_t ldw, int dtype, int reduction) {
     if (T < 0 || R < 1 || V < 1 || ldx < R || (w && ldw < R)) return RDB_ERR_SHAPE;
     if (dtype != RDB_F32 && dtype != RDB_BF16) return RDB_ERR_DTYPE;
     if (reduction != RDB_CE_NONE && reduction != RDB_CE_MEAN && reduction != RDB_CE_SUM) return RDB_ERR_UNSUPPORTED;
-    // coordinates of the tiled copies are 32-bit
-    if (T > (1LL << 28) || V > (1LL << 30) || R > (1LL << 24)) return RDB_ERR_TOO_LARGE;
+    // coordinates of the tiled copies and counts of tiles and k-blocks are 32-bit
+    if (T > (1LL << 28) || V > (1LL << 30) || R > (1LL << 20) || (double)T * (double)R > (double)(1LL << 36) || (double)T * (double)V > (double)(1LL << 45))
+        return RDB_ERR_TOO_LARGE;
     return RDB_OK;
 }
 
