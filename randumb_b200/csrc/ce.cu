@@ -184,17 +184,18 @@ struct Walk {
     }
 };
 
-// 32 rows x 64 bf16 columns of a warp, from registers through the swizzled staging box
-__device__ __forceinline__ void stage_bf16(uint32_t rowaddr, int lane, const float *v) {
+// 32 rows x 32 bf16 columns of a warp, from registers into a 2 KB staging box of 64-byte rows (the tiled copy's 64-byte swizzle:
+// 16-byte piece p of row r goes to p ^ ((r >> 1) & 3), which spreads eight lanes over all banks)
+__device__ __forceinline__ void stage_bf16(uint32_t box, int lane, const float *v) {
 #pragma unroll
-    for (int ch = 0; ch < 8; ++ch) {
+    for (int ch = 0; ch < 4; ++ch) {
         uint32_t pk[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const __nv_bfloat162 h = __floats2bfloat162_rn(v[ch * 8 + 2 * x], v[ch * 8 + 2 * x + 1]);
             pk[x] = *reinterpret_cast<const uint32_t *>(&h);
         }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (uint32_t)((ch ^ (lane & 7)) << 4)), "r"(pk[0]), "r"(pk[1]),
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + (uint32_t)lane * 64u + (((uint32_t)ch ^ (((uint32_t)lane >> 1) & 3u)) << 4)), "r"(pk[0]), "r"(pk[1]),
                      "r"(pk[2]), "r"(pk[3]) : "memory");
     }
     fence_proxy_async_smem();
@@ -425,6 +426,14 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             if (lane == 0) bulk_wait_group_read0();
             __syncwarp();
         };
+        // bf16: the box is two halves in turn, one being filled while the other is read; a group per use, empty or not
+        uint32_t turn = 0;
+        auto next_half = [&]() {
+            if (lane == 0) bulk_wait_group_read1();
+            __syncwarp();
+            turn ^= 2048u;
+            return stag + turn;
+        };
         uint32_t it = 0;
         bool ok = true;
         // this warp's 32 rows x 128 columns of the next accumulator, which goes back to the MMA thread
@@ -512,15 +521,18 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                         if (EPI != EPI_SUM) {
 #pragma unroll
                             for (int p = 0; p < PARTS; ++p) {
-                                box_free();
-                                stage_bf16(rowaddr, lane, e);
-                                if (p + 1 < PARTS) {
 #pragma unroll
-                                    for (int j = 0; j < 64; ++j) e[j] -= __bfloat162float(__float2bfloat16_rn(e[j]));
-                                }
-                                if (lane == 0) {
-                                    tma_store_2d(&tmap_d, stag, p * args.part_cols + c0, (int32_t)row_w);
-                                    bulk_commit_group();
+                                for (int b = 0; b < 2; ++b) {
+                                    const uint32_t box = next_half();
+                                    stage_bf16(box, lane, e + b * 32);
+                                    if (p + 1 < PARTS) {
+#pragma unroll
+                                        for (int j = b * 32; j < b * 32 + 32; ++j) e[j] -= __bfloat162float(__float2bfloat16_rn(e[j]));
+                                    }
+                                    if (lane == 0) {
+                                        tma_store_2d(&tmap_d, box, p * args.part_cols + c0 + b * 32, (int32_t)row_w);
+                                        bulk_commit_group();
+                                    }
                                 }
                             }
                         }
@@ -528,12 +540,12 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                     if (EPI != EPI_PROB) args.partial[(w.n * 2 + cg) * args.ld_partial + row_w + lane] = sum;
                 } else if (EPI == EPI_BF16 && w.slot < 0) {
 #pragma unroll
-                    for (int hb = 0; hb < 2; ++hb) {
-                        box_free();
-                        stage_bf16(rowaddr, lane, r + hb * 64);
-                        const int64_t c0 = n0 + hb * 64;
-                        if (lane == 0 && row_w < rows && c0 < args.N) {
-                            tma_store_2d(&tmap_d, stag, (int32_t)c0, (int32_t)row_w);
+                    for (int cb = 0; cb < 4; ++cb) {
+                        const uint32_t box = next_half();
+                        stage_bf16(box, lane, r + cb * 32);
+                        const int64_t c0 = n0 + cb * 32;
+                        if (lane == 0) {
+                            if (row_w < rows && c0 < args.N) tma_store_2d(&tmap_d, box, (int32_t)c0, (int32_t)row_w);
                             bulk_commit_group();
                         }
                     }
@@ -1235,7 +1247,7 @@ static int ce_logits(const CeCall &c, const void *b, int64_t ldb, int64_t v0, in
     td = ta;
     CeArgs a{};
     if (EPI != EPI_SUM) {
-        rc = make_tmap(&td, c.at<void>(p.e), p.piece * p.parts, p.Mpad, p.piece * p.parts, 64, 32);
+        rc = make_tmap(&td, c.at<void>(p.e), p.piece * p.parts, p.Mpad, p.piece * p.parts, 32, 32, false, CU_TENSOR_MAP_SWIZZLE_64B);
         if (rc) return rc;
     }
     a.count = c.at<int32_t>(p.count);
@@ -1296,7 +1308,7 @@ static int ce_dw(const CeCall &c, void *dw, int64_t v0, int64_t n) {
     if (rc) return rc;
     rc = make_tmap(&tb, c.at<void>(p.a), p.parts == 1 ? c.R : p.lda, p.Mpad, p.lda, 64, BK);
     if (rc) return rc;
-    rc = c.dtype == RDB_F32 ? make_tmap(&td, out, c.R, n, ldd, 32, 32, true) : make_tmap(&td, out, c.R, n, ldd, 64, 32);
+    rc = c.dtype == RDB_F32 ? make_tmap(&td, out, c.R, n, ldd, 32, 32, true) : make_tmap(&td, out, c.R, n, ldd, 32, 32, false, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
     CeArgs a{};
     a.count = c.at<int32_t>(p.count);

@@ -1473,7 +1473,7 @@ static void ensure_context() {
 
 // bf16 matrix with `inner` contiguous elements per row, `outer` rows, row pitch ld elements.
 int make_tmap(CUtensorMap *m, const void *base, int64_t inner, int64_t outer, int64_t ld, uint32_t box_inner,
-                     uint32_t box_outer, bool f32) {
+                     uint32_t box_outer, bool f32, CUtensorMapSwizzle swizzle) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return RDB_ERR_DRIVER;
     ensure_context();
@@ -1482,7 +1482,7 @@ int make_tmap(CUtensorMap *m, const void *base, int64_t inner, int64_t outer, in
     cuuint32_t box[2] = {box_inner, box_outer};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         if (getenv("RDB_DEBUG"))

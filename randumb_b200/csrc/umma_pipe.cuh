@@ -26,9 +26,10 @@ __device__ __forceinline__ void raise_abort(volatile int *abort_flag, int32_t *s
 }
 
 // ---- implemented in umma_gemm.cu ----------------------------------------------------------------
-// bf16 (or float32) matrix with `inner` contiguous elements per row, `outer` rows, row pitch ld elements, 128-byte swizzle
+// bf16 (or float32) matrix with `inner` contiguous elements per row, `outer` rows, row pitch ld elements.  A row of a box takes the
+// swizzle's width in shared memory: boxes are 128 bytes wide, or 64 with the 64-byte swizzle.
 int make_tmap(CUtensorMap *m, const void *base, int64_t inner, int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer,
-              bool f32 = false);
+              bool f32 = false, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 int max_resident_pairs();          // CTA pairs (one CTA per SM) that can be resident at once
 int sm_count();
 
