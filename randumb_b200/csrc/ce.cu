@@ -85,6 +85,27 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// L2 policies: what is read again soon (rows, the piece of the matrix) should outlive what streams past (E and P, several hundred MB)
+__device__ __forceinline__ uint64_t l2_keep() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t l2_stream() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void tma_load_pair_hint(uint32_t smem_dst, const CUtensorMap *m, uint32_t cluster_bar, int32_t x, int32_t y, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+        ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(cluster_bar), "r"(x), "r"(y), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store_hint(const CUtensorMap *m, uint32_t smem_src, int32_t x, int32_t y, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;"
+                 ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_src), "r"(x), "r"(y), "l"(policy) : "memory");
+}
 __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *m, uint32_t smem_src, int32_t x, int32_t y) {
     asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
                  ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_src), "r"(x), "r"(y) : "memory");
@@ -270,6 +291,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         if (lane == 0) {
             prefetch_tmap(&tmap_a);
             prefetch_tmap(&tmap_b);
+            const uint64_t pol_a = EPI <= EPI_PROB ? l2_keep() : l2_stream(), pol_b = EPI <= EPI_PROB ? l2_stream() : l2_keep();
             PipeState st;
             bool ok = true;
             while (ok && walk.take(w)) {
@@ -291,16 +313,16 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                         if (A_MN) {
 #pragma unroll
                             for (int i = 0; i < BM / 64; ++i)
-                                tma_load_2d_pair(sa + s * SUB_BYTES + i * (64 * BK * 2), &tmap_a, fb, ax + m0 + s * CE_TILE + i * 64, k0);
+                                tma_load_pair_hint(sa + s * SUB_BYTES + i * (64 * BK * 2), &tmap_a, fb, ax + m0 + s * CE_TILE + i * 64, k0, pol_a);
                         } else {
-                            tma_load_2d_pair(sa + s * SUB_BYTES, &tmap_a, fb, ax + k0, m0 + s * CE_TILE);
+                            tma_load_pair_hint(sa + s * SUB_BYTES, &tmap_a, fb, ax + k0, m0 + s * CE_TILE, pol_a);
                         }
                     }
                     if (B_MN) {
 #pragma unroll
-                        for (int i = 0; i < BM / 64; ++i) tma_load_2d_pair(sb + i * (64 * BK * 2), &tmap_b, fb, bx + n0 + i * 64, k0);
+                        for (int i = 0; i < BM / 64; ++i) tma_load_pair_hint(sb + i * (64 * BK * 2), &tmap_b, fb, bx + n0 + i * 64, k0, pol_b);
                     } else {
-                        tma_load_2d_pair(sb, &tmap_b, fb, bx + k0, n0);
+                        tma_load_pair_hint(sb, &tmap_b, fb, bx + k0, n0, pol_b);
                     }
                     st.advance<STAGES>();
                     if (++kk == kbs) { kk = 0; ++term; }
@@ -434,6 +456,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             turn ^= 2048u;
             return stag + turn;
         };
+        const uint64_t pol_e = l2_stream();
         uint32_t it = 0;
         bool ok = true;
         // this warp's 32 rows x 128 columns of the next accumulator, which goes back to the MMA thread
@@ -530,7 +553,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                                         for (int j = b * 32; j < b * 32 + 32; ++j) e[j] -= __bfloat162float(__float2bfloat16_rn(e[j]));
                                     }
                                     if (lane == 0) {
-                                        tma_store_2d(&tmap_d, box, p * args.part_cols + c0 + b * 32, (int32_t)row_w);
+                                        tma_store_hint(&tmap_d, box, p * args.part_cols + c0 + b * 32, (int32_t)row_w, pol_e);
                                         bulk_commit_group();
                                     }
                                 }
