@@ -127,12 +127,8 @@ struct Cut {
         tiles_n = (int)((cols + CE_TILE - 1) / CE_TILE);
         per_row = (tiles_n + 7) / 8;
         size = (tiles_n + per_row - 1) / per_row;
-        if (size > pairs) {
-            size = pairs;
-            per_row = (tiles_n + size - 1) / size;
-        }
         total = (int)((rows + tile_rows - 1) / tile_rows) * per_row * KB;
-        groups = pairs / size;
+        groups = pairs / size;      // pairs >= 8: every part of this GPU that the kernels run on has 16 SMs or more (ce_check)
         if (groups > total / 4) groups = total / 4 < 1 ? 1 : total / 4;
     }
     __host__ __device__ __forceinline__ int begin(int g) const { return (int)((int64_t)total * g / groups); }
@@ -633,7 +629,8 @@ __global__ void __launch_bounds__(CE_TILE) ce_tail_kernel(T *__restrict__ out, i
 __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict__ target, int64_t T, int64_t ignore, int use_ignore,
                                                        int32_t *__restrict__ idx, int32_t *__restrict__ map, int32_t *__restrict__ count,
                                                        float *__restrict__ zero_a, float *__restrict__ zero_b, float *__restrict__ zero_c,
-                                                       float *__restrict__ count_f, int32_t *__restrict__ far) {
+                                                       float *__restrict__ count_f, int32_t *__restrict__ far, int2 *__restrict__ parts,
+                                                       int64_t cols, int KB, int pairs, int tile_rows) {
     constexpr int PER = 8;
     __shared__ int warp_sum[2][32];
     pdl_launch_dependents();
@@ -641,25 +638,18 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int base = 0, turn = 0;
     for (int64_t b = 0; b < T; b += 1024 * PER, turn ^= 1) {
-        const int64_t i0 = b + threadIdx.x * PER;
+        const int64_t i0 = b + warp * (32 * PER) + lane;        // a warp takes 256 rows in a stretch, a lane every 32nd
         int64_t t[PER];
+        unsigned keep[PER];
         int n = 0;
-        unsigned keep = 0;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) t[k] = i0 + k < T ? target[i0 + k] : 0;
+        for (int k = 0; k < PER; ++k) t[k] = i0 + k * 32 < T ? target[i0 + k * 32] : 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            const bool ok = i0 + k < T && !(use_ignore && t[k] == ignore);
-            keep |= (unsigned)ok << k;
-            n += ok;
+            keep[k] = __ballot_sync(0xffffffffu, i0 + k * 32 < T && !(use_ignore && t[k] == ignore));
+            n += __popc(keep[k]);
         }
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
-        }
-        if (lane == 31) warp_sum[turn][warp] = incl;
+        if (lane == 0) warp_sum[turn][warp] = n;
         __syncthreads();
         int ws = warp_sum[turn][lane];               // every warp scans the warps' sums itself
 #pragma unroll
@@ -667,20 +657,33 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict
             const int y = __shfl_up_sync(0xffffffffu, ws, o);
             if (lane >= o) ws += y;
         }
-        const int before = warp ? __shfl_sync(0xffffffffu, ws, warp - 1) : 0;
-        int at = base + before + incl - n;
+        const int before = __shfl_sync(0xffffffffu, ws, warp) - n;
+        int at = base + before;
         base += __shfl_sync(0xffffffffu, ws, 31);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            if (i0 + k >= T) break;
-            const bool ok = (keep >> k) & 1u;
-            map[i0 + k] = ok ? at : -1;
-            if (ok) idx[at++] = (int32_t)(i0 + k);
-            else {
-                if (zero_a) zero_a[i0 + k] = 0.0f;
-                if (zero_b) zero_b[i0 + k] = 0.0f;
-                if (zero_c) zero_c[i0 + k] = 0.0f;
+            const int64_t i = i0 + k * 32;
+            const int j = at + __popc(keep[k] & ((1u << lane) - 1u));
+            at += __popc(keep[k]);
+            if (i < T) {
+                const bool ok = (keep[k] >> lane) & 1u;
+                map[i] = ok ? j : -1;
+                if (ok) idx[j] = (int32_t)i;
+                else {
+                    if (zero_a) zero_a[i] = 0.0f;
+                    if (zero_b) zero_b[i] = 0.0f;
+                    if (zero_c) zero_c[i] = 0.0f;
+                }
             }
+        }
+    }
+    // where the parts of each panel of the x-gradient begin and how many there are, for the kernels that add them
+    if (parts) {
+        const Cut cut(base, cols, KB, pairs, tile_rows);
+        const int panels = (base + tile_rows - 1) / tile_rows * cut.per_row;
+        for (int p = threadIdx.x; p < panels; p += 1024) {
+            const int lo = cut.owner(p * KB);
+            parts[p] = make_int2(lo, cut.owner((p + 1) * KB - 1) - lo + 1);
         }
     }
     if (threadIdx.x == 0) {
@@ -854,12 +857,12 @@ __global__ void __launch_bounds__(256) ce_split_kernel(__nv_bfloat16 *__restrict
 // ================================================================================================
 // finishing
 // ================================================================================================
-// s of 32 rows per block: eight threads per row add every eighth partial sum, then the eight are added in order.
-__global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ partial, int64_t ld, int nparts, const int32_t *__restrict__ idx,
+// s of 32 rows per block: sixteen threads per row add every sixteenth partial sum, then the sixteen are added in order.
+__global__ void __launch_bounds__(512) ce_sum_kernel(const float *__restrict__ partial, int64_t ld, int nparts, const int32_t *__restrict__ idx,
                                                      const int32_t *__restrict__ count, const float *__restrict__ lt, float *__restrict__ s_out,
                                                      float *__restrict__ lse, float *__restrict__ loss, float *__restrict__ loss2,
                                                      int32_t *__restrict__ far) {
-    __shared__ float sh[8][33];
+    __shared__ float sh[16][33];
     pdl_launch_dependents();
     pdl_wait();
     const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
@@ -868,14 +871,14 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ p
     float a = 0.0f;
     if (j < n) {
 #pragma unroll 8
-        for (int p = g; p < nparts; p += 8) a += partial[(int64_t)p * ld + j];
+        for (int p = g; p < nparts; p += 16) a += partial[(int64_t)p * ld + j];
     }
     sh[g][r] = a;
     __syncthreads();
     if (g == 0 && j < n) {
         float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s += sh[k][r];
+        for (int k = 0; k < 16; ++k) s += sh[k][r];
         const float l = log1pf(s);
         s_out[j] = s;
         const int32_t row = idx[j];
@@ -886,20 +889,19 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float *__restrict__ p
     }
 }
 
-// The parts of a row tile's column tile n of the x-gradient: first() .. last() groups, row r and column c of the k-th at at(..).
-struct SlotView {
-    float *base;
-    Cut cut;
-    int panel, lo, hi, member, tile_rows;
-    __device__ __forceinline__ SlotView(float *slots, int64_t count, int64_t R, int KB, int pairs, int tile_rows_)
-        : base(slots), cut(count, R, KB, pairs, tile_rows_), tile_rows(tile_rows_) {}
-    __device__ __forceinline__ void tile(int64_t m, int n) {
-        panel = (int)m * cut.per_row + n / cut.size;
-        member = n % cut.size;
-        lo = cut.owner(panel * cut.KB);
-        hi = cut.owner((panel + 1) * cut.KB - 1);
+// The parts of row j, column tile n of the x-gradient: `first` is column 0 of the first part, `step` elements lie between the parts.
+struct SlotRow {
+    float *first;
+    int64_t step;
+    int n;
+    __device__ __forceinline__ SlotRow(float *slots, const int2 *parts, int tiles_n, int tile_rows, int64_t j, int nt) {
+        const int per_row = (tiles_n + 7) / 8, size = (tiles_n + per_row - 1) / per_row;      // as Cut has them
+        const int m = (int)j / tile_rows, panel = m * per_row + nt / size;
+        const int2 p = parts[panel];
+        first = slots + (((int64_t)(panel + p.x) * size + nt % size) * tile_rows + (j - (int64_t)m * tile_rows)) * CE_TILE;
+        step = (int64_t)size * tile_rows * CE_TILE;
+        n = p.y;
     }
-    __device__ __forceinline__ float *at(int64_t g, int r, int c) const { return base + ((int64_t)cut.slot(panel, (int)g, member) * tile_rows + r) * CE_TILE + c; }
 };
 
 // Rows whose sum left float32's range: logits once more on CUDA cores, first the maximum and the sum relative to it, then (grad)
@@ -907,13 +909,12 @@ struct SlotView {
 // far[0] rows, listed behind it.
 template <typename T>
 __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, float *__restrict__ s_io, float *__restrict__ lse,
-                                                        float *__restrict__ loss, float *__restrict__ loss2, float *__restrict__ slots, int KB, int pairs,
+                                                        float *__restrict__ loss, float *__restrict__ loss2, float *__restrict__ slots, const int2 *__restrict__ parts,
                                                         const int32_t *__restrict__ far) {
     __shared__ float sh_m[16], sh_s[16], sh_p[16];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t n = *a.count;
     const int nfar = far[0];
     for (int i = blockIdx.x; i < nfar; i += gridDim.x) {
         const int64_t j = far[1 + i];
@@ -948,11 +949,10 @@ __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, 
             s_io[j] = -1.0f;
         }
         if (slots) {
-            SlotView o(slots, n, a.R, KB, pairs, a.tile_rows);
-            const int r = (int)(j % a.tile_rows);
+            const int tiles_n = (int)((a.R + CE_TILE - 1) / CE_TILE);
             const float pt = expf(lt - full);
-            for (int nt = 0; nt < o.cut.tiles_n; ++nt) {          // columns of one tile at a time
-                o.tile(j / a.tile_rows, nt);
+            for (int nt = 0; nt < tiles_n; ++nt) {                // columns of one tile at a time
+                const SlotRow o(slots, parts, tiles_n, a.tile_rows, j, nt);
                 const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
                 const bool mine = threadIdx.x < CE_TILE && c < a.R;
                 float acc = mine ? (pt - 1.0f) * vocab_at<T>(voc, t, c) : 0.0f;
@@ -969,7 +969,7 @@ __global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, 
                     }
                     __syncthreads();
                 }
-                if (mine) *o.at(o.lo, r, threadIdx.x) = acc;
+                if (mine) o.first[threadIdx.x] = acc;
             }
         }
         __syncthreads();
@@ -999,57 +999,98 @@ __global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__
 
 // x's gradient from the slots: their sum, finished with s and the target's row (noise: voc.w null and s given), written to the
 // rows' own places; zeros at ignored rows.
-// A block takes DX_ROWS rows of one column tile, a thread one column; what concerns a row is worked out once, by one thread.
-constexpr int DX_ROWS = 8;
-template <typename T>
-__global__ void __launch_bounds__(CE_TILE) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int32_t *__restrict__ map,
-                                                    const int32_t *__restrict__ count, const float *__restrict__ s, const int32_t *__restrict__ tcol,
-                                                    Vocab voc, int64_t T_rows, int64_t R, int KB, int pairs, int tile_rows, int tiles_n) {
-    __shared__ const float *sh_at[DX_ROWS];
-    __shared__ int sh_parts[DX_ROWS], sh_t[DX_ROWS];
-    __shared__ float sh_s[DX_ROWS];
+// A block takes ROWS rows of one column tile, a thread four columns of every fourth row; what concerns a row is worked out once, by
+// one thread.
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&f)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+__device__ __forceinline__ void store4(float *p, const float (&f)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int2 *__restrict__ parts,
+                                                       const int32_t *__restrict__ map, const float *__restrict__ s, const int32_t *__restrict__ tcol,
+                                                       Vocab voc, int64_t T_rows, int64_t R, int tile_rows, int tiles_n) {
+    __shared__ const float *sh_at[ROWS];
+    __shared__ int sh_parts[ROWS];
+    __shared__ uint32_t sh_hash[ROWS];             // noise word position of the target's row, column 0
+    __shared__ float sh_s[ROWS], sh_inv[ROWS];  // v -> (v - s w_t) inv
     __shared__ int64_t sh_step;
     pdl_launch_dependents();
     pdl_wait();
     const int nt = (int)(blockIdx.x % (unsigned)tiles_n);
-    const int64_t i0 = (int64_t)(blockIdx.x / (unsigned)tiles_n) * DX_ROWS;
-    const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
-    if (threadIdx.x < DX_ROWS) {
+    const int64_t i0 = (int64_t)(blockIdx.x / (unsigned)tiles_n) * ROWS;
+    if (threadIdx.x < ROWS) {
         const int64_t i = i0 + threadIdx.x;
         const int64_t j = i < T_rows ? map[i] : -1;
-        int parts = 0;
+        int n = 0;
+        float sj = 0.0f, inv = 1.0f;
         if (j >= 0) {
-            SlotView o(slots, *count, R, KB, pairs, tile_rows);
-            o.tile(j / tile_rows, nt);
-            sh_at[threadIdx.x] = o.at(o.lo, (int)(j % tile_rows), 0);
-            sh_step = (int64_t)o.cut.size * tile_rows * CE_TILE;     // the same for every row
-            parts = (int)(o.hi - o.lo) + 1;
+            const SlotRow o(slots, parts, tiles_n, tile_rows, j, nt);
+            sh_at[threadIdx.x] = o.first;
+            sh_step = o.step;                         // the same for every row
+            n = o.n;
             if (s) {
-                sh_s[threadIdx.x] = s[j];
-                sh_t[threadIdx.x] = tcol[j];
-                if (s[j] < 0.0f) parts = -1;          // the row was finished by ce_rescue_kernel
+                sj = s[j];
+                const int32_t t = tcol[j];
+                if (sj < 0.0f) {                      // the row was finished by ce_rescue_kernel
+                    n = 1;
+                    sj = 0.0f;
+                } else {
+                    inv = t >= 0 ? 1.0f / (1.0f + sj) : NAN;
+                }
+                sh_hash[threadIdx.x] = sq5_lin_rows(voc.seed, voc.row0 + (uint32_t)t, 0u).base;
             }
         }
-        sh_parts[threadIdx.x] = parts;
+        sh_s[threadIdx.x] = sj;
+        sh_inv[threadIdx.x] = inv;
+        sh_parts[threadIdx.x] = n;
     }
     __syncthreads();
+    const int cl = (threadIdx.x & 63) * 4;
+    const int64_t c = (int64_t)nt * CE_TILE + cl;
     if (c >= R) return;
+    const bool vec = R % 4 == 0 && (reinterpret_cast<uintptr_t>(dx) & (4 * sizeof(T) - 1)) == 0;
+    float4 v[ROWS / 4];
+    int most = 0;
 #pragma unroll
-    for (int k = 0; k < DX_ROWS; ++k) {
-        const int64_t i = i0 + k;
-        if (i >= T_rows) return;
-        const int parts = sh_parts[k];
-        float v = 0.0f;
-        if (parts != 0) {
-            const float *at = sh_at[k] + threadIdx.x;
-            v = *at;
-            for (int g = 1; g < parts; ++g) v += at[g * sh_step];
-            if (s && parts > 0) {
-                const float sj = sh_s[k];
-                v = sh_t[k] >= 0 ? (v - sj * vocab_at<T>(voc, sh_t[k], c)) / (1.0f + sj) : NAN;
+    for (int q = 0; q < ROWS / 4; ++q) {
+        const int k = (threadIdx.x >> 6) + 4 * q;
+        v[q] = sh_parts[k] ? *reinterpret_cast<const float4 *>(sh_at[k] + cl) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        most = sh_parts[k] > most ? sh_parts[k] : most;
+    }
+#pragma unroll(ROWS == 4 ? 8 : 1)
+    for (int g = 1; g < most; ++g) {
+        const int64_t off = g * sh_step + cl;
+#pragma unroll
+        for (int q = 0; q < ROWS / 4; ++q) {
+            const int k = (threadIdx.x >> 6) + 4 * q;
+            if (g < sh_parts[k]) {
+                const float4 u = *reinterpret_cast<const float4 *>(sh_at[k] + off);
+                v[q].x += u.x; v[q].y += u.y; v[q].z += u.z; v[q].w += u.w;
             }
         }
-        dx[i * R + c] = from_f32<T>(v);
+    }
+#pragma unroll
+    for (int q = 0; q < ROWS / 4; ++q) {
+        const int k = (threadIdx.x >> 6) + 4 * q;
+        const int64_t i = i0 + k;
+        if (i >= T_rows) return;
+        float f[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+        if (s && sh_parts[k]) {
+            const float sj = sh_s[k], inv = sh_inv[k];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float w = to_f32<T>(from_f32<T>(sq5_to_float(sq5_tail(sh_hash[k] + (uint32_t)(c + e) * SQ5_N1))));
+                f[e] = (f[e] - sj * w) * inv;
+            }
+        }
+        T *out = dx + i * R + c;
+        if (vec) store4(out, f);
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < R) out[e] = from_f32<T>(f[e]);
+        }
     }
 }
 
@@ -1098,7 +1139,8 @@ struct CePlan {
     bool dw_direct;
     int64_t ld_dw;
     // workspace
-    size_t idx, map, count, off2, lt, scale, tval, tcol, s, far, a, b, e, partial, slots, dw, tail, total;
+    size_t idx, map, count, off2, lt, scale, tval, tcol, s, far, a, b, e, partial, slots, parts_at, dw, tail, total;
+    bool slots_used;
 };
 
 constexpr size_t E_BUDGET = 512ull << 20;
@@ -1156,7 +1198,9 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     p.b = take(p.stage_b ? (size_t)p.piece * p.lda * 2 : 0);
     p.e = take(op != 0 ? (size_t)p.Mpad * p.piece * p.parts * 2 : 0);
     p.partial = take(op != 2 ? (size_t)p.npieces * (p.piece / CE_TILE) * 2 * p.Mpad * 4 : 0);
-    p.slots = take(op == 1 || (op == 2 && want_dx) ? (size_t)p.slot_rows * CE_TILE * 4 : 0);
+    p.slots_used = op == 1 || (op == 2 && want_dx);
+    p.slots = take(p.slots_used ? (size_t)p.slot_rows * CE_TILE * 4 : 0);
+    p.parts_at = take(p.slots_used ? (size_t)(p.Mpad / p.tile_rows) * cdiv64(cdiv64(R, CE_TILE), 8) * 8 : 0);
     p.dw = take(op == 2 && want_dw && !p.dw_direct ? (size_t)p.piece * p.ld_dw * es : 0);
     p.tail = take(op == 2 && want_dw ? (size_t)p.pairs * p.tile_rows * CE_TILE * 4 : 0);
     p.total = o;
@@ -1213,7 +1257,8 @@ struct CeCall {
 
 static int ce_find_rows(const CeCall &c, int64_t ignore, int use_ignore, float *zero_a, float *zero_b, float *zero_c, float *count_f) {
     return launch_pdl(ce_rows_kernel, dim3(1), 1024, 0, c.st, c.target, c.T, ignore, use_ignore, c.at<int32_t>(c.p.idx), c.at<int32_t>(c.p.map),
-                      c.at<int32_t>(c.p.count), zero_a, zero_b, zero_c, count_f, c.at<int32_t>(c.p.far));
+                      c.at<int32_t>(c.p.count), zero_a, zero_b, zero_c, count_f, c.at<int32_t>(c.p.far), c.p.slots_used ? c.at<int2>(c.p.parts_at) : (int2 *)nullptr, c.R, ce_kb(c.p),
+                      c.p.pairs, c.p.tile_rows);
 }
 
 static CeRowArgs ce_row_args(const CeCall &c) {
@@ -1374,14 +1419,19 @@ static int ce_dw(const CeCall &c, void *dw, int64_t v0, int64_t n) {
 
 static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
     const CePlan &p = c.p;
-    const dim3 grid((unsigned)(cdiv64(c.T, DX_ROWS) * cdiv64(c.R, CE_TILE)));
+    const int tiles_n = (int)cdiv64(c.R, CE_TILE);
     const float *s = unit ? c.at<float>(p.s) : nullptr;
-    const int32_t *map = c.at<int32_t>(p.map), *count = c.at<int32_t>(p.count), *tcol = c.at<int32_t>(p.tcol);
+    const int32_t *map = c.at<int32_t>(p.map), *tcol = c.at<int32_t>(p.tcol);
+    const int2 *parts = c.at<int2>(p.parts_at);
     float *slots = c.at<float>(p.slots);
-    if (c.dtype == RDB_F32)
-        return launch_pdl(ce_dx_kernel<float>, grid, CE_TILE, 0, c.st, (float *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs, p.tile_rows, (int)cdiv64(c.R, CE_TILE));
-    return launch_pdl(ce_dx_kernel<__nv_bfloat16>, grid, CE_TILE, 0, c.st, (__nv_bfloat16 *)dx, slots, map, count, s, tcol, c.voc, c.T, c.R, ce_kb(p), p.pairs,
-                      p.tile_rows, (int)cdiv64(c.R, CE_TILE));
+    // few rows have many parts each and are bound by latency: four rows per block then (1531 rows of 200: 12 against 24 us)
+    const int rows = cdiv64(c.T, 16) * tiles_n >= 4 * 148 ? 16 : 4;
+    const dim3 grid((unsigned)(cdiv64(c.T, rows) * tiles_n));
+    auto go = [&](auto kern, auto *out) {
+        return launch_pdl(kern, grid, CE_TILE, 0, c.st, out, slots, parts, map, s, tcol, c.voc, c.T, c.R, p.tile_rows, tiles_n);
+    };
+    if (c.dtype == RDB_F32) return rows == 16 ? go(ce_dx_kernel<float, 16>, (float *)dx) : go(ce_dx_kernel<float, 4>, (float *)dx);
+    return rows == 16 ? go(ce_dx_kernel<__nv_bfloat16, 16>, (__nv_bfloat16 *)dx) : go(ce_dx_kernel<__nv_bfloat16, 4>, (__nv_bfloat16 *)dx);
 }
 
 static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w, int64_t ldw, int dtype, int reduction) {
@@ -1391,6 +1441,7 @@ static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w,
     // coordinates of the tiled copies and counts of tiles and k-blocks are 32-bit
     if (T > (1LL << 28) || V > (1LL << 30) || R > (1LL << 20) || (double)T * (double)R > (double)(1LL << 36) || (double)T * (double)V > (double)(1LL << 45))
         return RDB_ERR_TOO_LARGE;
+    if (max_resident_pairs() < 8) return RDB_ERR_UNSUPPORTED;      // the x-gradient's groups have up to eight pairs
     return RDB_OK;
 }
 
@@ -1444,13 +1495,13 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x,
         const int64_t last = V - (c.p.npieces - 1) * c.p.piece;
         int32_t *far = c.at<int32_t>(c.p.far);
         const int nparts = (int)((c.p.npieces - 1) * (c.p.piece / CE_TILE) * 2 + (dx_unit ? c.p.piece / CE_TILE : cdiv64(last, CE_TILE)) * 2);
-        rc = launch_pdl(ce_sum_kernel, dim3((unsigned)(c.p.Mpad / 32)), 256, 0, c.st, (const float *)c.at<float>(c.p.partial), c.p.Mpad, nparts, ra.idx,
+        rc = launch_pdl(ce_sum_kernel, dim3((unsigned)(c.p.Mpad / 32)), 512, 0, c.st, (const float *)c.at<float>(c.p.partial), c.p.Mpad, nparts, ra.idx,
                         ra.count, (const float *)ra.lt, c.at<float>(c.p.s), lse, rows, rows2, far);
         if (rc) return rc;
         float *slots = dx_unit ? c.at<float>(c.p.slots) : nullptr, *sums = c.at<float>(c.p.s);
-        const int pairs = c.p.pairs;
-        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, ce_kb(c.p), pairs, (const int32_t *)far)
-                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, ce_kb(c.p), pairs, (const int32_t *)far);
+        const int2 *parts = c.at<int2>(c.p.parts_at);
+        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, parts, (const int32_t *)far)
+                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, parts, (const int32_t *)far);
         if (rc) return rc;
         if (dx_unit && (rc = ce_finish_dx(c, dx_unit, true))) return rc;
     }
