@@ -429,10 +429,10 @@ int rdb_gemm_dense_scatter(void *const *dst_ptrs, int ndst, size_t dst_offset_by
  * train_gpt2.py:354-372).  For every element, with t the tensor's step count after this call has raised it by one:
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2          g: gradient times *grad_scale (1 when null)
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in float32.  `tensors` and `h` are HOST memory, read before the call returns; the pointers in them (`step`: the tensor's
+ * in float32.  `lists` and `h` are HOST memory, read before the call returns; the pointers in them (`step`: the tensor's
  * float32 count), `grad_scale` and `h->lr_dev` (one float32 each, may be null) are device memory, read and written on `stream`
  * only, so a captured call replays with new gradients, counts and learning rates.
- *   param_dtype   RDB_F32, or RDB_BF16 (rounded to nearest after each step; with `master` set -- for all tensors or none --
+ *   param_dtype   RDB_F32, or RDB_BF16 (rounded to nearest after each step; with the `master` list
  *                 the float32 master copy is what is updated and the parameter receives its rounding)
  *   grad_dtype    RDB_F32 or RDB_BF16, one type for all tensors
  *   state_bits    32: exp_avg and exp_avg_sq are float32.
@@ -449,23 +449,24 @@ int rdb_gemm_dense_scatter(void *const *dst_ptrs, int ndst, size_t dst_offset_by
  */
 #define RDB_ADAMW_BLOCK 256
 #define RDB_NORM_BLOCKS 1184
-typedef struct rdb_adamw_tensor {
-    void *param;
-    const void *grad;
-    float *master;
-    void *exp_avg;
-    void *exp_avg_sq;
-    float *exp_avg_scale;
-    float *exp_avg_sq_scale;
-    float *step;
-    int64_t numel;
-} rdb_adamw_tensor;
+typedef struct rdb_adamw_lists {      /* HOST arrays of n entries each; a list that does not apply is NULL */
+    void *const *param;
+    const void *const *grad;
+    void *const *exp_avg;
+    void *const *exp_avg_sq;
+    float *const *step;
+    const int64_t *numel;
+    float *const *master;
+    float *const *exp_avg_scale;
+    float *const *exp_avg_sq_scale;
+    int64_t n;
+} rdb_adamw_lists;
 typedef struct rdb_adamw_hyper {
     double lr, beta1, beta2, eps, weight_decay;
     const float *lr_dev;      /* not null: read instead of lr */
     uint32_t seed;
 } rdb_adamw_hyper;
-int rdb_adamw_step(const rdb_adamw_tensor *tensors, int n, int param_dtype, int grad_dtype, int state_bits,
+int rdb_adamw_step(const rdb_adamw_lists *lists, int param_dtype, int grad_dtype, int state_bits,
                    const rdb_adamw_hyper *h, const float *grad_scale, void *stream);
 size_t rdb_grad_norm_workspace_bytes(int n);
 int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int64_t *numels, const int32_t *dtypes, int n, float max_norm,

@@ -49,7 +49,12 @@ class AdamwHyper(ctypes.Structure):
                 ("weight_decay", ctypes.c_double), ("lr_dev", ctypes.c_void_p), ("seed", ctypes.c_uint32)]
 
 
-ADAMW_WORDS = 9            # rdb_adamw_tensor: eight pointers and an int64, nine 8-byte words
+class AdamwLists(ctypes.Structure):
+    """``rdb_adamw_lists``: addresses of host arrays."""
+    _fields_ = [(k, ctypes.c_void_p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "step", "numel", "master", "exp_avg_scale", "exp_avg_sq_scale")] \
+        + [("n", ctypes.c_int64)]
+
+
 ADAMW_BLOCK = 256          # RDB_ADAMW_BLOCK
 
 _op = ctypes.POINTER(CallOptions)
@@ -99,7 +104,7 @@ PROTOTYPES = {
     "rdb_scale_bias_bwd_workspace_bytes": (_sz, [_i64]),
     "rdb_scale_bias_bwd": (_i32, [_vp, _vp, _vp, _i64, _u32, _vp]),
     "rdb_embed_fwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _u32, _vp]),
-    "rdb_adamw_step": (_i32, [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(AdamwHyper), _vp, _vp]),
+    "rdb_adamw_step": (_i32, [ctypes.POINTER(AdamwLists), _i32, _i32, _i32, ctypes.POINTER(AdamwHyper), _vp, _vp]),
     "rdb_grad_norm_workspace_bytes": (_sz, [_i32]),
     "rdb_grad_norm": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, ctypes.c_float, _vp, _sz, _vp]),
     "rdb_ce_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64, _i32, _vp, _i64]),

@@ -29,6 +29,7 @@
 // second is still being read.  (256 x 256 tiles, whose MMAs all go to one accumulator, kept the tensor pipe 62 % busy.)  At most 256
 // rows: 256 x 256 tiles, six 32 KB stages.  float32: the same, and the accumulators, whose additions cut instead of rounding (about
 // 2^-26 of the sum per 16 products, all in one direction), are added up in the epilogue's registers every eight k-blocks.
+#include <atomic>
 #include <cmath>
 
 #include "umma.cuh"
@@ -1220,8 +1221,15 @@ template <int A_MN, int B_MN, int EPI, int PARTS, int MT>
 static int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &td, const CUtensorMap &ts, const CeArgs &args,
                        int64_t max_items, int pairs, cudaStream_t st) {
     auto kern = ce_pair_kernel<A_MN, B_MN, EPI, PARTS, MT>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CeCfg<MT>::SMEM);
+    static std::atomic<uint64_t> prepared{0};          // devices on which the kernel may use its shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
+    if (dev >= 64 || !((prepared.load() >> dev) & 1)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CeCfg<MT>::SMEM);
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) prepared.fetch_or(1ull << dev);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(CE_THREADS);
     cfg.dynamicSmemBytes = CeCfg<MT>::SMEM;

@@ -335,12 +335,11 @@ constexpr int NT_SMALL = 48, NT_LARGE = 384;      // tensors per launch: 3.5 KB 
 static_assert(sizeof(AdamwTable<NT_LARGE>) + 512 < 32764, "kernel parameters");
 
 template <int NT>
-static int fill_table(AdamwTable<NT> *tab, const rdb_adamw_tensor *t, int n, int index0) {
+static int count_chunks(AdamwTable<NT> *tab, int n, int index0) {
     uint64_t c = 0;
     for (int i = 0; i < n; ++i) {
-        tab->t[i] = AdamwDesc{t[i].param, t[i].grad, t[i].master, t[i].exp_avg, t[i].exp_avg_sq, t[i].exp_avg_scale, t[i].exp_avg_sq_scale, t[i].step, t[i].numel};
         tab->first[i] = (uint32_t)c;
-        c += (uint64_t)cdiv64(t[i].numel, ADAMW_CHUNK);
+        c += (uint64_t)cdiv64(tab->t[i].n, ADAMW_CHUNK);
         if (c >= (1ull << 32)) return RDB_ERR_TOO_LARGE;
     }
     tab->first[n] = (uint32_t)c;
@@ -350,12 +349,17 @@ static int fill_table(AdamwTable<NT> *tab, const rdb_adamw_tensor *t, int n, int
 }
 
 template <typename P, typename G, bool MASTER, bool BITS8, int NT>
-static int launch_adamw(const rdb_adamw_tensor *t, int n, int index0, const AdamwScalars &s, const float *gs, cudaStream_t st) {
+static int launch_adamw(const rdb_adamw_lists &l, int n, int at, const AdamwScalars &s, const float *gs, cudaStream_t st) {
     AdamwTable<NT> tab;
     StepTable<NT> steps;
-    int rc = fill_table(&tab, t, n, index0);
+    for (int i = 0; i < n; ++i) {
+        const int k = at + i;
+        tab.t[i] = AdamwDesc{l.param[k], l.grad[k], MASTER ? l.master[k] : nullptr, l.exp_avg[k], l.exp_avg_sq[k], BITS8 ? l.exp_avg_scale[k] : nullptr,
+                             BITS8 ? l.exp_avg_sq_scale[k] : nullptr, l.step[k], l.numel[k]};
+        steps.step[i] = l.step[k];
+    }
+    int rc = count_chunks(&tab, n, at);
     if (rc) return rc;
-    for (int i = 0; i < n; ++i) steps.step[i] = t[i].step;
     steps.count = n;
     rc = launch_pdl(adamw_count_kernel<NT>, dim3(1), 256, 0, st, steps);
     if (rc) return rc;
@@ -366,21 +370,32 @@ static int launch_adamw(const rdb_adamw_tensor *t, int n, int index0, const Adam
 }
 
 template <typename P, typename G, bool MASTER, bool BITS8>
-static int adamw_all(const rdb_adamw_tensor *t, int n, const AdamwScalars &s, const float *gs, cudaStream_t st) {
+static int adamw_all(const rdb_adamw_lists &l, const AdamwScalars &s, const float *gs, cudaStream_t st) {
+    const int n = (int)l.n;
     for (int i = 0; i < n;) {
         const int k = n - i < NT_LARGE ? n - i : NT_LARGE;
-        const int rc = k <= NT_SMALL ? launch_adamw<P, G, MASTER, BITS8, NT_SMALL>(t + i, k, i, s, gs, st)
-                                     : launch_adamw<P, G, MASTER, BITS8, NT_LARGE>(t + i, k, i, s, gs, st);
+        const int rc = k <= NT_SMALL ? launch_adamw<P, G, MASTER, BITS8, NT_SMALL>(l, k, i, s, gs, st)
+                                     : launch_adamw<P, G, MASTER, BITS8, NT_LARGE>(l, k, i, s, gs, st);
         if (rc) return rc;
         i += k;
     }
     return RDB_OK;
 }
 
+struct GradRef {
+    const void *p;
+    int64_t n;
+};
+
 template <typename G, int NT>
-static int launch_sumsq(const rdb_adamw_tensor *t, int n, double *partial, int *used, cudaStream_t st) {
+static int launch_sumsq(const GradRef *t, int n, double *partial, int *used, cudaStream_t st) {
     AdamwTable<NT> tab;
-    int rc = fill_table(&tab, t, n, 0);
+    for (int i = 0; i < n; ++i) {
+        tab.t[i] = AdamwDesc{};
+        tab.t[i].g = t[i].p;
+        tab.t[i].n = t[i].n;
+    }
+    int rc = count_chunks(&tab, n, 0);
     if (rc) return rc;
     *used = norm_blocks(tab.first[n]);
     return launch_pdl(sumsq_kernel<G, NT>, dim3(*used), ADAMW_THREADS, 0, st, tab, partial);
@@ -390,27 +405,30 @@ static int launch_sumsq(const rdb_adamw_tensor *t, int n, double *partial, int *
 
 using namespace rdb;
 
-extern "C" int rdb_adamw_step(const rdb_adamw_tensor *tensors, int n, int param_dtype, int grad_dtype, int state_bits,
-                              const rdb_adamw_hyper *h, const float *grad_scale, void *stream) {
-    if (n < 0 || !h) return n < 0 ? RDB_ERR_SHAPE : RDB_ERR_NULL;
-    if (n == 0) return RDB_OK;
-    if (!tensors) return RDB_ERR_NULL;
+extern "C" int rdb_adamw_step(const rdb_adamw_lists *lists, int param_dtype, int grad_dtype, int state_bits, const rdb_adamw_hyper *h,
+                              const float *grad_scale, void *stream) {
+    if (!lists || !h) return RDB_ERR_NULL;
+    const rdb_adamw_lists &l = *lists;
+    if (l.n < 0) return RDB_ERR_SHAPE;
+    if (l.n == 0) return RDB_OK;
+    if (l.n > (1 << 30)) return RDB_ERR_TOO_LARGE;
+    if (!l.param || !l.grad || !l.exp_avg || !l.exp_avg_sq || !l.step || !l.numel) return RDB_ERR_NULL;
     if ((param_dtype != RDB_F32 && param_dtype != RDB_BF16) || (grad_dtype != RDB_F32 && grad_dtype != RDB_BF16)) return RDB_ERR_DTYPE;
     if (state_bits != 32 && state_bits != 8) return RDB_ERR_DTYPE;
+    if (state_bits == 8 && (!l.exp_avg_scale || !l.exp_avg_sq_scale)) return RDB_ERR_NULL;
     if (!(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0) || !(h->eps >= 0.0)) return RDB_ERR_UNSUPPORTED;
-    bool master = false;
-    for (int i = 0; i < n; ++i) master = master || tensors[i].master != nullptr;
-    for (int i = 0; i < n; ++i) {
-        const rdb_adamw_tensor &t = tensors[i];
-        if (t.numel < 0) return RDB_ERR_SHAPE;
-        if (!t.step) return RDB_ERR_NULL;
-        if (t.numel == 0) continue;
-        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return RDB_ERR_NULL;
-        if (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return RDB_ERR_NULL;
-        if ((t.master != nullptr) != master || (master && param_dtype != RDB_BF16)) return RDB_ERR_UNSUPPORTED;
-        const uintptr_t pm = dtype_size(param_dtype) - 1, gm = dtype_size(grad_dtype) - 1, sm = state_bits == 8 ? 0 : 3;
-        if ((reinterpret_cast<uintptr_t>(t.param) & pm) || (reinterpret_cast<uintptr_t>(t.grad) & gm) || (reinterpret_cast<uintptr_t>(t.exp_avg) & sm) ||
-            (reinterpret_cast<uintptr_t>(t.exp_avg_sq) & sm) || (reinterpret_cast<uintptr_t>(t.master) & 3))
+    const bool master = l.master != nullptr;
+    if (master && param_dtype != RDB_BF16) return RDB_ERR_UNSUPPORTED;
+    const uintptr_t pm = dtype_size(param_dtype) - 1, gm = dtype_size(grad_dtype) - 1, sm = state_bits == 8 ? 0 : 3;
+    for (int64_t i = 0; i < l.n; ++i) {
+        if (l.numel[i] < 0) return RDB_ERR_SHAPE;
+        if (!l.step[i]) return RDB_ERR_NULL;
+        if (l.numel[i] == 0) continue;
+        if (!l.param[i] || !l.grad[i] || !l.exp_avg[i] || !l.exp_avg_sq[i] || (master && !l.master[i])) return RDB_ERR_NULL;
+        if (state_bits == 8 && (!l.exp_avg_scale[i] || !l.exp_avg_sq_scale[i])) return RDB_ERR_NULL;
+        if ((reinterpret_cast<uintptr_t>(l.param[i]) & pm) || (reinterpret_cast<uintptr_t>(l.grad[i]) & gm) || (reinterpret_cast<uintptr_t>(l.exp_avg[i]) & sm) ||
+            (reinterpret_cast<uintptr_t>(l.exp_avg_sq[i]) & sm) || (master && (reinterpret_cast<uintptr_t>(l.master[i]) & 3)) ||
+            (reinterpret_cast<uintptr_t>(l.step[i]) & 3))
             return RDB_ERR_ALIGN;
     }
     cudaStream_t st = (cudaStream_t)stream;
@@ -427,7 +445,7 @@ extern "C" int rdb_adamw_step(const rdb_adamw_tensor *tensors, int n, int param_
     s.weight_decay = h->weight_decay;
     s.seed = h->seed;
     const bool b8 = state_bits == 8;
-#define RDB_ADAMW(P, G, M) (b8 ? adamw_all<P, G, M, true>(tensors, n, s, grad_scale, st) : adamw_all<P, G, M, false>(tensors, n, s, grad_scale, st))
+#define RDB_ADAMW(P, G, M) (b8 ? adamw_all<P, G, M, true>(l, s, grad_scale, st) : adamw_all<P, G, M, false>(l, s, grad_scale, st))
     if (param_dtype == RDB_F32) return grad_dtype == RDB_F32 ? RDB_ADAMW(float, float, false) : RDB_ADAMW(float, __nv_bfloat16, false);
     if (master) return grad_dtype == RDB_F32 ? RDB_ADAMW(__nv_bfloat16, float, true) : RDB_ADAMW(__nv_bfloat16, __nv_bfloat16, true);
     return grad_dtype == RDB_F32 ? RDB_ADAMW(__nv_bfloat16, float, false) : RDB_ADAMW(__nv_bfloat16, __nv_bfloat16, false);
@@ -455,7 +473,7 @@ extern "C" int rdb_grad_norm(float *norm, float *coef, const void *const *grads,
     cudaStream_t st = (cudaStream_t)stream;
     double *partial = reinterpret_cast<double *>(workspace);
     int filled = 0;
-    rdb_adamw_tensor part[NT_LARGE];
+    GradRef part[NT_LARGE];
     for (int dtype = RDB_F32; dtype <= RDB_BF16; ++dtype) {       // one launch holds gradients of one type
         int k = 0;
         for (int i = 0; i <= n; ++i) {
@@ -473,9 +491,7 @@ extern "C" int rdb_grad_norm(float *norm, float *coef, const void *const *grads,
                 k = 0;
             }
             if (i < n) {
-                part[k] = rdb_adamw_tensor{};
-                part[k].grad = grads[i];
-                part[k++].numel = numels[i];
+                part[k++] = GradRef{grads[i], numels[i]};
             }
         }
     }

@@ -5,6 +5,7 @@ All functions require CUDA tensors and raise ``RuntimeError`` otherwise -- there
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional, Tuple
 
@@ -43,6 +44,19 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream of device ``index`` without building a Stream object (2 us, as much as a small call's launch)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(index: int):
+    """``torch.cuda.device(index)``, or nothing when that device is the current one."""
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def _seed(seed: int) -> int:
@@ -443,12 +457,12 @@ def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor
     aux = torch.empty((2 * T + 1,), dtype=torch.float32, device=dev)
     loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
     unit = torch.empty((T, R), dtype=x.dtype, device=dev) if need_unit else None
-    with torch.cuda.device(dev):
+    with _on(dev.index):
         ldw = _pitch(weight) if weight is not None else 0
         ws = _workspace(L.rdb_ce_workspace_bytes(_lib.CE_LOSS_GRAD if need_unit else _lib.CE_LOSS, T, R, V, dt, _ptr(weight), ldw), dev)
         rc = L.rdb_ce_fwd(_ptr(loss), _ptr(aux), _ptr(unit), _ptr(x), _pitch(x), _ptr(weight), ldw, _ptr(target), _ptr(ws), ws.numel(), T, R, V, row0,
                           _seed(seed), 0 if ignore_index is None else int(ignore_index), 0 if ignore_index is None else 1, dt, red,
-                          _ptr(status_buffer(dev)), _stream(dev))
+                          _ptr(status_buffer(dev)), _raw_stream(dev.index))
     _lib.check(rc, "rdb_ce_fwd")
     return loss, aux, unit
 
@@ -459,8 +473,8 @@ def ce_scale(unit: torch.Tensor, dloss: torch.Tensor, aux: torch.Tensor, reducti
     dloss = dloss.contiguous()
     T, R = unit.shape
     dz = torch.empty_like(unit)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().rdb_ce_scale(_ptr(dz), _ptr(unit), _ptr(dloss), _ptr(aux), T, R, _dt(unit.dtype), _lib.CE_REDUCTIONS[reduction], _stream(dev))
+    with _on(dev.index):
+        rc = _lib.lib().rdb_ce_scale(_ptr(dz), _ptr(unit), _ptr(dloss), _ptr(aux), T, R, _dt(unit.dtype), _lib.CE_REDUCTIONS[reduction], _raw_stream(dev.index))
     _lib.check(rc, "rdb_ce_scale")
     return dz
 
@@ -477,11 +491,11 @@ def ce_bwd(dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: t
     L = _lib.lib()
     dx = torch.empty((T, R), dtype=x.dtype, device=dev) if need_dx else None
     dw = torch.empty((V, R), dtype=x.dtype, device=dev) if need_dw else None
-    with torch.cuda.device(dev):
+    with _on(dev.index):
         ws = _workspace(L.rdb_ce_workspace_bytes(_lib.CE_GRADS, T, R, V, dt, _ptr(weight), _pitch(weight)), dev)
         rc = L.rdb_ce_bwd(_ptr(dx), _ptr(dw), _ptr(dloss), _ptr(x), _pitch(x), _ptr(weight), _pitch(weight), _ptr(target), _ptr(aux), _ptr(ws),
                           ws.numel(), T, R, V, 0 if ignore_index is None else int(ignore_index), 0 if ignore_index is None else 1, dt, red,
-                          _ptr(status_buffer(dev)), _stream(dev))
+                          _ptr(status_buffer(dev)), _raw_stream(dev.index))
     _lib.check(rc, "rdb_ce_bwd")
     return dx, dw
 

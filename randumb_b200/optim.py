@@ -10,6 +10,7 @@ All tensors must be CUDA tensors: there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -20,17 +21,22 @@ from . import kernels as K
 BLOCK = _lib.ADAMW_BLOCK
 
 
-def _uniform(what: str, ts: Sequence[torch.Tensor], dtypes, n: int, dev: torch.device) -> torch.dtype:
+def _uniform(what: str, ts: Sequence[torch.Tensor], dtypes, n: int, dev: int) -> torch.dtype:
+    """The one type of a list of n contiguous CUDA tensors on device ``dev``; raises otherwise."""
     if len(ts) != n:
         raise RuntimeError(f"adamw_step: {n} params but {len(ts)} {what}")
     kinds = {t.dtype for t in ts}
-    if len(kinds) != 1 or next(iter(kinds)) not in dtypes:
+    kind = next(iter(kinds))
+    if len(kinds) != 1 or kind not in dtypes:
         raise RuntimeError(f"adamw_step: {what} must all have one type out of {sorted(str(d) for d in dtypes)}, got {sorted(str(d) for d in kinds)}")
-    if {t.device for t in ts} != {dev}:
-        raise RuntimeError(f"adamw_step: {what} must live on {dev}")
-    if not all([t.is_contiguous() for t in ts]):
+    if {t.get_device() for t in ts} != {dev}:
+        raise RuntimeError(f"adamw_step: {what} must live on cuda:{dev}")
+    if False in [t.is_contiguous() for t in ts]:
         raise RuntimeError(f"adamw_step: {what} must be contiguous")
-    return next(iter(kinds))
+    return kind
+
+
+_PARAM, _GRAD, _F32, _E4M3, _U8 = (torch.float32, torch.bfloat16), (torch.float32, torch.bfloat16), (torch.float32,), (torch.float8_e4m3fn,), (torch.uint8,)
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
@@ -54,62 +60,71 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     n = len(params)
     if n == 0:
         return
-    dev = K._need_cuda(*params)
-    pd = _uniform("params", params, (torch.float32, torch.bfloat16), n, dev)
-    gd = _uniform("grads", grads, (torch.float32, torch.bfloat16), n, dev)
+    dev = params[0].get_device()
+    if dev < 0:
+        raise RuntimeError("randumb_b200 kernels run on CUDA tensors only (no CPU implementation)")
+    pd = _uniform("params", params, _PARAM, n, dev)
+    gd = _uniform("grads", grads, _GRAD, n, dev)
     eight = exp_avg_scales is not None or exp_avg_sq_scales is not None
-    if eight:
-        if exp_avg_scales is None or exp_avg_sq_scales is None:
-            raise RuntimeError("adamw_step: 8-bit moments need exp_avg_scales and exp_avg_sq_scales")
-        _uniform("exp_avg_scales", exp_avg_scales, (torch.float32,), n, dev)
-        _uniform("exp_avg_sq_scales", exp_avg_sq_scales, (torch.float32,), n, dev)
-    _uniform("exp_avgs", exp_avgs, (torch.float8_e4m3fn,) if eight else (torch.float32,), n, dev)
-    _uniform("exp_avg_sqs", exp_avg_sqs, (torch.uint8,) if eight else (torch.float32,), n, dev)
+    if eight and (exp_avg_scales is None or exp_avg_sq_scales is None):
+        raise RuntimeError("adamw_step: 8-bit moments need exp_avg_scales and exp_avg_sq_scales")
+    _uniform("exp_avgs", exp_avgs, _E4M3 if eight else _F32, n, dev)
+    _uniform("exp_avg_sqs", exp_avg_sqs, _U8 if eight else _F32, n, dev)
+    numels = [t.numel() for t in params]
+    lists = [params, grads, exp_avgs, exp_avg_sqs]
+    names = ["param", "grad", "exp_avg", "exp_avg_sq"]
     if masters is not None:
-        _uniform("masters", masters, (torch.float32,), n, dev)
+        _uniform("masters", masters, _F32, n, dev)
         if pd != torch.bfloat16:
             raise RuntimeError("adamw_step: masters are the float32 copies of bfloat16 params")
-    numels = [t.numel() for t in params]
-    for what, ts in (("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs), ("masters", masters)):
-        if ts is not None and [t.numel() for t in ts] != numels:
-            raise RuntimeError(f"adamw_step: {what} and params differ in size")
+        lists.append(masters)
+        names.append("master")
+    for what, ts in zip(names[1:], lists[1:]):
+        if [t.numel() for t in ts] != numels:
+            raise RuntimeError(f"adamw_step: {what}s and params differ in size")
     if eight:
         blocks = [-(-k // BLOCK) for k in numels]
-        if [t.numel() for t in exp_avg_scales] != blocks or [t.numel() for t in exp_avg_sq_scales] != blocks:
-            raise RuntimeError(f"adamw_step: scales hold one value per {BLOCK} elements of their tensor")
+        for what, ts in (("exp_avg_scale", exp_avg_scales), ("exp_avg_sq_scale", exp_avg_sq_scales)):
+            _uniform(what + "s", ts, _F32, n, dev)
+            if [t.numel() for t in ts] != blocks:
+                raise RuntimeError(f"adamw_step: scales hold one value per {BLOCK} elements of their tensor")
+            lists.append(ts)
+            names.append(what)
     if isinstance(steps, torch.Tensor):
-        if steps.dtype != torch.float32 or steps.device != dev or steps.numel() != n or not steps.is_contiguous():
-            raise RuntimeError(f"adamw_step: steps must be {n} contiguous float32 counts on {dev}")
-        sp = range(steps.data_ptr(), steps.data_ptr() + 4 * n, 4)
+        if steps.dtype != torch.float32 or steps.get_device() != dev or steps.numel() != n or not steps.is_contiguous():
+            raise RuntimeError(f"adamw_step: steps must be {n} contiguous float32 counts on cuda:{dev}")
+        at = steps.data_ptr()
+        sp = list(range(at, at + 4 * n, 4))
     else:
-        _uniform("steps", steps, (torch.float32,), n, dev)
+        _uniform("steps", steps, _F32, n, dev)
         if any([t.numel() != 1 for t in steps]):
             raise RuntimeError("adamw_step: every tensor has one step count")
         sp = [t.data_ptr() for t in steps]
-    pp = [t.data_ptr() for t in params]
-    if len(set(pp)) != n and len({a for a, k in zip(pp, numels) if k}) != sum(1 for k in numels if k):
-        raise RuntimeError("adamw_step: a param is in the list twice")
     _one_float("grad_scale", grad_scale, dev)
     lr_dev = None
     if isinstance(lr, torch.Tensor):
         _one_float("lr", lr, dev)
         lr, lr_dev = 0.0, lr.data_ptr()
-    none = [0] * n
-    cols = (pp, [t.data_ptr() for t in grads], [t.data_ptr() for t in masters] if masters is not None else none,
-            [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
-            [t.data_ptr() for t in exp_avg_scales] if eight else none, [t.data_ptr() for t in exp_avg_sq_scales] if eight else none, sp, numels)
-    words = (ctypes.c_uint64 * (_lib.ADAMW_WORDS * n))()
-    for i, col in enumerate(cols):
-        words[i::_lib.ADAMW_WORDS] = col
+    words = [t.data_ptr() for t in params]
+    if len(set(words)) != n and len({a for a, k in zip(words, numels) if k}) != sum(1 for k in numels if k):
+        raise RuntimeError("adamw_step: a param is in the list twice")
+    for ts in lists[1:]:
+        words += [t.data_ptr() for t in ts]
+    words += sp
+    words += numels
+    table = array("Q", words)                              # one list behind the other, in host memory
+    base = table.buffer_info()[0]
+    arg = _lib.AdamwLists(n=n, **{name: base + 8 * n * i for i, name in enumerate(names + ["step", "numel"])})
     h = _lib.AdamwHyper(float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), lr_dev, K._seed(seed))
-    with torch.cuda.device(dev):
-        rc = _lib.lib().rdb_adamw_step(words, n, K._dt(pd), K._dt(gd), 8 if eight else 32, ctypes.byref(h), K._ptr(grad_scale), K._stream(dev))
+    with K._on(dev):
+        rc = _lib.lib().rdb_adamw_step(ctypes.byref(arg), K._dt(pd), K._dt(gd), 8 if eight else 32, ctypes.byref(h), K._ptr(grad_scale),
+                                       K._raw_stream(dev))
     _lib.check(rc, "rdb_adamw_step")
 
 
-def _one_float(what: str, t: Optional[torch.Tensor], dev: torch.device) -> None:
-    if t is not None and (t.dtype != torch.float32 or t.numel() != 1 or t.device != dev):
-        raise RuntimeError(f"{what} must be a one-element float32 tensor on {dev}")
+def _one_float(what: str, t: Optional[torch.Tensor], dev: int) -> None:
+    if t is not None and (t.dtype != torch.float32 or t.numel() != 1 or t.get_device() != dev):
+        raise RuntimeError(f"{what} must be a one-element float32 tensor on cuda:{dev}")
 
 
 def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -120,21 +135,25 @@ def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -
     n = len(grads)
     if n == 0:
         raise RuntimeError("grad_norm: no gradients")
-    dev = K._need_cuda(*grads)
-    if not all([t.is_contiguous() for t in grads]):
+    dev = grads[0].get_device()
+    if dev < 0:
+        raise RuntimeError("randumb_b200 kernels run on CUDA tensors only (no CPU implementation)")
+    if {t.get_device() for t in grads} != {dev}:
+        raise RuntimeError("grad_norm: all gradients must live on the same device")
+    if False in [t.is_contiguous() for t in grads]:
         raise RuntimeError("grad_norm: gradients must be contiguous")
     if max_norm is not None and not max_norm >= 0.0:
         raise RuntimeError(f"grad_norm: max_norm must not be negative, got {max_norm}")
-    out = torch.empty((2,), dtype=torch.float32, device=dev)
+    out = torch.empty((2,), dtype=torch.float32, device=grads[0].device)
     L = _lib.lib()
-    ptrs = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in grads])
-    numels = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
-    kinds = (ctypes.c_int32 * n)(*[K._dt(t.dtype) for t in grads])
-    ws = K._workspace(L.rdb_grad_norm_workspace_bytes(n), dev)
+    ptrs, numels = array("Q", [t.data_ptr() for t in grads]), array("q", [t.numel() for t in grads])
+    kinds = {d: K._dt(d) for d in {t.dtype for t in grads}}
+    dtypes = array("i", [kinds[t.dtype] for t in grads])
+    ws = K._workspace(L.rdb_grad_norm_workspace_bytes(n), out.device)
     clip = max_norm is not None
-    with torch.cuda.device(dev):
-        rc = L.rdb_grad_norm(out.data_ptr(), out.data_ptr() + 4 if clip else None, ptrs, numels, kinds, n, float(max_norm) if clip else 0.0, K._ptr(ws),
-                             ws.numel(), K._stream(dev))
+    with K._on(dev):
+        rc = L.rdb_grad_norm(out.data_ptr(), out.data_ptr() + 4 if clip else None, ptrs.buffer_info()[0], numels.buffer_info()[0], dtypes.buffer_info()[0],
+                             n, float(max_norm) if clip else 0.0, K._ptr(ws), ws.numel(), K._raw_stream(dev))
     _lib.check(rc, "rdb_grad_norm")
     return out[0], out[1] if clip else None
 
