@@ -18,6 +18,7 @@ namespace rdb {
 
 constexpr int ADAMW_CHUNK = 8192;
 constexpr int ADAMW_THREADS = 256;
+static_assert(ADAMW_CHUNK == 8 * 4 * 256, "sumsq_kernel takes a chunk in four passes of its eight warps");
 constexpr int SEG = RDB_ADAMW_BLOCK;      // elements per warp pass, and per scale of an 8-bit moment
 static_assert(SEG == 256, "a warp pass is 32 lanes x 8 elements");
 
@@ -109,11 +110,24 @@ __device__ __forceinline__ float warp_max(float x) {
 
 // First moment in 8 bits: float8 e4m3 times the scale that puts the block's largest magnitude at 448, rounded to nearest
 // (off by at most 2^-4 of the value; b1 forgets it within a few steps).
-__device__ __forceinline__ float e4m3_value(uint8_t c) {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
-    return __half2float(__half(h));
+__device__ __forceinline__ float2 e4m3_values(uint8_t c0, uint8_t c1) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((uint32_t)c0 | ((uint32_t)c1 << 8)), __NV_E4M3);
+    return __half22float2(__half2(h));
 }
-__device__ __forceinline__ uint8_t e4m3_code(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint16_t e4m3_codes(float x0, float x1) { return __nv_cvt_float2_to_fp8x2(make_float2(x0, x1), __NV_SATFINITE, __NV_E4M3); }
+
+// x / d with 1 / d at hand, correctly rounded: quotient, exact residual, one correction (P. Markstein, "Computation of elementary
+// functions on the IBM RISC System/6000 processor", 1990).  The bytes of the second moment hang on every bit of it.
+__device__ __forceinline__ float divide_by(float x, float d, float inv) {
+    const float q = __fmul_rn(x, inv);
+    return __fmaf_rn(__fmaf_rn(-q, d, x), inv, q);
+}
+// square root within 2^-23
+__device__ __forceinline__ float sqrt_fast(float x) {
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // Second moment in 8 bits: no sign, 4 exponent bits (bias 15), 4 mantissa bits; byte 255 stands for 1.9375 and carries the
 // block's maximum.  Shifted into a float32 the byte sits on top of exponent and mantissa, so its value is that float32 times
@@ -147,24 +161,33 @@ __device__ __forceinline__ void adamw_segment(const AdamwDesc &d, int64_t at, in
     }
     float m[8], v[8];
     float mmax = 0.0f, vmax = 0.0f;
+    if (BITS8) {
+        const uint8_t *mc = reinterpret_cast<const uint8_t *>(m8), *vc = reinterpret_cast<const uint8_t *>(v8);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const float2 x = e4m3_values(mc[j], mc[j + 1]);
+            m[j] = __fmul_rn(x.x, mscale);
+            m[j + 1] = __fmul_rn(x.y, mscale);
+            v[j] = __fmul_rn(ue4m4_value(vc[j]), vscale);
+            v[j + 1] = __fmul_rn(ue4m4_value(vc[j + 1]), vscale);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            m[j] = *reinterpret_cast<float *>(&m8[j]);
+            v[j] = *reinterpret_cast<float *>(&v8[j]);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float g = __fmul_rn(to_f32<G>(g8[j]), gscale);
-        float m0, v0;
-        if (BITS8) {
-            m0 = __fmul_rn(e4m3_value(*reinterpret_cast<uint8_t *>(&m8[j])), mscale);
-            v0 = __fmul_rn(ue4m4_value(*reinterpret_cast<uint8_t *>(&v8[j])), vscale);
-        } else {
-            m0 = *reinterpret_cast<float *>(&m8[j]);
-            v0 = *reinterpret_cast<float *>(&v8[j]);
-        }
-        m[j] = __fadd_rn(__fmul_rn(m0, s.b1), __fmul_rn(g, s.omb1));
-        v[j] = __fadd_rn(__fmul_rn(v0, s.b2), __fmul_rn(__fmul_rn(g, g), s.omb2));
+        m[j] = __fadd_rn(__fmul_rn(m[j], s.b1), __fmul_rn(g, s.omb1));
+        v[j] = __fadd_rn(__fmul_rn(v[j], s.b2), __fmul_rn(__fmul_rn(g, g), s.omb2));
         mmax = fmaxf(mmax, fabsf(m[j]));
         vmax = fmaxf(vmax, v[j]);
         const float p = MASTER ? w8[j] : to_f32<P>(p8[j]);
-        const float upd = __fdiv_rn(m[j], __fadd_rn(__fmul_rn(__fsqrt_rn(v[j]), inv_root), s.eps));
-        const float q = __fsub_rn(__fmul_rn(p, decay), __fmul_rn(size, upd));
+        const float upd = __fdividef(m[j], __fmaf_rn(sqrt_fast(v[j]), inv_root, s.eps));   // within 2^-21
+        const float q = __fmaf_rn(p, decay, -size * upd);
         if (MASTER) w8[j] = q;
         p8[j] = from_f32<P>(q);
     }
@@ -173,14 +196,28 @@ __device__ __forceinline__ void adamw_segment(const AdamwDesc &d, int64_t at, in
     if (BITS8) {
         mscale = __fmul_rn(warp_max(mmax), 1.0f / 448.0f);
         vscale = __fmul_rn(warp_max(vmax), 1.0f / 1.9375f);
+        uint8_t *mc = reinterpret_cast<uint8_t *>(m8), *vc = reinterpret_cast<uint8_t *>(v8);
+        const uint32_t h0 = (uint32_t)at * SQ5_N1 + rseed;
+        // ordinary scales: multiply by the reciprocal; scales next to nothing (or not a number) divide, zero scales give zero
+        const bool easy = mscale > 1e-30f && vscale > 1e-30f && mscale < 1e30f && vscale < 1e30f;
+        const float minv = easy ? __frcp_rn(mscale) : 0.0f, vinv = easy ? __frcp_rn(vscale) : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float qm = mscale > 0.0f ? __fdiv_rn(m[j], mscale) : 0.0f;
-            const float qv = vscale > 0.0f ? __fdiv_rn(v[j], vscale) : 0.0f;
-            const uint32_t pos = (uint32_t)(at + elem_of<VEC>(lane, j));
-            const uint32_t r19 = sq5_tail(pos * SQ5_N1 + rseed) >> 13;
-            *reinterpret_cast<uint8_t *>(&m8[j]) = e4m3_code(qm);
-            *reinterpret_cast<uint8_t *>(&v8[j]) = ue4m4_code(qv, v[j], r19);
+        for (int j = 0; j < 8; j += 2) {
+            float qm[2], qv[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (easy) {
+                    qm[e] = divide_by(m[j + e], mscale, minv);
+                    qv[e] = divide_by(v[j + e], vscale, vinv);
+                } else {
+                    qm[e] = mscale > 0.0f ? __fdiv_rn(m[j + e], mscale) : 0.0f;
+                    qv[e] = vscale > 0.0f ? __fdiv_rn(v[j + e], vscale) : 0.0f;
+                }
+                vc[j + e] = ue4m4_code(qv[e], v[j + e], sq5_tail(h0 + (uint32_t)elem_of<VEC>(lane, j + e) * SQ5_N1) >> 13);
+            }
+            const uint16_t c = e4m3_codes(qm[0], qm[1]);
+            mc[j] = (uint8_t)c;
+            mc[j + 1] = (uint8_t)(c >> 8);
         }
         if (lane == 0) {
             d.ms[at / SEG] = mscale;
@@ -282,11 +319,25 @@ sumsq_kernel(const __grid_constant__ AdamwTable<NT> tab, double *__restrict__ pa
         const int64_t lo = (int64_t)(c - tab.first[ti]) * ADAMW_CHUNK;
         const int64_t hi = lo + ADAMW_CHUNK < d.n ? lo + ADAMW_CHUNK : d.n;
         const bool vec = (reinterpret_cast<uintptr_t>(d.g) & (sizeof(G) * 4 - 1)) == 0;
+        const G *g = reinterpret_cast<const G *>(d.g);
+        if (vec && hi - lo == ADAMW_CHUNK) {         // a whole chunk: four 256-element passes of the warp, all loads in flight
+            G g8[4][8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load8<true>(g8[u], g + lo + (warp * 4 + u) * SEG, lane, SEG);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float f = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f += to_f32<G>(g8[u][j]) * to_f32<G>(g8[u][j]);
+                acc += (double)f;
+            }
+            continue;
+        }
         for (int64_t at = lo + warp * SEG; at < hi; at += (ADAMW_THREADS / 32) * SEG) {
             const int left = (int)(hi - at < SEG ? hi - at : SEG);
             G g8[8];
-            if (vec && left == SEG) load8<true>(g8, reinterpret_cast<const G *>(d.g) + at, lane, left);
-            else load8<false>(g8, reinterpret_cast<const G *>(d.g) + at, lane, left);
+            if (vec && left == SEG) load8<true>(g8, g + at, lane, left);
+            else load8<false>(g8, g + at, lane, left);
             float f = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) f += to_f32<G>(g8[j]) * to_f32<G>(g8[j]);
