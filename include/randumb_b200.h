@@ -483,7 +483,8 @@ int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int6
  * when none does).  x, w and the gradients are of type dtype, losses float32.
  *
  * rdb_ce_fwd   loss (one float32, or T of them for RDB_CE_NONE) and aux, float32 [2T + 1]: log-sum-exp per row, loss per row,
- *              number of rows that count.  dx_unit (may be null, only with w null): d(row's loss)/dx, contiguous [T, R].
+ *              number of rows that count.  dx_unit (may be null, only with w null): d(row's loss)/dx, float32, contiguous [T, R]: the gradient is
+ *              rounded to dtype once, when the loss's own gradient is known.
  * rdb_ce_scale dz = dx_unit times the gradient of the loss: *dloss (RDB_CE_SUM), *dloss / count (RDB_CE_MEAN), dloss[row] (NONE).
  * rdb_ce_bwd   gradients for a stored matrix from the forward's aux: dx [T, R] and dw [V, R], contiguous, either may be null.
  * workspace: 256-byte aligned, rdb_ce_workspace_bytes(op, ...) bytes with op RDB_CE_LOSS (fwd), RDB_CE_LOSS_GRAD (fwd with
@@ -498,10 +499,10 @@ int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int6
 #define RDB_CE_MEAN 1
 #define RDB_CE_SUM 2
 size_t rdb_ce_workspace_bytes(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw);
-int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
+int rdb_ce_fwd(float *loss, float *aux, float *dx_unit, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
                void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t V, int64_t row0, uint32_t seed, int64_t ignore_index,
                int use_ignore, int dtype, int reduction, int32_t *status, void *stream);
-int rdb_ce_scale(void *dz, const void *dx_unit, const float *dloss, const float *aux, int64_t T, int64_t R, int dtype, int reduction,
+int rdb_ce_scale(void *dz, const float *dx_unit, const float *dloss, const float *aux, int64_t T, int64_t R, int dtype, int reduction,
                  void *stream);
 int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
                const float *aux, void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t V, int64_t ignore_index,

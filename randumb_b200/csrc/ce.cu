@@ -1007,8 +1007,8 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&f)[4]) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
 }
 __device__ __forceinline__ void store4(float *p, const float (&f)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]); }
-template <typename T, int ROWS>
-__global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(T *__restrict__ dx, float *__restrict__ slots, const int2 *__restrict__ parts,
+template <typename T, typename O, int ROWS>
+__global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(O *__restrict__ dx, float *__restrict__ slots, const int2 *__restrict__ parts,
                                                        const int32_t *__restrict__ map, const float *__restrict__ s, const int32_t *__restrict__ tcol,
                                                        Vocab voc, int64_t T_rows, int64_t R, int tile_rows, int tiles_n) {
     __shared__ const float *sh_at[ROWS];
@@ -1050,7 +1050,7 @@ __global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(T *_
     const int cl = (threadIdx.x & 63) * 4;
     const int64_t c = (int64_t)nt * CE_TILE + cl;
     if (c >= R) return;
-    const bool vec = R % 4 == 0 && (reinterpret_cast<uintptr_t>(dx) & (4 * sizeof(T) - 1)) == 0;
+    const bool vec = R % 4 == 0 && (reinterpret_cast<uintptr_t>(dx) & (4 * sizeof(O) - 1)) == 0;
     float4 v[ROWS / 4];
     int most = 0;
 #pragma unroll
@@ -1085,12 +1085,12 @@ __global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(T *_
                 f[e] = (f[e] - sj * w) * inv;
             }
         }
-        T *out = dx + i * R + c;
+        O *out = dx + i * R + c;
         if (vec) store4(out, f);
         else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < R) out[e] = from_f32<T>(f[e]);
+                if (c + e < R) out[e] = from_f32<O>(f[e]);
         }
     }
 }
@@ -1104,7 +1104,7 @@ __device__ __forceinline__ void store_f8(float *p, const float (&f)[8]) {
 // ignored rows stay zero whatever the factor (no row counts: 1 / 0)
 __device__ __forceinline__ float scaled(float u, float g) { return u == 0.0f ? 0.0f : u * g; }
 template <typename T>
-__global__ void __launch_bounds__(256) ce_scale_kernel(T *__restrict__ dz, const T *__restrict__ unit, const float *__restrict__ dloss,
+__global__ void __launch_bounds__(256) ce_scale_kernel(T *__restrict__ dz, const float *__restrict__ unit, const float *__restrict__ dloss,
                                                        const float *__restrict__ count, int64_t rows, int64_t R, int reduction) {
     pdl_launch_dependents();
     pdl_wait();
@@ -1124,7 +1124,7 @@ __global__ void __launch_bounds__(256) ce_scale_kernel(T *__restrict__ dz, const
         return;
     }
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x)
-        dz[i] = from_f32<T>(scaled(to_f32<T>(unit[i]), reduction == RDB_CE_NONE ? dloss[i / R] : g0));
+        dz[i] = from_f32<T>(scaled(unit[i], reduction == RDB_CE_NONE ? dloss[i / R] : g0));
 }
 
 // ================================================================================================
@@ -1438,8 +1438,10 @@ static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
     auto go = [&](auto kern, auto *out) {
         return launch_pdl(kern, grid, CE_TILE, 0, c.st, out, slots, parts, map, s, tcol, c.voc, c.T, c.R, p.tile_rows, tiles_n);
     };
-    if (c.dtype == RDB_F32) return rows == 16 ? go(ce_dx_kernel<float, 16>, (float *)dx) : go(ce_dx_kernel<float, 4>, (float *)dx);
-    return rows == 16 ? go(ce_dx_kernel<__nv_bfloat16, 16>, (__nv_bfloat16 *)dx) : go(ce_dx_kernel<__nv_bfloat16, 4>, (__nv_bfloat16 *)dx);
+    using H = __nv_bfloat16;
+    if (c.dtype == RDB_F32) return rows == 16 ? go(ce_dx_kernel<float, float, 16>, (float *)dx) : go(ce_dx_kernel<float, float, 4>, (float *)dx);
+    if (unit) return rows == 16 ? go(ce_dx_kernel<H, float, 16>, (float *)dx) : go(ce_dx_kernel<H, float, 4>, (float *)dx);
+    return rows == 16 ? go(ce_dx_kernel<H, H, 16>, (H *)dx) : go(ce_dx_kernel<H, H, 4>, (H *)dx);
 }
 
 static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w, int64_t ldw, int dtype, int reduction) {
@@ -1462,7 +1464,7 @@ extern "C" size_t rdb_ce_workspace_bytes(int op, int64_t T, int64_t R, int64_t V
     return ce_plan(op, T, R, V, dtype, w, ldw, nullptr, 1, 1).total;
 }
 
-extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
+extern "C" int rdb_ce_fwd(float *loss, float *aux, float *dx_unit, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
                           void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t V, int64_t row0, uint32_t seed,
                           int64_t ignore_index, int use_ignore, int dtype, int reduction, int32_t *status, void *stream) {
     int rc = ce_check(T, R, V, ldx, w, ldw, dtype, reduction);
@@ -1471,7 +1473,7 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, void *dx_unit, const void *x,
     if (!aux || (!loss && (T > 0 || reduction != RDB_CE_NONE))) return RDB_ERR_NULL;
     if (T > 0 && (!x || !target)) return RDB_ERR_NULL;
     const size_t es = dtype_size(dtype);
-    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(dx_unit)) & (es - 1)) || (reinterpret_cast<uintptr_t>(target) & 7))
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & (es - 1)) || (reinterpret_cast<uintptr_t>(dx_unit) & 3) || (reinterpret_cast<uintptr_t>(target) & 7))
         return RDB_ERR_ALIGN;
     CeCall c{};
     c.p = ce_plan(dx_unit ? 1 : 0, T, R, V, dtype, w, ldw, nullptr, 1, 0);
@@ -1564,7 +1566,7 @@ extern "C" int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x,
     return RDB_OK;
 }
 
-extern "C" int rdb_ce_scale(void *dz, const void *unit, const float *dloss, const float *aux, int64_t T, int64_t R, int dtype, int reduction,
+extern "C" int rdb_ce_scale(void *dz, const float *unit, const float *dloss, const float *aux, int64_t T, int64_t R, int dtype, int reduction,
                             void *stream) {
     int rc = ce_check(T, R, 1, R, nullptr, 0, dtype, reduction);
     if (rc) return rc;
@@ -1574,6 +1576,6 @@ extern "C" int rdb_ce_scale(void *dz, const void *unit, const float *dloss, cons
     const int64_t want = cdiv64(T * R, 256 * 8);
     const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8));
     if (dtype == RDB_F32)
-        return launch_pdl(ce_scale_kernel<float>, grid, 256, 0, st, (float *)dz, (const float *)unit, dloss, aux + 2 * T, T, R, reduction);
-    return launch_pdl(ce_scale_kernel<__nv_bfloat16>, grid, 256, 0, st, (__nv_bfloat16 *)dz, (const __nv_bfloat16 *)unit, dloss, aux + 2 * T, T, R, reduction);
+        return launch_pdl(ce_scale_kernel<float>, grid, 256, 0, st, (float *)dz, unit, dloss, aux + 2 * T, T, R, reduction);
+    return launch_pdl(ce_scale_kernel<__nv_bfloat16>, grid, 256, 0, st, (__nv_bfloat16 *)dz, unit, dloss, aux + 2 * T, T, R, reduction);
 }

@@ -1,10 +1,10 @@
 // AdamW over a list of tensors and the norm of a list of gradients (CUDA cores, HBM-bound).
 //
-// One launch walks up to ADAMW_TENSORS tensors: their pointers travel in the kernel's parameters, the elements are cut into
-// chunks of ADAMW_CHUNK, and a block finds the tensor of its chunk by bisection.  A warp owns 256 consecutive elements at a
-// time -- the block of elements that shares the scale of an 8-bit moment, so its maximum is one shuffle reduction and nothing
-// is read twice.  Arithmetic is float32 throughout, one rounding per operation as written (no contraction), so the bytes of
-// the 8-bit moments follow from the inputs alone.
+// One launch walks up to NT_LARGE tensors: their pointers travel in the kernel's parameters.  The tensors are cut into segments of
+// 256 elements, the warps of the grid take segments in turn (each by itself: no barrier), and since a warp's segments only move
+// forward, the tensor of the next one is found by stepping on from the last one's.  256 consecutive elements share the scale of an
+// 8-bit moment, so its maximum is one shuffle reduction and nothing is read twice.  Arithmetic is float32; what the 8-bit
+// moments are made of has one rounding per operation as written (no contraction), so their bytes follow from the inputs alone.
 //
 //   m' = b1 m + (1 - b1) g        v' = b2 v + (1 - b2) g^2
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
@@ -16,9 +16,9 @@
 
 namespace rdb {
 
-constexpr int ADAMW_CHUNK = 8192;
+constexpr int NORM_CHUNK = 8192;
 constexpr int ADAMW_THREADS = 256;
-static_assert(ADAMW_CHUNK == 8 * 4 * 256, "sumsq_kernel takes a chunk in four passes of its eight warps");
+static_assert(NORM_CHUNK == 8 * 4 * 256, "sumsq_kernel takes a chunk in four passes of its eight warps");
 constexpr int SEG = RDB_ADAMW_BLOCK;      // elements per warp pass, and per scale of an 8-bit moment
 static_assert(SEG == 256, "a warp pass is 32 lanes x 8 elements");
 
@@ -32,7 +32,7 @@ struct AdamwDesc {
     int64_t n;
 };
 
-// NT tensors; first[i] is the first chunk of tensor i, first[count] the number of chunks
+// NT tensors; first[i] is the first segment (AdamW) or chunk (norm) of tensor i, first[count] their number
 template <int NT>
 struct AdamwTable {
     AdamwDesc t[NT];
@@ -122,116 +122,165 @@ __device__ __forceinline__ float divide_by(float x, float d, float inv) {
     const float q = __fmul_rn(x, inv);
     return __fmaf_rn(__fmaf_rn(-q, d, x), inv, q);
 }
-// square root within 2^-23
-__device__ __forceinline__ float sqrt_fast(float x) {
-    float y;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // Second moment in 8 bits: no sign, 4 exponent bits (bias 15), 4 mantissa bits; byte 255 stands for 1.9375 and carries the
 // block's maximum.  Shifted into a float32 the byte sits on top of exponent and mantissa, so its value is that float32 times
-// 2^112 (subnormals included).  (1 - b2) is far below a step of any 8-bit format: rounding to nearest would leave v where it
+// 2^112 = 5.19e33 (subnormals included).  (1 - b2) is far below a step of any 8-bit format: rounding to nearest would leave v where it
 // is however small the gradients become, so v is rounded to one of its two neighbours at random with the odds that keep its
 // expectation: add 19 random bits below the byte and cut.  A positive v never becomes 0: it divides.
-__device__ __forceinline__ float ue4m4_value(uint8_t c) { return __fmul_rn(__uint_as_float((uint32_t)c << 19), 5.192296858534828e33f); }
-__device__ __forceinline__ uint8_t ue4m4_code(float q, float v, uint32_t r19) {
+__device__ __forceinline__ uint32_t ue4m4_code(float q, float v, uint32_t r19) {
     uint32_t c = (__float_as_uint(__fmul_rn(q, 1.925929944387236e-34f)) + r19) >> 19;
     c = c > 255u ? 255u : c;
-    return (uint8_t)((c == 0u && v > 0.0f) ? 1u : c);
+    return (c == 0u && v > 0.0f) ? 1u : c;
 }
 
-template <typename P, typename G, bool MASTER, bool BITS8, bool VEC>
-__device__ __forceinline__ void adamw_segment(const AdamwDesc &d, int64_t at, int left, int lane, const AdamwScalars &s, float gscale,
-                                              float size, float inv_root, float decay, uint32_t rseed) {
-    using S = typename std::conditional<BITS8, uint8_t, float>::type;
+// division and square root of the update, within 2^-21.  An eps near zero could meet a denominator that the fast forms flush.
+__device__ __forceinline__ float update_of(float m, float v, float inv_root, float eps, bool fast) {
+    if (fast) {
+        float r, q;
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+        r = __fmaf_rn(r, inv_root, eps);
+        asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(r));
+        return q;
+    }
+    return __fdiv_rn(m, __fmaf_rn(__fsqrt_rn(v), inv_root, eps));
+}
+
+struct StepScalars {
+    float size, inv_root, decay, eps;
+    bool fast;
+};
+
+// parameter (or its master) after the step
+template <typename P, bool MASTER>
+__device__ __forceinline__ void move(P &p8, float &w8, float m, float v, const StepScalars &c) {
+    const float p = MASTER ? w8 : to_f32<P>(p8);
+    const float q = __fmaf_rn(p, c.decay, -c.size * update_of(m, v, c.inv_root, c.eps, c.fast));
+    if (MASTER) w8 = q;
+    p8 = from_f32<P>(q);
+}
+
+__device__ __forceinline__ void new_moments(float &m, float &v, float g, const AdamwScalars &s) {
+    m = __fadd_rn(__fmul_rn(m, s.b1), __fmul_rn(g, s.omb1));
+    v = __fadd_rn(__fmul_rn(v, s.b2), __fmul_rn(__fmul_rn(g, g), s.omb2));
+}
+
+template <typename P, typename G, bool MASTER, bool VEC>
+__device__ __forceinline__ void adamw_segment32(const AdamwDesc &d, int64_t at, int left, int lane, const AdamwScalars &s, float gscale,
+                                                const StepScalars &c) {
     P p8[8];
     G g8[8];
-    S m8[8], v8[8];
-    float w8[8];
-    float mscale = 0.0f, vscale = 0.0f;
+    float m[8], v[8], w8[8];
     load8<VEC>(g8, reinterpret_cast<const G *>(d.g) + at, lane, left);
-    load8<VEC>(m8, reinterpret_cast<const S *>(d.m) + at, lane, left);
-    load8<VEC>(v8, reinterpret_cast<const S *>(d.v) + at, lane, left);
+    load8<VEC>(m, const_cast<const float *>(reinterpret_cast<float *>(d.m)) + at, lane, left);
+    load8<VEC>(v, const_cast<const float *>(reinterpret_cast<float *>(d.v)) + at, lane, left);
     if (MASTER) load8<VEC>(w8, const_cast<const float *>(d.master) + at, lane, left);
     else load8<VEC>(p8, const_cast<const P *>(reinterpret_cast<P *>(d.p)) + at, lane, left);
-    if (BITS8) {
-        mscale = d.ms[at / SEG];
-        vscale = d.vs[at / SEG];
-    }
-    float m[8], v[8];
-    float mmax = 0.0f, vmax = 0.0f;
-    if (BITS8) {
-        const uint8_t *mc = reinterpret_cast<const uint8_t *>(m8), *vc = reinterpret_cast<const uint8_t *>(v8);
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const float2 x = e4m3_values(mc[j], mc[j + 1]);
-            m[j] = __fmul_rn(x.x, mscale);
-            m[j + 1] = __fmul_rn(x.y, mscale);
-            v[j] = __fmul_rn(ue4m4_value(vc[j]), vscale);
-            v[j + 1] = __fmul_rn(ue4m4_value(vc[j + 1]), vscale);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            m[j] = *reinterpret_cast<float *>(&m8[j]);
-            v[j] = *reinterpret_cast<float *>(&v8[j]);
-        }
-    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float g = __fmul_rn(to_f32<G>(g8[j]), gscale);
-        m[j] = __fadd_rn(__fmul_rn(m[j], s.b1), __fmul_rn(g, s.omb1));
-        v[j] = __fadd_rn(__fmul_rn(v[j], s.b2), __fmul_rn(__fmul_rn(g, g), s.omb2));
-        mmax = fmaxf(mmax, fabsf(m[j]));
-        vmax = fmaxf(vmax, v[j]);
-        const float p = MASTER ? w8[j] : to_f32<P>(p8[j]);
-        const float upd = __fdividef(m[j], __fmaf_rn(sqrt_fast(v[j]), inv_root, s.eps));   // within 2^-21
-        const float q = __fmaf_rn(p, decay, -size * upd);
-        if (MASTER) w8[j] = q;
-        p8[j] = from_f32<P>(q);
+        new_moments(m[j], v[j], __fmul_rn(to_f32<G>(g8[j]), gscale), s);
+        move<P, MASTER>(p8[j], w8[j], m[j], v[j], c);
     }
     store8<VEC>(reinterpret_cast<P *>(d.p) + at, p8, lane, left);
     if (MASTER) store8<VEC>(d.master + at, w8, lane, left);
-    if (BITS8) {
-        mscale = __fmul_rn(warp_max(mmax), 1.0f / 448.0f);
-        vscale = __fmul_rn(warp_max(vmax), 1.0f / 1.9375f);
-        uint8_t *mc = reinterpret_cast<uint8_t *>(m8), *vc = reinterpret_cast<uint8_t *>(v8);
-        const uint32_t h0 = (uint32_t)at * SQ5_N1 + rseed;
-        // ordinary scales: multiply by the reciprocal; scales next to nothing (or not a number) divide, zero scales give zero
-        const bool easy = mscale > 1e-30f && vscale > 1e-30f && mscale < 1e30f && vscale < 1e30f;
-        const float minv = easy ? __frcp_rn(mscale) : 0.0f, vinv = easy ? __frcp_rn(vscale) : 0.0f;
+    store8<VEC>(reinterpret_cast<float *>(d.m) + at, m, lane, left);
+    store8<VEC>(reinterpret_cast<float *>(d.v) + at, v, lane, left);
+}
+
+// four bytes of a lane: words in the vector form, gathered bytes otherwise
+template <bool VEC> __device__ __forceinline__ uint32_t load_bytes(const uint8_t *base, int h, int lane, int left) {
+    if (VEC) return *reinterpret_cast<const uint32_t *>(base + h * 128 + lane * 4);
+    uint32_t w = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            float qm[2], qv[2];
+    for (int k = 0; k < 4; ++k) {
+        const int e = elem_of<false>(lane, h * 4 + k);
+        w |= (e < left ? (uint32_t)base[e] : 0u) << (8 * k);
+    }
+    return w;
+}
+template <bool VEC> __device__ __forceinline__ void store_bytes(uint8_t *base, uint32_t w, int h, int lane, int left) {
+    if (VEC) *reinterpret_cast<uint32_t *>(base + h * 128 + lane * 4) = w;
+    else {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (easy) {
-                    qm[e] = divide_by(m[j + e], mscale, minv);
-                    qv[e] = divide_by(v[j + e], vscale, vinv);
-                } else {
-                    qm[e] = mscale > 0.0f ? __fdiv_rn(m[j + e], mscale) : 0.0f;
-                    qv[e] = vscale > 0.0f ? __fdiv_rn(v[j + e], vscale) : 0.0f;
-                }
-                vc[j + e] = ue4m4_code(qv[e], v[j + e], sq5_tail(h0 + (uint32_t)elem_of<VEC>(lane, j + e) * SQ5_N1) >> 13);
-            }
-            const uint16_t c = e4m3_codes(qm[0], qm[1]);
-            mc[j] = (uint8_t)c;
-            mc[j + 1] = (uint8_t)(c >> 8);
-        }
-        if (lane == 0) {
-            d.ms[at / SEG] = mscale;
-            d.vs[at / SEG] = vscale;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            *reinterpret_cast<float *>(&m8[j]) = m[j];
-            *reinterpret_cast<float *>(&v8[j]) = v[j];
+        for (int k = 0; k < 4; ++k) {
+            const int e = elem_of<false>(lane, h * 4 + k);
+            if (e < left) base[e] = (uint8_t)(w >> (8 * k));
         }
     }
-    store8<VEC>(reinterpret_cast<S *>(d.m) + at, m8, lane, left);
-    store8<VEC>(reinterpret_cast<S *>(d.v) + at, v8, lane, left);
+}
+
+template <typename P, typename G, bool MASTER, bool VEC>
+__device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, int left, int lane, const AdamwScalars &s, float gscale,
+                                               const StepScalars &c, uint32_t rseed) {
+    P p8[8];
+    G g8[8];
+    float m[8], v[8], w8[8];
+    uint8_t *mb = reinterpret_cast<uint8_t *>(d.m) + at, *vb = reinterpret_cast<uint8_t *>(d.v) + at;
+    load8<VEC>(g8, reinterpret_cast<const G *>(d.g) + at, lane, left);
+    uint32_t mw[2], vw[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        mw[h] = load_bytes<VEC>(mb, h, lane, left);
+        vw[h] = load_bytes<VEC>(vb, h, lane, left);
+    }
+    if (MASTER) load8<VEC>(w8, const_cast<const float *>(d.master) + at, lane, left);
+    else load8<VEC>(p8, const_cast<const P *>(reinterpret_cast<P *>(d.p)) + at, lane, left);
+    float mscale = d.ms[at / SEG], vscale = d.vs[at / SEG];
+    // byte << 19 as a float32 is the value times 2^-112: one product where the scale leaves room for 2^112
+    const bool room = vscale < 16384.0f;
+    const float vup = room ? __fmul_rn(vscale, 5.192296858534828e33f) : vscale;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float2 x0 = e4m3_values((uint8_t)mw[h], (uint8_t)(mw[h] >> 8)), x1 = e4m3_values((uint8_t)(mw[h] >> 16), (uint8_t)(mw[h] >> 24));
+        m[h * 4] = __fmul_rn(x0.x, mscale);
+        m[h * 4 + 1] = __fmul_rn(x0.y, mscale);
+        m[h * 4 + 2] = __fmul_rn(x1.x, mscale);
+        m[h * 4 + 3] = __fmul_rn(x1.y, mscale);
+        const uint32_t b0 = (vw[h] & 0xFFu) << 19, b1 = (vw[h] & 0xFF00u) << 11, b2 = (vw[h] & 0xFF0000u) << 3, b3 = (vw[h] >> 5) & 0x7F80000u;
+        const uint32_t b[4] = {b0, b1, b2, b3};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            v[h * 4 + k] = room ? __fmul_rn(__uint_as_float(b[k]), vup) : __fmul_rn(__fmul_rn(__uint_as_float(b[k]), 5.192296858534828e33f), vup);
+    }
+    float mmax = 0.0f, vmax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        new_moments(m[j], v[j], __fmul_rn(to_f32<G>(g8[j]), gscale), s);
+        mmax = fmaxf(mmax, fabsf(m[j]));
+        vmax = fmaxf(vmax, v[j]);
+        move<P, MASTER>(p8[j], w8[j], m[j], v[j], c);
+    }
+    store8<VEC>(reinterpret_cast<P *>(d.p) + at, p8, lane, left);
+    if (MASTER) store8<VEC>(d.master + at, w8, lane, left);
+    mscale = __fmul_rn(warp_max(mmax), 1.0f / 448.0f);
+    vscale = __fmul_rn(warp_max(vmax), 1.0f / 1.9375f);
+    const uint32_t h0 = (uint32_t)at * SQ5_N1 + rseed;
+    // ordinary scales: multiply by the reciprocal; scales next to nothing (or not a number) divide, zero scales give zero
+    const bool easy = mscale > 1e-30f && vscale > 1e-30f && mscale < 1e30f && vscale < 1e30f;
+    const float minv = easy ? __frcp_rn(mscale) : 0.0f, vinv = easy ? __frcp_rn(vscale) : 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float qm[4], qv[4];
+        uint32_t code[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int j = h * 4 + k;
+            if (easy) {
+                qm[k] = divide_by(m[j], mscale, minv);
+                qv[k] = divide_by(v[j], vscale, vinv);
+            } else {
+                qm[k] = mscale > 0.0f ? __fdiv_rn(m[j], mscale) : 0.0f;
+                qv[k] = vscale > 0.0f ? __fdiv_rn(v[j], vscale) : 0.0f;
+            }
+            code[k] = ue4m4_code(qv[k], v[j], sq5_tail(h0 + (uint32_t)elem_of<VEC>(lane, j) * SQ5_N1) >> 13);
+        }
+        store_bytes<VEC>(mb, (uint32_t)e4m3_codes(qm[0], qm[1]) | ((uint32_t)e4m3_codes(qm[2], qm[3]) << 16), h, lane, left);
+        store_bytes<VEC>(vb, code[0] | (code[1] << 8) | (code[2] << 16) | (code[3] << 24), h, lane, left);
+    }
+    if (lane == 0) {
+        d.ms[at / SEG] = mscale;
+        d.vs[at / SEG] = vscale;
+    }
 }
 
 template <typename Table>
@@ -259,44 +308,43 @@ __global__ void adamw_count_kernel(const __grid_constant__ StepTable<NT> tab) {
 }
 
 template <typename P, typename G, bool MASTER, bool BITS8, int NT>
-__global__ void __launch_bounds__(ADAMW_THREADS)
+__global__ void __launch_bounds__(ADAMW_THREADS, 4)
 adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, const float *__restrict__ grad_scale) {
-    __shared__ float sh[3];
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t warps = gridDim.x * (ADAMW_THREADS / 32);
     const float gscale = grad_scale ? *grad_scale : 1.0f;
-    const uint32_t chunks = tab.first[tab.count];
-    int cur = -1;
-    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int ti = find_tensor(tab, c);
+    const uint32_t segs = tab.first[tab.count];
+    StepScalars c{};
+    c.eps = s.eps;
+    c.fast = s.eps > 1e-30f;
+    float t_have = -1.0f;
+    int ti = 0;
+    for (uint32_t g = blockIdx.x * (ADAMW_THREADS / 32) + (threadIdx.x >> 5); g < segs; g += warps) {
+        while (g >= tab.first[ti + 1]) ++ti;
         const AdamwDesc &d = tab.t[ti];
-        if (ti != cur) {                  // bias corrections of this tensor's step, in float64
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const double t = (double)*d.step;
-                const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
-                sh[0] = (float)(lr / (1.0 - pow(s.beta1, t)));
-                sh[1] = (float)(1.0 / sqrt(1.0 - pow(s.beta2, t)));
-                sh[2] = (float)(1.0 - lr * s.weight_decay);
-            }
-            __syncthreads();
-            cur = ti;
+        const float t = *d.step;
+        if (t != t_have) {                // bias corrections of this step, in float64; tensors that began together share them
+            const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
+            c.size = (float)(lr / (1.0 - pow(s.beta1, (double)t)));
+            c.inv_root = (float)(1.0 / sqrt(1.0 - pow(s.beta2, (double)t)));
+            c.decay = (float)(1.0 - lr * s.weight_decay);
+            t_have = t;
         }
-        const float size = sh[0], inv_root = sh[1], decay = sh[2];
-        const uint32_t rseed = BITS8 ? s.seed + (uint32_t)(int64_t)*d.step * 0x9E3779B1u + (uint32_t)(tab.index0 + ti) * 0x85EBCA6Bu : 0u;
-        const int64_t lo = (int64_t)(c - tab.first[ti]) * ADAMW_CHUNK;
-        const int64_t hi = lo + ADAMW_CHUNK < d.n ? lo + ADAMW_CHUNK : d.n;
+        const int64_t at = (int64_t)(g - tab.first[ti]) * SEG;
+        const int left = (int)(d.n - at < SEG ? d.n - at : SEG);
         constexpr uintptr_t PV = sizeof(P) * 4 - 1, GV = sizeof(G) * 4 - 1, SV = BITS8 ? 3 : 15;
-        const bool vec = ((reinterpret_cast<uintptr_t>(d.p) & PV) | (reinterpret_cast<uintptr_t>(d.g) & GV) |
-                          (reinterpret_cast<uintptr_t>(d.m) & SV) | (reinterpret_cast<uintptr_t>(d.v) & SV) |
-                          (MASTER ? reinterpret_cast<uintptr_t>(d.master) & 15 : 0)) == 0;
-        for (int64_t at = lo + warp * SEG; at < hi; at += (ADAMW_THREADS / 32) * SEG) {
-            const int left = (int)(hi - at < SEG ? hi - at : SEG);
-            if (vec && left == SEG)
-                adamw_segment<P, G, MASTER, BITS8, true>(d, at, left, lane, s, gscale, size, inv_root, decay, rseed);
-            else
-                adamw_segment<P, G, MASTER, BITS8, false>(d, at, left, lane, s, gscale, size, inv_root, decay, rseed);
+        const bool vec = left == SEG && ((reinterpret_cast<uintptr_t>(d.p) & PV) | (reinterpret_cast<uintptr_t>(d.g) & GV) |
+                                         (reinterpret_cast<uintptr_t>(d.m) & SV) | (reinterpret_cast<uintptr_t>(d.v) & SV) |
+                                         (MASTER ? reinterpret_cast<uintptr_t>(d.master) & 15 : 0)) == 0;
+        if (BITS8) {
+            const uint32_t rseed = s.seed + (uint32_t)(int64_t)t * 0x9E3779B1u + (uint32_t)(tab.index0 + ti) * 0x85EBCA6Bu;
+            if (vec) adamw_segment8<P, G, MASTER, true>(d, at, left, lane, s, gscale, c, rseed);
+            else adamw_segment8<P, G, MASTER, false>(d, at, left, lane, s, gscale, c, rseed);
+        } else {
+            if (vec) adamw_segment32<P, G, MASTER, true>(d, at, left, lane, s, gscale, c);
+            else adamw_segment32<P, G, MASTER, false>(d, at, left, lane, s, gscale, c);
         }
     }
 }
@@ -316,11 +364,11 @@ sumsq_kernel(const __grid_constant__ AdamwTable<NT> tab, double *__restrict__ pa
     for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
         const int ti = find_tensor(tab, c);
         const AdamwDesc &d = tab.t[ti];
-        const int64_t lo = (int64_t)(c - tab.first[ti]) * ADAMW_CHUNK;
-        const int64_t hi = lo + ADAMW_CHUNK < d.n ? lo + ADAMW_CHUNK : d.n;
+        const int64_t lo = (int64_t)(c - tab.first[ti]) * NORM_CHUNK;
+        const int64_t hi = lo + NORM_CHUNK < d.n ? lo + NORM_CHUNK : d.n;
         const bool vec = (reinterpret_cast<uintptr_t>(d.g) & (sizeof(G) * 4 - 1)) == 0;
         const G *g = reinterpret_cast<const G *>(d.g);
-        if (vec && hi - lo == ADAMW_CHUNK) {         // a whole chunk: four 256-element passes of the warp, all loads in flight
+        if (vec && hi - lo == NORM_CHUNK) {         // a whole chunk: four 256-element passes of the warp, all loads in flight
             G g8[4][8];
 #pragma unroll
             for (int u = 0; u < 4; ++u) load8<true>(g8[u], g + lo + (warp * 4 + u) * SEG, lane, SEG);
@@ -386,11 +434,11 @@ constexpr int NT_SMALL = 48, NT_LARGE = 384;      // tensors per launch: 3.5 KB 
 static_assert(sizeof(AdamwTable<NT_LARGE>) + 512 < 32764, "kernel parameters");
 
 template <int NT>
-static int count_chunks(AdamwTable<NT> *tab, int n, int index0) {
+static int count_parts(AdamwTable<NT> *tab, int n, int index0, int part) {
     uint64_t c = 0;
     for (int i = 0; i < n; ++i) {
         tab->first[i] = (uint32_t)c;
-        c += (uint64_t)cdiv64(tab->t[i].n, ADAMW_CHUNK);
+        c += (uint64_t)cdiv64(tab->t[i].n, part);
         if (c >= (1ull << 32)) return RDB_ERR_TOO_LARGE;
     }
     tab->first[n] = (uint32_t)c;
@@ -409,15 +457,17 @@ static int launch_adamw(const rdb_adamw_lists &l, int n, int at, const AdamwScal
                              BITS8 ? l.exp_avg_sq_scale[k] : nullptr, l.step[k], l.numel[k]};
         steps.step[i] = l.step[k];
     }
-    int rc = count_chunks(&tab, n, at);
+    int rc = count_parts(&tab, n, at, SEG);
     if (rc) return rc;
     steps.count = n;
     rc = launch_pdl(adamw_count_kernel<NT>, dim3(1), 256, 0, st, steps);
     if (rc) return rc;
-    const uint32_t chunks = tab.first[n];
-    if (chunks == 0) return RDB_OK;
-    const uint32_t cap = 148 * 8;
-    return launch_pdl(adamw_kernel<P, G, MASTER, BITS8, NT>, dim3(chunks < cap ? chunks : cap), ADAMW_THREADS, 0, st, tab, s, gs);
+    const uint32_t want = (tab.first[n] + ADAMW_THREADS / 32 - 1) / (ADAMW_THREADS / 32);
+    if (want == 0) return RDB_OK;
+    // Four blocks are resident per SM.  32-bit moments, bound by memory: many short blocks (69 M elements, float32: 4, 8, 16, 64
+    // blocks per SM take 318, 307, 298, 287 us); 8-bit moments pay a block's float64 bias corrections more dearly (232, 229, 228, 251).
+    const uint32_t cap = 148 * (BITS8 ? 16 : 64);
+    return launch_pdl(adamw_kernel<P, G, MASTER, BITS8, NT>, dim3(want < cap ? want : cap), ADAMW_THREADS, 0, st, tab, s, gs);
 }
 
 template <typename P, typename G, bool MASTER, bool BITS8>
@@ -446,7 +496,7 @@ static int launch_sumsq(const GradRef *t, int n, double *partial, int *used, cud
         tab.t[i].g = t[i].p;
         tab.t[i].n = t[i].n;
     }
-    int rc = count_chunks(&tab, n, 0);
+    int rc = count_parts(&tab, n, 0, NORM_CHUNK);
     if (rc) return rc;
     *used = norm_blocks(tab.first[n]);
     return launch_pdl(sumsq_kernel<G, NT>, dim3(*used), ADAMW_THREADS, 0, st, tab, partial);

@@ -448,7 +448,8 @@ def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor
            seed: int = 0, vocab: int = 0, row0: int = 0, need_unit: bool = False
            ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """(loss, aux, unit): cross entropy of ``x @ W.T`` against ``target`` (see rdb_ce_fwd).  ``weight`` None: ``vocab`` noise rows
-    from ``row0`` on.  loss: float32, 0-d or (reduction "none") [T]; unit: the rows' own gradients in x, with ``need_unit``."""
+    from ``row0`` on.  loss: float32, 0-d or (reduction "none") [T]; unit: the rows' own gradients in x, float32, with
+    ``need_unit``."""
     V = int(vocab) if weight is None else weight.shape[0]
     dev, dt, red = _ce_args(x, weight, target, V, reduction)
     x, weight, target = _ce_rows(x), _ce_rows(weight), target.contiguous()
@@ -456,7 +457,7 @@ def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor
     L = _lib.lib()
     aux = torch.empty((2 * T + 1,), dtype=torch.float32, device=dev)
     loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
-    unit = torch.empty((T, R), dtype=x.dtype, device=dev) if need_unit else None
+    unit = torch.empty((T, R), dtype=torch.float32, device=dev) if need_unit else None
     with _on(dev.index):
         ldw = _pitch(weight) if weight is not None else 0
         ws = _workspace(L.rdb_ce_workspace_bytes(_lib.CE_LOSS_GRAD if need_unit else _lib.CE_LOSS, T, R, V, dt, _ptr(weight), ldw), dev)
@@ -467,14 +468,15 @@ def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor
     return loss, aux, unit
 
 
-def ce_scale(unit: torch.Tensor, dloss: torch.Tensor, aux: torch.Tensor, reduction: str) -> torch.Tensor:
+def ce_scale(unit: torch.Tensor, dloss: torch.Tensor, aux: torch.Tensor, reduction: str, dtype: torch.dtype) -> torch.Tensor:
+    """The gradient in x, of type ``dtype``, from the rows' own and the loss's (see rdb_ce_scale)."""
     dev = _need_cuda(unit, dloss, aux)
-    assert unit.is_contiguous() and aux.is_contiguous() and dloss.dtype == torch.float32
+    assert unit.is_contiguous() and unit.dtype == torch.float32 and aux.is_contiguous() and dloss.dtype == torch.float32
     dloss = dloss.contiguous()
     T, R = unit.shape
-    dz = torch.empty_like(unit)
+    dz = torch.empty((T, R), dtype=dtype, device=dev)
     with _on(dev.index):
-        rc = _lib.lib().rdb_ce_scale(_ptr(dz), _ptr(unit), _ptr(dloss), _ptr(aux), T, R, _dt(unit.dtype), _lib.CE_REDUCTIONS[reduction], _raw_stream(dev.index))
+        rc = _lib.lib().rdb_ce_scale(_ptr(dz), _ptr(unit), _ptr(dloss), _ptr(aux), T, R, _dt(dtype), _lib.CE_REDUCTIONS[reduction], _raw_stream(dev.index))
     _lib.check(rc, "rdb_ce_scale")
     return dz
 

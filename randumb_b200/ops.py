@@ -124,27 +124,27 @@ def _(rows, cols, seed, row0, dtype, device):
 def noise_ce_fwd(z: torch.Tensor, target: torch.Tensor, seed: int, out_features: int, row0: int, ignore_index: Optional[int], reduction: str,
                  need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     loss, aux, unit = K.ce_fwd(z, None, target, ignore_index, reduction, seed, out_features, row0, need_grad)
-    return loss, aux, unit if unit is not None else z.new_empty((0,))
+    return loss, aux, unit if unit is not None else aux.new_empty((0,))
 
 
 @noise_ce_fwd.register_fake
 def _(z, target, seed, out_features, row0, ignore_index, reduction, need_grad):
     T = z.shape[0]
     return (z.new_empty((T,) if reduction == "none" else (), dtype=torch.float32), z.new_empty((2 * T + 1,), dtype=torch.float32),
-            z.new_empty(z.shape if need_grad else (0,)))
+            z.new_empty(z.shape if need_grad else (0,), dtype=torch.float32))
 
 
 noise_ce_fwd.register_kernel("cpu")(_cpu_raises("noise_ce_fwd"))
 
 
 @custom_op("rten::noise_ce_bwd", mutates_args=(), device_types="cuda")
-def noise_ce_bwd(dloss: torch.Tensor, unit: torch.Tensor, aux: torch.Tensor, reduction: str) -> torch.Tensor:
-    return K.ce_scale(unit, dloss, aux, reduction)
+def noise_ce_bwd(dloss: torch.Tensor, unit: torch.Tensor, aux: torch.Tensor, reduction: str, dtype: torch.dtype) -> torch.Tensor:
+    return K.ce_scale(unit, dloss, aux, reduction, dtype)
 
 
 @noise_ce_bwd.register_fake
-def _(dloss, unit, aux, reduction):
-    return torch.empty_like(unit)
+def _(dloss, unit, aux, reduction, dtype):
+    return torch.empty_like(unit, dtype=dtype)
 
 
 noise_ce_bwd.register_kernel("cpu")(_cpu_raises("noise_ce_bwd"))
@@ -155,7 +155,7 @@ def _noise_ce_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
     ctx.mark_non_differentiable(aux, unit)
     ctx.save_for_backward(aux, unit)
-    ctx.reduction, ctx.has_unit = inputs[6], inputs[7]
+    ctx.reduction, ctx.has_unit, ctx.dtype = inputs[6], inputs[7], inputs[0].dtype
 
 
 def _noise_ce_backward(ctx, dloss, daux, dunit):
@@ -164,7 +164,7 @@ def _noise_ce_backward(ctx, dloss, daux, dunit):
         return (None,) * 8
     if not ctx.has_unit:
         raise RuntimeError("noise_ce_fwd was called with need_grad=False: it kept nothing for a backward pass")
-    return (noise_ce_bwd(dloss, unit, aux, ctx.reduction),) + (None,) * 7
+    return (noise_ce_bwd(dloss, unit, aux, ctx.reduction, ctx.dtype),) + (None,) * 7
 
 
 noise_ce_fwd.register_autograd(_noise_ce_backward, setup_context=_noise_ce_setup)
@@ -234,14 +234,14 @@ class _NoiseCE(torch.autograd.Function):
     def forward(ctx, z, target, seed, out_features, row0, ignore_index, reduction):
         loss, aux, unit = K.ce_fwd(z, None, target, ignore_index, reduction, seed, out_features, row0, True)
         ctx.save_for_backward(aux, unit)
-        ctx.reduction = reduction
+        ctx.reduction, ctx.dtype = reduction, z.dtype
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         aux, unit = ctx.saved_tensors
-        return K.ce_scale(unit, dloss, aux, ctx.reduction), None, None, None, None, None, None
+        return K.ce_scale(unit, dloss, aux, ctx.reduction, ctx.dtype), None, None, None, None, None, None
 
 
 class _LinearCE(torch.autograd.Function):
