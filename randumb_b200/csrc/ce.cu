@@ -8,8 +8,8 @@
 //
 // so no running maximum is needed: the sum never falls below the target's own 1, and small losses and the gradients of tokens
 // the model already knows come out of log1p and of a sum without the target, not of a difference of nearly equal numbers.  e_v
-// exceeds float32 only where another logit lies more than 69 above the target's (s beyond 2^100); such rows are counted as
-// they are found and done again, one by one, with their true maximum (ce_rescue_kernel).
+// exceeds float32 only where another logit lies more than 69 above the target's (s beyond 2^100); such rows are
+// noticed and done again, one by one, with their true maximum (ce_rescue_row).
 //
 // Rows whose target is ignored are left out: the remaining rows are gathered to the front, and every later kernel works on that
 // many rows, a number that only the device knows.
@@ -626,11 +626,11 @@ __global__ void __launch_bounds__(CE_TILE) ce_tail_kernel(T *__restrict__ out, i
 // rows
 // ================================================================================================
 // Positions of the rows that count, in order: idx[compact] = row, map[row] = compact or -1.  One block; the losses (zero_*, may be
-// null) are cleared at ignored rows, the list of far rows is emptied.
+// null) are cleared at ignored rows, the ticket of the kernel that sums them is reset.
 __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict__ target, int64_t T, int64_t ignore, int use_ignore,
                                                        int32_t *__restrict__ idx, int32_t *__restrict__ map, int32_t *__restrict__ count,
                                                        float *__restrict__ zero_a, float *__restrict__ zero_b, float *__restrict__ zero_c,
-                                                       float *__restrict__ count_f, int32_t *__restrict__ far, int2 *__restrict__ parts,
+                                                       float *__restrict__ count_f, uint32_t *__restrict__ ticket, int2 *__restrict__ parts,
                                                        int64_t cols, int KB, int pairs, int tile_rows) {
     constexpr int PER = 8;
     __shared__ int warp_sum[2][32];
@@ -689,7 +689,7 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const int64_t *__restrict
     }
     if (threadIdx.x == 0) {
         *count = base;
-        *far = 0;
+        *ticket = 0;
         if (count_f) *count_f = (float)base;
     }
 }
@@ -858,38 +858,6 @@ __global__ void __launch_bounds__(256) ce_split_kernel(__nv_bfloat16 *__restrict
 // ================================================================================================
 // finishing
 // ================================================================================================
-// s of 32 rows per block: sixteen threads per row add every sixteenth partial sum, then the sixteen are added in order.
-__global__ void __launch_bounds__(512) ce_sum_kernel(const float *__restrict__ partial, int64_t ld, int nparts, const int32_t *__restrict__ idx,
-                                                     const int32_t *__restrict__ count, const float *__restrict__ lt, float *__restrict__ s_out,
-                                                     float *__restrict__ lse, float *__restrict__ loss, float *__restrict__ loss2,
-                                                     int32_t *__restrict__ far) {
-    __shared__ float sh[16][33];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int64_t j = (int64_t)blockIdx.x * 32 + r, n = *count;
-    if ((int64_t)blockIdx.x * 32 >= n) return;
-    float a = 0.0f;
-    if (j < n) {
-#pragma unroll 8
-        for (int p = g; p < nparts; p += 16) a += partial[(int64_t)p * ld + j];
-    }
-    sh[g][r] = a;
-    __syncthreads();
-    if (g == 0 && j < n) {
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) s += sh[k][r];
-        const float l = log1pf(s);
-        s_out[j] = s;
-        const int32_t row = idx[j];
-        loss[row] = l;
-        if (loss2) loss2[row] = l;
-        lse[row] = lt[j] + l;
-        if (s >= S_LIMIT) far[1 + atomicAdd(far, 1)] = (int32_t)j;    // in any order: each row is redone by itself
-    }
-}
-
 // The parts of row j, column tile n of the x-gradient: `first` is column 0 of the first part, `step` elements lie between the parts.
 struct SlotRow {
     float *first;
@@ -905,96 +873,143 @@ struct SlotRow {
     }
 };
 
-// Rows whose sum left float32's range: logits once more on CUDA cores, first the maximum and the sum relative to it, then (grad)
-// the gradient itself.  One row per block at a time; the row's first slot receives the finished gradient and s becomes -1.
-// far[0] rows, listed behind it.
+// What is known of the rows once all their logits have been seen.
+struct CeSumArgs {
+    CeRowArgs rows;
+    Vocab voc;
+    const float *partial;
+    int64_t ld_partial;
+    int nparts;
+    float *s;                     // per gathered row: s, or -1: its gradient is finished
+    float *lse, *loss_rows, *loss_rows2;
+    float *slots;                 // null: no gradient
+    const int2 *parts;
+    float *loss;                  // null: no total
+    int mean;
+    uint32_t *ticket;             // zero at the start
+};
+
+// A row whose sum left float32's range: its logits once more on CUDA cores, first the maximum and the sum relative to it, then, with
+// slots, the gradient itself, which goes to the row's first slot.  By the whole block.
 template <typename T>
-__global__ void __launch_bounds__(512) ce_rescue_kernel(CeRowArgs a, Vocab voc, float *__restrict__ s_io, float *__restrict__ lse,
-                                                        float *__restrict__ loss, float *__restrict__ loss2, float *__restrict__ slots, const int2 *__restrict__ parts,
-                                                        const int32_t *__restrict__ far) {
+__device__ __noinline__ void ce_rescue_row(const CeSumArgs &g, int64_t j) {
     __shared__ float sh_m[16], sh_s[16], sh_p[16];
-    pdl_launch_dependents();
-    pdl_wait();
+    const CeRowArgs &a = g.rows;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int nfar = far[0];
-    for (int i = blockIdx.x; i < nfar; i += gridDim.x) {
-        const int64_t j = far[1 + i];
-        const int64_t row = a.idx[j], t = a.target[row];
-        const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
-        const float lt = a.lt[j];
-        auto logit = [&](int64_t v) {
-            float d = 0.0f;
-            for (int64_t c = lane; c < a.R; c += 32) d = fmaf(to_f32<T>(x[c]), vocab_at<T>(voc, v, c), d);
+    const int64_t row = a.idx[j], t = a.target[row];
+    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    const float lt = a.lt[j];
+    auto logit = [&](int64_t v) {
+        float d = 0.0f;
+        for (int64_t c = lane; c < a.R; c += 32) d = fmaf(to_f32<T>(x[c]), vocab_at<T>(g.voc, v, c), d);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-            return d;
-        };
-        float m = lt, s = 0.0f;                        // sum of exp(l - m) over the columns other than t, m the maximum so far
-        for (int64_t v = warp; v < a.V; v += 16) {
-            if (v == t) continue;
-            const float l = logit(v);
-            if (l > m) { s = s * expf(m - l) + 1.0f; m = l; }
-            else s += expf(l - m);
-        }
-        if (lane == 0) { sh_m[warp] = m; sh_s[warp] = s; }
-        __syncthreads();
-        float mm = sh_m[0], ss = 0.0f;
-        for (int k = 1; k < 16; ++k) mm = fmaxf(mm, sh_m[k]);
-        for (int k = 0; k < 16; ++k) ss += sh_s[k] * expf(sh_m[k] - mm);
-        const float full = mm + logf(ss + expf(lt - mm));
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            loss[row] = full - lt;
-            if (loss2) loss2[row] = full - lt;
-            lse[row] = full;
-            s_io[j] = -1.0f;
-        }
-        if (slots) {
-            const int tiles_n = (int)((a.R + CE_TILE - 1) / CE_TILE);
-            const float pt = expf(lt - full);
-            for (int nt = 0; nt < tiles_n; ++nt) {                // columns of one tile at a time
-                const SlotRow o(slots, parts, tiles_n, a.tile_rows, j, nt);
-                const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
-                const bool mine = threadIdx.x < CE_TILE && c < a.R;
-                float acc = mine ? (pt - 1.0f) * vocab_at<T>(voc, t, c) : 0.0f;
-                for (int64_t v0 = 0; v0 < a.V; v0 += 16) {
-                    const int64_t v = v0 + warp;
-                    float p = 0.0f;
-                    if (v < a.V && v != t) p = expf(logit(v) - full);
-                    if (lane == 0) sh_p[warp] = p;
-                    __syncthreads();
-                    if (mine) {
+        for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        return d;
+    };
+    float m = lt, s = 0.0f;                        // sum of exp(l - m) over the columns other than t, m the maximum so far
+    for (int64_t v = warp; v < a.V; v += 16) {
+        if (v == t) continue;
+        const float l = logit(v);
+        if (l > m) { s = s * expf(m - l) + 1.0f; m = l; }
+        else s += expf(l - m);
+    }
+    __syncthreads();                               // the row before is done with the arrays
+    if (lane == 0) { sh_m[warp] = m; sh_s[warp] = s; }
+    __syncthreads();
+    float mm = sh_m[0], ss = 0.0f;
+    for (int k = 1; k < 16; ++k) mm = fmaxf(mm, sh_m[k]);
+    for (int k = 0; k < 16; ++k) ss += sh_s[k] * expf(sh_m[k] - mm);
+    const float full = mm + logf(ss + expf(lt - mm));
+    if (threadIdx.x == 0) {
+        g.loss_rows[row] = full - lt;
+        if (g.loss_rows2) g.loss_rows2[row] = full - lt;
+        g.lse[row] = full;
+        g.s[j] = -1.0f;
+    }
+    if (!g.slots) return;
+    const int tiles_n = (int)((a.R + CE_TILE - 1) / CE_TILE);
+    const float pt = expf(lt - full);
+    for (int nt = 0; nt < tiles_n; ++nt) {         // columns of one tile at a time
+        const SlotRow o(g.slots, g.parts, tiles_n, a.tile_rows, j, nt);
+        const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
+        const bool mine = threadIdx.x < CE_TILE && c < a.R;
+        float acc = mine ? (pt - 1.0f) * vocab_at<T>(g.voc, t, c) : 0.0f;
+        for (int64_t v0 = 0; v0 < a.V; v0 += 16) {
+            const int64_t v = v0 + warp;
+            float p = 0.0f;
+            if (v < a.V && v != t) p = expf(logit(v) - full);
+            if (lane == 0) sh_p[warp] = p;
+            __syncthreads();
+            if (mine) {
 #pragma unroll 1
-                        for (int k = 0; k < 16; ++k)
-                            if (sh_p[k] != 0.0f) acc = fmaf(sh_p[k], vocab_at<T>(voc, v0 + k, c), acc);
-                    }
-                    __syncthreads();
-                }
-                if (mine) o.first[threadIdx.x] = acc;
+                for (int k = 0; k < 16; ++k)
+                    if (sh_p[k] != 0.0f) acc = fmaf(sh_p[k], vocab_at<T>(g.voc, v0 + k, c), acc);
             }
+            __syncthreads();
         }
-        __syncthreads();
+        if (mine) o.first[threadIdx.x] = acc;
     }
 }
 
-// ignored rows hold 0: all T are added, in one fixed order
-__global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__ loss_rows, int64_t T, const int32_t *__restrict__ count,
-                                                       float *__restrict__ loss, int mean) {
-    __shared__ double sh[32];
+// s, log-sum-exp and loss of 32 rows per block: sixteen threads per row add every sixteenth partial sum, then the sixteen are added in
+// order; rows beyond float32's range are redone.  The block that finishes last adds up the losses of all rows (ignored ones hold
+// 0) in one fixed order.
+template <typename T>
+__global__ void __launch_bounds__(512) ce_sum_kernel(const CeSumArgs g) {
+    __shared__ float sh[16][33];
+    __shared__ double sh_d[16];
+    __shared__ unsigned far;
+    __shared__ bool last;
     pdl_launch_dependents();
     pdl_wait();
+    const int r = threadIdx.x & 31, grp = threadIdx.x >> 5;
+    const int64_t j0 = (int64_t)blockIdx.x * 32, j = j0 + r, n = *g.rows.count;
+    if (j0 < n) {
+        float a = 0.0f;
+        if (j < n) {
+#pragma unroll 8
+            for (int p = grp; p < g.nparts; p += 16) a += g.partial[(int64_t)p * g.ld_partial + j];
+        }
+        sh[grp][r] = a;
+        __syncthreads();
+        if (grp == 0) {
+            float s = 0.0f;
+            if (j < n) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) s += sh[k][r];
+                const float l = log1pf(s);
+                const int32_t row = g.rows.idx[j];
+                g.s[j] = s;
+                g.loss_rows[row] = l;
+                if (g.loss_rows2) g.loss_rows2[row] = l;
+                g.lse[row] = g.rows.lt[j] + l;
+            }
+            const unsigned f = __ballot_sync(0xffffffffu, s >= S_LIMIT);     // not-a-number is the answer already
+            if (r == 0) far = f;
+        }
+        __syncthreads();
+        for (unsigned f = far; f; f &= f - 1) ce_rescue_row<T>(g, j0 + __ffs(f) - 1);
+    }
+    if (!g.loss) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(g.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
     double a = 0.0;
 #pragma unroll 8
-    for (int64_t i = threadIdx.x; i < T; i += 1024) a += (double)loss_rows[i];
+    for (int64_t i = threadIdx.x; i < g.rows.T; i += 512) a += (double)__ldcg(g.loss_rows + i);
 #pragma unroll
     for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
+    if (r == 0) sh_d[grp] = a;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        a = sh[threadIdx.x];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-        if (threadIdx.x == 0) *loss = (float)(mean ? a / (double)*count : a);
+    if (threadIdx.x == 0) {
+        a = 0.0;
+        for (int k = 0; k < 16; ++k) a += sh_d[k];
+        *g.loss = (float)(g.mean ? a / (double)n : a);
     }
 }
 
@@ -1033,7 +1048,7 @@ __global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(O *_
             if (s) {
                 sj = s[j];
                 const int32_t t = tcol[j];
-                if (sj < 0.0f) {                      // the row was finished by ce_rescue_kernel
+                if (sj < 0.0f) {                      // the row was finished by ce_rescue_row
                     n = 1;
                     sj = 0.0f;
                 } else {
@@ -1140,7 +1155,7 @@ struct CePlan {
     bool dw_direct;
     int64_t ld_dw;
     // workspace
-    size_t idx, map, count, off2, lt, scale, tval, tcol, s, far, a, b, e, partial, slots, parts_at, dw, tail, total;
+    size_t idx, map, count, off2, lt, scale, tval, tcol, s, ticket, a, b, e, partial, slots, parts_at, dw, tail, total;
     bool slots_used;
 };
 
@@ -1192,7 +1207,7 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     p.tcol = take((size_t)p.Mpad * 4);
     p.lt = take((size_t)p.Mpad * 4);
     p.s = take((size_t)p.Mpad * 4);
-    p.far = take((size_t)p.Mpad * 4 + 4);
+    p.ticket = take(16);
     p.scale = take(op == 2 ? (size_t)p.Mpad * 4 : 0);
     p.tval = take(op == 2 ? (size_t)p.Mpad * 4 : 0);
     p.a = take((size_t)p.Mpad * p.lda * 2);
@@ -1265,7 +1280,7 @@ struct CeCall {
 
 static int ce_find_rows(const CeCall &c, int64_t ignore, int use_ignore, float *zero_a, float *zero_b, float *zero_c, float *count_f) {
     return launch_pdl(ce_rows_kernel, dim3(1), 1024, 0, c.st, c.target, c.T, ignore, use_ignore, c.at<int32_t>(c.p.idx), c.at<int32_t>(c.p.map),
-                      c.at<int32_t>(c.p.count), zero_a, zero_b, zero_c, count_f, c.at<int32_t>(c.p.far), c.p.slots_used ? c.at<int2>(c.p.parts_at) : (int2 *)nullptr, c.R, ce_kb(c.p),
+                      c.at<int32_t>(c.p.count), zero_a, zero_b, zero_c, count_f, c.at<uint32_t>(c.p.ticket), c.p.slots_used ? c.at<int2>(c.p.parts_at) : (int2 *)nullptr, c.R, ce_kb(c.p),
                       c.p.pairs, c.p.tile_rows);
 }
 
@@ -1460,7 +1475,7 @@ static int ce_check(int64_t T, int64_t R, int64_t V, int64_t ldx, const void *w,
 using namespace rdb;
 
 extern "C" size_t rdb_ce_workspace_bytes(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw) {
-    if (op < RDB_CE_LOSS || op > RDB_CE_GRADS || ce_check(T, R, V, R, w, ldw, dtype, RDB_CE_SUM) != RDB_OK || T == 0) return 1024;
+    if (op < RDB_CE_LOSS || op > RDB_CE_GRADS || ce_check(T, R, V, R, w, ldw, dtype, RDB_CE_SUM) != RDB_OK) return 1024;
     return ce_plan(op, T, R, V, dtype, w, ldw, nullptr, 1, 1).total;
 }
 
@@ -1477,7 +1492,7 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, float *dx_unit, const void *x
         return RDB_ERR_ALIGN;
     CeCall c{};
     c.p = ce_plan(dx_unit ? 1 : 0, T, R, V, dtype, w, ldw, nullptr, 1, 0);
-    if (!workspace || workspace_bytes < (T ? c.p.total : 1024) || (reinterpret_cast<uintptr_t>(workspace) & 255)) return RDB_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < c.p.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return RDB_ERR_WORKSPACE;
     c.ws = reinterpret_cast<uint8_t *>(workspace);
     c.x = x; c.ldx = ldx; c.T = T; c.R = R; c.V = V;
     c.voc = Vocab{w, ldw, seed, (uint32_t)row0};
@@ -1501,22 +1516,28 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, float *dx_unit, const void *x
                 if ((rc = ce_accumulate(c, b, ldb, n, i > 0))) return rc;
             } else if ((rc = ce_logits<EPI_SUM>(c, b, ldb, v0, n, i))) return rc;
         }
-        // row sums: a full piece leaves two per column tile; without the gradient the last piece has only the tiles that exist
-        const int64_t last = V - (c.p.npieces - 1) * c.p.piece;
-        int32_t *far = c.at<int32_t>(c.p.far);
-        const int nparts = (int)((c.p.npieces - 1) * (c.p.piece / CE_TILE) * 2 + (dx_unit ? c.p.piece / CE_TILE : cdiv64(last, CE_TILE)) * 2);
-        rc = launch_pdl(ce_sum_kernel, dim3((unsigned)(c.p.Mpad / 32)), 512, 0, c.st, (const float *)c.at<float>(c.p.partial), c.p.Mpad, nparts, ra.idx,
-                        ra.count, (const float *)ra.lt, c.at<float>(c.p.s), lse, rows, rows2, far);
-        if (rc) return rc;
-        float *slots = dx_unit ? c.at<float>(c.p.slots) : nullptr, *sums = c.at<float>(c.p.s);
-        const int2 *parts = c.at<int2>(c.p.parts_at);
-        rc = dtype == RDB_F32 ? launch_pdl(ce_rescue_kernel<float>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, parts, (const int32_t *)far)
-                              : launch_pdl(ce_rescue_kernel<__nv_bfloat16>, dim3(148), 512, 0, c.st, ra, c.voc, sums, lse, rows, rows2, slots, parts, (const int32_t *)far);
-        if (rc) return rc;
-        if (dx_unit && (rc = ce_finish_dx(c, dx_unit, true))) return rc;
     }
-    if (reduction == RDB_CE_NONE) return RDB_OK;
-    return launch_pdl(ce_loss_kernel, dim3(1), 1024, 0, c.st, (const float *)rows, T, (const int32_t *)c.at<int32_t>(c.p.count), loss, reduction == RDB_CE_MEAN ? 1 : 0);
+    // row sums: a full piece leaves two per column tile; without the gradient the last piece has only the tiles that exist
+    const int64_t last = V - (c.p.npieces - 1) * c.p.piece;
+    CeSumArgs g{};
+    g.rows = ce_row_args(c);
+    g.voc = c.voc;
+    g.partial = c.at<float>(c.p.partial);
+    g.ld_partial = c.p.Mpad;
+    g.nparts = (int)((c.p.npieces - 1) * (c.p.piece / CE_TILE) * 2 + (dx_unit ? c.p.piece / CE_TILE : cdiv64(last, CE_TILE)) * 2);
+    g.s = c.at<float>(c.p.s);
+    g.lse = lse;
+    g.loss_rows = rows;
+    g.loss_rows2 = rows2;
+    g.slots = dx_unit ? c.at<float>(c.p.slots) : nullptr;
+    g.parts = c.at<int2>(c.p.parts_at);
+    g.loss = reduction == RDB_CE_NONE ? nullptr : loss;
+    g.mean = reduction == RDB_CE_MEAN ? 1 : 0;
+    g.ticket = c.at<uint32_t>(c.p.ticket);
+    const dim3 grid((unsigned)(T ? c.p.Mpad / 32 : 1));
+    rc = dtype == RDB_F32 ? launch_pdl(ce_sum_kernel<float>, grid, 512, 0, c.st, g) : launch_pdl(ce_sum_kernel<__nv_bfloat16>, grid, 512, 0, c.st, g);
+    if (rc || T == 0 || !dx_unit) return rc;
+    return ce_finish_dx(c, dx_unit, true);
 }
 
 extern "C" int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x, int64_t ldx, const void *w, int64_t ldw, const int64_t *target,
