@@ -604,22 +604,41 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
 }
 
-// Output rows of the tiles whose contraction was cut (CeArgs::tail): their parts, added in order.
+// Output rows of the tiles whose contraction was cut (CeArgs::tail): their parts, added in order.  A block takes four rows, a thread
+// four columns of one.
 template <typename T>
-__global__ void __launch_bounds__(CE_TILE) ce_tail_kernel(T *__restrict__ out, int64_t ldo, const float *__restrict__ slots, int64_t M, int64_t N,
-                                                          int64_t first, int parts, int tile_rows) {
+__global__ void __launch_bounds__(256) ce_tail_kernel(T *__restrict__ out, int64_t ldo, const float *__restrict__ slots, int64_t M, int64_t N,
+                                                      int first, int parts, int tile_rows) {
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t tiles_n = (N + CE_TILE - 1) / CE_TILE;
-    const int64_t i = blockIdx.x / tile_rows, r = blockIdx.x % tile_rows;
-    const int64_t tile = first + i;
-    const int64_t row = tile / tiles_n * tile_rows + r, col = tile % tiles_n * CE_TILE + threadIdx.x;
+    const int tiles_n = (int)((N + CE_TILE - 1) / CE_TILE);
+    const int r4 = tile_rows / 4, i = blockIdx.x / r4;
+    const int r = (blockIdx.x % r4) * 4 + (threadIdx.x >> 6), cl = (threadIdx.x & 63) * 4;
+    const int tile = first + i;
+    const int64_t row = (int64_t)(tile / tiles_n) * tile_rows + r, col = (int64_t)(tile % tiles_n) * CE_TILE + cl;
     if (row >= M || col >= N) return;
-    const float *p = slots + (i * parts * tile_rows + r) * CE_TILE + threadIdx.x;
-    float v = *p;
+    const float *p = slots + ((int64_t)i * parts * tile_rows + r) * CE_TILE + cl;
+    float4 v = *reinterpret_cast<const float4 *>(p);
 #pragma unroll 4
-    for (int k = 1; k < parts; ++k) v += p[(int64_t)k * tile_rows * CE_TILE];
-    out[row * ldo + col] = from_f32<T>(v);
+    for (int k = 1; k < parts; ++k) {
+        const float4 u = *reinterpret_cast<const float4 *>(p + (int64_t)k * tile_rows * CE_TILE);
+        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    T *o = out + row * ldo + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (col + e < N) o[e] = from_f32<T>(f[e]);
+}
+
+// rows of a padded matrix to a dense one whose rows start on no vector boundary
+template <typename T>
+__global__ void __launch_bounds__(256) ce_copy_kernel(T *__restrict__ dst, const T *__restrict__ src, int64_t rows, int64_t cols, int64_t ld) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    for (int64_t c = threadIdx.x & 63; c < cols; c += 64) dst[r * cols + c] = src[r * ld + c];
 }
 
 // ================================================================================================
@@ -842,16 +861,26 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) 
     }
 }
 
-// rows of the matrix in bf16 parts, zero between R and part_cols
+// rows of the matrix in bf16 parts, zero between R and part_cols; a thread takes eight columns of a row
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(256) ce_split_kernel(__nv_bfloat16 *__restrict__ dst, int64_t ldd, int64_t part_cols, int64_t rows, int64_t R,
                                                        int64_t v0, Vocab voc) {
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t total = rows * part_cols;
+    const uint32_t per = (uint32_t)(part_cols / 8);
+    const int64_t total = rows * per;
+    const bool vec = voc.w && rows_aligned<T>(voc.w, voc.ldw);
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / part_cols, c = i - r * part_cols;
-        split_store<PARTS>(dst + r * ldd, part_cols, c, c < R ? vocab_at<T>(voc, v0 + r, c) : 0.0f);
+        const int64_t r = i >> 32 ? i / per : (uint32_t)i / per;
+        const int64_t c = (i - r * per) * 8;
+        float f[8];
+        if (vec && c + 8 <= R) {
+            load_f8(f, reinterpret_cast<const T *>(voc.w) + (v0 + r) * voc.ldw + c);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = c + k < R ? vocab_at<T>(voc, v0 + r, c + k) : 0.0f;
+        }
+        split_store8<PARTS>(dst + r * ldd + c, part_cols, f);
     }
 }
 
@@ -1319,7 +1348,7 @@ static int ce_stage(const CeCall &c, int64_t v0, int64_t n, const void **base, i
     *ld = c.p.lda;
     if (!c.voc.w && c.dtype == RDB_BF16)
         return rdb_noise(b, RDB_BF16, n, c.R, c.p.lda, (int64_t)c.voc.row0 + v0, 0, c.voc.seed, c.st);
-    const int64_t want = cdiv64(n * c.p.Rp, 256 * 4);
+    const int64_t want = cdiv64(n * c.p.Rp / 8, 256);
     const dim3 grid((unsigned)(want < 148 * 8 ? (want < 1 ? 1 : want) : 148 * 8));
     if (c.dtype == RDB_F32) return launch_pdl(ce_split_kernel<float, 3>, grid, 256, 0, c.st, b, c.p.lda, c.p.Rp, n, c.R, v0, c.voc);
     return launch_pdl(ce_split_kernel<__nv_bfloat16, 1>, grid, 256, 0, c.st, b, c.p.lda, c.p.Rp, n, c.R, v0, c.voc);
@@ -1430,14 +1459,23 @@ static int ce_dw(const CeCall &c, void *dw, int64_t v0, int64_t n) {
          : tile_rows == CE_TILE ? launch_pair<1, 1, EPI_BF16, 1, 1>(ta, tb, td, ts, a, items, p.pairs, c.st)
                                 : launch_pair<1, 1, EPI_BF16, 1, 2>(ta, tb, td, ts, a, items, p.pairs, c.st);
     if (rc) return rc;
-    if (a.tail) {
-        const dim3 grid((unsigned)(a.tail * tile_rows));
-        rc = c.dtype == RDB_F32 ? launch_pdl(ce_tail_kernel<float>, grid, CE_TILE, 0, c.st, (float *)out, ldd, (const float *)tail, n, c.R, tiles - a.tail, a.tail_parts, tile_rows)
-                                : launch_pdl(ce_tail_kernel<__nv_bfloat16>, grid, CE_TILE, 0, c.st, (__nv_bfloat16 *)out, ldd, (const float *)tail, n, c.R, tiles - a.tail, a.tail_parts, tile_rows);
+    uint8_t *mine = static_cast<uint8_t *>(dw) + (size_t)v0 * c.R * es;
+    if (!p.dw_direct && tiles > a.tail) {
+        // whole tiles came to the padded copy: as many rows as have one
+        const int64_t rows = round_up(tiles - a.tail, cdiv64(c.R, CE_TILE)) / cdiv64(c.R, CE_TILE) * tile_rows;
+        const int64_t m = rows < n ? rows : n;
+        const dim3 grid((unsigned)cdiv64(m, 4));
+        rc = c.dtype == RDB_F32 ? launch_pdl(ce_copy_kernel<float>, grid, 256, 0, c.st, (float *)mine, (const float *)out, m, c.R, ldd)
+                                : launch_pdl(ce_copy_kernel<__nv_bfloat16>, grid, 256, 0, c.st, (__nv_bfloat16 *)mine, (const __nv_bfloat16 *)out, m, c.R, ldd);
+        if (rc) return rc;
     }
-    if (rc || p.dw_direct) return rc;
-    cudaError_t e = cudaMemcpy2DAsync(static_cast<uint8_t *>(dw) + (size_t)v0 * c.R * es, c.R * es, out, ldd * es, c.R * es, n, cudaMemcpyDeviceToDevice, c.st);
-    return e == cudaSuccess ? RDB_OK : (int)e;
+    if (a.tail) {
+        const dim3 grid((unsigned)(a.tail * (tile_rows / 4)));
+        const int first = (int)(tiles - a.tail);
+        rc = c.dtype == RDB_F32 ? launch_pdl(ce_tail_kernel<float>, grid, 256, 0, c.st, (float *)mine, c.R, (const float *)tail, n, c.R, first, a.tail_parts, tile_rows)
+                                : launch_pdl(ce_tail_kernel<__nv_bfloat16>, grid, 256, 0, c.st, (__nv_bfloat16 *)mine, c.R, (const float *)tail, n, c.R, first, a.tail_parts, tile_rows);
+    }
+    return rc;
 }
 
 static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
