@@ -319,7 +319,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, c
     StepScalars c{};
     c.eps = s.eps;
     c.fast = s.eps > 1e-30f;
-    float t_have = -1.0f;
+    float t_have = NAN;
     int ti = 0;
     for (uint32_t g = blockIdx.x * (ADAMW_THREADS / 32) + (threadIdx.x >> 5); g < segs; g += warps) {
         while (g >= tab.first[ti + 1]) ++ti;

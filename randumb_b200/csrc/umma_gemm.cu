@@ -1466,7 +1466,11 @@ static EncodeTiledFn encode_fn() {
 static void ensure_context() {
     thread_local bool done = false;
     if (!done) {
+        // not an operation of a stream, but one that a capture in its strict mode would be invalidated by
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        (void)cudaThreadExchangeStreamCaptureMode(&mode);
         (void)cudaFree(nullptr);
+        (void)cudaThreadExchangeStreamCaptureMode(&mode);
         done = true;
     }
 }

@@ -441,7 +441,10 @@ def _ce_args(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tens
 
 
 def _ce_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or _rows_ok(t) else t.contiguous()
+    """The matrix itself when its rows are dense and follow one another at some pitch, else a contiguous copy."""
+    if t is None or t.is_contiguous() or (t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1])):
+        return t
+    return t.contiguous()
 
 
 def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor, ignore_index: Optional[int] = -100, reduction: str = "mean",

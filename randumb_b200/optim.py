@@ -57,69 +57,85 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     seed        of the random rounding of the 8-bit second moments.
     grad_scale  one-element float32 CUDA tensor the gradients are multiplied with (the factor ``grad_norm`` returns).
     """
-    n = len(params)
-    if n == 0:
+    if len(params) == 0:
         return
-    dev = params[0].get_device()
-    if dev < 0:
-        raise RuntimeError("randumb_b200 kernels run on CUDA tensors only (no CPU implementation)")
-    pd = _uniform("params", params, _PARAM, n, dev)
-    gd = _uniform("grads", grads, _GRAD, n, dev)
-    eight = exp_avg_scales is not None or exp_avg_sq_scales is not None
-    if eight and (exp_avg_scales is None or exp_avg_sq_scales is None):
-        raise RuntimeError("adamw_step: 8-bit moments need exp_avg_scales and exp_avg_sq_scales")
-    _uniform("exp_avgs", exp_avgs, _E4M3 if eight else _F32, n, dev)
-    _uniform("exp_avg_sqs", exp_avg_sqs, _U8 if eight else _F32, n, dev)
-    numels = [t.numel() for t in params]
-    lists = [params, grads, exp_avgs, exp_avg_sqs]
-    names = ["param", "grad", "exp_avg", "exp_avg_sq"]
-    if masters is not None:
-        _uniform("masters", masters, _F32, n, dev)
-        if pd != torch.bfloat16:
-            raise RuntimeError("adamw_step: masters are the float32 copies of bfloat16 params")
-        lists.append(masters)
-        names.append("master")
-    for what, ts in zip(names[1:], lists[1:]):
-        if [t.numel() for t in ts] != numels:
-            raise RuntimeError(f"adamw_step: {what}s and params differ in size")
-    if eight:
-        blocks = [-(-k // BLOCK) for k in numels]
-        for what, ts in (("exp_avg_scale", exp_avg_scales), ("exp_avg_sq_scale", exp_avg_sq_scales)):
-            _uniform(what + "s", ts, _F32, n, dev)
-            if [t.numel() for t in ts] != blocks:
-                raise RuntimeError(f"adamw_step: scales hold one value per {BLOCK} elements of their tensor")
-            lists.append(ts)
-            names.append(what)
-    if isinstance(steps, torch.Tensor):
-        if steps.dtype != torch.float32 or steps.get_device() != dev or steps.numel() != n or not steps.is_contiguous():
-            raise RuntimeError(f"adamw_step: steps must be {n} contiguous float32 counts on cuda:{dev}")
-        at = steps.data_ptr()
-        sp = list(range(at, at + 4 * n, 4))
-    else:
-        _uniform("steps", steps, _F32, n, dev)
-        if any([t.numel() != 1 for t in steps]):
-            raise RuntimeError("adamw_step: every tensor has one step count")
-        sp = [t.data_ptr() for t in steps]
-    _one_float("grad_scale", grad_scale, dev)
-    lr_dev = None
-    if isinstance(lr, torch.Tensor):
-        _one_float("lr", lr, dev)
-        lr, lr_dev = 0.0, lr.data_ptr()
-    words = [t.data_ptr() for t in params]
-    if len(set(words)) != n and len({a for a, k in zip(words, numels) if k}) != sum(1 for k in numels if k):
-        raise RuntimeError("adamw_step: a param is in the list twice")
-    for ts in lists[1:]:
-        words += [t.data_ptr() for t in ts]
-    words += sp
-    words += numels
-    table = array("Q", words)                              # one list behind the other, in host memory
-    base = table.buffer_info()[0]
-    arg = _lib.AdamwLists(n=n, **{name: base + 8 * n * i for i, name in enumerate(names + ["step", "numel"])})
-    h = _lib.AdamwHyper(float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), lr_dev, K._seed(seed))
-    with K._on(dev):
-        rc = _lib.lib().rdb_adamw_step(ctypes.byref(arg), K._dt(pd), K._dt(gd), 8 if eight else 32, ctypes.byref(h), K._ptr(grad_scale),
-                                       K._raw_stream(dev))
-    _lib.check(rc, "rdb_adamw_step")
+    state = _State(params, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales)
+    state.launch(params, grads, lr, betas, eps, weight_decay, seed, grad_scale)
+
+
+class _State:
+    """What a list of parameters keeps between steps, checked once: moments, scales, masters and counts."""
+
+    def __init__(self, params, exp_avgs, exp_avg_sqs, steps, masters=None, exp_avg_scales=None, exp_avg_sq_scales=None):
+        n = self.n = len(params)
+        dev = self.dev = params[0].get_device()
+        if dev < 0:
+            raise RuntimeError("randumb_b200 kernels run on CUDA tensors only (no CPU implementation)")
+        self.dtype = _uniform("params", params, _PARAM, n, dev)
+        eight = self.eight = exp_avg_scales is not None or exp_avg_sq_scales is not None
+        if eight and (exp_avg_scales is None or exp_avg_sq_scales is None):
+            raise RuntimeError("adamw_step: 8-bit moments need exp_avg_scales and exp_avg_sq_scales")
+        _uniform("exp_avgs", exp_avgs, _E4M3 if eight else _F32, n, dev)
+        _uniform("exp_avg_sqs", exp_avg_sqs, _U8 if eight else _F32, n, dev)
+        numels = self.numels = [t.numel() for t in params]
+        lists = [("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)]
+        if masters is not None:
+            _uniform("masters", masters, _F32, n, dev)
+            if self.dtype != torch.bfloat16:
+                raise RuntimeError("adamw_step: masters are the float32 copies of bfloat16 params")
+            lists.append(("master", masters))
+        for what, ts in lists:
+            if [t.numel() for t in ts] != numels:
+                raise RuntimeError(f"adamw_step: {what}s and params differ in size")
+        if eight:
+            blocks = [-(-k // BLOCK) for k in numels]
+            for what, ts in (("exp_avg_scale", exp_avg_scales), ("exp_avg_sq_scale", exp_avg_sq_scales)):
+                _uniform(what + "s", ts, _F32, n, dev)
+                if [t.numel() for t in ts] != blocks:
+                    raise RuntimeError(f"adamw_step: scales hold one value per {BLOCK} elements of their tensor")
+                lists.append((what, ts))
+        if isinstance(steps, torch.Tensor):
+            if steps.dtype != torch.float32 or steps.get_device() != dev or steps.numel() != n or not steps.is_contiguous():
+                raise RuntimeError(f"adamw_step: steps must be {n} contiguous float32 counts on cuda:{dev}")
+            at = steps.data_ptr()
+            words = list(range(at, at + 4 * n, 4))
+        else:
+            _uniform("steps", steps, _F32, n, dev)
+            if any([t.numel() != 1 for t in steps]):
+                raise RuntimeError("adamw_step: every tensor has one step count")
+            words = [t.data_ptr() for t in steps]
+        words += numels
+        for _, ts in lists:
+            words += [t.data_ptr() for t in ts]
+        self.names = ["step", "numel"] + [what for what, _ in lists]
+        self.words = array("Q", words)                         # one list behind the other, in host memory
+        self.keep = (steps, [ts for _, ts in lists])           # the tensors the addresses belong to
+        self.some = sum(1 for k in numels if k)
+
+    def launch(self, params, grads, lr, betas, eps, weight_decay, seed, grad_scale) -> None:
+        n, dev = self.n, self.dev
+        if _uniform("params", params, _PARAM, n, dev) != self.dtype or [t.numel() for t in params] != self.numels:
+            raise RuntimeError("adamw_step: params changed their type or size")
+        gd = _uniform("grads", grads, _GRAD, n, dev)
+        if [t.numel() for t in grads] != self.numels:
+            raise RuntimeError("adamw_step: grads and params differ in size")
+        pp = [t.data_ptr() for t in params]
+        if len(set(pp)) != n and len({a for a, k in zip(pp, self.numels) if k}) != self.some:
+            raise RuntimeError("adamw_step: a param is in the list twice")
+        _one_float("grad_scale", grad_scale, dev)
+        lr_dev = None
+        if isinstance(lr, torch.Tensor):
+            _one_float("lr", lr, dev)
+            lr, lr_dev = 0.0, lr.data_ptr()
+        pp += [t.data_ptr() for t in grads]
+        moving = array("Q", pp)
+        base, held = moving.buffer_info()[0], self.words.buffer_info()[0]
+        arg = _lib.AdamwLists(n=n, param=base, grad=base + 8 * n, **{name: held + 8 * n * i for i, name in enumerate(self.names)})
+        h = _lib.AdamwHyper(float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), lr_dev, K._seed(seed))
+        with K._on(dev):
+            rc = _lib.lib().rdb_adamw_step(ctypes.byref(arg), K._dt(self.dtype), K._dt(gd), 8 if self.eight else 32, ctypes.byref(h),
+                                           K._ptr(grad_scale), K._raw_stream(dev))
+        _lib.check(rc, "rdb_adamw_step")
 
 
 def _one_float(what: str, t: Optional[torch.Tensor], dev: int) -> None:
@@ -199,6 +215,7 @@ class AdamW(torch.optim.Optimizer):
         if max_grad_norm is not None and not max_grad_norm >= 0.0:
             raise ValueError(f"invalid max_grad_norm: {max_grad_norm}")
         self.max_grad_norm, self.seed, self.last_grad_norm = max_grad_norm, int(seed), None
+        self._lists: dict = {}                                      # (group, kind) -> state tensors of the parameters with a gradient, their lists
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights))
 
     def _new_state(self, p: torch.Tensor, group: dict) -> dict:
@@ -219,6 +236,25 @@ class AdamW(torch.optim.Optimizer):
             st["master"] = p.detach().float()
         return st
 
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        self._lists = {}
+
+    def _state_of(self, key, params: list, group: dict, master: bool) -> _State:
+        """The checked lists of these parameters' states; kept while the same parameters have gradients and the same tensors as state."""
+        sts = [self.state[p] for p in params]
+        have = self._lists.get(key)
+        parts = [v for s in sts for v in s.values()]
+        if have is not None and len(have[0]) == len(parts) and all([a is b for a, b in zip(have[0], parts)]):
+            return have[1]
+        eight = {}
+        if group["state_bits"] == 8:
+            eight = dict(exp_avg_scales=[s["exp_avg_scale"] for s in sts], exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in sts])
+        made = _State([_flat(p) for p in params], [_flat(s["exp_avg"]) for s in sts], [_flat(s["exp_avg_sq"]) for s in sts], [s["step"] for s in sts],
+                      [_flat(s["master"]) for s in sts] if master else None, **eight)
+        self._lists[key] = (parts, made)
+        return made
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -229,35 +265,37 @@ class AdamW(torch.optim.Optimizer):
         for gi, group in enumerate(self.param_groups):
             kinds: dict = {}
             for p in group["params"]:
-                if p.grad is None:
-                    continue
-                if p.grad.is_sparse:
-                    raise RuntimeError("AdamW does not take sparse gradients")
-                if not self.state[p]:
-                    self.state[p].update(self._new_state(p, group))
                 g = p.grad
-                if g.stride() != p.stride() or g.dtype not in (torch.float32, torch.bfloat16):
-                    g = torch.empty_like(p).copy_(g)               # the parameter's own order of elements
-                kinds.setdefault((p.device, p.dtype, g.dtype, "master" in self.state[p]), []).append((p, _flat(g)))
-            for kind, pairs in kinds.items():
-                todo.append((gi, group, kind, pairs))
-                all_grads.setdefault(kind[0], []).extend(g for _, g in pairs)
-        scales = {}
+                if g is None:
+                    continue
+                st = self.state[p]
+                if not st:
+                    if g.is_sparse:
+                        raise RuntimeError("AdamW does not take sparse gradients")
+                    st.update(self._new_state(p, group))
+                if p.is_contiguous() and g.is_contiguous() and g.dtype in _GRAD:
+                    flat, g = p, g.detach()
+                else:
+                    if g.is_sparse:
+                        raise RuntimeError("AdamW does not take sparse gradients")
+                    if g.stride() != p.stride() or g.dtype not in _GRAD:
+                        g = torch.empty_like(p).copy_(g)               # the parameter's own order of elements
+                    flat, g = _flat(p), _flat(g)
+                ps, flats, gs = kinds.setdefault((p.device, p.dtype, g.dtype, "master" in st), ([], [], []))
+                ps.append(p)
+                flats.append(flat)
+                gs.append(g)
+            for kind, (ps, flats, gs) in kinds.items():
+                todo.append((gi, group, kind, ps, flats, gs))
+                all_grads.setdefault(kind[0], []).extend(gs)
+        scale = None
         if self.max_grad_norm is not None and all_grads:
             if len(all_grads) > 1:
                 raise RuntimeError("max_grad_norm: the parameters must live on one device")
-            for dev, grads in all_grads.items():
-                self.last_grad_norm, scales[dev] = grad_norm(grads, self.max_grad_norm)
-        for k, (gi, group, kind, pairs) in enumerate(todo):
-            states = [self.state[p] for p, _ in pairs]
-            eight = {}
-            if group["state_bits"] == 8:
-                eight = dict(exp_avg_scales=[s["exp_avg_scale"] for s in states], exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states],
-                             seed=self.seed + 0x632BE5AB * k)
-            adamw_step([_flat(p) for p, _ in pairs], [g for _, g in pairs], [_flat(s["exp_avg"]) for s in states],
-                       [_flat(s["exp_avg_sq"]) for s in states], [s["step"] for s in states], lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                       weight_decay=group["weight_decay"], masters=[_flat(s["master"]) for s in states] if kind[3] else None,
-                       grad_scale=scales.get(kind[0]), **eight)
+            self.last_grad_norm, scale = grad_norm(next(iter(all_grads.values())), self.max_grad_norm)
+        for k, (gi, group, kind, ps, flats, gs) in enumerate(todo):
+            self._state_of((gi,) + kind, ps, group, kind[3]).launch(flats, gs, group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                                                                    self.seed + 0x632BE5AB * k, scale)
         return loss
 
     def load_state_dict(self, state_dict) -> None:
@@ -266,6 +304,7 @@ class AdamW(torch.optim.Optimizer):
         torch.optim.AdamW does not have keeps this optimiser's values, and its float32 moments load into 32-bit ones."""
         here = [dict(g) for g in self.param_groups]
         super().load_state_dict(state_dict)
+        self._lists = {}
         for group, old in zip(self.param_groups, here):
             for k in ("state_bits", "master_weights"):
                 group.setdefault(k, old[k])

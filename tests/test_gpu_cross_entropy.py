@@ -316,6 +316,86 @@ def test_captured_and_on_a_side_stream(rb):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_capture_as_the_first_call_of_a_process():
+    """Forward and backward captured before the library has been used: nothing in a first call may disturb a capture."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, randumb_b200 as rb
+x = torch.randn(70, 64, device="cuda").bfloat16().requires_grad_()
+w = torch.randn(300, 64, device="cuda").bfloat16().requires_grad_()
+t = torch.randint(0, 300, (70,), device="cuda")
+rb.kernels.status_buffer(x.device)
+st = torch.cuda.Stream()
+st.wait_stream(torch.cuda.current_stream())
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=st):
+    out = [rb.linear_cross_entropy(x, w, t), *torch.autograd.grad(rb.linear_cross_entropy(x, w, t), [x, w]),
+           *torch.autograd.grad(rb.noise_cross_entropy(x, 5, 300, t), x)]
+g.replay()
+torch.cuda.synchronize()
+want = [rb.linear_cross_entropy(x, w, t), *torch.autograd.grad(rb.linear_cross_entropy(x, w, t), [x, w]),
+        *torch.autograd.grad(rb.noise_cross_entropy(x, 5, 300, t), x)]
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_one_row_of_a_strided_matrix(rb):
+    x, w, target = inputs("linear", 1, 128, 50, torch.bfloat16, 1)
+    wide = torch.zeros(1, 256, device="cuda", dtype=torch.bfloat16)
+    wide[:, ::2] = x
+    assert torch.equal(rb.linear_cross_entropy(wide[:, ::2], w, target), rb.linear_cross_entropy(x, w, target))
+    one = w[:1].clone()
+    widew = torch.zeros(1, 256, device="cuda", dtype=torch.bfloat16)
+    widew[:, ::2] = one
+    z = torch.zeros(1, dtype=torch.int64, device="cuda")
+    assert rb.linear_cross_entropy(x, widew[:, ::2], z).item() == 0.0
+
+
+def test_two_streams_at_once(rb):
+    """Two calls whose kernels may run side by side give what they give alone."""
+    sets = [inputs("linear", 900, 128, 5003, torch.bfloat16, s) for s in (1, 2)]
+    alone = [_value(rb, *s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for st, s, out in zip(streams, sets, outs):
+            with torch.cuda.stream(st):
+                out.append(_value(rb, *s))
+    torch.cuda.synchronize()
+    for a, out in zip(alone, outs):
+        for o in out:
+            assert all(torch.equal(x, y) for x, y in zip(a, o))
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+def test_operators_through_the_dispatcher(rb, kind):
+    """rten::*_ce_*: schema, fake kernels and autograd registration; the same numbers as the eager functions."""
+    x, w, target = inputs(kind, 60, 40, 90, torch.float32, 3)
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    checks = ("test_schema", "test_faketensor", "test_autograd_registration")
+    if kind == "noise":
+        args = (xl, target, 1003, 90, 5, -100, "mean", True)
+        torch.library.opcheck(torch.ops.rten.noise_ce_fwd.default, args, test_utils=checks)
+        loss = torch.ops.rten.noise_ce_fwd(*args)[0]
+        leaves = [xl]
+    else:
+        args = (xl, wl, target, -100, "mean")
+        torch.library.opcheck(torch.ops.rten.linear_ce_fwd.default, args, test_utils=checks)
+        loss = torch.ops.rten.linear_ce_fwd(*args)[0]
+        leaves = [xl, wl]
+    grads = torch.autograd.grad(loss, leaves)
+    x2, w2 = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss2 = call(rb, kind, x2, w2, target, 3)
+    grads2 = torch.autograd.grad(loss2, [x2] if kind == "noise" else [x2, w2])
+    assert torch.equal(loss, loss2) and all(torch.equal(a, b) for a, b in zip(grads, grads2))
+
+
 @pytest.mark.parametrize("dtype,tol", [(torch.bfloat16, 2e-2), (torch.float32, 2e-5)])
 def test_layer_loss(rb, dtype, tol):
     """RandumbLinear.cross_entropy against the layer's weight in 64 bits.  bf16: z and dz are rounded to bf16 on the way, as the

@@ -302,3 +302,54 @@ def test_refusals(rb):
         step([p], [g], [m.to(torch.float8_e4m3fn)], [v.to(torch.uint8)], s, exp_avg_scales=[m[:2]], exp_avg_sq_scales=[m[:1]])
     step([], [], [], [], s)
     assert p.abs().sum() == 0
+
+
+def test_more_tensors_than_one_launch_holds(rb):
+    """500 tensors, some empty, in 8 bits and 32: each as if it were alone (tensor i of the list rounds with its own seed)."""
+    sizes = [(7 * i) % 600 for i in range(500)]
+    g = torch.Generator().manual_seed(2)
+    p0 = [torch.randn(k, generator=g).cuda() for k in sizes]
+    gr = [torch.randn(k, generator=g).cuda() for k in sizes]
+    for bits in (32, 8):
+        def state():
+            if bits == 32:
+                return [torch.zeros(k, device="cuda") for k in sizes], [torch.zeros(k, device="cuda") for k in sizes], {}
+            m = [torch.zeros(k, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for k in sizes]
+            v = [torch.zeros(k, dtype=torch.uint8, device="cuda") for k in sizes]
+            return m, v, dict(exp_avg_scales=[torch.zeros(-(-k // 256), device="cuda") for k in sizes],
+                              exp_avg_sq_scales=[torch.zeros(-(-k // 256), device="cuda") for k in sizes])
+        p = [t.clone() for t in p0]
+        m, v, sc = state()
+        steps = torch.zeros(500, device="cuda")
+        rb.optim.adamw_step(p, gr, m, v, steps, lr=1e-2, seed=11, **sc)
+        assert (steps == 1).all()
+        q = [t.clone() for t in p0]
+        m2, v2, sc2 = state()
+        s2 = [torch.zeros((), device="cuda") for _ in sizes]
+        for i in (1, 44, 383, 384, 385, 499):
+            one = {k: [x[i]] for k, x in sc2.items()}
+            # tensor i of a list of its own rounds with seed + i * 0x85EBCA6B
+            rb.optim.adamw_step([q[i]], [gr[i]], [m2[i]], [v2[i]], [s2[i]], lr=1e-2, seed=11 + i * 0x85EBCA6B, **one)
+            assert torch.equal(p[i], q[i]) and torch.equal(m[i].view(torch.uint8), m2[i].view(torch.uint8)) and torch.equal(v[i], v2[i])
+
+
+def test_optimizer_follows_its_parameters(rb):
+    """Between steps a parameter's storage is exchanged, another gets its first gradient, one group is added."""
+    a, b, c = (torch.nn.Parameter(torch.ones(k, device="cuda")) for k in (300, 40, 5))
+    opt = rb.optim.AdamW([a, b], lr=0.1, weight_decay=0.0)
+    ref = [torch.nn.Parameter(torch.ones(k, device="cuda")) for k in (300, 40, 5)]
+    topt = torch.optim.AdamW(ref[:2], lr=0.1, weight_decay=0.0)
+    for k in range(5):
+        for p, r in zip((a, b, c), ref):
+            if p is not b or k >= 2:
+                p.grad = torch.full_like(p, 0.5 + k)
+                r.grad = p.grad.clone()
+        if k == 3:
+            a.data = a.data.clone()
+            opt.add_param_group({"params": [c], "lr": 0.01, "weight_decay": 0.0})
+            topt.add_param_group({"params": [ref[2]], "lr": 0.01, "weight_decay": 0.0})
+        opt.step()
+        topt.step()
+        for p, r in zip((a, b, c), ref):
+            # a few roundings of values of size 1 in either program
+            assert (p - r).abs().max() < 8 * 2.0 ** -23
