@@ -813,10 +813,12 @@ def gpt2_whole_step(args, dev, world, rank, rb, randumb_ms):
             self.ln_f = nn.LayerNorm(d)
             self.lm_head = nn.Linear(d, vocab, bias=False)
 
-        def forward(self, idx, targets):
+        def forward(self, idx, targets, own=False):
             x = self.wte(idx) + self.wpe(torch.arange(idx.shape[1], device=idx.device))
             for blk in self.blocks:
                 x = blk(x)
+            if own:
+                return rb.linear_cross_entropy(self.ln_f(x), self.lm_head.weight, targets)
             logits = self.lm_head(self.ln_f(x))
             return F.cross_entropy(logits.float().view(-1, vocab), targets.view(-1))
 
@@ -831,17 +833,19 @@ def gpt2_whole_step(args, dev, world, rank, rb, randumb_ms):
     idx_host = torch.randint(0, vocab, (B, S), generator=g).pin_memory()
     tgt_host = torch.randint(0, vocab, (B, S), generator=g).pin_memory()
     out = {}
-    for variant in ("frozen", "all_trainable"):
+    for variant in ("frozen", "all_trainable", "all_trainable_own_loss_and_adamw"):
+        own = variant.endswith("own_loss_and_adamw")
         for n, p in model.named_parameters():
-            p.requires_grad_(variant == "all_trainable" or n.endswith("weight_coef"))
+            p.requires_grad_(variant.startswith("all_trainable") or n.endswith("weight_coef"))
             p.grad = None
         params = [p for p in model.parameters() if p.requires_grad]
-        opt = torch.optim.Adam(params, lr=1e-4, fused=True)
+        opt = rb.optim.AdamW(params, lr=1e-4, weight_decay=0.0) if own else torch.optim.Adam(params, lr=1e-4, fused=True)
+        torch.cuda.reset_peak_memory_stats()
 
         def step():
             idx = idx_host.to(dev, non_blocking=True)
             tgt = tgt_host.to(dev, non_blocking=True)
-            loss = model(idx, tgt)
+            loss = model(idx, tgt, own)
             loss.backward()
             if world > 1:
                 rb.parallel.allreduce_coef_grads(params)          # one flat bucket: the coefficients, or every weight
@@ -870,11 +874,13 @@ def gpt2_whole_step(args, dev, world, rank, rb, randumb_ms):
         ms = float(t.item())
         out[variant] = {"ms_per_step": ms, "tokens_per_s": world * B * S / (ms * 1e-3),
                         "trainable_parameters": sum(p.numel() for p in params), "loss": first_loss,
+                        "peak_memory_gb": torch.cuda.max_memory_allocated() / 1e9,
                         "pseudorandom_layers_share": randumb_ms / ms}
         del opt
     out["what"] = ("GPT-2-small-shaped step (12 blocks, d 768, 12 heads, MLP 3072, vocabulary 50257, 8 x 1024 tokens per GPU): forward, "
                    "cross-entropy, backward, flat gradient all-reduce, fused Adam; 'frozen' trains the 24 coefficient matrices only (the "
-                   "all-reduce carries only dC), 'all_trainable' every weight.  pseudorandom_layers_share = the 24 layers' own time "
+                   "all-reduce carries only dC), 'all_trainable' every weight, '..._own_loss_and_adamw' the same with linear_cross_entropy and "
+                   "optim.AdamW (32-bit moments, float32 masters).  pseudorandom_layers_share = the 24 layers' own time "
                    "(this line's ms_per_step) over the whole step; the rest is PyTorch's attention, layer norms, dense projections, "
                    "embedding and loss kernels")
     out["expected_initial_loss"] = "about ln(50257) = 10.82 for random weights (modded-nanogpt/train_gpt2.py:241 of the reference)"
