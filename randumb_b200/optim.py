@@ -175,14 +175,22 @@ def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -
 
 
 def second_moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
-    """float32 values of an 8-bit second moment (uint8 codes of ``adamw_step`` and their scales), in the shape of ``codes``."""
-    v = (codes.reshape(-1).to(torch.int32) << 19).view(torch.float32) * 2.0 ** 112
-    return (v * scales.repeat_interleave(BLOCK)[:v.numel()]).reshape(codes.shape)
+    """float32 values of an 8-bit second moment (uint8 codes of ``adamw_step`` and their scales), laid out like ``codes``."""
+    flat = _flat(codes)
+    v = (flat.to(torch.int32) << 19).view(torch.float32) * 2.0 ** 112
+    return _like(codes, v * scales.repeat_interleave(BLOCK)[:v.numel()].view(v.shape))
 
 
 def first_moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
-    """float32 values of an 8-bit first moment (float8_e4m3fn codes of ``adamw_step`` and their scales)."""
-    return (codes.reshape(-1).float() * scales.repeat_interleave(BLOCK)[:codes.numel()]).reshape(codes.shape)
+    """float32 values of an 8-bit first moment (float8_e4m3fn codes of ``adamw_step`` and their scales), laid out like ``codes``."""
+    v = _flat(codes).float()
+    return _like(codes, v * scales.repeat_interleave(BLOCK)[:v.numel()].view(v.shape))
+
+
+def _like(codes: torch.Tensor, values: torch.Tensor) -> torch.Tensor:
+    out = torch.empty_like(codes, dtype=torch.float32)
+    _flat(out).copy_(values)
+    return out
 
 
 class AdamW(torch.optim.Optimizer):

@@ -253,6 +253,10 @@ def test_optimizer_class(rb):
                 ps = ps2
         assert opt.state[ps[0]]["step"].item() == 4 and opt.state[ps[2]]["step"].item() == 3
         assert opt.state[ps[1]]["exp_avg"].stride() == ps[1].stride()
+        if bits == 8:                                              # the channels-last moment decodes in its own layout, near the float32 one
+            st, want = opt.state[ps[1]], topt.state[ref[1]]["exp_avg"]
+            got = rb.optim.first_moment_values(st["exp_avg"], st["exp_avg_scale"])
+            assert got.stride() == ps[1].stride() and (got - want).norm() < 0.1 * want.norm()
         for i, (p, r) in enumerate(zip(ps, ref)):
             got = opt.state[p]["master"] if "master" in opt.state[p] else p
             # each of the four updates is at most lr * (1 + a few) in size; 8-bit moments are within 2^-4 (first), and the second's random rounding
