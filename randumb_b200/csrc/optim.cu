@@ -2,7 +2,7 @@
 //
 // One launch walks up to NT_LARGE tensors: their pointers travel in the kernel's parameters.  The tensors are cut into segments of
 // 256 elements, the warps of the grid take segments in turn (each by itself: no barrier), and since a warp's segments only move
-// forward, the tensor of the next one is found by stepping on from the last one's.  256 consecutive elements share the scale of an
+// forward, the tensor of the next one is found by stepping on from the last one's (of the first by bisection).  256 consecutive elements share the scale of an
 // 8-bit moment, so its maximum is one shuffle reduction and nothing is read twice.  Arithmetic is float32; what the 8-bit
 // moments are made of has one rounding per operation as written (no contraction), so their bytes follow from the inputs alone.
 //
@@ -43,7 +43,7 @@ struct AdamwTable {
 
 struct AdamwScalars {
     float b1, omb1, b2, omb2, eps;
-    double lr, beta1, beta2;
+    double lr, ln_beta1, ln_beta2;         // natural logarithms; -inf for 0
     const float *lr_dev;                  // one float32 in device memory, or null: `lr`
     double weight_decay;
     uint32_t seed;
@@ -283,6 +283,7 @@ __device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, i
     }
 }
 
+// the tensor that part `chunk` belongs to (the last one when there is none)
 template <typename Table>
 __device__ __forceinline__ int find_tensor(const Table &tab, uint32_t chunk) {
     int lo = 0, hi = tab.count - 1;
@@ -320,15 +321,16 @@ adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, c
     c.eps = s.eps;
     c.fast = s.eps > 1e-30f;
     float t_have = NAN;
-    int ti = 0;
-    for (uint32_t g = blockIdx.x * (ADAMW_THREADS / 32) + (threadIdx.x >> 5); g < segs; g += warps) {
+    uint32_t g = blockIdx.x * (ADAMW_THREADS / 32) + (threadIdx.x >> 5);
+    int ti = find_tensor(tab, g);
+    for (; g < segs; g += warps) {
         while (g >= tab.first[ti + 1]) ++ti;
         const AdamwDesc &d = tab.t[ti];
         const float t = *d.step;
         if (t != t_have) {                // bias corrections of this step, in float64; tensors that began together share them
             const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
-            c.size = (float)(lr / (1.0 - pow(s.beta1, (double)t)));
-            c.inv_root = (float)(1.0 / sqrt(1.0 - pow(s.beta2, (double)t)));
+            c.size = (float)(lr / -expm1((double)t * s.ln_beta1));            // 1 - beta^t
+            c.inv_root = 1.0f / sqrtf((float)-expm1((double)t * s.ln_beta2));
             c.decay = (float)(1.0 - lr * s.weight_decay);
             t_have = t;
         }
@@ -540,8 +542,8 @@ extern "C" int rdb_adamw_step(const rdb_adamw_lists *lists, int param_dtype, int
     s.omb2 = (float)(1.0 - h->beta2);
     s.eps = (float)h->eps;
     s.lr = h->lr;
-    s.beta1 = h->beta1;
-    s.beta2 = h->beta2;
+    s.ln_beta1 = log(h->beta1);
+    s.ln_beta2 = log(h->beta2);
     s.lr_dev = h->lr_dev;
     s.weight_decay = h->weight_decay;
     s.seed = h->seed;

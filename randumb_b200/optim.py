@@ -60,7 +60,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if len(params) == 0:
         return
     state = _State(params, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales)
-    state.launch(params, grads, lr, betas, eps, weight_decay, seed, grad_scale)
+    state.launch(params, grads, lr, betas, eps, weight_decay, seed, grad_scale, fresh=True)
 
 
 class _State:
@@ -112,9 +112,9 @@ class _State:
         self.keep = (steps, [ts for _, ts in lists])           # the tensors the addresses belong to
         self.some = sum(1 for k in numels if k)
 
-    def launch(self, params, grads, lr, betas, eps, weight_decay, seed, grad_scale) -> None:
+    def launch(self, params, grads, lr, betas, eps, weight_decay, seed, grad_scale, fresh: bool = False) -> None:
         n, dev = self.n, self.dev
-        if _uniform("params", params, _PARAM, n, dev) != self.dtype or [t.numel() for t in params] != self.numels:
+        if not fresh and (_uniform("params", params, _PARAM, n, dev) != self.dtype or [t.numel() for t in params] != self.numels):
             raise RuntimeError("adamw_step: params changed their type or size")
         gd = _uniform("grads", grads, _GRAD, n, dev)
         if [t.numel() for t in grads] != self.numels:
