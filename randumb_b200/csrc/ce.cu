@@ -26,8 +26,8 @@
 // The products run on CTA pairs (cta_group::2).  bf16: 512 x 256 tiles, two 256 x 256 accumulators that fill TMEM and take MMAs in
 // turn, four 48 KB stages of TMA-fed operands; an epilogue warp takes its 32 rows x 128 columns of an accumulator into registers,
 // hands the accumulator back and computes from the registers, and the MMA thread runs ahead on the first accumulator while the
-// second is still being read.  (256 x 256 tiles, whose MMAs all go to one accumulator, kept the tensor pipe 62 % busy.)  At most 256
-// rows: 256 x 256 tiles, six 32 KB stages.  float32: the same, and the accumulators, whose additions cut instead of rounding (about
+// second is still being read.  (256 x 256 tiles, whose MMAs all go to one accumulator, kept the tensor pipe 62 % busy.)  Few rows
+// (ce_tile_rows): 256 x 256 tiles, six 32 KB stages.  float32: the same, and the accumulators, whose additions cut instead of rounding (about
 // 2^-26 of the sum per 16 products, all in one direction), are added up in the epilogue's registers every eight k-blocks.
 #include <atomic>
 #include <cmath>
@@ -1195,13 +1195,23 @@ static int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 static int ce_kb(const CePlan &p) { return p.nterm * (int)cdiv64(p.piece, BK); }     // k-blocks of the x-gradient's product
 
+// Rows per tile.  float32: 256 (the registers hold one sub-tile).  bf16: 512-row tiles are the faster ones where rows fill them (8192
+// rows; 4000 of R = 1024, V = 50257, loss and gradient: 683 against 724 us), by about a tenth: 256-row tiles win when they round the
+// rows up to a tenth less (600 rows: 183 against 214; 2100: 410 against 454; 1200: even), and for short contractions of few rows, where
+// the exponentials bound the logits and twice the tiles spread better (R = 200, V = 32003: 512 rows 61 against 64, 1600 rows 99 against
+// 106, 2100 rows 117 against 125; 4000 rows 177 against 173).
+static int ce_tile_rows(int64_t T, int64_t R, int dtype) {
+    if (dtype == RDB_F32) return CE_TILE;
+    const int64_t r256 = round_up(T, CE_TILE), r512 = round_up(T, 2 * CE_TILE);
+    return r256 * 11 < r512 * 10 || (R <= 512 && T <= 2048) ? CE_TILE : 2 * CE_TILE;
+}
+
 // op 0: loss; 1: loss and unit gradient of x (noise); 2: gradients of a stored matrix
 static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw, const void *dw, int want_dx, int want_dw) {
     CePlan p{};
     p.parts = dtype == RDB_F32 ? 3 : 1;
     p.nterm = dtype == RDB_F32 ? 6 : 1;
-    // 512-row tiles unless all rows fit 256 or the numbers are float32 (see the top)
-    p.tile_rows = p.parts == 3 || T <= CE_TILE ? CE_TILE : 2 * CE_TILE;
+    p.tile_rows = ce_tile_rows(T, R, dtype);
     p.Mpad = round_up(T, p.tile_rows);
     p.Rp = round_up(R, p.parts == 3 ? 64 : 8);
     p.lda = p.Rp * p.parts;

@@ -115,7 +115,7 @@ def check(rb, kind, x, w, target, seed, ignore, reduction, gout=None):
 
 
 SHAPES = [(1, 8, 1), (1, 128, 50257), (2, 1, 3), (3, 5, 300), (31, 64, 256), (128, 72, 257), (129, 256, 1000), (255, 250, 511), (257, 264, 513),
-          (600, 40, 2049), (1000, 513, 777), (2048, 128, 4096)]
+          (600, 40, 2049), (1000, 513, 777), (2048, 128, 4096), (2500, 136, 700)]
 
 
 @pytest.mark.parametrize("kind", ["noise", "linear"])
