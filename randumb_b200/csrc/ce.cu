@@ -7,9 +7,11 @@
 //   d loss / dx = (sum over v != t of e_v w_v  -  s w_t) / (1 + s)
 //
 // so no running maximum is needed: the sum never falls below the target's own 1, and small losses and the gradients of tokens
-// the model already knows come out of log1p and of a sum without the target, not of a difference of nearly equal numbers.  e_v
-// exceeds float32 only where another logit lies more than 69 above the target's (s beyond 2^100); such rows are
-// noticed and done again, one by one, with their true maximum (ce_rescue_row).
+// the model already knows come out of log1p and of a sum without the target, not of a difference of nearly equal numbers.  Float32
+// holds e_v up to 69 above the target's logit (s below 2^100 leaves room for the gradient).  Where the row's length says that the
+// largest of V random logits will lie 40 or more above the target's (|x| |w_t| / sqrt(R) is their standard deviation, times sqrt(2 ln
+// V)), that estimate takes the target's place:  e_v = exp(l_v - l_t - d),  loss = log(s + exp(-d)) + d.  A row that leaves the range
+// all the same, at either end, is noticed and done again with its true maximum (ce_rescue_row).
 //
 // Rows whose target is ignored are left out: the remaining rows are gathered to the front, and every later kernel works on that
 // many rows, a number that only the device knows.
@@ -741,7 +743,8 @@ struct CeRowArgs {
     const int32_t *idx, *count;
     __nv_bfloat16 *a;             // gathered rows [rows, PARTS * part_cols]
     int64_t lda, part_cols;
-    float *off2, *lt, *scale, *tval;
+    float *off2, *lt, *dist, *scale, *tval;
+    float spread;                 // sqrt(2 ln V)
     int32_t *tcol;
     // backward
     const float *dloss;           // null: forward
@@ -813,7 +816,7 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) 
     const bool known = t >= 0 && t < a.V;
     const bool dot_it = !a.dloss && known;
     const T *src = reinterpret_cast<const T *>(a.x) + row * a.ldx;
-    float dot = 0.0f;
+    float dot = 0.0f, xx = 0.0f, ww = 0.0f;
     // the same order of additions whether or not the operands start on vector boundaries
     const bool vx = rows_aligned<T>(a.x, a.ldx), vw = voc.w && rows_aligned<T>(voc.w, voc.ldw);
     const T *wrow = reinterpret_cast<const T *>(voc.w) + (voc.w && dot_it ? t * voc.ldw : 0);
@@ -835,23 +838,39 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) 
                     w[k] = voc.w ? to_f32<T>(wrow[c + k]) : to_f32<T>(from_f32<T>(sq5_to_float(sq5_tail(lin.base + ((uint32_t)c + k) * lin.sk))));
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) dot = fmaf(f[k], w[k], dot);
+            for (int k = 0; k < 8; ++k) {
+                dot = fmaf(f[k], w[k], dot);
+                xx = fmaf(f[k], f[k], xx);
+                ww = fmaf(w[k], w[k], ww);
+            }
         }
         split_store8<PARTS>(dst + c, a.part_cols, f);
     }
     for (int64_t c = done + lane; c < a.part_cols; c += 32) {
         const float v = c < a.R ? to_f32<T>(src[c]) : 0.0f;
         split_store<PARTS>(dst, a.part_cols, c, v);
-        if (dot_it && c < a.R) dot = fmaf(v, vocab_at<T>(voc, t, c), dot);
+        if (dot_it && c < a.R) {
+            const float w = vocab_at<T>(voc, t, c);
+            dot = fmaf(v, w, dot);
+            xx = fmaf(v, v, xx);
+            ww = fmaf(w, w, ww);
+        }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    for (int o = 16; o; o >>= 1) {
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        xx += __shfl_xor_sync(0xffffffffu, xx, o);
+        ww += __shfl_xor_sync(0xffffffffu, ww, o);
+    }
     if (lane == 0) {
         a.tcol[j] = known ? (int32_t)t : -1;
         if (!a.dloss) {
             if (!known) dot = NAN;                    // a target outside the vocabulary: the row's loss says so
+            const float top = sqrtf(xx) * sqrtf(ww / (float)a.R) * a.spread;
+            const float d = top - dot >= 40.0f && top < 1e6f ? top - dot : 0.0f;
             a.lt[j] = dot;
-            a.off2[j] = dot * LOG2E;
+            a.dist[j] = d;
+            a.off2[j] = (dot + d) * LOG2E;
         } else {
             const float g = a.reduction == RDB_CE_NONE ? a.dloss[row] : a.reduction == RDB_CE_MEAN ? a.dloss[0] / (float)n : a.dloss[0];
             a.off2[j] = a.lse[row] * LOG2E;
@@ -1003,17 +1022,20 @@ __global__ void __launch_bounds__(512) ce_sum_kernel(const CeSumArgs g) {
         __syncthreads();
         if (grp == 0) {
             float s = 0.0f;
+            bool lost = false;
             if (j < n) {
 #pragma unroll
                 for (int k = 0; k < 16; ++k) s += sh[k][r];
-                const float l = log1pf(s);
+                const float d = g.rows.dist[j], total = s + expf(-d);
+                const float l = d == 0.0f ? log1pf(s) : logf(total) + d;
+                lost = s >= S_LIMIT || total < 1.0f / S_LIMIT;          // not-a-number is the answer already
                 const int32_t row = g.rows.idx[j];
                 g.s[j] = s;
                 g.loss_rows[row] = l;
                 if (g.loss_rows2) g.loss_rows2[row] = l;
                 g.lse[row] = g.rows.lt[j] + l;
             }
-            const unsigned f = __ballot_sync(0xffffffffu, s >= S_LIMIT);     // not-a-number is the answer already
+            const unsigned f = __ballot_sync(0xffffffffu, lost);
             if (r == 0) far = f;
         }
         __syncthreads();
@@ -1053,12 +1075,12 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&f)[4]) {
 __device__ __forceinline__ void store4(float *p, const float (&f)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]); }
 template <typename T, typename O, int ROWS>
 __global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(O *__restrict__ dx, float *__restrict__ slots, const int2 *__restrict__ parts,
-                                                       const int32_t *__restrict__ map, const float *__restrict__ s, const int32_t *__restrict__ tcol,
-                                                       Vocab voc, int64_t T_rows, int64_t R, int tile_rows, int tiles_n) {
+                                                       const int32_t *__restrict__ map, const float *__restrict__ s, const float *__restrict__ dist,
+                                                       const int32_t *__restrict__ tcol, Vocab voc, int64_t T_rows, int64_t R, int tile_rows, int tiles_n) {
     __shared__ const float *sh_at[ROWS];
     __shared__ int sh_parts[ROWS];
     __shared__ uint32_t sh_hash[ROWS];             // noise word position of the target's row, column 0
-    __shared__ float sh_s[ROWS], sh_inv[ROWS];  // v -> (v - s w_t) inv
+    __shared__ float sh_s[ROWS], sh_inv[ROWS];  // v -> (v - s w_t) / (s + exp(-d))
     __shared__ int64_t sh_step;
     pdl_launch_dependents();
     pdl_wait();
@@ -1081,7 +1103,7 @@ __global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(O *_
                     n = 1;
                     sj = 0.0f;
                 } else {
-                    inv = t >= 0 ? 1.0f / (1.0f + sj) : NAN;
+                    inv = t >= 0 ? 1.0f / (expf(-dist[j]) + sj) : NAN;
                 }
                 sh_hash[threadIdx.x] = sq5_lin_rows(voc.seed, voc.row0 + (uint32_t)t, 0u).base;
             }
@@ -1184,7 +1206,7 @@ struct CePlan {
     bool dw_direct;
     int64_t ld_dw;
     // workspace
-    size_t idx, map, count, off2, lt, scale, tval, tcol, s, ticket, a, b, e, partial, slots, parts_at, dw, tail, total;
+    size_t idx, map, count, off2, lt, dist, scale, tval, tcol, s, ticket, a, b, e, partial, slots, parts_at, dw, tail, total;
     bool slots_used;
 };
 
@@ -1245,6 +1267,7 @@ static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const 
     p.off2 = take((size_t)p.Mpad * 4);
     p.tcol = take((size_t)p.Mpad * 4);
     p.lt = take((size_t)p.Mpad * 4);
+    p.dist = take((size_t)p.Mpad * 4);
     p.s = take((size_t)p.Mpad * 4);
     p.ticket = take(16);
     p.scale = take(op == 2 ? (size_t)p.Mpad * 4 : 0);
@@ -1333,6 +1356,8 @@ static CeRowArgs ce_row_args(const CeCall &c) {
     a.lda = c.p.lda; a.part_cols = c.p.Rp;
     a.off2 = c.at<float>(c.p.off2);
     a.lt = c.at<float>(c.p.lt);
+    a.dist = c.at<float>(c.p.dist);
+    a.spread = (float)sqrt(2.0 * log((double)c.V));
     a.scale = c.at<float>(c.p.scale);
     a.tval = c.at<float>(c.p.tval);
     a.tcol = c.at<int32_t>(c.p.tcol);
@@ -1491,7 +1516,7 @@ static int ce_dw(const CeCall &c, void *dw, int64_t v0, int64_t n) {
 static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
     const CePlan &p = c.p;
     const int tiles_n = (int)cdiv64(c.R, CE_TILE);
-    const float *s = unit ? c.at<float>(p.s) : nullptr;
+    const float *s = unit ? c.at<float>(p.s) : nullptr, *dist = c.at<float>(p.dist);
     const int32_t *map = c.at<int32_t>(p.map), *tcol = c.at<int32_t>(p.tcol);
     const int2 *parts = c.at<int2>(p.parts_at);
     float *slots = c.at<float>(p.slots);
@@ -1499,7 +1524,7 @@ static int ce_finish_dx(const CeCall &c, void *dx, bool unit) {
     const int rows = cdiv64(c.T, 16) * tiles_n >= 4 * 148 ? 16 : 4;
     const dim3 grid((unsigned)(cdiv64(c.T, rows) * tiles_n));
     auto go = [&](auto kern, auto *out) {
-        return launch_pdl(kern, grid, CE_TILE, 0, c.st, out, slots, parts, map, s, tcol, c.voc, c.T, c.R, p.tile_rows, tiles_n);
+        return launch_pdl(kern, grid, CE_TILE, 0, c.st, out, slots, parts, map, s, dist, tcol, c.voc, c.T, c.R, p.tile_rows, tiles_n);
     };
     using H = __nv_bfloat16;
     if (c.dtype == RDB_F32) return rows == 16 ? go(ce_dx_kernel<float, float, 16>, (float *)dx) : go(ce_dx_kernel<float, float, 4>, (float *)dx);

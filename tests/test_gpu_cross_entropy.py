@@ -170,10 +170,12 @@ def test_no_row_counts(rb, kind):
 
 @pytest.mark.parametrize("kind", ["noise", "linear"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_logits_far_above_the_target(rb, kind, dtype):
+@pytest.mark.parametrize("shape", [(300, 128, 900), (2500, 520, 600)])
+def test_logits_far_above_the_target(rb, kind, dtype, shape):
     """Rows whose sum relative to the target's logit leaves float32 (other logits hundreds above it), beside ordinary rows and rows
     that the model knows almost for sure."""
-    T, R, V, seed = 300, 128, 900, 8
+    T, R, V = shape
+    seed = 8
     x, w, target = inputs(kind, T, R, V, dtype, seed)
     far = torch.arange(0, T, 7, device="cuda")
     sure = torch.arange(3, T, 7, device="cuda")
@@ -182,6 +184,18 @@ def test_logits_far_above_the_target(rb, kind, dtype):
     x[sure] = (w[target[sure]].float() / norm[target[sure]] * torch.linspace(15, 300, sure.numel(), device="cuda")[:, None]).to(dtype)
     loss, grads = check(rb, kind, x, w, target, seed, -100, "none", torch.ones(T, device="cuda"))
     assert loss[far].max() > 300 and loss[sure].min() < 1e-6
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("std", [15.0, 40.0, 300.0])
+def test_logits_of_large_scale(rb, kind, dtype, std):
+    """Logits spread far wider than a trained model's: the largest lies 60, 150 or 1000 above the target's in an ordinary row."""
+    T, R, V, seed = 400, 200, 3000, 12
+    x, w, target = inputs(kind, T, R, V, dtype, seed, std)
+    x[::50] *= 0.01
+    loss, _ = check(rb, kind, x, w, target, seed, -100, "none", torch.ones(T, device="cuda"))
+    assert loss.median() > 2 * std
 
 
 def test_target_outside_the_vocabulary(rb):
@@ -240,12 +254,13 @@ def test_only_what_is_asked_for(rb):
 
 
 @pytest.mark.parametrize("kind", ["noise", "linear"])
-def test_several_pieces_and_repeatability(rb, kind):
+@pytest.mark.parametrize("T,R,V,dtype", [(40000, 64, 20000, torch.bfloat16), (30000, 250, 20000, torch.bfloat16), (20000, 36, 8100, torch.float32)])
+def test_several_pieces_and_repeatability(rb, kind, T, R, V, dtype):
     """Enough rows that the vocabulary is taken in several pieces; the same call gives the same bits."""
-    T, R, V, seed = 40000, 64, 20000, 11
+    seed = 11
     g = torch.Generator(device="cuda").manual_seed(1)
-    x = (torch.randn(T, R, device="cuda", generator=g) * (3.0 / R) ** 0.5 * 2).bfloat16()
-    w = (noise_matrix(V, R, 1000 + seed, 5, torch.bfloat16).cuda() if kind == "noise" else (torch.randn(V, R, device="cuda", generator=g) * 2 / R ** 0.5).bfloat16())
+    x = (torch.randn(T, R, device="cuda", generator=g) * (3.0 / R) ** 0.5 * 2).to(dtype)
+    w = (noise_matrix(V, R, 1000 + seed, 5, dtype).cuda() if kind == "noise" else (torch.randn(V, R, device="cuda", generator=g) * 2 / R ** 0.5).to(dtype))
     target = torch.randint(0, V, (T,), device="cuda", generator=g)
     target[torch.rand(T, device="cuda", generator=g) < 0.2] = -100
     out = []
@@ -258,12 +273,25 @@ def test_several_pieces_and_repeatability(rb, kind):
     xs, ws = x.float().requires_grad_(), w.float().requires_grad_()
     want = F.cross_entropy(xs @ ws.t(), target)
     gx, gw = torch.autograd.grad(want, [xs, ws])
-    # norms: rounding errors of single elements average out; 2^-8 covers the two bf16 roundings
+    # norms: rounding errors of single elements average out; 2^-8 covers the two bf16 roundings; float32 either side's sums of up to 20000 terms
+    tol = 2.0 ** -8 if dtype == torch.bfloat16 else 1e-5
     assert abs(out[0][0].item() / want.item() - 1) < 1e-5
-    assert O.rel_fro(out[0][1].float().cpu(), gx.cpu()) < 2.0 ** -8
+    assert O.rel_fro(out[0][1].float().cpu(), gx.cpu()) < tol
     if kind == "linear":
-        assert O.rel_fro(out[0][2].float().cpu(), gw.cpu()) < 2.0 ** -8
+        assert O.rel_fro(out[0][2].float().cpu(), gw.cpu()) < tol
 
+
+def test_noise_in_several_pieces_without_a_gradient(rb):
+    """The noise matrix is staged 256 MB at a time."""
+    T, R, V = 70, 512, 300001
+    x = (torch.randn(T, R, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * (3.0 / R) ** 0.5 * 2).bfloat16()
+    target = torch.randint(0, V, (T,), device="cuda")
+    target[0], target[1] = V - 1, 262144                             # the last row; the first of the second piece
+    S = rb.kernels.noise(V, R, 77, 9, 0, torch.bfloat16).float()
+    want = F.cross_entropy(x.float() @ S.t(), target, reduction="none")
+    got = rb.noise_cross_entropy(x, 77, V, target, row0=9, reduction="none")
+    # float32 sums of 512 products either side, logits up to 10: 2^-23 * 48 * 30 at most
+    assert (got - want).abs().max() < 2.0 ** -23 * 48 * 30
 
 def test_gradient_is_the_slope(rb):
     """float32: the loss along a direction, by differences, against the gradient."""
