@@ -136,7 +136,6 @@ struct Cut {
     }
     __host__ __device__ __forceinline__ int begin(int g) const { return (int)((int64_t)total * g / groups); }
     __host__ __device__ __forceinline__ int owner(int at) const { return (int)((((int64_t)at + 1) * groups + total - 1) / total - 1); }
-    __host__ __device__ __forceinline__ int slot(int panel, int g, int member) const { return (panel + g) * size + member; }
     __host__ __device__ __forceinline__ int slots(int pairs) const { return (total / (KB ? KB : 1) + pairs / size) * size; }
 };
 
@@ -1194,6 +1193,237 @@ __global__ void __launch_bounds__(256) ce_scale_kernel(T *__restrict__ dz, const
 }
 
 // ================================================================================================
+// a few rows, loss only
+// ================================================================================================
+// Scoring a token or a few: the matrix is read (or hashed) once and multiplied on CUDA cores; a tile of the tensor-core path would
+// be 250 rows of padding, behind four kernels that prepare it.  A warp takes FEW_ROWS vocabulary rows at a time, 32 lanes along the
+// columns, the rows of x in shared memory; each lane ends up with the logits of some (vocabulary row, x row) pairs and keeps a running
+// maximum and a sum relative to it.  Bound by the launches where small, by the hash (noise) or the matrix's bytes (stored) where large.
+// Against the tensor-core path, on the device, us, V = 50257 but where said:
+//   bf16   1 x 128  noise 33 -> 18, stored 31 -> 16     4 x 768  noise 66 -> 55, stored 40 -> 41
+//          V = 128256: 1 x 4096  noise 608 -> 424, stored 221 -> 211 (5.0 TB/s)     4 x 2048  noise 401 -> 250, stored 123 -> 127
+//   fp32   1 x 128  noise 53 -> 18, stored 51 -> 18     4 x 768  noise 174 -> 53, stored 182 -> 51
+// Four rows of bf16 are where the two meet for a stored matrix: each value is loaded once, but converted and multiplied per row.
+constexpr int FEW_T = 4;                      // rows of x at most
+constexpr int FEW_ROWS = 4;                   // vocabulary rows per warp and pass
+constexpr int FEW_WARPS = 8;
+// blocks per SM, as many as the registers and shared memory of each form hold at once: every warp has the same share of the rows
+constexpr int few_blocks(int nt, bool noise) { return noise ? 4 : nt == 1 ? 3 : 2; }
+
+struct FewArgs {
+    const void *x;
+    int64_t ldx, T, R, V;
+    const int64_t *target;
+    Vocab voc;
+    float2 *partial;                          // (maximum, sum relative to it) per block and row of x
+    int64_t ignore;
+    int use_ignore, mean;
+    float *lse, *loss_rows, *loss_rows2, *count, *loss;
+};
+
+// add one logit to a running (maximum, sum relative to it)
+__device__ __forceinline__ void online(float &m, float &s, float l) {
+    if (l > m) {
+        s = s * ex2((m - l) * LOG2E) + 1.0f;
+        m = l;
+    } else if (l == m) {
+        s += l == -INFINITY ? 0.0f : 1.0f;    // a difference of two infinities would be NaN
+    } else {
+        s += ex2((l - m) * LOG2E);
+    }
+}
+__device__ __forceinline__ void online_join(float &m, float &s, float m2, float s2) {
+    const float mm = fmaxf(m, m2);
+    s = (m == mm ? s : s * ex2((m - mm) * LOG2E)) + (m2 == mm ? s2 : s2 * ex2((m2 - mm) * LOG2E));
+    m = mm;
+}
+
+// rows of x in shared memory start at 16 bytes
+__host__ __device__ __forceinline__ int few_stride(int64_t R) { return (int)((R + 3) / 4 * 4); }
+
+template <typename T, int NT, bool NOISE>
+__global__ void __launch_bounds__(FEW_WARPS * 32, few_blocks(NT, NOISE)) ce_few_kernel(const FewArgs a) {
+    extern __shared__ __align__(16) float xs[];   // [NT][RS]
+    __shared__ float2 sh[FEW_WARPS][NT];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int R = (int)a.R, RS = few_stride(R);
+    for (int t = 0; t < NT; ++t)
+        for (int c = threadIdx.x; c < R; c += FEW_WARPS * 32)
+            xs[t * RS + c] = t < a.T ? to_f32<T>(reinterpret_cast<const T *>(a.x)[t * a.ldx + c]) : 0.0f;
+    __syncthreads();
+    // after the exchange below lane i holds pair i of (vocabulary row, x row): row i / NT, x row i % NT
+    constexpr int PAIRS = FEW_ROWS * NT;
+    const int my_row = (lane % PAIRS) / NT, my_t = lane % NT;
+    const int64_t my_target = my_t < a.T ? a.target[my_t] : -1;
+    float m = -INFINITY, s = 0.0f;
+    const bool vec = !NOISE && rows_aligned<T>(a.voc.w, a.voc.ldw);
+    constexpr int W = 16 / sizeof(T);         // elements of a 16-byte load
+    const int64_t step = (int64_t)gridDim.x * FEW_WARPS * FEW_ROWS;
+    for (int64_t v0 = ((int64_t)blockIdx.x * FEW_WARPS + warp) * FEW_ROWS; v0 < a.V; v0 += step) {
+        float acc[PAIRS];
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) acc[i] = 0.0f;
+        int c = 0;                            // columns done
+        if (NOISE) {
+            uint32_t h[FEW_ROWS];
+#pragma unroll
+            for (int r = 0; r < FEW_ROWS; ++r) h[r] = sq5_lin_rows(a.voc.seed, a.voc.row0 + (uint32_t)(v0 + r), (uint32_t)lane).base;
+#pragma unroll 2
+            for (c = lane; c < R; c += 32) {
+                float w[FEW_ROWS];
+#pragma unroll
+                for (int r = 0; r < FEW_ROWS; ++r) {
+                    w[r] = to_f32<T>(from_f32<T>(sq5_to_float(sq5_tail(h[r]))));
+                    h[r] += 32u * SQ5_N1;
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const float x = xs[t * RS + c];
+#pragma unroll
+                    for (int r = 0; r < FEW_ROWS; ++r) acc[r * NT + t] = fmaf(x, w[r], acc[r * NT + t]);
+                }
+            }
+        } else {
+            const T *row[FEW_ROWS];
+#pragma unroll
+            for (int r = 0; r < FEW_ROWS; ++r) row[r] = reinterpret_cast<const T *>(a.voc.w) + (v0 + r < a.V ? v0 + r : a.V - 1) * a.voc.ldw;
+            const int whole = vec ? R / W * W : 0;
+#pragma unroll 2
+            for (c = lane * W; c < whole; c += 32 * W) {
+                uint4 u[FEW_ROWS];
+#pragma unroll
+                for (int r = 0; r < FEW_ROWS; ++r) u[r] = __ldg(reinterpret_cast<const uint4 *>(row[r] + c));
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (int e = 0; e < W; e += 4) {
+                        const float4 q = *reinterpret_cast<const float4 *>(xs + t * RS + c + e);
+                        const float x[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int r = 0; r < FEW_ROWS; ++r)
+                                acc[r * NT + t] = fmaf(x[k], to_f32<T>(reinterpret_cast<const T *>(&u[r])[e + k]), acc[r * NT + t]);
+                    }
+                }
+            }
+            for (c = whole + lane; c < R; c += 32) {
+#pragma unroll
+                for (int r = 0; r < FEW_ROWS; ++r) {
+                    const float w = to_f32<T>(row[r][c]);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[r * NT + t] = fmaf(xs[t * RS + c], w, acc[r * NT + t]);
+                }
+            }
+        }
+        // sums over the lanes, each step halving what a lane keeps; then over the lanes that keep the same pair
+#pragma unroll
+        for (int o = PAIRS / 2; o; o >>= 1) {
+            const bool upper = lane & o;
+#pragma unroll
+            for (int i = 0; i < PAIRS / 2; ++i) {
+                if (i < o) {
+                    const float give = upper ? acc[i] : acc[i + o];
+                    const float got = __shfl_xor_sync(0xffffffffu, give, o);
+                    acc[i] = (upper ? acc[i + o] : acc[i]) + got;
+                }
+            }
+        }
+        float l = acc[0];
+#pragma unroll
+        for (int o = PAIRS; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int64_t v = v0 + my_row;
+        if (lane < PAIRS && v < a.V && v != my_target) online(m, s, l);
+    }
+    // lanes of the same x row, then the warps
+#pragma unroll
+    for (int o = NT; o < 32; o <<= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        online_join(m, s, m2, s2);
+    }
+    if (lane < NT) sh[warp][lane] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x < NT) {
+        float2 r = sh[0][threadIdx.x];
+        for (int k = 1; k < FEW_WARPS; ++k) online_join(r.x, r.y, sh[k][threadIdx.x].x, sh[k][threadIdx.x].y);
+        a.partial[(int64_t)blockIdx.x * NT + threadIdx.x] = r;
+    }
+}
+
+// one block: a warp per row joins the blocks' sums and computes the target's logit
+template <typename T, int NT>
+__global__ void __launch_bounds__(FEW_T * 32) ce_few_finish_kernel(const FewArgs a, int blocks) {
+    __shared__ float sh_loss[FEW_T];
+    __shared__ int sh_kept[FEW_T];
+    pdl_wait();
+    // not before: blocks of a next call that come while this call's still run would fill some SMs twice over, and the shares
+    // are fixed (1 row of 4096, V = 128256, noise, calls in a row: 790 us, against 465 us for one alone)
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, t = threadIdx.x >> 5;
+    if (t < a.T) {
+        float m = -INFINITY, s = 0.0f, lt = 0.0f;
+        for (int b = lane; b < blocks; b += 32) {
+            const float2 p = a.partial[(int64_t)b * NT + t];
+            online_join(m, s, p.x, p.y);
+        }
+        const int64_t target = a.target[t];
+        const bool known = target >= 0 && target < a.V;
+        const T *x = reinterpret_cast<const T *>(a.x) + t * a.ldx;
+        if (known)
+            for (int64_t c = lane; c < a.R; c += 32) lt = fmaf(to_f32<T>(x[c]), vocab_at<T>(a.voc, target, c), lt);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+            online_join(m, s, m2, s2);
+            lt += __shfl_xor_sync(0xffffffffu, lt, o);
+        }
+        const bool kept = !(a.use_ignore && target == a.ignore);
+        // relative to the target's logit while that holds, as everywhere else
+        const float up = m - lt;
+        float loss = s == 0.0f ? 0.0f : up < 60.0f ? log1pf(s * expf(up)) : up + logf(s + expf(-up));
+        if (!known) loss = NAN;
+        if (!(lt == lt) || !(m == m)) loss = NAN;
+        if (!kept) loss = 0.0f;
+        if (lane == 0) {
+            a.loss_rows[t] = loss;
+            if (a.loss_rows2) a.loss_rows2[t] = loss;
+            a.lse[t] = kept ? lt + loss : 0.0f;
+            sh_loss[t] = loss;
+            sh_kept[t] = kept;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0.0;
+        int n = 0;
+        for (int k = 0; k < a.T; ++k) {
+            sum += sh_loss[k];
+            n += sh_kept[k];
+        }
+        *a.count = (float)n;
+        if (a.loss) *a.loss = (float)(a.mean ? sum / n : sum);
+    }
+}
+
+template <typename T, int NT>
+static int launch_few(const FewArgs &a, cudaStream_t st) {
+    const int64_t want = cdiv64(a.V, FEW_WARPS * FEW_ROWS);
+    const int64_t most = (int64_t)sm_count() * few_blocks(NT, !a.voc.w);
+    const int blocks = (int)(want < most ? want : most);
+    const size_t smem = (size_t)NT * few_stride(a.R) * sizeof(float);
+    const int rc = a.voc.w ? launch_pdl(ce_few_kernel<T, NT, false>, dim3(blocks), FEW_WARPS * 32, smem, st, a)
+                           : launch_pdl(ce_few_kernel<T, NT, true>, dim3(blocks), FEW_WARPS * 32, smem, st, a);
+    if (rc) return rc;
+    return launch_pdl(ce_few_finish_kernel<T, NT>, dim3(1), FEW_T * 32, 0, st, a, blocks);
+}
+
+// whether a loss without a gradient takes this way: its rows of x fit the 48 KB of shared memory that
+// need no opting in, with the kernel's own few hundred bytes
+static bool few_rows(int64_t T, int64_t R) { return T >= 1 && T <= FEW_T && R <= 47 * 1024 / (int64_t)sizeof(float) / (T == 1 ? 1 : FEW_T) - 4; }
+
+// ================================================================================================
 // host side
 // ================================================================================================
 struct CePlan {
@@ -1231,6 +1461,10 @@ static int ce_tile_rows(int64_t T, int64_t R, int dtype) {
 // op 0: loss; 1: loss and unit gradient of x (noise); 2: gradients of a stored matrix
 static CePlan ce_plan(int op, int64_t T, int64_t R, int64_t V, int dtype, const void *w, int64_t ldw, const void *dw, int want_dx, int want_dw) {
     CePlan p{};
+    if (op == 0 && few_rows(T, R)) {          // partial sums of ce_few_kernel only
+        p.total = (size_t)sm_count() * few_blocks(1, true) * FEW_T * sizeof(float2);
+        return p;
+    }
     p.parts = dtype == RDB_F32 ? 3 : 1;
     p.nterm = dtype == RDB_F32 ? 6 : 1;
     p.tile_rows = ce_tile_rows(T, R, dtype);
@@ -1575,6 +1809,20 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, float *dx_unit, const void *x
     c.st = (cudaStream_t)stream;
     float *lse = aux, *rows = aux + T, *count_f = aux + 2 * T;
     float *rows2 = reduction == RDB_CE_NONE ? loss : nullptr;       // the caller's own copy of the rows' losses
+    if (!dx_unit && few_rows(T, R)) {
+        FewArgs f{};
+        f.x = x; f.ldx = ldx; f.T = T; f.R = R; f.V = V;
+        f.target = target;
+        f.voc = c.voc;
+        f.partial = c.at<float2>(0);
+        f.ignore = ignore_index;
+        f.use_ignore = use_ignore;
+        f.mean = reduction == RDB_CE_MEAN ? 1 : 0;
+        f.lse = lse; f.loss_rows = rows; f.loss_rows2 = rows2; f.count = count_f;
+        f.loss = reduction == RDB_CE_NONE ? nullptr : loss;
+        if (dtype == RDB_F32) return T == 1 ? launch_few<float, 1>(f, c.st) : launch_few<float, FEW_T>(f, c.st);
+        return T == 1 ? launch_few<__nv_bfloat16, 1>(f, c.st) : launch_few<__nv_bfloat16, FEW_T>(f, c.st);
+    }
     if ((rc = ce_find_rows(c, ignore_index, use_ignore, lse, rows, rows2, count_f))) return rc;
     if (T > 0) {
         const CeRowArgs ra = ce_row_args(c);

@@ -401,6 +401,57 @@ def test_two_streams_at_once(rb):
             assert all(torch.equal(x, y) for x, y in zip(a, o))
 
 
+# up to four rows without a gradient have a kernel of their own; 3004 (four rows) and 12028 (one) are the widest that take it
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,R,V", [(1, 1, 1), (1, 3, 2), (2, 31, 5), (3, 33, 1000), (4, 250, 511), (4, 513, 40003), (5, 64, 300), (4, 3004, 70), (4, 3005, 70),
+                                   (1, 12028, 90), (1, 12029, 90)])
+@pytest.mark.parametrize("std", [2.0, 40.0, 300.0])
+def test_a_few_rows(rb, kind, dtype, T, R, V, std):
+    x, w, target = inputs(kind, T, R, V, dtype, T + R, std)
+    _, losses, _, _, _, _, terms = plain(x, w, target, None, "none", torch.ones(T, device="cuda"))
+    logit, _ = tolerances(dtype, R, V, terms)
+    for reduction, want in (("none", losses), ("mean", losses.mean()), ("sum", losses.sum())):
+        with torch.no_grad():
+            got = call(rb, kind, x, w, target, T + R, None, reduction)
+            again = call(rb, kind, x, w, target, T + R, None, reduction)
+        assert torch.equal(got, again)
+        assert torch.allclose(got.double(), want, rtol=2.0 ** -21, atol=logit * (T if reduction == "sum" else 1)), (got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_few_rows_ignored_strided_and_infinite(rb, dtype):
+    g = torch.Generator().manual_seed(5)
+    wide = torch.randn(700, 131, generator=g).to(dtype).cuda()
+    x = torch.randn(4, 140, generator=g).to(dtype).cuda()[:, 3:132]
+    for w in (wide[:, 1:130], wide[:, :129]):
+        target = torch.tensor([5, -100, 699, -100]).cuda()
+        with torch.no_grad():
+            want = torch.nn.functional.cross_entropy(x.double() @ w.double().t(), target, reduction="none")
+            terms = (x.double().abs() @ w.double().abs().t()).max().item()
+            bad = x.clone()
+            bad[1], bad[3, 0] = float("nan"), float("inf")
+            for xx in (x, bad):
+                got = rb.ops.linear_cross_entropy(xx, w, target, reduction="none")
+                assert torch.allclose(got.double(), want, rtol=2.0 ** -21, atol=tolerances(dtype, 129, 700, terms)[0])
+                mean = rb.ops.linear_cross_entropy(xx, w, target)
+                assert torch.allclose(mean.double(), want.sum() / 2, rtol=2.0 ** -20, atol=tolerances(dtype, 129, 700, terms)[0])
+            none = torch.full((4,), -100).cuda()
+            assert torch.isnan(rb.ops.linear_cross_entropy(bad, w, none))
+            assert rb.ops.linear_cross_entropy(bad, w, none, reduction="sum") == 0
+            out = rb.ops.linear_cross_entropy(x, w, torch.tensor([5, 700, 699, -1]).cuda(), reduction="none", ignore_index=None)
+            assert torch.equal(torch.isnan(out).cpu(), torch.tensor([False, True, False, True]))
+    # a logit of minus infinity leaves the sum alone; one of plus infinity beside a finite target makes the loss infinite
+    w = torch.ones(40, 8, dtype=dtype).cuda()
+    one = torch.ones(1, 8, dtype=dtype).cuda()
+    t = torch.tensor([0]).cuda()
+    with torch.no_grad():
+        w[7, 0] = float("-inf")
+        assert abs(rb.ops.linear_cross_entropy(one, w, t).item() - math.log(39)) < 1e-5
+        w[9, 0] = w[33, 0] = float("inf")
+        assert rb.ops.linear_cross_entropy(one, w, t).item() == float("inf")
+
+
 @pytest.mark.parametrize("kind", ["noise", "linear"])
 def test_operators_through_the_dispatcher(rb, kind):
     """rten::*_ce_*: schema, fake kernels and autograd registration; the same numbers as the eager functions."""
