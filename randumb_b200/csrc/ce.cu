@@ -283,156 +283,156 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     WorkItem w;
 
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CE_REGS_CONTROL));
-    if (warp == 0) {
-        // ------------------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            prefetch_tmap(&tmap_a);
-            prefetch_tmap(&tmap_b);
-            const uint64_t pol_a = EPI <= EPI_PROB ? l2_keep() : l2_stream(), pol_b = EPI <= EPI_PROB ? l2_stream() : l2_keep();
-            PipeState st;
-            bool ok = true;
-            while (ok && walk.take(w)) {
-                const int32_t m0 = (int32_t)(w.m * Cfg::ROWS + half * BM);
-                const int32_t n0 = (int32_t)(w.n * CE_TILE + half * BM);
-                int term = kbs ? w.kb0 / kbs : 0, kk = w.kb0 - term * kbs;
-                for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    if (!mbar_wait_cluster(smem_u32(&bar_free[st.idx]), st.phase ^ 1, abortp)) {
-                        raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_PRODUCER);
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t fb = mapa(smem_u32(&bar_full[st.idx]), rank & ~1u);
-                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[st.idx]), 2 * Cfg::STAGE);
-                    const uint32_t sa = smem_base + st.idx * Cfg::STAGE, sb = sa + MT * SUB_BYTES;
-                    const int32_t ax = args.a_off[term], bx = args.b_off[term], k0 = kk * BK;
-#pragma unroll
-                    for (int s = 0; s < MT; ++s) {
-                        if (A_MN) {
-#pragma unroll
-                            for (int i = 0; i < BM / 64; ++i)
-                                tma_load_pair_hint(sa + s * SUB_BYTES + i * (64 * BK * 2), &tmap_a, fb, ax + m0 + s * CE_TILE + i * 64, k0, pol_a);
-                        } else {
-                            tma_load_pair_hint(sa + s * SUB_BYTES, &tmap_a, fb, ax + k0, m0 + s * CE_TILE, pol_a);
-                        }
-                    }
-                    if (B_MN) {
-#pragma unroll
-                        for (int i = 0; i < BM / 64; ++i) tma_load_pair_hint(sb + i * (64 * BK * 2), &tmap_b, fb, bx + n0 + i * 64, k0, pol_b);
-                    } else {
-                        tma_load_pair_hint(sb, &tmap_b, fb, bx + k0, n0, pol_b);
-                    }
-                    st.advance<STAGES>();
-                    if (++kk == kbs) { kk = 0; ++term; }
-                }
-            }
-            if (!ok) {
-                // gave up: let the loads already in flight land before the CTA may retire
-                const long long t0 = clock64();
-                while (clock64() - t0 < 4000000LL) {
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer (even CTA of the pair)
-        if (lane == 0 && leader) {
-            constexpr uint32_t idesc = idesc_bf16_f32(2 * BM, CE_TILE, A_MN, B_MN);
-            constexpr uint32_t desc_hi = smem_desc_hi_sw128(1024);
-            constexpr uint32_t A_LBO = A_MN ? 64 * BK * 2 : 0, A_KSTEP = A_MN ? 2048 : UMMA_K * 2;
-            constexpr uint32_t B_LBO = B_MN ? 64 * BK * 2 : 0, B_KSTEP = B_MN ? 2048 : UMMA_K * 2;
-            const uint32_t peer = rank ^ 1u;
-            bool ok = true;
-            auto issue = [&](uint32_t stage, int sub, int acc, int k, bool fresh) {
-                const uint32_t sa = smem_base + stage * Cfg::STAGE;
-                const uint32_t a_lo = smem_desc_lo(sa + sub * SUB_BYTES, A_LBO), b_lo = smem_desc_lo(sa + MT * SUB_BYTES, B_LBO);
-                umma_bf16_pair(tmem_base + acc * CE_TILE, pack_desc(a_lo + ((k * A_KSTEP) >> 4), desc_hi),
-                               pack_desc(b_lo + ((k * B_KSTEP) >> 4), desc_hi), idesc, fresh ? 0u : 1u);
-            };
-            auto wait = [&](uint32_t bar, uint32_t parity) {
-                if (!mbar_wait_cluster(bar, parity, abortp)) {
-                    raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_MMA);
-                    ok = false;
-                } else {
-                    tc_fence_after_sync();
-                }
-                return ok;
-            };
-            auto commit_both = [&](uint32_t bar) {          // to the barrier of both CTAs
-                umma_commit_pair(bar);
-                umma_commit_pair(mapa(bar, peer));
-            };
-            if (MT == 1) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CE_REGS_CONTROL));
+        if (warp == 0) {
+            // ------------------------------------------------------------------ TMA producer
+            if (lane == 0) {
+                prefetch_tmap(&tmap_a);
+                prefetch_tmap(&tmap_b);
+                const uint64_t pol_a = EPI <= EPI_PROB ? l2_keep() : l2_stream(), pol_b = EPI <= EPI_PROB ? l2_stream() : l2_keep();
                 PipeState st;
-                uint32_t it = 0;
+                bool ok = true;
                 while (ok && walk.take(w)) {
-                    for (int c0 = w.kb0; c0 < w.kb1 && ok;) {
-                        const int c1 = ADD && c0 + CE_CHUNK < w.kb1 ? c0 + CE_CHUNK : w.kb1;
-                        const int acc = (int)(it & 1);
-                        if (!wait(smem_u32(&bar_tmem_empty[acc]), ((it >> 1) & 1) ^ 1)) break;
-                        for (int kb = c0; kb < c1; ++kb) {
-                            if (!wait(smem_u32(&bar_full[st.idx]), st.phase)) break;
-#pragma unroll
-                            for (int k = 0; k < BK / UMMA_K; ++k) issue(st.idx, 0, acc, k, ((kb - c0) | k) == 0);
-                            commit_both(smem_u32(&bar_free[st.idx]));
-                            st.advance<STAGES>();
+                    const int32_t m0 = (int32_t)(w.m * Cfg::ROWS + half * BM);
+                    const int32_t n0 = (int32_t)(w.n * CE_TILE + half * BM);
+                    int term = kbs ? w.kb0 / kbs : 0, kk = w.kb0 - term * kbs;
+                    for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                        if (!mbar_wait_cluster(smem_u32(&bar_free[st.idx]), st.phase ^ 1, abortp)) {
+                            raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_PRODUCER);
+                            ok = false;
+                            break;
                         }
-                        if (ok) commit_both(smem_u32(&bar_tmem_full[acc]));
-                        ++it;
-                        c0 = c1;
+                        const uint32_t fb = mapa(smem_u32(&bar_full[st.idx]), rank & ~1u);
+                        if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[st.idx]), 2 * Cfg::STAGE);
+                        const uint32_t sa = smem_base + st.idx * Cfg::STAGE, sb = sa + MT * SUB_BYTES;
+                        const int32_t ax = args.a_off[term], bx = args.b_off[term], k0 = kk * BK;
+#pragma unroll
+                        for (int s = 0; s < MT; ++s) {
+                            if (A_MN) {
+#pragma unroll
+                                for (int i = 0; i < BM / 64; ++i)
+                                    tma_load_pair_hint(sa + s * SUB_BYTES + i * (64 * BK * 2), &tmap_a, fb, ax + m0 + s * CE_TILE + i * 64, k0, pol_a);
+                            } else {
+                                tma_load_pair_hint(sa + s * SUB_BYTES, &tmap_a, fb, ax + k0, m0 + s * CE_TILE, pol_a);
+                            }
+                        }
+                        if (B_MN) {
+#pragma unroll
+                            for (int i = 0; i < BM / 64; ++i) tma_load_pair_hint(sb + i * (64 * BK * 2), &tmap_b, fb, bx + n0 + i * 64, k0, pol_b);
+                        } else {
+                            tma_load_pair_hint(sb, &tmap_b, fb, bx + k0, n0, pol_b);
+                        }
+                        st.advance<STAGES>();
+                        if (++kk == kbs) { kk = 0; ++term; }
                     }
                 }
-            } else {
-                // Two accumulators per tile.  While the epilogue still reads accumulator 1 of the tile before, the k-blocks that
-                // are staged already go to accumulator 0 alone (ahead of accumulator 1 by at most the ring); then both in turn:
-                // consecutive MMAs to one accumulator are a quarter slower.
-                PipeState st0, st1;
-                uint32_t it = 0;
-                while (ok && walk.take(w)) {
-                    const int n = w.kb1 - w.kb0;
-                    if (n == 0) continue;
-                    const uint32_t par = (it & 1) ^ 1;
-                    bool have1 = false;
-                    int i0 = 0, i1 = 0;
-                    while (i1 < n && ok) {
-                        if (!have1 && (i0 - i1 == STAGES || i0 == n || mbar_try_wait_cluster(smem_u32(&bar_tmem_empty[1]), par))) {
-                            if (!wait(smem_u32(&bar_tmem_empty[1]), par)) break;
-                            have1 = true;
-                        }
-                        if (have1 && i1 < i0) {
-#pragma unroll
-                            for (int k = 0; k < BK / UMMA_K; ++k) issue(st1.idx, 1, 1, k, (i1 | k) == 0);
-                            commit_both(smem_u32(&bar_free[st1.idx]));
-                            st1.advance<STAGES>();
-                            if (++i1 == n) commit_both(smem_u32(&bar_tmem_full[1]));
-                            continue;
-                        }
-                        if (i0 == 0 && !wait(smem_u32(&bar_tmem_empty[0]), par)) break;
-                        if (!wait(smem_u32(&bar_full[st0.idx]), st0.phase)) break;
-                        const bool last = i0 == n - 1;
-                        if (!have1 || last) {
-#pragma unroll
-                            for (int k = 0; k < BK / UMMA_K; ++k) issue(st0.idx, 0, 0, k, (i0 | k) == 0);
-                            if (last) commit_both(smem_u32(&bar_tmem_full[0]));     // drained while accumulator 1 finishes
-                            st0.advance<STAGES>();
-                            ++i0;
-                            continue;                                                // accumulator 1 catches up at the loop's top
-                        }
-#pragma unroll
-                        for (int k = 0; k < BK / UMMA_K; ++k) {
-                            issue(st0.idx, 0, 0, k, (i0 | k) == 0);
-                            issue(st0.idx, 1, 1, k, (i0 | k) == 0);
-                        }
-                        commit_both(smem_u32(&bar_free[st0.idx]));
-                        st0.advance<STAGES>();
-                        st1.advance<STAGES>();
-                        ++i0;
-                        ++i1;
+                if (!ok) {
+                    // gave up: let the loads already in flight land before the CTA may retire
+                    const long long t0 = clock64();
+                    while (clock64() - t0 < 4000000LL) {
                     }
-                    ++it;
+                }
+            }
+        } else if (warp == 1) {
+            // ------------------------------------------------------------------ MMA issuer (even CTA of the pair)
+            if (lane == 0 && leader) {
+                constexpr uint32_t idesc = idesc_bf16_f32(2 * BM, CE_TILE, A_MN, B_MN);
+                constexpr uint32_t desc_hi = smem_desc_hi_sw128(1024);
+                constexpr uint32_t A_LBO = A_MN ? 64 * BK * 2 : 0, A_KSTEP = A_MN ? 2048 : UMMA_K * 2;
+                constexpr uint32_t B_LBO = B_MN ? 64 * BK * 2 : 0, B_KSTEP = B_MN ? 2048 : UMMA_K * 2;
+                const uint32_t peer = rank ^ 1u;
+                bool ok = true;
+                auto issue = [&](uint32_t stage, int sub, int acc, int k, bool fresh) {
+                    const uint32_t sa = smem_base + stage * Cfg::STAGE;
+                    const uint32_t a_lo = smem_desc_lo(sa + sub * SUB_BYTES, A_LBO), b_lo = smem_desc_lo(sa + MT * SUB_BYTES, B_LBO);
+                    umma_bf16_pair(tmem_base + acc * CE_TILE, pack_desc(a_lo + ((k * A_KSTEP) >> 4), desc_hi),
+                                   pack_desc(b_lo + ((k * B_KSTEP) >> 4), desc_hi), idesc, fresh ? 0u : 1u);
+                };
+                auto wait = [&](uint32_t bar, uint32_t parity) {
+                    if (!mbar_wait_cluster(bar, parity, abortp)) {
+                        raise_abort(abortp, args.status, RDB_STATUS_TIMEOUT_MMA);
+                        ok = false;
+                    } else {
+                        tc_fence_after_sync();
+                    }
+                    return ok;
+                };
+                auto commit_both = [&](uint32_t bar) {          // to the barrier of both CTAs
+                    umma_commit_pair(bar);
+                    umma_commit_pair(mapa(bar, peer));
+                };
+                if (MT == 1) {
+                    PipeState st;
+                    uint32_t it = 0;
+                    while (ok && walk.take(w)) {
+                        for (int c0 = w.kb0; c0 < w.kb1 && ok;) {
+                            const int c1 = ADD && c0 + CE_CHUNK < w.kb1 ? c0 + CE_CHUNK : w.kb1;
+                            const int acc = (int)(it & 1);
+                            if (!wait(smem_u32(&bar_tmem_empty[acc]), ((it >> 1) & 1) ^ 1)) break;
+                            for (int kb = c0; kb < c1; ++kb) {
+                                if (!wait(smem_u32(&bar_full[st.idx]), st.phase)) break;
+#pragma unroll
+                                for (int k = 0; k < BK / UMMA_K; ++k) issue(st.idx, 0, acc, k, ((kb - c0) | k) == 0);
+                                commit_both(smem_u32(&bar_free[st.idx]));
+                                st.advance<STAGES>();
+                            }
+                            if (ok) commit_both(smem_u32(&bar_tmem_full[acc]));
+                            ++it;
+                            c0 = c1;
+                        }
+                    }
+                } else {
+                    // Two accumulators per tile.  While the epilogue still reads accumulator 1 of the tile before, the k-blocks that
+                    // are staged already go to accumulator 0 alone (ahead of accumulator 1 by at most the ring); then both in turn:
+                    // consecutive MMAs to one accumulator are a quarter slower.
+                    PipeState st0, st1;
+                    uint32_t it = 0;
+                    while (ok && walk.take(w)) {
+                        const int n = w.kb1 - w.kb0;
+                        if (n == 0) continue;
+                        const uint32_t par = (it & 1) ^ 1;
+                        bool have1 = false;
+                        int i0 = 0, i1 = 0;
+                        while (i1 < n && ok) {
+                            if (!have1 && (i0 - i1 == STAGES || i0 == n || mbar_try_wait_cluster(smem_u32(&bar_tmem_empty[1]), par))) {
+                                if (!wait(smem_u32(&bar_tmem_empty[1]), par)) break;
+                                have1 = true;
+                            }
+                            if (have1 && i1 < i0) {
+#pragma unroll
+                                for (int k = 0; k < BK / UMMA_K; ++k) issue(st1.idx, 1, 1, k, (i1 | k) == 0);
+                                commit_both(smem_u32(&bar_free[st1.idx]));
+                                st1.advance<STAGES>();
+                                if (++i1 == n) commit_both(smem_u32(&bar_tmem_full[1]));
+                                continue;
+                            }
+                            if (i0 == 0 && !wait(smem_u32(&bar_tmem_empty[0]), par)) break;
+                            if (!wait(smem_u32(&bar_full[st0.idx]), st0.phase)) break;
+                            const bool last = i0 == n - 1;
+                            if (!have1 || last) {
+#pragma unroll
+                                for (int k = 0; k < BK / UMMA_K; ++k) issue(st0.idx, 0, 0, k, (i0 | k) == 0);
+                                if (last) commit_both(smem_u32(&bar_tmem_full[0]));     // drained while accumulator 1 finishes
+                                st0.advance<STAGES>();
+                                ++i0;
+                                continue;                                                // accumulator 1 catches up at the loop's top
+                            }
+#pragma unroll
+                            for (int k = 0; k < BK / UMMA_K; ++k) {
+                                issue(st0.idx, 0, 0, k, (i0 | k) == 0);
+                                issue(st0.idx, 1, 1, k, (i0 | k) == 0);
+                            }
+                            commit_both(smem_u32(&bar_free[st0.idx]));
+                            st0.advance<STAGES>();
+                            st1.advance<STAGES>();
+                            ++i0;
+                            ++i1;
+                        }
+                        ++it;
+                    }
                 }
             }
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CE_REGS_EPI));
         // ------------------------------------------------------------------ epilogue: 8 warps, this CTA's 128 rows of a sub-tile
