@@ -1795,7 +1795,8 @@ extern "C" int rdb_ce_fwd(float *loss, float *aux, float *dx_unit, const void *x
     if (!aux || (!loss && (T > 0 || reduction != RDB_CE_NONE))) return RDB_ERR_NULL;
     if (T > 0 && (!x || !target)) return RDB_ERR_NULL;
     const size_t es = dtype_size(dtype);
-    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & (es - 1)) || (reinterpret_cast<uintptr_t>(dx_unit) & 3) || (reinterpret_cast<uintptr_t>(target) & 7))
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & (es - 1)) || ((reinterpret_cast<uintptr_t>(dx_unit) | reinterpret_cast<uintptr_t>(loss) | reinterpret_cast<uintptr_t>(aux)) & 3) ||
+        (reinterpret_cast<uintptr_t>(target) & 7))
         return RDB_ERR_ALIGN;
     CeCall c{};
     c.p = ce_plan(dx_unit ? 1 : 0, T, R, V, dtype, w, ldw, nullptr, 1, 0);
@@ -1870,7 +1871,7 @@ extern "C" int rdb_ce_bwd(void *dx, void *dw, const float *dloss, const void *x,
     if (T > 0 && (!w || !dloss || !aux || !x || !target)) return RDB_ERR_NULL;
     const size_t es = dtype_size(dtype);
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & (es - 1)) ||
-        (reinterpret_cast<uintptr_t>(target) & 7))
+        ((reinterpret_cast<uintptr_t>(dloss) | reinterpret_cast<uintptr_t>(aux)) & 3) || (reinterpret_cast<uintptr_t>(target) & 7))
         return RDB_ERR_ALIGN;
     cudaStream_t st = (cudaStream_t)stream;
     if (T == 0) {
@@ -1914,6 +1915,9 @@ extern "C" int rdb_ce_scale(void *dz, const float *unit, const float *dloss, con
     if (rc) return rc;
     if (T == 0) return RDB_OK;
     if (!dz || !unit || !dloss || !aux) return RDB_ERR_NULL;
+    if ((reinterpret_cast<uintptr_t>(dz) & (dtype_size(dtype) - 1)) ||
+        ((reinterpret_cast<uintptr_t>(unit) | reinterpret_cast<uintptr_t>(dloss) | reinterpret_cast<uintptr_t>(aux)) & 3))
+        return RDB_ERR_ALIGN;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t want = cdiv64(T * R, 256 * 8);
     const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8));

@@ -520,6 +520,7 @@ extern "C" int rdb_adamw_step(const rdb_adamw_lists *lists, int param_dtype, int
     if (state_bits != 32 && state_bits != 8) return RDB_ERR_DTYPE;
     if (state_bits == 8 && (!l.exp_avg_scale || !l.exp_avg_sq_scale)) return RDB_ERR_NULL;
     if (!(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0) || !(h->eps >= 0.0)) return RDB_ERR_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(h->lr_dev) | reinterpret_cast<uintptr_t>(grad_scale)) & 3) return RDB_ERR_ALIGN;
     const bool master = l.master != nullptr;
     if (master && param_dtype != RDB_BF16) return RDB_ERR_UNSUPPORTED;
     const uintptr_t pm = dtype_size(param_dtype) - 1, gm = dtype_size(grad_dtype) - 1, sm = state_bits == 8 ? 0 : 3;
@@ -531,7 +532,8 @@ extern "C" int rdb_adamw_step(const rdb_adamw_lists *lists, int param_dtype, int
         if (state_bits == 8 && (!l.exp_avg_scale[i] || !l.exp_avg_sq_scale[i])) return RDB_ERR_NULL;
         if ((reinterpret_cast<uintptr_t>(l.param[i]) & pm) || (reinterpret_cast<uintptr_t>(l.grad[i]) & gm) || (reinterpret_cast<uintptr_t>(l.exp_avg[i]) & sm) ||
             (reinterpret_cast<uintptr_t>(l.exp_avg_sq[i]) & sm) || (master && (reinterpret_cast<uintptr_t>(l.master[i]) & 3)) ||
-            (reinterpret_cast<uintptr_t>(l.step[i]) & 3))
+            (reinterpret_cast<uintptr_t>(l.step[i]) & 3) ||
+            (state_bits == 8 && ((reinterpret_cast<uintptr_t>(l.exp_avg_scale[i]) | reinterpret_cast<uintptr_t>(l.exp_avg_sq_scale[i])) & 3)))
             return RDB_ERR_ALIGN;
     }
     cudaStream_t st = (cudaStream_t)stream;

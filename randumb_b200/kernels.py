@@ -440,6 +440,15 @@ def _ce_args(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tens
     return dev, _dt(x.dtype), _lib.CE_REDUCTIONS[reduction]
 
 
+def _ce_ignore(ignore_index: Optional[int]) -> Tuple[int, int]:
+    if ignore_index is None:
+        return 0, 0
+    value = int(ignore_index)
+    if not -2 ** 63 <= value < 2 ** 63:
+        raise RuntimeError(f"cross entropy: ignore_index must be an int64, got {ignore_index}")
+    return value, 1
+
+
 def _ce_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """The matrix itself when its rows are dense and follow one another at some pitch, else a contiguous copy."""
     if t is None or t.is_contiguous() or (t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1])):
@@ -454,6 +463,7 @@ def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor
     from ``row0`` on.  loss: float32, 0-d or (reduction "none") [T]; unit: the rows' own gradients in x, float32, with
     ``need_unit``."""
     V = int(vocab) if weight is None else weight.shape[0]
+    ignore, use_ignore = _ce_ignore(ignore_index)
     dev, dt, red = _ce_args(x, weight, target, V, reduction)
     x, weight, target = _ce_rows(x), _ce_rows(weight), target.contiguous()
     T, R = x.shape
@@ -465,7 +475,7 @@ def ce_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], target: torch.Tensor
         ldw = _pitch(weight) if weight is not None else 0
         ws = _workspace(L.rdb_ce_workspace_bytes(_lib.CE_LOSS_GRAD if need_unit else _lib.CE_LOSS, T, R, V, dt, _ptr(weight), ldw), dev)
         rc = L.rdb_ce_fwd(_ptr(loss), _ptr(aux), _ptr(unit), _ptr(x), _pitch(x), _ptr(weight), ldw, _ptr(target), _ptr(ws), ws.numel(), T, R, V, row0,
-                          _seed(seed), 0 if ignore_index is None else int(ignore_index), 0 if ignore_index is None else 1, dt, red,
+                          _seed(seed), ignore, use_ignore, dt, red,
                           _ptr(status_buffer(dev)), _raw_stream(dev.index))
     _lib.check(rc, "rdb_ce_fwd")
     return loss, aux, unit
@@ -488,6 +498,7 @@ def ce_bwd(dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: t
            reduction: str = "mean", need_dx: bool = True, need_dw: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dweight) of a stored matrix, contiguous, from the forward's ``aux``; either may be skipped."""
     V = weight.shape[0]
+    ignore, use_ignore = _ce_ignore(ignore_index)
     dev, dt, red = _ce_args(x, weight, target, V, reduction)
     x, weight, target, dloss = _ce_rows(x), _ce_rows(weight), target.contiguous(), dloss.contiguous()
     assert dloss.dtype == torch.float32 and dloss.device == dev and dloss.numel() == (x.shape[0] if reduction == "none" else 1)
@@ -499,7 +510,7 @@ def ce_bwd(dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: t
     with _on(dev.index):
         ws = _workspace(L.rdb_ce_workspace_bytes(_lib.CE_GRADS, T, R, V, dt, _ptr(weight), _pitch(weight)), dev)
         rc = L.rdb_ce_bwd(_ptr(dx), _ptr(dw), _ptr(dloss), _ptr(x), _pitch(x), _ptr(weight), _pitch(weight), _ptr(target), _ptr(aux), _ptr(ws),
-                          ws.numel(), T, R, V, 0 if ignore_index is None else int(ignore_index), 0 if ignore_index is None else 1, dt, red,
+                          ws.numel(), T, R, V, ignore, use_ignore, dt, red,
                           _ptr(status_buffer(dev)), _raw_stream(dev.index))
     _lib.check(rc, "rdb_ce_bwd")
     return dx, dw

@@ -104,12 +104,21 @@ class _State:
             if any([t.numel() != 1 for t in steps]):
                 raise RuntimeError("adamw_step: every tensor has one step count")
             words = [t.data_ptr() for t in steps]
+        counts = len(words)
         words += numels
         for _, ts in lists:
             words += [t.data_ptr() for t in ts]
+        # every address once: two tensors in one place would be updated by two threads at a time
+        at = words[:counts] + words[counts + n:]
+        if len(set(at)) != len(at):
+            empty = [k == 0 for k in numels]
+            at = words[:counts] + [a for i, a in enumerate(words[counts + n:]) if not empty[i % n]]
+            if len(set(at)) != len(at):
+                raise RuntimeError("adamw_step: a step count, moment, scale or master is in the lists twice")
         self.names = ["step", "numel"] + [what for what, _ in lists]
         self.words = array("Q", words)                         # one list behind the other, in host memory
-        self.keep = (steps, [ts for _, ts in lists])           # the tensors the addresses belong to
+        # the tensors the addresses belong to
+        self.keep = ([steps] if isinstance(steps, torch.Tensor) else list(steps)) + [t for _, ts in lists for t in ts]
         self.some = sum(1 for k in numels if k)
 
     def launch(self, params, grads, lr, betas, eps, weight_decay, seed, grad_scale, fresh: bool = False) -> None:
@@ -136,6 +145,8 @@ class _State:
             rc = _lib.lib().rdb_adamw_step(ctypes.byref(arg), K._dt(self.dtype), K._dt(gd), 8 if self.eight else 32, ctypes.byref(h),
                                            K._ptr(grad_scale), K._raw_stream(dev))
         _lib.check(rc, "rdb_adamw_step")
+        # autograd learns that these were written: a graph that kept one refuses to run backward
+        torch.autograd.graph.increment_version([*params, *self.keep])
 
 
 def _one_float(what: str, t: Optional[torch.Tensor], dev: int) -> None:
@@ -244,23 +255,28 @@ class AdamW(torch.optim.Optimizer):
             st["master"] = p.detach().float()
         return st
 
+    def __getstate__(self) -> dict:                                 # copies and pickles; the lists are made again
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "seed": self.seed, "last_grad_norm": self.last_grad_norm}
+
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
         self._lists = {}
 
     def _state_of(self, key, params: list, group: dict, master: bool) -> _State:
-        """The checked lists of these parameters' states; kept while the same parameters have gradients and the same tensors as state."""
+        """The checked lists of these parameters' states; kept while the same parameters have gradients and the same tensors, in the
+        same places, as state."""
         sts = [self.state[p] for p in params]
         have = self._lists.get(key)
         parts = [v for s in sts for v in s.values()]
-        if have is not None and len(have[0]) == len(parts) and all([a is b for a, b in zip(have[0], parts)]):
+        at = [t.data_ptr() for t in parts]
+        if have is not None and at == have[2] and all([a is b for a, b in zip(have[0], parts)]):
             return have[1]
         eight = {}
         if group["state_bits"] == 8:
             eight = dict(exp_avg_scales=[s["exp_avg_scale"] for s in sts], exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in sts])
         made = _State([_flat(p) for p in params], [_flat(s["exp_avg"]) for s in sts], [_flat(s["exp_avg_sq"]) for s in sts], [s["step"] for s in sts],
                       [_flat(s["master"]) for s in sts] if master else None, **eight)
-        self._lists[key] = (parts, made)
+        self._lists[key] = (parts, made, at)
         return made
 
     @torch.no_grad()

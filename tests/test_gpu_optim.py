@@ -4,6 +4,7 @@ Tolerances.  One float32 operation is off by at most half a step, u = 2^-24 of i
 |dm| <= 2 u (|b1 m| + |(1 - b1) g|) and one u more where the gradient is scaled first.  The update m / (sqrt(v) / root + eps) adds
 the roundings of v (3 u, halved by the root), sqrt, product, sum, quotient, size: below 10 u relative to the update's own terms.
 """
+import copy
 import math
 
 import numpy as np
@@ -282,6 +283,13 @@ def test_refusals(rb):
     step = rb.optim.adamw_step
     with pytest.raises(RuntimeError, match="twice"):
         step([p, p], [g, g], [m, m], [v, v], torch.zeros(2, device="cuda"))
+    two = lambda: [torch.zeros(4, device="cuda") for _ in range(2)]                   # noqa: E731
+    with pytest.raises(RuntimeError, match="twice"):
+        step(two(), [g, g], two(), two(), [s, s])
+    with pytest.raises(RuntimeError, match="twice"):
+        step(two(), [g, g], [m, m], two(), torch.zeros(2, device="cuda"))
+    with pytest.raises(RuntimeError, match="twice"):
+        step([p], [g], [m], [m], s)
     with pytest.raises(RuntimeError, match="differ in size"):
         step([p], [torch.zeros(5, device="cuda")], [m], [v], s)
     with pytest.raises(RuntimeError, match="one type"):
@@ -357,3 +365,50 @@ def test_optimizer_follows_its_parameters(rb):
         for p, r in zip((a, b, c), ref):
             # a few roundings of values of size 1 in either program
             assert (p - r).abs().max() < 8 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_that_moves(rb, bits):
+    """The state's memory is exchanged between steps (moved to the host and back): the next step works on the new one."""
+    g = torch.Generator().manual_seed(4)
+    start = torch.randn(700, generator=g).cuda()
+    a, b = torch.nn.Parameter(start.clone()), torch.nn.Parameter(start.clone())
+    opt, ref = (rb.optim.AdamW([p], lr=0.01, state_bits=bits) for p in (a, b))
+    old = []
+    for _ in range(4):
+        a.grad = torch.randn(700, generator=g).cuda()
+        b.grad = a.grad.clone()
+        opt.step()
+        ref.step()
+        assert torch.equal(a, b)
+        for t in opt.state[a].values():
+            old.append((t.data, t.data.clone()))
+            t.data = t.data.cpu().cuda()
+    for t, before in old:
+        assert torch.equal(t.float(), before.float())         # what was left behind is not written any more
+
+
+def test_a_graph_that_kept_a_parameter_notices_the_step(rb):
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    q = torch.nn.Parameter(torch.ones(4, 2, device="cuda").t())
+    opt = rb.optim.AdamW([p, q])
+    loss = (p * p).sum() + (q * q).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    assert p._version > 0 and q._version > 0
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+
+
+def test_a_copied_optimizer_steps_by_itself(rb):
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = rb.optim.AdamW([p], lr=0.1, max_grad_norm=1.0, state_bits=8)
+    for k in range(2):
+        p.grad = torch.full_like(p, 1.0 + k)
+        opt.step()
+    q, twin = copy.deepcopy((p, opt))
+    q.grad = p.grad = torch.full_like(p, 3.0)
+    opt.step()
+    assert not torch.equal(p, q)
+    twin.step()
+    assert torch.equal(p, q) and torch.equal(opt.last_grad_norm, twin.last_grad_norm)

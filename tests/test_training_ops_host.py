@@ -1,6 +1,8 @@
 """Host side of the training operators (cross entropy, AdamW, gradient norm): refusals before any launch, CPU tensors, tracing,
 planning.  CPU only -- no kernel runs here."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -76,6 +78,8 @@ def test_adamw_and_norm_refusals(built_lib):
     assert step(param=None) == -1 and step(numel=-1) == -2 and step(step=0) == -1 and step(grad=0) == -1
     assert step(pd=7) == -3 and step(bits=16) == -3 and step(bits=8) == -1
     assert step(param=OK + 2) == -4 and step(pd=_lib.BF16, param=OK + 1) == -4 and step(exp_avg=OK + 1) == -4 and step(step=OK + 2) == -4
+    assert step(bits=8, exp_avg_scale=OK + 2, exp_avg_sq_scale=OK) == -4 and step(bits=8, exp_avg_scale=OK, exp_avg_sq_scale=OK + 1) == -4
+    assert step(hyper=_lib.AdamwHyper(1e-3, 0.9, 0.99, 1e-8, 0.0, OK + 2, 0)) == -4
     assert step(master=OK) == -6                                    # masters are the float32 copies of bf16 parameters
     for bad in (_lib.AdamwHyper(1e-3, 1.0, 0.99, 1e-8, 0.0, None, 0), _lib.AdamwHyper(1e-3, 0.9, float("nan"), 1e-8, 0.0, None, 0),
                 _lib.AdamwHyper(1e-3, 0.9, 0.99, -1.0, 0.0, None, 0)):
@@ -100,6 +104,9 @@ def test_cpu_tensors_are_refused():
         rb.linear_cross_entropy(x, w, t)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         rb.kernels.ce_fwd(x, w, t)
+    for far in (2 ** 63, -2 ** 63 - 1, 2 ** 64):                     # would be another value in 64 bits
+        with pytest.raises(RuntimeError, match="ignore_index"):
+            rb.kernels.ce_fwd(x, w, t, far)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         rb.optim.adamw_step([x], [x], [x], [x], torch.zeros(1))
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
@@ -136,6 +143,10 @@ def test_optimizer_arguments():
             rb.optim.AdamW([p], **bad)
     opt = rb.optim.AdamW([p])
     opt.step()                                                      # no gradients: nothing to do
+    two = rb.optim.AdamW([p], max_grad_norm=0.5, seed=7, state_bits=8)
+    for c in (copy.deepcopy(two), pickle.loads(pickle.dumps(two))):
+        assert (c.max_grad_norm, c.seed, c.last_grad_norm, c.param_groups[0]["state_bits"]) == (0.5, 7, None, 8)
+        c.step()
     p.grad = torch.ones(3)
     with pytest.raises(RuntimeError, match="CUDA parameters"):
         opt.step()
