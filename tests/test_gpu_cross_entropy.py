@@ -452,6 +452,29 @@ def test_a_few_rows_ignored_strided_and_infinite(rb, dtype):
         assert rb.ops.linear_cross_entropy(one, w, t).item() == float("inf")
 
 
+@pytest.mark.parametrize("T", [3, 1060])
+def test_offsets_past_32_bits(rb, T):
+    """Rows 2^22 elements apart: the last ones lie more than 2^32 elements behind the first."""
+    R, V, pitch = 72, 1060, 2 ** 22
+    x, w, target = inputs("linear", T, R, V, torch.bfloat16, 6)
+    target[:2] = torch.tensor([V - 1, 0])
+    far = torch.empty((V - 1) * pitch + R, dtype=torch.bfloat16, device="cuda").as_strided((V, R), (pitch, 1))
+    far.copy_(w)
+    check(rb, "linear", x, w, target, 6, -100, "mean")
+    with torch.no_grad():
+        assert torch.equal(rb.ops.linear_cross_entropy(x, far, target, reduction="none"), rb.ops.linear_cross_entropy(x, w, target, reduction="none"))
+    one, other = ([t.requires_grad_() for t in (x.clone(), m)] for m in (w, far.detach()))
+    want, got = (torch.autograd.grad(rb.ops.linear_cross_entropy(a, m, target), [a, m]) for a, m in (one, other))
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    far = far.detach()
+    rows = far[V - T:]
+    rows.copy_(x.detach())
+    for call_it in (lambda a: rb.ops.linear_cross_entropy(a, w.detach(), target), lambda a: rb.ops.noise_cross_entropy(a, 9, V, target)):
+        (a, b) = (t.detach().requires_grad_() for t in (x, rows))
+        la, lb = call_it(a), call_it(b)
+        assert torch.equal(la, lb) and torch.equal(torch.autograd.grad(la, a)[0], torch.autograd.grad(lb, b)[0])
+
+
 @pytest.mark.parametrize("kind", ["noise", "linear"])
 def test_operators_through_the_dispatcher(rb, kind):
     """rten::*_ce_*: schema, fake kernels and autograd registration; the same numbers as the eager functions."""

@@ -412,3 +412,29 @@ def test_a_copied_optimizer_steps_by_itself(rb):
     assert not torch.equal(p, q)
     twin.step()
     assert torch.equal(p, q) and torch.equal(opt.last_grad_norm, twin.last_grad_norm)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_past_32_bit_offsets(rb, bits):
+    """2^31 + 300 elements: what lies behind 2^31 is updated as in a small tensor."""
+    n, head = 2 ** 31 + 300, 2 ** 31 - 256
+    kw = dict(device="cuda")
+    p, g = torch.zeros(n, dtype=torch.bfloat16, **kw), torch.zeros(n, dtype=torch.bfloat16, **kw)
+    tail = torch.randn(n - head, generator=torch.Generator().manual_seed(9)).bfloat16().cuda()
+    p[head:], g[head:] = tail, tail.flip(0)
+
+    def state(k):
+        if bits == 32:
+            return [torch.zeros(k, **kw)], [torch.zeros(k, **kw)], {}
+        return [torch.zeros(k, dtype=torch.uint8, **kw).view(torch.float8_e4m3fn)], [torch.zeros(k, dtype=torch.uint8, **kw)], \
+            dict(exp_avg_scales=[torch.zeros(-(-k // 256), **kw)], exp_avg_sq_scales=[torch.zeros(-(-k // 256), **kw)])
+
+    m, v, sc = state(n)
+    assert torch.equal(rb.optim.grad_norm([g])[0], rb.optim.grad_norm([g[head:].clone()])[0])
+    rb.optim.adamw_step([p], [g], m, v, torch.zeros(1, **kw), lr=0.1, weight_decay=0.0, **sc)
+    q, m2, v2 = [tail.clone()], *state(n - head)[:2]
+    sc2 = state(n - head)[2]
+    rb.optim.adamw_step(q, [tail.flip(0)], m2, v2, torch.zeros(1, **kw), lr=0.1, weight_decay=0.0, **sc2)
+    assert torch.equal(m[0].view(torch.uint8)[(head if bits == 8 else 4 * head):], m2[0].view(torch.uint8))
+    # the random rounding of an 8-bit second moment goes by the element's place, the update of a first step does not hang on it
+    assert torch.equal(p[head:], q[0]) and (p[:head:1 << 20] == 0).all()
