@@ -9,9 +9,9 @@
 // so no running maximum is needed: the sum never falls below the target's own 1, and small losses and the gradients of tokens
 // the model already knows come out of log1p and of a sum without the target, not of a difference of nearly equal numbers.  Float32
 // holds e_v up to 69 above the target's logit (s below 2^100 leaves room for the gradient).  Where the row's length says that the
-// largest of V random logits will lie 40 or more above the target's (|x| |w_t| / sqrt(R) is their standard deviation, times sqrt(2 ln
-// V)), that estimate takes the target's place:  e_v = exp(l_v - l_t - d),  loss = log(s + exp(-d)) + d.  A row that leaves the range
-// all the same, at either end, is noticed and done again with its true maximum (ce_rescue_row).
+// largest of V random logits will lie 40 or more above the target's (|x| |w_t| / sqrt(R) is their standard deviation, largest_of(V) of
+// those the mean of the largest), that estimate takes the target's place:  e_v = exp(l_v - l_t - d),  loss = log(s + exp(-d)) + d.  A row that leaves the range
+// all the same, at either end, is noticed and done again with its true maximum (ce_far_rows).
 //
 // Rows whose target is ignored are left out: the remaining rows are gathered to the front, and every later kernel works on that
 // many rows, a number that only the device knows.
@@ -743,7 +743,7 @@ struct CeRowArgs {
     __nv_bfloat16 *a;             // gathered rows [rows, PARTS * part_cols]
     int64_t lda, part_cols;
     float *off2, *lt, *dist, *scale, *tval;
-    float spread;                 // sqrt(2 ln V)
+    float spread;                 // mean of the largest of V standard normal values
     int32_t *tcol;
     // backward
     const float *dloss;           // null: forward
@@ -936,65 +936,200 @@ struct CeSumArgs {
     uint32_t *ticket;             // zero at the start
 };
 
-// A row whose sum left float32's range: its logits once more on CUDA cores, first the maximum and the sum relative to it, then, with
-// slots, the gradient itself, which goes to the row's first slot.  By the whole block.
-template <typename T>
-__device__ __noinline__ void ce_rescue_row(const CeSumArgs &g, int64_t j) {
-    __shared__ float sh_m[16], sh_s[16], sh_p[16];
-    const CeRowArgs &a = g.rows;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = a.idx[j], t = a.target[row];
-    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
-    const float lt = a.lt[j];
-    auto logit = [&](int64_t v) {
-        float d = 0.0f;
-        for (int64_t c = lane; c < a.R; c += 32) d = fmaf(to_f32<T>(x[c]), vocab_at<T>(g.voc, v, c), d);
+// Sums over the warp of N values per lane (N a power of two): lane i gets that of value i % N.  Each step halves what a lane keeps.
+template <int N> __device__ __forceinline__ float warp_sums(float (&v)[N], int lane) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        return d;
-    };
-    float m = lt, s = 0.0f;                        // sum of exp(l - m) over the columns other than t, m the maximum so far
-    for (int64_t v = warp; v < a.V; v += 16) {
-        if (v == t) continue;
-        const float l = logit(v);
-        if (l > m) { s = s * expf(m - l) + 1.0f; m = l; }
-        else s += expf(l - m);
+    for (int o = N / 2; o; o >>= 1) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if (i < o) {
+                const float give = upper ? v[i] : v[i + o];
+                const float got = __shfl_xor_sync(0xffffffffu, give, o);
+                v[i] = (upper ? v[i + o] : v[i]) + got;
+            }
+        }
     }
-    __syncthreads();                               // the row before is done with the arrays
-    if (lane == 0) { sh_m[warp] = m; sh_s[warp] = s; }
+    float l = v[0];
+#pragma unroll
+    for (int o = N; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    return l;
+}
+
+// add one logit to a running (maximum, sum relative to it)
+__device__ __forceinline__ void online(float &m, float &s, float l) {
+    if (l > m) {
+        s = s * ex2((m - l) * LOG2E) + 1.0f;
+        m = l;
+    } else if (l == m) {
+        s += l == -INFINITY ? 0.0f : 1.0f;    // a difference of two infinities would be NaN
+    } else {
+        s += ex2((l - m) * LOG2E);
+    }
+}
+__device__ __forceinline__ void online_join(float &m, float &s, float m2, float s2) {
+    const float mm = fmaxf(m, m2);
+    s = (m == mm ? s : s * ex2((m - mm) * LOG2E)) + (m2 == mm ? s2 : s2 * ex2((m2 - mm) * LOG2E));
+    m = mm;
+}
+
+// Rows whose sum left float32's range: their logits once more on CUDA cores, first the maximum and the sum relative to it, then, with
+// slots, the gradient itself, which goes to a row's first slot.  By the whole block (512 threads), for up to FAR of its rows at a time
+// (`far`: bit r is row j0 + r): a warp multiplies FAR_ROWS rows of the matrix with all of them.  Bound by what one SM can load
+// (stored) or hash (noise).  Among 8192 rows of 768, V = 50257, the call takes, ms: stored, loss, no such row 0.5, one 3.6, 1024 7.7 (one row at a
+// time, a logit per warp: 25 and 84); noise, loss and gradient 1.0, 16, 52 (53, 337); all logits of standard deviation 150, loss, 15 (478).
+constexpr int FAR = 2, FAR_ROWS = 4, FAR_COLS = 4;
+
+template <typename T>
+__device__ __noinline__ void ce_far_rows(const CeSumArgs &g, int64_t j0, unsigned far) {
+    __shared__ float2 sh_ms[16][FAR];
+    __shared__ float sh_full[FAR];
+    __shared__ __align__(16) float sh_p[16 * FAR_ROWS][FAR];
+    const CeRowArgs &a = g.rows;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = (int)a.R;
+    const int n = __popc(far) < FAR ? __popc(far) : FAR;
+    int64_t j[FAR];
+    const T *x[FAR];
+    int64_t target[FAR];
+    unsigned left = far;
+#pragma unroll
+    for (int t = 0; t < FAR; ++t) {                // past the last one: the last one again, whose results nothing reads
+        j[t] = j0 + __ffs(left) - 1;
+        if (t + 1 < n) left &= left - 1;
+        const int64_t row = a.idx[j[t]];
+        x[t] = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+        target[t] = a.target[row];
+    }
+    constexpr int PAIRS = FAR_ROWS * FAR;
+    static_assert(FAR == 2, "two rows");
+    const int my_row = lane % PAIRS / FAR, my_t = lane % FAR;      // whose logit the lane gets
+    const int64_t my_target = target[my_t ? 1 : 0];
+    constexpr int W = 16 / sizeof(T);              // elements of a 16-byte load
+    const bool vec = g.voc.w && rows_aligned<T>(g.voc.w, g.voc.ldw) && rows_aligned<T>(a.x, a.ldx);
+    const int whole = vec ? R / W * W : 0;
+    // logits of matrix rows v0 .. v0 + 3 (rows past the end: the last one's)
+    auto logits = [&](int64_t v0) {
+        float acc[PAIRS];
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) acc[i] = 0.0f;
+        if (g.voc.w) {
+            const T *w[FAR_ROWS];
+#pragma unroll
+            for (int r = 0; r < FAR_ROWS; ++r) w[r] = reinterpret_cast<const T *>(g.voc.w) + (v0 + r < a.V ? v0 + r : a.V - 1) * g.voc.ldw;
+#pragma unroll 2
+            for (int c = lane * W; c < whole; c += 32 * W) {
+                uint4 u[FAR_ROWS];
+#pragma unroll
+                for (int r = 0; r < FAR_ROWS; ++r) u[r] = __ldg(reinterpret_cast<const uint4 *>(w[r] + c));
+#pragma unroll
+                for (int t = 0; t < FAR; ++t) {
+                    const uint4 f = __ldg(reinterpret_cast<const uint4 *>(x[t] + c));
+#pragma unroll
+                    for (int e = 0; e < W; ++e)
+#pragma unroll
+                        for (int r = 0; r < FAR_ROWS; ++r)
+                            acc[r * FAR + t] = fmaf(to_f32<T>(reinterpret_cast<const T *>(&f)[e]), to_f32<T>(reinterpret_cast<const T *>(&u[r])[e]), acc[r * FAR + t]);
+                }
+            }
+#pragma unroll 2
+            for (int c = whole + lane; c < R; c += 32)
+#pragma unroll
+                for (int r = 0; r < FAR_ROWS; ++r) {
+                    const float f = to_f32<T>(w[r][c]);
+#pragma unroll
+                    for (int t = 0; t < FAR; ++t) acc[r * FAR + t] = fmaf(to_f32<T>(x[t][c]), f, acc[r * FAR + t]);
+                }
+        } else {
+            uint32_t h = sq5_lin_rows(g.voc.seed, g.voc.row0 + (uint32_t)v0, (uint32_t)lane).base;
+#pragma unroll 2
+            for (int c = lane; c < R; c += 32, h += 32u * SQ5_N1) {
+                float f[FAR];
+#pragma unroll
+                for (int t = 0; t < FAR; ++t) f[t] = to_f32<T>(x[t][c]);
+#pragma unroll
+                for (int r = 0; r < FAR_ROWS; ++r) {
+                    const float w = to_f32<T>(from_f32<T>(sq5_to_float(sq5_tail(h + (uint32_t)r * (SQ5_PRIME * SQ5_N1)))));
+#pragma unroll
+                    for (int t = 0; t < FAR; ++t) acc[r * FAR + t] = fmaf(f[t], w, acc[r * FAR + t]);
+                }
+            }
+        }
+        return warp_sums(acc, lane);
+    };
+    float m = -INFINITY, s = 0.0f;                 // over the columns other than the target
+    for (int64_t v0 = warp * FAR_ROWS; v0 < a.V; v0 += 16 * FAR_ROWS) {
+        const float l = logits(v0);
+        if (lane < PAIRS && v0 + my_row < a.V && v0 + my_row != my_target) online(m, s, l);
+    }
+#pragma unroll
+    for (int o = FAR; o < 32; o <<= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        online_join(m, s, m2, s2);
+    }
+    __syncthreads();                               // the rows before are done with the arrays
+    if (lane < FAR) sh_ms[warp][lane] = make_float2(m, s);
     __syncthreads();
-    float mm = sh_m[0], ss = 0.0f;
-    for (int k = 1; k < 16; ++k) mm = fmaxf(mm, sh_m[k]);
-    for (int k = 0; k < 16; ++k) ss += sh_s[k] * expf(sh_m[k] - mm);
-    const float full = mm + logf(ss + expf(lt - mm));
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < n) {
+        const int t = threadIdx.x;
+        float2 r = sh_ms[0][t];
+        for (int k = 1; k < 16; ++k) online_join(r.x, r.y, sh_ms[k][t].x, sh_ms[k][t].y);
+        const int64_t jt = j[t ? 1 : 0], row = a.idx[jt];
+        const float lt = a.lt[jt];
+        online_join(r.x, r.y, lt, 1.0f);
+        const float full = r.x + logf(r.y);
         g.loss_rows[row] = full - lt;
         if (g.loss_rows2) g.loss_rows2[row] = full - lt;
         g.lse[row] = full;
-        g.s[j] = -1.0f;
+        g.s[jt] = -1.0f;
+        sh_full[t] = full;
     }
     if (!g.slots) return;
+    __syncthreads();
+    const float my_full = sh_full[my_t < n ? my_t : n - 1];
     const int tiles_n = (int)((a.R + CE_TILE - 1) / CE_TILE);
-    const float pt = expf(lt - full);
-    for (int nt = 0; nt < tiles_n; ++nt) {         // columns of one tile at a time
-        const SlotRow o(g.slots, g.parts, tiles_n, a.tile_rows, j, nt);
-        const int64_t c = (int64_t)nt * CE_TILE + threadIdx.x;
-        const bool mine = threadIdx.x < CE_TILE && c < a.R;
-        float acc = mine ? (pt - 1.0f) * vocab_at<T>(g.voc, t, c) : 0.0f;
-        for (int64_t v0 = 0; v0 < a.V; v0 += 16) {
-            const int64_t v = v0 + warp;
-            float p = 0.0f;
-            if (v < a.V && v != t) p = expf(logit(v) - full);
-            if (lane == 0) sh_p[warp] = p;
+    for (int c0 = 0; c0 < R; c0 += 512 * FAR_COLS) {              // so many columns at a time, FAR_COLS per thread
+        float acc[FAR_COLS][FAR];
+#pragma unroll
+        for (int k = 0; k < FAR_COLS; ++k) {
+            const int c = c0 + k * 512 + (int)threadIdx.x;
+#pragma unroll
+            for (int t = 0; t < FAR; ++t) {
+                const float full = sh_full[t < n ? t : n - 1];
+                acc[k][t] = c < R ? (expf(a.lt[j[t]] - full) - 1.0f) * vocab_at<T>(g.voc, target[t], c) : 0.0f;
+            }
+        }
+        for (int64_t v0 = 0; v0 < a.V; v0 += 16 * FAR_ROWS) {
+            const int64_t v = v0 + warp * FAR_ROWS + my_row;
+            if (v0 + warp * FAR_ROWS < a.V) {
+                const float l = logits(v0 + warp * FAR_ROWS);
+                if (lane < PAIRS) sh_p[warp * FAR_ROWS + my_row][my_t] = v < a.V && v != my_target ? expf(l - my_full) : 0.0f;
+            }
             __syncthreads();
-            if (mine) {
+            const int rows = a.V - v0 < 16 * FAR_ROWS ? (int)(a.V - v0) : 16 * FAR_ROWS;
 #pragma unroll 1
-                for (int k = 0; k < 16; ++k)
-                    if (sh_p[k] != 0.0f) acc = fmaf(sh_p[k], vocab_at<T>(g.voc, v0 + k, c), acc);
+            for (int k = 0; k < rows; ++k) {
+                const float2 p = *reinterpret_cast<const float2 *>(sh_p[k]);
+                if (p.x == 0.0f && p.y == 0.0f) continue;
+#pragma unroll
+                for (int q = 0; q < FAR_COLS; ++q) {
+                    const int c = c0 + q * 512 + (int)threadIdx.x;
+                    if (c < R) {
+                        const float w = vocab_at<T>(g.voc, v0 + k, c);
+                        acc[q][0] = fmaf(p.x, w, acc[q][0]);
+                        acc[q][1] = fmaf(p.y, w, acc[q][1]);
+                    }
+                }
             }
             __syncthreads();
         }
-        if (mine) o.first[threadIdx.x] = acc;
+#pragma unroll
+        for (int q = 0; q < FAR_COLS; ++q) {
+            const int c = c0 + q * 512 + (int)threadIdx.x;
+            if (c >= R) continue;
+#pragma unroll
+            for (int t = 0; t < FAR; ++t)
+                if (t < n) SlotRow(g.slots, g.parts, tiles_n, a.tile_rows, j[t], c / CE_TILE).first[c % CE_TILE] = acc[q][t];
+        }
     }
 }
 
@@ -1002,7 +1137,7 @@ __device__ __noinline__ void ce_rescue_row(const CeSumArgs &g, int64_t j) {
 // order; rows beyond float32's range are redone.  The block that finishes last adds up the losses of all rows (ignored ones hold
 // 0) in one fixed order.
 template <typename T>
-__global__ void __launch_bounds__(512) ce_sum_kernel(const CeSumArgs g) {
+__global__ void __launch_bounds__(512, 2) ce_sum_kernel(const CeSumArgs g) {
     __shared__ float sh[16][33];
     __shared__ double sh_d[16];
     __shared__ unsigned far;
@@ -1038,7 +1173,10 @@ __global__ void __launch_bounds__(512) ce_sum_kernel(const CeSumArgs g) {
             if (r == 0) far = f;
         }
         __syncthreads();
-        for (unsigned f = far; f; f &= f - 1) ce_rescue_row<T>(g, j0 + __ffs(f) - 1);
+        for (unsigned f = far; f;) {
+            ce_far_rows<T>(g, j0, f);
+            for (int k = 0; k < FAR; ++k) f &= f - 1;
+        }
     }
     if (!g.loss) return;
     __syncthreads();
@@ -1098,7 +1236,7 @@ __global__ void __launch_bounds__(CE_TILE, ROWS == 16 ? 4 : 2) ce_dx_kernel(O *_
             if (s) {
                 sj = s[j];
                 const int32_t t = tcol[j];
-                if (sj < 0.0f) {                      // the row was finished by ce_rescue_row
+                if (sj < 0.0f) {                      // the row was finished by ce_far_rows
                     n = 1;
                     sj = 0.0f;
                 } else {
@@ -1221,23 +1359,6 @@ struct FewArgs {
     float *lse, *loss_rows, *loss_rows2, *count, *loss;
 };
 
-// add one logit to a running (maximum, sum relative to it)
-__device__ __forceinline__ void online(float &m, float &s, float l) {
-    if (l > m) {
-        s = s * ex2((m - l) * LOG2E) + 1.0f;
-        m = l;
-    } else if (l == m) {
-        s += l == -INFINITY ? 0.0f : 1.0f;    // a difference of two infinities would be NaN
-    } else {
-        s += ex2((l - m) * LOG2E);
-    }
-}
-__device__ __forceinline__ void online_join(float &m, float &s, float m2, float s2) {
-    const float mm = fmaxf(m, m2);
-    s = (m == mm ? s : s * ex2((m - mm) * LOG2E)) + (m2 == mm ? s2 : s2 * ex2((m2 - mm) * LOG2E));
-    m = mm;
-}
-
 // rows of x in shared memory start at 16 bytes
 __host__ __device__ __forceinline__ int few_stride(int64_t R) { return (int)((R + 3) / 4 * 4); }
 
@@ -1253,7 +1374,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, few_blocks(NT, NOISE)) ce_few_
         for (int c = threadIdx.x; c < R; c += FEW_WARPS * 32)
             xs[t * RS + c] = t < a.T ? to_f32<T>(reinterpret_cast<const T *>(a.x)[t * a.ldx + c]) : 0.0f;
     __syncthreads();
-    // after the exchange below lane i holds pair i of (vocabulary row, x row): row i / NT, x row i % NT
+    // lane i takes the sum of pair i of (vocabulary row, x row): row i / NT, x row i % NT
     constexpr int PAIRS = FEW_ROWS * NT;
     const int my_row = (lane % PAIRS) / NT, my_t = lane % NT;
     const int64_t my_target = my_t < a.T ? a.target[my_t] : -1;
@@ -1318,22 +1439,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, few_blocks(NT, NOISE)) ce_few_
                 }
             }
         }
-        // sums over the lanes, each step halving what a lane keeps; then over the lanes that keep the same pair
-#pragma unroll
-        for (int o = PAIRS / 2; o; o >>= 1) {
-            const bool upper = lane & o;
-#pragma unroll
-            for (int i = 0; i < PAIRS / 2; ++i) {
-                if (i < o) {
-                    const float give = upper ? acc[i] : acc[i + o];
-                    const float got = __shfl_xor_sync(0xffffffffu, give, o);
-                    acc[i] = (upper ? acc[i + o] : acc[i]) + got;
-                }
-            }
-        }
-        float l = acc[0];
-#pragma unroll
-        for (int o = PAIRS; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float l = warp_sums(acc, lane);
         const int64_t v = v0 + my_row;
         if (lane < PAIRS && v < a.V && v != my_target) online(m, s, l);
     }
@@ -1580,6 +1686,12 @@ static int ce_find_rows(const CeCall &c, int64_t ignore, int use_ignore, float *
                       c.p.pairs, c.p.tile_rows);
 }
 
+// Mean of the largest of n standard normal values, by its limiting (Gumbel) distribution; its spread is 1.28 / sqrt(2 ln n).
+static float largest_of(int64_t n) {
+    const double a = sqrt(2.0 * log((double)n));
+    return n < 16 ? (float)a : (float)(a + (0.5772 - 0.5 * (log(log((double)n)) + log(4.0 * 3.14159265))) / a);
+}
+
 static CeRowArgs ce_row_args(const CeCall &c) {
     CeRowArgs a{};
     a.x = c.x; a.ldx = c.ldx; a.T = c.T; a.R = c.R; a.V = c.V;
@@ -1591,7 +1703,7 @@ static CeRowArgs ce_row_args(const CeCall &c) {
     a.off2 = c.at<float>(c.p.off2);
     a.lt = c.at<float>(c.p.lt);
     a.dist = c.at<float>(c.p.dist);
-    a.spread = (float)sqrt(2.0 * log((double)c.V));
+    a.spread = largest_of(c.V);
     a.scale = c.at<float>(c.p.scale);
     a.tval = c.at<float>(c.p.tval);
     a.tcol = c.at<int32_t>(c.p.tcol);
