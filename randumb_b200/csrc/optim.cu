@@ -134,7 +134,10 @@ __device__ __forceinline__ uint32_t ue4m4_code(float q, float v, uint32_t r19) {
     return (c == 0u && v > 0.0f) ? 1u : c;
 }
 
-// division and square root of the update, within 2^-21.  An eps near zero could meet a denominator that the fast forms flush.
+// Division and square root of the update, within 2^-21.  The fast forms take values below 2^-126 for 0.  A v below it then misses from the
+// denominator with up to 2^-63 inv_root, so they are taken where eps is 2^21 times that (the usual 1e-8 is); an m below it has an
+// update of at most 2^-126 / eps < 2^-84, which becomes 0.
+constexpr float FAST_EPS = 2.2737368e-13f;     // 2^21 * 2^-63
 __device__ __forceinline__ float update_of(float m, float v, float inv_root, float eps, bool fast) {
     if (fast) {
         float r, q;
@@ -319,7 +322,6 @@ adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, c
     const uint32_t segs = tab.first[tab.count];
     StepScalars c{};
     c.eps = s.eps;
-    c.fast = s.eps > 1e-30f;
     float t_have = NAN;
     uint32_t g = blockIdx.x * (ADAMW_THREADS / 32) + (threadIdx.x >> 5);
     int ti = find_tensor(tab, g);
@@ -331,6 +333,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, c
             const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
             c.size = (float)(lr / -expm1((double)t * s.ln_beta1));            // 1 - beta^t
             c.inv_root = 1.0f / sqrtf((float)-expm1((double)t * s.ln_beta2));
+            c.fast = s.eps >= FAST_EPS * c.inv_root;
             c.decay = (float)(1.0 - lr * s.weight_decay);
             t_have = t;
         }

@@ -438,3 +438,29 @@ def test_a_tensor_past_32_bit_offsets(rb, bits):
     assert torch.equal(m[0].view(torch.uint8)[(head if bits == 8 else 4 * head):], m2[0].view(torch.uint8))
     # the random rounding of an 8-bit second moment goes by the element's place, the update of a first step does not hang on it
     assert torch.equal(p[head:], q[0]) and (p[:head:1 << 20] == 0).all()
+
+
+@pytest.mark.parametrize("pdtype,bits", [(torch.float32, 32), (torch.float32, 8), (torch.bfloat16, 32)])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-25, 1e-20, 1e-18, 1e-16, 1e-15, 1e-13, 1e-11, 1e-8])
+def test_a_small_eps_and_small_gradients(rb, pdtype, bits, eps):
+    """First step from zero with lr 1, gradients of 1e-19 to 1e-15: v is below float32's normal range for most of them, its root is not, and eps
+    may be far below that.  The moments are taken as float32 rounds them (v by steps of 2^-149 here); what is left is the update:
+    quotient and root within 2^-21 as the kernel states, and eight roundings of 2^-24 each, 2^-21 together."""
+    b1, b2, n = 0.9, 0.999, 600
+    g = torch.logspace(-19, -15, n, dtype=torch.float64).float() * (1 - 2 * (torch.arange(n) % 2))
+    p = torch.zeros(n, dtype=pdtype, device="cuda")
+    kw = {}
+    if bits == 32:
+        m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    else:
+        m, v = torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn), torch.zeros(n, dtype=torch.uint8, device="cuda")
+        kw = dict(exp_avg_scales=[torch.zeros(3, device="cuda")], exp_avg_sq_scales=[torch.zeros(3, device="cuda")])
+    if pdtype == torch.bfloat16:
+        kw["masters"] = [torch.zeros(n, device="cuda")]
+    rb.optim.adamw_step([p], [g.cuda()], [m], [v], torch.zeros(1, device="cuda"), lr=1.0, betas=(b1, b2), eps=eps, weight_decay=0.0, **kw)
+    m64 = (g * np.float32(1 - b1)).double()
+    v64 = torch.from_numpy((g.numpy() * g.numpy()) * np.float32(1 - b2)).double()
+    assert (v64 > 0).all() and (v64 < 2.0 ** -126).sum() > 100
+    want = -(m64 / (1 - b1)) / (torch.sqrt(v64 / (1 - b2)) + float(np.float32(eps)))
+    got = (kw["masters"][0] if pdtype == torch.bfloat16 else p).double().cpu()
+    assert ((got - want).abs() <= 2.0 ** -20 * want.abs()).all(), ((got - want).abs() / want.abs()).max()
