@@ -973,6 +973,11 @@ __device__ __forceinline__ void online_join(float &m, float &s, float m2, float 
     m = mm;
 }
 
+// log(1 + s e^up): the loss of a row whose other logits have a largest one `up` above the target's and a sum s relative to that
+__device__ __forceinline__ float loss_above(float up, float s) {
+    return s == 0.0f ? 0.0f : up < 60.0f ? log1pf(s * expf(up)) : up + logf(s + expf(-up));
+}
+
 // Rows whose sum left float32's range: their logits once more on CUDA cores, first the maximum and the sum relative to it, then, with
 // slots, the gradient itself, which goes to a row's first slot.  By the whole block (512 threads), for up to FAR of its rows at a time
 // (`far`: bit r is row j0 + r): a warp multiplies FAR_ROWS rows of the matrix with all of them.  Bound by what one SM can load
@@ -983,7 +988,7 @@ constexpr int FAR = 2, FAR_ROWS = 4, FAR_COLS = 4;
 template <typename T>
 __device__ __noinline__ void ce_far_rows(const CeSumArgs &g, int64_t j0, unsigned far) {
     __shared__ float2 sh_ms[16][FAR];
-    __shared__ float sh_full[FAR];
+    __shared__ float3 sh_ref[FAR];                 // the larger of target's and others' largest logit, log-sum-exp above it, loss
     __shared__ __align__(16) float sh_p[16 * FAR_ROWS][FAR];
     const CeRowArgs &a = g.rows;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = (int)a.R;
@@ -1074,18 +1079,17 @@ __device__ __noinline__ void ce_far_rows(const CeSumArgs &g, int64_t j0, unsigne
         float2 r = sh_ms[0][t];
         for (int k = 1; k < 16; ++k) online_join(r.x, r.y, sh_ms[k][t].x, sh_ms[k][t].y);
         const int64_t jt = j[t ? 1 : 0], row = a.idx[jt];
-        const float lt = a.lt[jt];
-        online_join(r.x, r.y, lt, 1.0f);
-        const float full = r.x + logf(r.y);
-        g.loss_rows[row] = full - lt;
-        if (g.loss_rows2) g.loss_rows2[row] = full - lt;
-        g.lse[row] = full;
+        const float lt = a.lt[jt], up = r.x - lt, l = loss_above(up, r.y);
+        const float ref = up > 0.0f ? r.x : lt, rest = up > 0.0f ? logf(r.y + expf(-up)) : l;
+        g.loss_rows[row] = l;
+        if (g.loss_rows2) g.loss_rows2[row] = l;
+        g.lse[row] = ref + rest;
         g.s[jt] = -1.0f;
-        sh_full[t] = full;
+        sh_ref[t] = make_float3(ref, rest, l);
     }
     if (!g.slots) return;
     __syncthreads();
-    const float my_full = sh_full[my_t < n ? my_t : n - 1];
+    const float3 my_ref = sh_ref[my_t < n ? my_t : n - 1];
     const int tiles_n = (int)((a.R + CE_TILE - 1) / CE_TILE);
     for (int c0 = 0; c0 < R; c0 += 512 * FAR_COLS) {              // so many columns at a time, FAR_COLS per thread
         float acc[FAR_COLS][FAR];
@@ -1094,15 +1098,14 @@ __device__ __noinline__ void ce_far_rows(const CeSumArgs &g, int64_t j0, unsigne
             const int c = c0 + k * 512 + (int)threadIdx.x;
 #pragma unroll
             for (int t = 0; t < FAR; ++t) {
-                const float full = sh_full[t < n ? t : n - 1];
-                acc[k][t] = c < R ? (expf(a.lt[j[t]] - full) - 1.0f) * vocab_at<T>(g.voc, target[t], c) : 0.0f;
+                acc[k][t] = c < R ? expm1f(-sh_ref[t < n ? t : n - 1].z) * vocab_at<T>(g.voc, target[t], c) : 0.0f;
             }
         }
         for (int64_t v0 = 0; v0 < a.V; v0 += 16 * FAR_ROWS) {
             const int64_t v = v0 + warp * FAR_ROWS + my_row;
             if (v0 + warp * FAR_ROWS < a.V) {
                 const float l = logits(v0 + warp * FAR_ROWS);
-                if (lane < PAIRS) sh_p[warp * FAR_ROWS + my_row][my_t] = v < a.V && v != my_target ? expf(l - my_full) : 0.0f;
+                if (lane < PAIRS) sh_p[warp * FAR_ROWS + my_row][my_t] = v < a.V && v != my_target ? expf((l - my_ref.x) - my_ref.y) : 0.0f;
             }
             __syncthreads();
             const int rows = a.V - v0 < 16 * FAR_ROWS ? (int)(a.V - v0) : 16 * FAR_ROWS;
@@ -1488,7 +1491,7 @@ __global__ void __launch_bounds__(FEW_T * 32) ce_few_finish_kernel(const FewArgs
         const bool kept = !(a.use_ignore && target == a.ignore);
         // relative to the target's logit while that holds, as everywhere else
         const float up = m - lt;
-        float loss = s == 0.0f ? 0.0f : up < 60.0f ? log1pf(s * expf(up)) : up + logf(s + expf(-up));
+        float loss = loss_above(up, s);
         if (!known) loss = NAN;
         if (!(lt == lt) || !(m == m)) loss = NAN;
         if (!kept) loss = 0.0f;

@@ -581,3 +581,52 @@ def test_refusals(rb):
         rb.rlinear_cross_entropy(x, torch.zeros(4, 15, device="cuda", dtype=torch.bfloat16), 1, 20, target)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         ce(x, w, target.cpu())
+
+
+def planned(kind, dtype, logits, ups, seed, R=160):
+    """Rows of x, a matrix of few rows and targets with chosen logits: logits [T, V] with V < R fixes x up to the matrix's null space, from which each
+    row gets as much as makes |x| |w_t| / sqrt(R) * (mean of the largest of V standard normal values) lie ups[i] above its target's logit (the largest
+    one): long rows that are not well aligned with their targets."""
+    T, V = logits.shape
+    g = torch.Generator().manual_seed(seed)
+    w = (noise_matrix(V, R, 1000 + seed, 5, dtype) if kind == "noise" else (torch.randn(V, R, generator=g) * 0.5).to(dtype)).double()
+    target = logits.argmax(1)
+    x = logits.double() @ torch.linalg.pinv(w).t()
+    n = torch.randn(T, R, generator=g, dtype=torch.float64)
+    n -= n @ torch.linalg.pinv(w) @ w
+    a = math.sqrt(2 * math.log(V))
+    spread = a + (0.5772 - 0.5 * (math.log(math.log(V)) + math.log(4 * 3.14159265))) / a
+    want = (logits.amax(1).double() + ups) * math.sqrt(R) / spread / w[target].norm(dim=1)
+    more = want ** 2 - (x ** 2).sum(1)
+    assert (more > 0).all()
+    x += n * (more.sqrt() / n.norm(dim=1))[:, None]
+    return x.to(dtype).cuda(), w.to(dtype).cuda(), target.cuda()
+
+
+def small_losses(x, w, target):
+    """(losses, largest sum of a logit's terms) in 64 bits, without the difference of log-sum-exp and logit: 2^-52 of a logit is more than
+    2^-20 of the smallest of these losses."""
+    xd, wd = x.double(), w.double()
+    logits = xd @ wd.t()
+    e = torch.exp(logits - logits.gather(1, target[:, None]))
+    e[torch.arange(x.shape[0]), target] = 0
+    return torch.log1p(e.sum(1)), (xd.abs() @ wd.abs().t()).amax().item()
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("top", [0.0, 30.0])
+@pytest.mark.parametrize("ups", [(76.0, 85.0, 110.0, 150.0, 400.0)])
+def test_a_likely_target_of_a_long_row(rb, kind, dtype, top, ups):
+    """The target is the most likely token by 10 to 35, in rows whose length says that some other logit should lie `ups` above it."""
+    gaps = (10.0, 15.0, 18.8, 22.0, 25.0, 35.0)
+    T, V, seed = len(gaps) * len(ups), 50, 4
+    g = torch.Generator().manual_seed(3)
+    logits = top - torch.tensor(gaps).repeat_interleave(len(ups))[:, None] + torch.randn(T, V, generator=g)
+    logits[torch.arange(T), torch.randint(0, V, (T,), generator=g)] = top
+    x, w, target = planned(kind, dtype, logits, torch.tensor(ups, dtype=torch.float64).repeat(len(gaps)), seed)
+    loss, _ = check(rb, kind, x, w, target, seed, -100, "none", torch.ones(T, device="cuda"))
+    # such a loss is the sum of e^(l_v - l_t): it is off, relative to itself, by the error of a difference of logits
+    losses, terms = small_losses(x, w, target)
+    logit, _ = tolerances(dtype, x.shape[1], V, terms)
+    assert losses.max() < 0.1 and ((loss.double() - losses).abs() <= 2 * logit * losses).all(), ((loss.double() - losses) / losses)
