@@ -9,9 +9,10 @@
 // so no running maximum is needed: the sum never falls below the target's own 1, and small losses and the gradients of tokens
 // the model already knows come out of log1p and of a sum without the target, not of a difference of nearly equal numbers.  Float32
 // holds e_v up to 69 above the target's logit (s below 2^100 leaves room for the gradient).  Where the row's length says that the
-// largest of V random logits will lie 40 or more above the target's (|x| |w_t| / sqrt(R) is their standard deviation, largest_of(V) of
-// those the mean of the largest), that estimate takes the target's place:  e_v = exp(l_v - l_t - d),  loss = log(s + exp(-d)) + d.  A row that leaves the range
-// all the same, at either end, is noticed and done again with its true maximum (ce_far_rows).
+// largest of V random logits will lie 40 or more above the target's (|x| |w_t| / sqrt(R) is their standard deviation, largest_of(V)
+// of those the mean of the largest), that estimate takes the target's place:  e_v = exp(l_v - l_t - d),  loss = log(1 + s exp(d)).
+// A row that leaves the range all the same, at either end, or whose target then turns out to be likelier than all others together,
+// is noticed and done again with its true maximum (ce_far_rows).
 //
 // Rows whose target is ignored are left out: the remaining rows are gathered to the front, and every later kernel works on that
 // many rows, a number that only the device knows.
@@ -43,6 +44,7 @@ using namespace ptx;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float S_LIMIT = 1.2676506e30f;       // 2^100: rows above are redone with their maximum
+constexpr float S_LEAST = 8.2718061e-25f;      // 2^-80: rows below, too; terms under 2^-126 are 0, and 2^20 of them are 2^-26 of this
 constexpr int CE_TILE = 256;
 constexpr int CE_EPI = 8;
 constexpr int CE_THREADS = (4 + CE_EPI) * 32;   // a control warpgroup (TMA, MMA, two idle warps) and two epilogue warpgroups
@@ -1163,9 +1165,11 @@ __global__ void __launch_bounds__(512, 2) ce_sum_kernel(const CeSumArgs g) {
             if (j < n) {
 #pragma unroll
                 for (int k = 0; k < 16; ++k) s += sh[k][r];
-                const float d = g.rows.dist[j], total = s + expf(-d);
-                const float l = d == 0.0f ? log1pf(s) : logf(total) + d;
-                lost = s >= S_LIMIT || total < 1.0f / S_LIMIT;          // not-a-number is the answer already
+                // d != 0: the others together are at least as likely as the target, or the row is redone: a small loss would come out of
+                // terms that float32 no longer holds, and of a difference (not-a-number is the answer already)
+                const float d = g.rows.dist[j], own = expf(-d);
+                const float l = d == 0.0f ? log1pf(s) : s < 1.0f && d < 85.0f ? log1pf(s * expf(d)) : logf(s + own) + d;
+                lost = s >= S_LIMIT || (d != 0.0f && (s < S_LEAST || s < own));
                 const int32_t row = g.rows.idx[j];
                 g.s[j] = s;
                 g.loss_rows[row] = l;

@@ -583,7 +583,7 @@ def test_refusals(rb):
         ce(x, w, target.cpu())
 
 
-def planned(kind, dtype, logits, ups, seed, R=160):
+def planned(kind, dtype, logits, ups, seed, R=400):
     """Rows of x, a matrix of few rows and targets with chosen logits: logits [T, V] with V < R fixes x up to the matrix's null space, from which each
     row gets as much as makes |x| |w_t| / sqrt(R) * (mean of the largest of V standard normal values) lie ups[i] above its target's logit (the largest
     one): long rows that are not well aligned with their targets."""
@@ -616,7 +616,7 @@ def small_losses(x, w, target):
 @pytest.mark.parametrize("kind", ["noise", "linear"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("top", [0.0, 30.0])
-@pytest.mark.parametrize("ups", [(76.0, 85.0, 110.0, 150.0, 400.0)])
+@pytest.mark.parametrize("ups", [(41.0, 48.0, 55.0, 62.0, 69.0), (76.0, 85.0, 110.0, 150.0, 400.0)])
 def test_a_likely_target_of_a_long_row(rb, kind, dtype, top, ups):
     """The target is the most likely token by 10 to 35, in rows whose length says that some other logit should lie `ups` above it."""
     gaps = (10.0, 15.0, 18.8, 22.0, 25.0, 35.0)
@@ -630,3 +630,23 @@ def test_a_likely_target_of_a_long_row(rb, kind, dtype, top, ups):
     losses, terms = small_losses(x, w, target)
     logit, _ = tolerances(dtype, x.shape[1], V, terms)
     assert losses.max() < 0.1 and ((loss.double() - losses).abs() <= 2 * logit * losses).all(), ((loss.double() - losses) / losses)
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_likeliest_of_widely_spread_logits(rb, kind, dtype):
+    """Logits of deviation 200, rows whose target is the largest by 5 to 30 and lies far below where the largest usually does."""
+    R, V, seed = 64, 1000, 6
+    x, w, _ = inputs(kind, 30000, R, V, dtype, seed, 200.0)
+    logits = x.double() @ w.double().t()
+    two = logits.topk(2)
+    gap = two.values[:, 0] - two.values[:, 1]
+    rows = torch.nonzero((gap > 5) & (gap < 30))[:, 0]
+    rows = rows[two.values[rows, 0].argsort()[:80]]
+    target = two.indices[rows, 0]
+    assert rows.numel() == 80 and two.values[rows, 0].max() < 560
+    x = x[rows].contiguous()
+    loss, _ = check(rb, kind, x, w, target, seed, -100, "none", torch.ones(80, device="cuda"))
+    losses, terms = small_losses(x, w, target)
+    logit, _ = tolerances(dtype, R, V, terms)
+    assert ((loss.double() - losses).abs() <= 2 * logit * losses).all(), ((loss.double() - losses) / losses)
