@@ -650,3 +650,45 @@ def test_the_likeliest_of_widely_spread_logits(rb, kind, dtype):
     losses, terms = small_losses(x, w, target)
     logit, _ = tolerances(dtype, R, V, terms)
     assert ((loss.double() - losses).abs() <= 2 * logit * losses).all(), ((loss.double() - losses) / losses)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("common", [-100.0, 60.0])
+def test_logits_with_a_common_part(rb, dtype, common):
+    """Rows of a stored matrix that share a component, as trained ones do: all logits about `common`, of deviation 3."""
+    T, R, V, seed = 700, 96, 2000, 9
+    g = torch.Generator().manual_seed(seed)
+    u = torch.randn(R, generator=g)
+    u /= u.norm()
+    x = torch.randn(T, R, generator=g)
+    x += (10 - x @ u)[:, None] * u
+    w = torch.randn(V, R, generator=g) * 0.3
+    w += (common / 10 - w @ u)[:, None] * u
+    target = torch.randint(0, V, (T,), generator=g).cuda()
+    check(rb, "linear", x.to(dtype).cuda(), w.to(dtype).cuda(), target, seed, -100, "none", torch.ones(T, device="cuda"))
+
+
+def test_logits_with_a_common_part_take_the_ordinary_way(rb):
+    """Rows about -100 with deviation 3 are no harder than rows about 0: no row needs the slow way (which takes a hundred times as long)."""
+    T, R, V = 2048, 256, 20000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    u = torch.randn(R, device="cuda", generator=g)
+    u /= u.norm()
+    x = torch.randn(T, R, device="cuda", generator=g)
+    x += (10 - x @ u)[:, None] * u
+    w = torch.randn(V, R, device="cuda", generator=g) * (3 / R ** 0.5)
+    target = torch.randint(0, V, (T,), device="cuda", generator=g)
+    took = []
+    for common in (0.0, -100.0):
+        ww, xx = (w + (common / 10 - w @ u)[:, None] * u).bfloat16(), x.bfloat16()
+        times = []
+        with torch.no_grad():
+            for _ in range(8):
+                a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                a.record()
+                rb.linear_cross_entropy(xx, ww, target)
+                b.record()
+                b.synchronize()
+                times.append(a.elapsed_time(b))
+        took.append(sorted(times)[2])
+    assert took[1] < 8 * took[0], took
