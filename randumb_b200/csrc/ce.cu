@@ -529,6 +529,10 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                         if (EPI == EPI_PROB) {
 #pragma unroll
                             for (int j = 0; j < 64; ++j) e[j] *= scale;
+                            if (row_w + 32 > rows) {             // padding, which the weight gradient contracts with: 0 even against an infinite weight
+#pragma unroll
+                                for (int j = 0; j < 64; ++j) e[j] = row_w + lane < rows ? e[j] : 0.0f;
+                            }
                         }
                         if (__any_sync(0xffffffffu, (unsigned)tr < 64u)) {      // a target among these columns: left out of the sum
                             const float tv = EPI == EPI_PROB ? tval : 0.0f;

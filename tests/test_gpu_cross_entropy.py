@@ -692,3 +692,25 @@ def test_logits_with_a_common_part_take_the_ordinary_way(rb):
                 times.append(a.elapsed_time(b))
         took.append(sorted(times)[2])
     assert took[1] < 8 * took[0], took
+
+
+@pytest.mark.parametrize("T", [5, 70, 700])
+def test_vocabulary_rows_masked_by_minus_infinity(rb, T):
+    """Vocabulary rows that hold minus infinity in a column where every x is positive have probability 0: they reach neither the loss nor another
+    row's weight gradient, and their own is 0, whatever number of rows the last tile holds."""
+    R, V, seed, dtype = 40, 300, 2, torch.bfloat16
+    x, w, target = inputs("linear", T, R, V, dtype, seed)
+    x[:, 0] = x[:, 0].abs() + 0.5
+    off = torch.tensor([7, 100, 299], device="cuda")
+    target[torch.isin(target, off)] = 3
+    w[off, 0] = -math.inf
+    keep = torch.ones(V, dtype=torch.bool, device="cuda")
+    keep[off] = False
+    place = keep.cumsum(0) - 1
+    wl, kl = w.clone().requires_grad_(), w[keep].clone().requires_grad_()
+    loss, want = rb.linear_cross_entropy(x, wl, target), rb.linear_cross_entropy(x, kl, place[target])
+    dw, dk = torch.autograd.grad(loss, wl)[0], torch.autograd.grad(want, kl)[0]
+    assert (dw[off] == 0).all()
+    # the same numbers added in another order
+    assert abs(loss.item() / want.item() - 1) < 2.0 ** -19
+    assert (dw[keep].double() - dk.double()).abs().max() <= 2.0 ** -8 * dk.double().abs().max()
