@@ -9,6 +9,7 @@
 //   m' = b1 m + (1 - b1) g        v' = b2 v + (1 - b2) g^2
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 #include <cuda_fp8.h>
+#include <float.h>
 #include <math.h>
 #include <type_traits>
 
@@ -122,6 +123,8 @@ __device__ __forceinline__ float divide_by(float x, float d, float inv) {
     const float q = __fmul_rn(x, inv);
     return __fmaf_rn(__fmaf_rn(-q, d, x), inv, q);
 }
+
+constexpr float V_MOST = 3e38f;         // largest second moment in 8 bits: 1.9375 times its scale is still finite
 
 // Second moment in 8 bits: no sign, 4 exponent bits (bias 15), 4 mantissa bits; byte 255 stands for 1.9375 and carries the
 // block's maximum.  Shifted into a float32 the byte sits on top of exponent and mantissa, so its value is that float32 times
@@ -255,8 +258,25 @@ __device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, i
     }
     store8<VEC>(reinterpret_cast<P *>(d.p) + at, p8, lane, left);
     if (MASTER) store8<VEC>(d.master + at, w8, lane, left);
-    mscale = __fmul_rn(warp_max(mmax), 1.0f / 448.0f);
-    vscale = __fmul_rn(warp_max(vmax), 1.0f / 1.9375f);
+    mmax = warp_max(mmax);
+    vmax = warp_max(vmax);
+    if (!(mmax <= FLT_MAX && vmax <= V_MOST)) {
+        // Some element's moments have left the range: it is lost (first moment NaN from here on), and its block's others go on as if it were
+        // not there.  An infinite scale would turn them all into 0 * infinity.
+        mmax = vmax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (!(fabsf(m[j]) <= FLT_MAX && v[j] <= V_MOST)) m[j] = NAN;
+            else {
+                mmax = fmaxf(mmax, fabsf(m[j]));
+                vmax = fmaxf(vmax, v[j]);
+            }
+        }
+        mmax = warp_max(mmax);
+        vmax = warp_max(vmax);
+    }
+    mscale = __fmul_rn(mmax, 1.0f / 448.0f);
+    vscale = __fmul_rn(vmax, 1.0f / 1.9375f);
     const uint32_t h0 = (uint32_t)at * SQ5_N1 + rseed;
     // ordinary scales: multiply by the reciprocal; scales next to nothing (or not a number) divide, zero scales give zero
     const bool easy = mscale > 1e-30f && vscale > 1e-30f && mscale < 1e30f && vscale < 1e30f;

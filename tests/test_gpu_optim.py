@@ -464,3 +464,50 @@ def test_a_small_eps_and_small_gradients(rb, pdtype, bits, eps):
     want = -(m64 / (1 - b1)) / (torch.sqrt(v64 / (1 - b2)) + float(np.float32(eps)))
     got = (kw["masters"][0] if pdtype == torch.bfloat16 else p).double().cpu()
     assert ((got - want).abs() <= 2.0 ** -20 * want.abs()).all(), ((got - want).abs() / want.abs()).max()
+
+
+def _eight(k):
+    return [torch.zeros(k, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)], [torch.zeros(k, dtype=torch.uint8, device="cuda")], \
+        dict(exp_avg_scales=[torch.zeros(-(-k // 256), device="cuda")], exp_avg_sq_scales=[torch.zeros(-(-k // 256), device="cuda")])
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan, 1e25])
+def test_8_bit_moments_lose_one_element_to_a_gradient_out_of_range(rb, bad, shift):
+    """One infinity, NaN or value whose square is infinite in one step: that element's parameter and first moment are NaN from then on, and
+    every other element has the bytes of a run in which the gradient was 0 there."""
+    n, at = 700, 261
+    runs = []
+    for first in (bad, 0.0):
+        p = torch.zeros(n + shift, device="cuda")[shift:]
+        m, v, kw = _eight(n + shift)
+        m, v = [m[0][shift:]], [v[0][shift:]]
+        kw = {k: [t[0][:3].clone()] for k, t in kw.items()}
+        steps = torch.zeros(1, device="cuda")
+        for k in range(4):
+            g = torch.randn(n, generator=torch.Generator().manual_seed(k)).cuda()
+            g[at] = first if k == 0 else 0.0
+            rb.optim.adamw_step([p], [g], m, v, steps, lr=0.1, **kw)
+        runs.append((p, m[0].view(torch.uint8), v[0], rb.optim.first_moment_values(m[0], kw["exp_avg_scales"][0]), *[t[0] for t in kw.values()]))
+    rest = torch.arange(n, device="cuda") != at
+    assert torch.isnan(runs[0][0][at]) and torch.isnan(runs[0][3][at])
+    for a, b in zip(*runs):
+        keep = rest if a.numel() == n else slice(None)
+        assert torch.equal(a[keep], b[keep])
+
+
+def test_8_bit_moments_of_a_gradient_just_in_range(rb):
+    """g = 1e19: the second moment, 1e35, is the largest of its block and stays finite; the parameters stay numbers."""
+    n = 300
+    p = torch.zeros(n, device="cuda")
+    m, v, kw = _eight(n)
+    steps = torch.zeros(1, device="cuda")
+    for k in range(4):
+        g = torch.randn(n, generator=torch.Generator().manual_seed(k)).cuda()
+        if k == 0:
+            g[7] = 1e19
+        rb.optim.adamw_step([p], [g], m, v, steps, lr=0.1, **kw)
+        assert torch.isfinite(p).all() and p.abs().max() < 0.1 * 40 * (k + 1)
+        values = rb.optim.second_moment_values(v[0], kw["exp_avg_sq_scales"][0])
+        assert torch.isfinite(rb.optim.first_moment_values(m[0], kw["exp_avg_scales"][0])).all()
+        assert torch.isfinite(values).all() and values[7] == values.max() and values[7] > 9e34
