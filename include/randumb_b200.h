@@ -444,7 +444,8 @@ int rdb_gemm_dense_scatter(void *const *dst_ptrs, int ndst, size_t dst_offset_by
  *                 the upper 19 of the 1-D noise word of (element index mod 2^32) under the seed
  *                 h->seed + t * 0x9E3779B1 + i * 0x85EBCA6B (tensor i of the list): the same call gives the same bytes.
  *                 An element whose new moments leave float32's range (an infinite gradient, one whose square is infinite) is left out of its
- *                 block's scales; its first moment is NaN from then on, the other elements are as if its gradient had been 0.
+ *                 block's scales; its first moment is NaN from then on, the other elements are as if its gradient had been 0.  So is
+ *                 an element whose gradient is NaN (its second moment, whose code has no NaN, is stored as the block's largest).
  * Tensors may start at any address their element type allows (vector accesses where all of a tensor's pointers allow them).
  * Entries of the list must not overlap.  rdb_grad_norm (grads, numels, dtypes: HOST arrays): 2-norm over all gradients in float64 partial sums, repeatable;
  * coef (may be null) = min(1, max_norm / (norm + 1e-6)), the factor to pass as grad_scale.  workspace: 8-byte aligned.

@@ -278,7 +278,8 @@ __device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, i
     mscale = __fmul_rn(mmax, 1.0f / 448.0f);
     vscale = __fmul_rn(vmax, 1.0f / 1.9375f);
     const uint32_t h0 = (uint32_t)at * SQ5_N1 + rseed;
-    // ordinary scales: multiply by the reciprocal; scales next to nothing (or not a number) divide, zero scales give zero
+    // ordinary scales: multiply by the reciprocal; others divide, and a scale of zero gives zero, or NaN where the first moment is: its code
+    // holds NaN.  (The second moment's has none: 255, the block's largest.  An element never has it NaN alone.)
     const bool easy = mscale > 1e-30f && vscale > 1e-30f && mscale < 1e30f && vscale < 1e30f;
     const float minv = easy ? __frcp_rn(mscale) : 0.0f, vinv = easy ? __frcp_rn(vscale) : 0.0f;
 #pragma unroll
@@ -292,7 +293,7 @@ __device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, i
                 qm[k] = divide_by(m[j], mscale, minv);
                 qv[k] = divide_by(v[j], vscale, vinv);
             } else {
-                qm[k] = mscale > 0.0f ? __fdiv_rn(m[j], mscale) : 0.0f;
+                qm[k] = mscale > 0.0f || m[j] != m[j] ? __fdiv_rn(m[j], mscale) : 0.0f;
                 qv[k] = vscale > 0.0f ? __fdiv_rn(v[j], vscale) : 0.0f;
             }
             code[k] = ue4m4_code(qv[k], v[j], sq5_tail(h0 + (uint32_t)elem_of<VEC>(lane, j) * SQ5_N1) >> 13);

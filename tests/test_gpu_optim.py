@@ -511,3 +511,15 @@ def test_8_bit_moments_of_a_gradient_just_in_range(rb):
         values = rb.optim.second_moment_values(v[0], kw["exp_avg_sq_scales"][0])
         assert torch.isfinite(rb.optim.first_moment_values(m[0], kw["exp_avg_scales"][0])).all()
         assert torch.isfinite(values).all() and values[7] == values.max() and values[7] > 9e34
+
+
+def test_8_bit_moments_that_are_nothing_but_nan(rb):
+    """A tensor of one element, and a clipping factor that is NaN: no element of the block is a number, and the state says so."""
+    for n, gs in ((1, None), (300, torch.full((), math.nan, device="cuda"))):
+        p = torch.ones(n, device="cuda")
+        m, v, kw = _eight(n)
+        steps = torch.zeros(1, device="cuda")
+        rb.optim.adamw_step([p], [torch.full((n,), math.nan if gs is None else 1.0, device="cuda")], m, v, steps, grad_scale=gs, **kw)
+        assert torch.isnan(p).all() and torch.isnan(rb.optim.first_moment_values(m[0], kw["exp_avg_scales"][0])).all()
+        rb.optim.adamw_step([p.fill_(1.0)], [torch.ones(n, device="cuda")], m, v, steps, **kw)
+        assert torch.isnan(p).all()
