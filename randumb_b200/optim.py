@@ -238,6 +238,10 @@ class AdamW(torch.optim.Optimizer):
         self._lists: dict = {}                                      # (group, kind) -> state tensors of the parameters with a gradient, their lists
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights))
 
+    def add_param_group(self, param_group) -> None:
+        _refuse_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
+
     def _new_state(self, p: torch.Tensor, group: dict) -> dict:
         if p.dtype not in (torch.float32, torch.bfloat16) or not p.is_cuda:
             raise RuntimeError(f"AdamW takes float32 and bfloat16 CUDA parameters, got {p.dtype} on {p.device}")
@@ -326,8 +330,11 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but every state tensor keeps its own type (moments and masters of a bfloat16 parameter are not bfloat16).  The
         groups' hyperparameters, ``state_bits`` and ``master_weights`` among them, become the checkpoint's; what a checkpoint of
-        torch.optim.AdamW does not have keeps this optimiser's values, and its float32 moments load into 32-bit ones."""
+        torch.optim.AdamW does not have keeps this optimiser's values, and its float32 moments load into 32-bit ones.  Options that
+        this optimiser does not have (``maximize``, ``amsgrad``, ``differentiable``, torch.optim.Adam's weight decay) are refused."""
         here = [dict(g) for g in self.param_groups]
+        for group, old in zip(state_dict["param_groups"], here):
+            _refuse_options({**old, **group})
         super().load_state_dict(state_dict)
         self._lists = {}
         for group, old in zip(self.param_groups, here):
@@ -351,6 +358,17 @@ class AdamW(torch.optim.Optimizer):
                     t, v = t.view(torch.uint8), v.view(torch.uint8)
                 t.copy_(v.reshape(t.shape))
             self.state[p] = dst
+
+
+def _refuse_options(group: dict) -> None:
+    """Raises for what torch's optimisers can do and ``step`` would leave undone."""
+    for k in ("maximize", "amsgrad", "differentiable"):
+        if group.get(k):
+            raise ValueError(f"AdamW does not have the option {k}")
+    if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+        raise ValueError("AdamW's weight decay is decoupled from the gradient; the group asks for torch.optim.Adam's")
+    if group["state_bits"] not in (8, 32):
+        raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
 
 
 def _flat(t: torch.Tensor) -> torch.Tensor:

@@ -153,3 +153,23 @@ def test_optimizer_arguments():
     with pytest.raises(RuntimeError, match="one block of memory"):
         rb.optim._flat(torch.zeros(4, 4)[:, :2])
     assert rb.optim._flat(torch.arange(12).view(3, 4).t()).tolist() == list(range(12))
+
+
+def test_optimizer_refuses_options_that_it_does_not_have():
+    """maximize, amsgrad, differentiable and coupled weight decay (torch.optim.Adam's) are refused where a group or a checkpoint asks for them, and
+    a refused checkpoint leaves the optimiser as it was."""
+    p = torch.nn.Parameter(torch.zeros(3))
+    for bad in (dict(maximize=True), dict(amsgrad=True), dict(differentiable=True), dict(decoupled_weight_decay=False, weight_decay=0.1), dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            rb.optim.AdamW([{"params": [p], **bad}])
+    rb.optim.AdamW([{"params": [p], "maximize": False, "decoupled_weight_decay": False, "weight_decay": 0.0}])
+    q = torch.nn.Parameter(torch.zeros(3))
+    for other in (torch.optim.AdamW([q], maximize=True), torch.optim.AdamW([q], amsgrad=True), torch.optim.Adam([q], weight_decay=0.1)):
+        opt = rb.optim.AdamW([p], lr=0.5, state_bits=8)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == 0.5 and opt.param_groups[0]["state_bits"] == 8 and "maximize" not in opt.param_groups[0]
+    for other in (torch.optim.AdamW([q], lr=0.25), torch.optim.Adam([q], lr=0.25)):      # without weight decay the two are the same
+        opt = rb.optim.AdamW([p], lr=0.5)
+        opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == 0.25
