@@ -331,12 +331,22 @@ class AdamW(torch.optim.Optimizer):
         """As torch's, but every state tensor keeps its own type (moments and masters of a bfloat16 parameter are not bfloat16).  The
         groups' hyperparameters, ``state_bits`` and ``master_weights`` among them, become the checkpoint's; what a checkpoint of
         torch.optim.AdamW does not have keeps this optimiser's values, and its float32 moments load into 32-bit ones.  Options that
-        this optimiser does not have (``maximize``, ``amsgrad``, ``differentiable``, torch.optim.Adam's weight decay) are refused."""
+        this optimiser does not have (``maximize``, ``amsgrad``, ``differentiable``, torch.optim.Adam's weight decay) are refused.  A checkpoint that does not load
+        changes nothing."""
         here = [dict(g) for g in self.param_groups]
         for group, old in zip(state_dict["param_groups"], here):
             _refuse_options({**old, **group})
-        super().load_state_dict(state_dict)
-        self._lists = {}
+        before = self.state, self.param_groups
+        try:
+            super().load_state_dict(state_dict)
+            self._load_own(state_dict, here)
+        except Exception:                                           # as it was
+            self.state, self.param_groups = before
+            raise
+        finally:
+            self._lists = {}
+
+    def _load_own(self, state_dict, here: list) -> None:
         for group, old in zip(self.param_groups, here):
             for k in ("state_bits", "master_weights"):
                 group.setdefault(k, old[k])

@@ -173,3 +173,15 @@ def test_optimizer_refuses_options_that_it_does_not_have():
         opt = rb.optim.AdamW([p], lr=0.5)
         opt.load_state_dict(other.state_dict())
         assert opt.param_groups[0]["lr"] == 0.25
+
+
+def test_a_checkpoint_that_does_not_fit_changes_nothing():
+    p = torch.nn.Parameter(torch.zeros(3, dtype=torch.bfloat16))
+    opt = rb.optim.AdamW([p], lr=0.5)
+    opt.state[p]["step"] = torch.zeros(())
+    groups, state = opt.param_groups, opt.state
+    other = rb.optim.AdamW([torch.nn.Parameter(torch.zeros(3))], lr=0.25).state_dict()
+    other["state"] = {0: {"step": torch.tensor(3.0)}}
+    with pytest.raises(RuntimeError):
+        opt.load_state_dict(other)
+    assert opt.param_groups is groups and opt.state is state and groups[0]["lr"] == 0.5
