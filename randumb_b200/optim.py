@@ -218,7 +218,7 @@ class AdamW(torch.optim.Optimizer):
         seed: of the random rounding of 8-bit second moments.
 
     ``step()`` returns the closure's loss; ``last_grad_norm`` holds the norm of the last step (a device tensor) with ``max_grad_norm``.
-    The first step creates the state and cannot be captured; later ones can.
+    The first step creates the state and cannot be captured (it raises); later ones can.
     """
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -301,6 +301,9 @@ class AdamW(torch.optim.Optimizer):
                 if not st:
                     if g.is_sparse:
                         raise RuntimeError("AdamW does not take sparse gradients")
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: a parameter's first step creates its state and cannot be captured (a replay would begin again from "
+                                           "zero): take one step first")
                     st.update(self._new_state(p, group))
                 if p.is_contiguous() and g.is_contiguous() and g.dtype in _GRAD:
                     flat, g = p, g.detach()

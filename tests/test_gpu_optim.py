@@ -523,3 +523,20 @@ def test_8_bit_moments_that_are_nothing_but_nan(rb):
         assert torch.isnan(p).all() and torch.isnan(rb.optim.first_moment_values(m[0], kw["exp_avg_scales"][0])).all()
         rb.optim.adamw_step([p.fill_(1.0)], [torch.ones(n, device="cuda")], m, v, steps, **kw)
         assert torch.isnan(p).all()
+
+
+def test_the_first_step_is_not_captured(rb):
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = rb.optim.AdamW([p], lr=0.1)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            opt.step()
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert opt.state[p]["step"].item() == 2
