@@ -27,6 +27,7 @@ a CPU registration that raises ``NotImplementedError``: there is no CPU implemen
 """
 from __future__ import annotations
 
+import functools
 from typing import List, Optional, Tuple
 
 import torch
@@ -120,6 +121,32 @@ def _(rows, cols, seed, row0, dtype, device):
 # ------------------------------------------------------------------------------------------------
 # cross entropy over a large vocabulary
 # ------------------------------------------------------------------------------------------------
+class _Once(torch.autograd.Function):
+    """A gradient whose own gradient does not exist: it says so when it is asked for."""
+
+    @staticmethod
+    def forward(ctx, t):
+        return t.view_as(t)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("cross entropy: second derivatives are not implemented")
+
+
+def _first_order(backward):
+    """Marks the gradients that ``backward`` returns under create_graph=True.  (torch's once_differentiable does that only where the
+    incoming gradient takes part in autograd; that of a loss does not, and a penalty on the gradient would drop out silently.)"""
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        again = torch.is_grad_enabled()
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not again:
+            return out
+        return tuple(_Once.apply(t.detach().requires_grad_()) if isinstance(t, torch.Tensor) else t for t in out)
+    return wrapper
+
+
 @custom_op("rten::noise_ce_fwd", mutates_args=(), device_types="cuda")
 def noise_ce_fwd(z: torch.Tensor, target: torch.Tensor, seed: int, out_features: int, row0: int, ignore_index: Optional[int], reduction: str,
                  need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -158,6 +185,7 @@ def _noise_ce_setup(ctx, inputs, output):
     ctx.reduction, ctx.has_unit, ctx.dtype = inputs[6], inputs[7], inputs[0].dtype
 
 
+@_first_order
 def _noise_ce_backward(ctx, dloss, daux, dunit):
     aux, unit = ctx.saved_tensors
     if dloss is None or not ctx.needs_input_grad[0]:
@@ -208,6 +236,7 @@ def _linear_ce_setup(ctx, inputs, output):
     ctx.save_for_backward(x, weight, target, output[1])
 
 
+@_first_order
 def _linear_ce_backward(ctx, dloss, daux):
     x, weight, target, aux = ctx.saved_tensors
     need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
@@ -238,7 +267,7 @@ class _NoiseCE(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dloss):
         aux, unit = ctx.saved_tensors
         return K.ce_scale(unit, dloss, aux, ctx.reduction, ctx.dtype), None, None, None, None, None, None
@@ -255,7 +284,7 @@ class _LinearCE(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dloss):
         x, weight, target, aux = ctx.saved_tensors
         dx, dw = K.ce_bwd(dloss, x, weight, target, aux, ctx.ignore_index, ctx.reduction, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
@@ -498,6 +527,7 @@ class _DenseMMT(torch.autograd.Function):
         return K.gemm_dense(a.contiguous(), b.contiguous(), True, True)
 
     @staticmethod
+    @_first_order
     def backward(ctx, grad):
         a, b = ctx.saved_tensors
         grad = grad.contiguous()

@@ -714,3 +714,20 @@ def test_vocabulary_rows_masked_by_minus_infinity(rb, T):
     # the same numbers added in another order
     assert abs(loss.item() / want.item() - 1) < 2.0 ** -19
     assert (dw[keep].double() - dk.double()).abs().max() <= 2.0 ** -8 * dk.double().abs().max()
+
+
+def test_no_second_derivatives(rb):
+    """A gradient of a gradient is refused by every form of the loss; none of its parts drops out silently."""
+    x, w, target = inputs("linear", 20, 16, 30, torch.float32, 1)
+    c = torch.randn(8, 16, device="cuda")
+    for make in (lambda a: rb.linear_cross_entropy(a, w, target), lambda a: rb.noise_cross_entropy(a, 3, 30, target),
+                 lambda a: rb.rlinear_cross_entropy(a, c, 3, 30, target), lambda a: rb.rlinear_cross_entropy(a, c.requires_grad_(), 3, 30, target),
+                 lambda a: rb.linear_cross_entropy(a, w.requires_grad_(), target, reduction="none").square().sum(),
+                 lambda a: torch.ops.rten.noise_ce_fwd(a, target, 3, 30, 0, -100, "mean", True)[0],
+                 lambda a: torch.ops.rten.linear_ce_fwd(a, w.detach(), target, -100, "mean")[0]):
+        a = x.clone().requires_grad_()
+        grad = torch.autograd.grad(make(a), a, create_graph=True)[0]
+        b = x.clone().requires_grad_()
+        assert torch.equal(grad, torch.autograd.grad(make(b), b)[0])
+        with pytest.raises(RuntimeError):
+            (make(a) + grad.pow(2).sum()).backward()
