@@ -19,6 +19,7 @@ modded-nanogpt/train_gpt2.py:236-240):
 
   rten::noise_ce_fwd / rten::noise_ce_bwd     logits z S^T over regenerated noise rows
   rten::linear_ce_fwd / rten::linear_ce_bwd   logits x W^T over a stored matrix
+  rten::matmul_nt_fwd / rten::matmul_nt_bwd   z = x C^T in front of a noise head
   noise_cross_entropy, rlinear_cross_entropy, linear_cross_entropy   the differentiable functions on top of them
 
 Every operator is functional (fresh outputs, current stream), has a fake (meta) kernel so
@@ -249,6 +250,50 @@ def _linear_ce_backward(ctx, dloss, daux):
 linear_ce_fwd.register_autograd(_linear_ce_backward, setup_context=_linear_ce_setup)
 
 
+@custom_op("rten::matmul_nt_fwd", mutates_args=(), device_types="cuda")
+def matmul_nt_fwd(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    return K.gemm_dense(a.contiguous(), b.contiguous(), True, True)
+
+
+@matmul_nt_fwd.register_fake
+def _(a, b):
+    return a.new_empty((a.shape[0], b.shape[0]))
+
+
+matmul_nt_fwd.register_kernel("cpu")(_cpu_raises("matmul_nt_fwd"))
+
+
+@custom_op("rten::matmul_nt_bwd", mutates_args=(), device_types="cuda")
+def matmul_nt_bwd(grad: torch.Tensor, a: torch.Tensor, b: torch.Tensor, need_da: bool, need_db: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    da, db = _matmul_nt_grads(grad, a, b, need_da, need_db)
+    return da if need_da else a.new_empty((0,)), db if need_db else b.new_empty((0,))
+
+
+@matmul_nt_bwd.register_fake
+def _(grad, a, b, need_da, need_db):
+    return a.new_empty(a.shape if need_da else (0,)), b.new_empty(b.shape if need_db else (0,))
+
+
+matmul_nt_bwd.register_kernel("cpu")(_cpu_raises("matmul_nt_bwd"))
+
+
+def _matmul_nt_grads(grad, a, b, need_da, need_db):
+    grad = grad.contiguous()
+    return (K.gemm_dense(grad, b.contiguous(), True, False) if need_da else None,       # grad @ b
+            K.gemm_dense(grad, a.contiguous(), False, False) if need_db else None)      # grad^T @ a
+
+
+@_first_order
+def _matmul_nt_backward(ctx, grad):
+    a, b = ctx.saved_tensors
+    need_da, need_db = ctx.needs_input_grad
+    da, db = matmul_nt_bwd(grad, a, b, need_da, need_db)
+    return da if need_da else None, db if need_db else None
+
+
+matmul_nt_fwd.register_autograd(_matmul_nt_backward, setup_context=lambda ctx, inputs, output: ctx.save_for_backward(*inputs))
+
+
 def _eager(*ts: torch.Tensor) -> bool:
     """Plain CUDA tensors outside of any tracing: the kernels can be called without going through the dispatcher, which costs more
     than they do on small problems."""
@@ -289,6 +334,20 @@ class _LinearCE(torch.autograd.Function):
         x, weight, target, aux = ctx.saved_tensors
         dx, dw = K.ce_bwd(dloss, x, weight, target, aux, ctx.ignore_index, ctx.reduction, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dx, dw, None, None, None
+
+
+class _MatmulNT(torch.autograd.Function):
+    """a[L, P] @ b[Q, P].T on the library's product kernels: matmul_nt_fwd / matmul_nt_bwd for eager calls that take part in autograd."""
+
+    @staticmethod
+    def forward(ctx, a, b):
+        ctx.save_for_backward(a, b)
+        return K.gemm_dense(a.contiguous(), b.contiguous(), True, True)
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, grad):
+        return _matmul_nt_grads(grad, *ctx.saved_tensors, *ctx.needs_input_grad)
 
 
 def noise_cross_entropy(z: torch.Tensor, seed: int, out_features: int, target: torch.Tensor, row0: int = 0, ignore_index: Optional[int] = -100,
@@ -345,7 +404,7 @@ def rlinear_cross_entropy(x: torch.Tensor, coef: torch.Tensor, seed: int, out_fe
     x2 = x.reshape(-1, x.shape[-1])
     if ignore_index is not None:
         x2 = x2.masked_fill((target.reshape(-1) == ignore_index).unsqueeze(1), 0.0)
-    z = _DenseMMT.apply(x2, coef)
+    z = _MatmulNT.apply(x2, coef) if _eager(x2, coef) else matmul_nt_fwd(x2, coef)
     loss = noise_cross_entropy(z, seed, out_features, target.reshape(-1), row0, ignore_index, reduction)
     return loss.reshape(lead) if reduction == "none" else loss
 
@@ -515,24 +574,6 @@ class _DenseMM(torch.autograd.Function):
         grad = grad.contiguous()
         da = K.gemm_dense(grad, b.contiguous(), True, True) if ctx.needs_input_grad[0] else None      # grad @ b^T
         db = K.gemm_dense(a.contiguous(), grad, False, False) if ctx.needs_input_grad[1] else None   # a^T @ grad
-        return da, db
-
-
-class _DenseMMT(torch.autograd.Function):
-    """a[L, P] @ b[Q, P].T on the library's product kernels."""
-
-    @staticmethod
-    def forward(ctx, a, b):
-        ctx.save_for_backward(a, b)
-        return K.gemm_dense(a.contiguous(), b.contiguous(), True, True)
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, grad):
-        a, b = ctx.saved_tensors
-        grad = grad.contiguous()
-        da = K.gemm_dense(grad, b.contiguous(), True, False) if ctx.needs_input_grad[0] else None     # grad @ b
-        db = K.gemm_dense(grad, a.contiguous(), False, False) if ctx.needs_input_grad[1] else None    # grad^T @ a
         return da, db
 
 

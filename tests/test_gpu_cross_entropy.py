@@ -731,3 +731,17 @@ def test_no_second_derivatives(rb):
         assert torch.equal(grad, torch.autograd.grad(make(b), b)[0])
         with pytest.raises(RuntimeError):
             (make(a) + grad.pow(2).sum()).backward()
+
+
+def test_layer_loss_through_the_dispatcher(rb):
+    """The product in front of the noise head as an operator: schema, fake kernel, autograd, the same numbers as the eager function."""
+    x, _, target = inputs("linear", 60, 40, 90, torch.bfloat16, 3)
+    c = (torch.randn(24, 40, device="cuda") * 0.2).bfloat16()
+    xl, cl = x.clone().requires_grad_(), c.clone().requires_grad_()
+    torch.library.opcheck(torch.ops.rten.matmul_nt_fwd.default, (xl, cl), test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+    loss = torch.ops.rten.noise_ce_fwd(torch.ops.rten.matmul_nt_fwd(xl, cl), target, 1003, 90, 5, -100, "mean", True)[0]
+    grads = torch.autograd.grad(loss, [xl, cl])
+    x2, c2 = x.clone().requires_grad_(), c.clone().requires_grad_()
+    loss2 = rb.rlinear_cross_entropy(x2, c2, 1003, 90, target, row0=5)
+    grads2 = torch.autograd.grad(loss2, [x2, c2])
+    assert torch.equal(loss, loss2) and all(torch.equal(a, b) for a, b in zip(grads, grads2))

@@ -185,3 +185,24 @@ def test_a_checkpoint_that_does_not_fit_changes_nothing():
     with pytest.raises(RuntimeError):
         opt.load_state_dict(other)
     assert opt.param_groups is groups and opt.state is state and groups[0]["lr"] == 0.5
+
+
+def test_fake_tensors_through_the_layer_loss():
+    """rlinear_cross_entropy and RandumbLinear.cross_entropy can be traced like their parts; on CPU tensors they say what the parts say."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    layer = rb.RandumbLinear(16, 30, 8, seed=1, device="cpu", dtype=torch.bfloat16)
+    with FakeTensorMode():
+        x = torch.empty(4, 6, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        c = torch.empty(8, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        t = torch.empty(4, 6, device="cuda", dtype=torch.int64)
+        loss = rb.rlinear_cross_entropy(x, c, 1, 30, t)
+        assert loss.shape == () and loss.dtype == torch.float32 and loss.requires_grad
+        assert rb.rlinear_cross_entropy(x, c, 1, 30, t, reduction="none", ignore_index=None).shape == (4, 6)
+        layer.weight_coef = torch.nn.Parameter(torch.empty(8, 16, device="cuda", dtype=torch.bfloat16))
+        assert layer.cross_entropy(x, t).shape == ()
+        z = rb.ops.matmul_nt_fwd(x.reshape(24, 16), c)
+        assert z.shape == (24, 8) and z.dtype == torch.bfloat16
+        da, db = rb.ops.matmul_nt_bwd(z, x.reshape(24, 16), c, False, True)
+        assert da.shape == (0,) and db.shape == c.shape and db.dtype == c.dtype
+    with pytest.raises(NotImplementedError, match="Unsupported CPU implementation"):
+        rb.rlinear_cross_entropy(torch.ones(2, 3), torch.ones(4, 3), 1, 5, torch.zeros(2, dtype=torch.int64))
