@@ -32,6 +32,7 @@ import functools
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.library import custom_op
 
 from . import kernels as K
@@ -301,6 +302,12 @@ def _eager(*ts: torch.Tensor) -> bool:
         and not torch._C._len_torch_dispatch_stack()
 
 
+def _no_tangents(*ts: torch.Tensor) -> None:
+    """Forward-mode differentiation is not implemented: raises where a tangent would be dropped."""
+    if forward_ad._current_level >= 0 and any([forward_ad.unpack_dual(t).tangent is not None for t in ts]):
+        raise RuntimeError("cross entropy: forward-mode differentiation is not implemented")
+
+
 class _NoiseCE(torch.autograd.Function):
     """noise_ce_fwd / noise_ce_bwd for eager calls that take part in autograd."""
 
@@ -362,6 +369,7 @@ def noise_cross_entropy(z: torch.Tensor, seed: int, out_features: int, target: t
     lead = z.shape[:-1]
     if tuple(target.shape) != tuple(lead):
         raise RuntimeError(f"noise_cross_entropy: target {tuple(target.shape)} does not match z {tuple(z.shape)}")
+    _no_tangents(z)
     z2, t = z.reshape(-1, z.shape[-1]), target.reshape(-1)
     need = torch.is_grad_enabled() and z.requires_grad
     if not _eager(z2, t):
@@ -381,6 +389,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     lead = x.shape[:-1]
     if tuple(target.shape) != tuple(lead):
         raise RuntimeError(f"linear_cross_entropy: target {tuple(target.shape)} does not match x {tuple(x.shape)}")
+    _no_tangents(x, weight)
     x2, t = x.reshape(-1, x.shape[-1]), target.reshape(-1)
     if not _eager(x2, weight, t):
         loss = linear_ce_fwd(x2, weight, t, ignore_index, reduction)[0]
@@ -401,6 +410,7 @@ def rlinear_cross_entropy(x: torch.Tensor, coef: torch.Tensor, seed: int, out_fe
         raise RuntimeError(f"rlinear_cross_entropy: target {tuple(target.shape)} does not match x {tuple(x.shape)}")
     if coef.dim() != 2 or coef.shape[1] != x.shape[-1] or coef.dtype != x.dtype:
         raise RuntimeError(f"rlinear_cross_entropy: coef {tuple(coef.shape)} {coef.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    _no_tangents(x, coef)
     x2 = x.reshape(-1, x.shape[-1])
     if ignore_index is not None:
         x2 = x2.masked_fill((target.reshape(-1) == ignore_index).unsqueeze(1), 0.0)

@@ -206,3 +206,20 @@ def test_fake_tensors_through_the_layer_loss():
         assert da.shape == (0,) and db.shape == c.shape and db.dtype == c.dtype
     with pytest.raises(NotImplementedError, match="Unsupported CPU implementation"):
         rb.rlinear_cross_entropy(torch.ones(2, 3), torch.ones(4, 3), 1, 5, torch.zeros(2, dtype=torch.int64))
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation is not implemented, and says so where a tangent would be dropped."""
+    import torch.autograd.forward_ad as fw
+    x, w, c, t = torch.ones(2, 3), torch.ones(5, 3), torch.ones(4, 3), torch.zeros(2, dtype=torch.int64)
+    calls = (lambda a: rb.noise_cross_entropy(a, 1, 5, t), lambda a: rb.linear_cross_entropy(a, w, t), lambda a: rb.rlinear_cross_entropy(a, c, 1, 5, t))
+    for call in calls + (lambda a: rb.linear_cross_entropy(x, a.repeat(3, 1)[:5], t), lambda a: rb.rlinear_cross_entropy(x, a.repeat(2, 1), 1, 5, t)):
+        with fw.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(fw.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
+    with fw.dual_level():                                           # no tangent among the inputs: as ever
+        for call in calls:
+            with pytest.raises((NotImplementedError, RuntimeError), match="CPU"):
+                call(x)
