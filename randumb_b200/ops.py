@@ -296,10 +296,10 @@ matmul_nt_fwd.register_autograd(_matmul_nt_backward, setup_context=lambda ctx, i
 
 
 def _eager(*ts: torch.Tensor) -> bool:
-    """Plain CUDA tensors outside of any tracing: the kernels can be called without going through the dispatcher, which costs more
-    than they do on small problems."""
+    """Plain CUDA tensors outside of any tracing and of torch.func's transforms: the kernels can be called without going through the
+    dispatcher, which costs more than they do on small problems."""
     return not torch.compiler.is_compiling() and all([t.is_cuda and type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts]) \
-        and not torch._C._len_torch_dispatch_stack()
+        and not torch._C._len_torch_dispatch_stack() and not torch._C._are_functorch_transforms_active()
 
 
 def _no_tangents(*ts: torch.Tensor) -> None:

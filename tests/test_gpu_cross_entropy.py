@@ -745,3 +745,13 @@ def test_layer_loss_through_the_dispatcher(rb):
     loss2 = rb.rlinear_cross_entropy(x2, c2, 1003, 90, target, row0=5)
     grads2 = torch.autograd.grad(loss2, [x2, c2])
     assert torch.equal(loss, loss2) and all(torch.equal(a, b) for a, b in zip(grads, grads2))
+
+
+def test_vmap_takes_the_calls_one_by_one(rb):
+    x, w, target = inputs("linear", 40, 16, 30, torch.float32, 1)
+    c = torch.randn(8, 16, device="cuda")
+    xs, ts = x.view(4, 10, 16), target.view(4, 10)
+    for f in (lambda a, t: rb.linear_cross_entropy(a, w, t), lambda a, t: rb.noise_cross_entropy(a, 3, 30, t), lambda a, t: rb.rlinear_cross_entropy(a, c, 3, 30, t)):
+        with torch.no_grad():
+            got = torch.func.vmap(f)(xs, ts)
+            assert torch.equal(got, torch.stack([f(a, t) for a, t in zip(xs, ts)]))
