@@ -893,7 +893,7 @@ __device__ __noinline__ float sampled_top(const CeRowArgs &a, const Vocab &voc, 
 // One warp per gathered row: the row in bf16 parts, its target's logit (forward), or exponent offset, factor and target value of
 // the probabilities (backward).  Rows up to the tile's end are zeros that contribute nothing anywhere.
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) ce_gather_kernel(CeRowArgs a, Vocab voc) {
+__global__ void __launch_bounds__(256, 4) ce_gather_kernel(const __grid_constant__ CeRowArgs a, const __grid_constant__ Vocab voc) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;

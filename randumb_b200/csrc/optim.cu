@@ -44,6 +44,7 @@ struct AdamwTable {
 
 struct AdamwScalars {
     float b1, omb1, b2, omb2, eps;
+    bool fast;                            // see update_of
     double lr, ln_beta1, ln_beta2;         // natural logarithms; -inf for 0
     const float *lr_dev;                  // one float32 in device memory, or null: `lr`
     double weight_decay;
@@ -55,7 +56,6 @@ struct AdamwScalars {
 template <typename T> struct Vec4;
 template <> struct Vec4<float> { using V = float4; };
 template <> struct Vec4<__nv_bfloat16> { using V = uint2; };
-template <> struct Vec4<uint8_t> { using V = uint32_t; };
 
 template <bool VEC> __device__ __forceinline__ int elem_of(int lane, int j) {
     return VEC ? ((j >> 2) * 128 + lane * 4 + (j & 3)) : (j * 32 + lane);
@@ -125,6 +125,7 @@ __device__ __forceinline__ float divide_by(float x, float d, float inv) {
 }
 
 constexpr float V_MOST = 3e38f;         // largest second moment in 8 bits: 1.9375 times its scale is still finite
+__device__ __forceinline__ bool is_lost(float m, float v) { return !(fabsf(m) <= FLT_MAX && v <= V_MOST); }
 
 // Second moment in 8 bits: no sign, 4 exponent bits (bias 15), 4 mantissa bits; byte 255 stands for 1.9375 and carries the
 // block's maximum.  Shifted into a float32 the byte sits on top of exponent and mantissa, so its value is that float32 times
@@ -260,17 +261,16 @@ __device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, i
     if (MASTER) store8<VEC>(d.master + at, w8, lane, left);
     mmax = warp_max(mmax);
     vmax = warp_max(vmax);
-    if (!(mmax <= FLT_MAX && vmax <= V_MOST)) {
+    const bool in_range = mmax <= FLT_MAX && vmax <= V_MOST;
+    if (!in_range) {
         // Some element's moments have left the range: it is lost (first moment NaN from here on), and its block's others go on as if it were
         // not there.  An infinite scale would turn them all into 0 * infinity.
         mmax = vmax = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (!(fabsf(m[j]) <= FLT_MAX && v[j] <= V_MOST)) m[j] = NAN;
-            else {
-                mmax = fmaxf(mmax, fabsf(m[j]));
-                vmax = fmaxf(vmax, v[j]);
-            }
+            if (is_lost(m[j], v[j])) continue;
+            mmax = fmaxf(mmax, fabsf(m[j]));
+            vmax = fmaxf(vmax, v[j]);
         }
         mmax = warp_max(mmax);
         vmax = warp_max(vmax);
@@ -278,9 +278,9 @@ __device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, i
     mscale = __fmul_rn(mmax, 1.0f / 448.0f);
     vscale = __fmul_rn(vmax, 1.0f / 1.9375f);
     const uint32_t h0 = (uint32_t)at * SQ5_N1 + rseed;
-    // ordinary scales: multiply by the reciprocal; others divide, and a scale of zero gives zero, or NaN where the first moment is: its code
-    // holds NaN.  (The second moment's has none: 255, the block's largest.  An element never has it NaN alone.)
-    const bool easy = mscale > 1e-30f && vscale > 1e-30f && mscale < 1e30f && vscale < 1e30f;
+    // ordinary scales: multiply by the reciprocal (a NaN stays one); others divide, and a scale of zero gives zero, but NaN where an element is
+    // lost: the first moment's code holds NaN.  (The second moment's has none: 255, the block's largest.  An element never has it NaN alone.)
+    const bool easy = in_range && mscale > 1e-30f && vscale > 1e-30f && mscale < 1e30f && vscale < 1e30f;
     const float minv = easy ? __frcp_rn(mscale) : 0.0f, vinv = easy ? __frcp_rn(vscale) : 0.0f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -293,7 +293,7 @@ __device__ __forceinline__ void adamw_segment8(const AdamwDesc &d, int64_t at, i
                 qm[k] = divide_by(m[j], mscale, minv);
                 qv[k] = divide_by(v[j], vscale, vinv);
             } else {
-                qm[k] = mscale > 0.0f || m[j] != m[j] ? __fdiv_rn(m[j], mscale) : 0.0f;
+                qm[k] = is_lost(m[j], v[j]) ? NAN : mscale > 0.0f ? __fdiv_rn(m[j], mscale) : 0.0f;
                 qv[k] = vscale > 0.0f ? __fdiv_rn(v[j], vscale) : 0.0f;
             }
             code[k] = ue4m4_code(qv[k], v[j], sq5_tail(h0 + (uint32_t)elem_of<VEC>(lane, j) * SQ5_N1) >> 13);
@@ -343,6 +343,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, c
     const uint32_t segs = tab.first[tab.count];
     StepScalars c{};
     c.eps = s.eps;
+    c.fast = s.fast;
     float t_have = NAN;
     uint32_t g = blockIdx.x * (ADAMW_THREADS / 32) + (threadIdx.x >> 5);
     int ti = find_tensor(tab, g);
@@ -354,7 +355,6 @@ adamw_kernel(const __grid_constant__ AdamwTable<NT> tab, const AdamwScalars s, c
             const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
             c.size = (float)(lr / -expm1((double)t * s.ln_beta1));            // 1 - beta^t
             c.inv_root = 1.0f / sqrtf((float)-expm1((double)t * s.ln_beta2));
-            c.fast = s.eps >= FAST_EPS * c.inv_root;
             c.decay = (float)(1.0 - lr * s.weight_decay);
             t_have = t;
         }
@@ -567,6 +567,7 @@ extern "C" int rdb_adamw_step(const rdb_adamw_lists *lists, int param_dtype, int
     s.b2 = (float)h->beta2;
     s.omb2 = (float)(1.0 - h->beta2);
     s.eps = (float)h->eps;
+    s.fast = h->eps >= FAST_EPS / sqrt(1.0 - h->beta2);               // inv_root is largest at the first step
     s.lr = h->lr;
     s.ln_beta1 = log(h->beta1);
     s.ln_beta2 = log(h->beta2);
