@@ -755,3 +755,26 @@ def test_vmap_takes_the_calls_one_by_one(rb):
         with torch.no_grad():
             got = torch.func.vmap(f)(xs, ts)
             assert torch.equal(got, torch.stack([f(a, t) for a, t in zip(xs, ts)]))
+
+
+@pytest.mark.parametrize("kind", ["noise", "linear"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [1, 2, 5, 31, 32, 33, 40, 70])
+def test_wide_logits_of_small_vocabularies(rb, kind, dtype, V):
+    """Rows whose length asks for a look at other logits, over vocabularies that are all looked at, and just not."""
+    T, R, seed = 90, 72, V
+    x, w, target = inputs(kind, T, R, V, dtype, seed, 60.0)
+    check(rb, kind, x, w, target, seed, -100, "none", torch.ones(T, device="cuda"))
+
+
+def test_traced_by_torch_compile(rb):
+    """One graph without breaks, forward and backward, and the eager numbers."""
+    x, w, target = inputs("linear", 40, 16, 30, torch.float32, 1)
+    c = torch.randn(8, 16, device="cuda", requires_grad=True)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    for f, leaves in ((lambda: rb.linear_cross_entropy(x, w, target), [x, w]), (lambda: rb.noise_cross_entropy(x, 3, 30, target), [x]),
+                      (lambda: rb.rlinear_cross_entropy(x, c, 3, 30, target), [x, c])):
+        want = f()
+        got = torch.compile(f, backend="aot_eager", fullgraph=True)()
+        assert torch.equal(got, want)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves), torch.autograd.grad(want, leaves)))
