@@ -483,7 +483,8 @@ int rdb_grad_norm(float *norm, float *coef, const void *const *grads, const int6
  * target: int64 [T], the row's column in [0, V); with use_ignore, rows whose target equals ignore_index count for nothing: their
  * contents (infinities and NaN included) reach no result, their loss and gradient are 0.  Any other target outside [0, V) makes
  * the row's loss and gradient NaN.  reduction RDB_CE_NONE: loss per row; RDB_CE_SUM; RDB_CE_MEAN: over the rows that count (NaN
- * when none does).  x, w and the gradients are of type dtype, losses float32.
+ * when none does).  x, w and the gradients are of type dtype, losses float32.  float32 operands are split into three bf16 parts where
+ * there are more than four rows or a gradient is wanted: finite values of any size are exact, an infinity makes NaN of what it meets.
  *
  * rdb_ce_fwd   loss (one float32, or T of them for RDB_CE_NONE) and aux, float32 [2T + 1]: log-sum-exp per row, loss per row,
  *              number of rows that count.  dx_unit (may be null, only with w null): d(row's loss)/dx, float32, contiguous [T, R]: the gradient is

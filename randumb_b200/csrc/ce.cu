@@ -732,10 +732,15 @@ template <typename T> __device__ __forceinline__ float vocab_at(const Vocab &v, 
     return to_f32<T>(from_f32<T>(sq5_to_float(sq5_bits(v.row0 + (uint32_t)row, (uint32_t)col, v.seed))));
 }
 
+// The first of several bf16 parts: a finite value beyond bf16's largest (float32's lowest, as masks have it) must not round to infinity.
+__device__ __forceinline__ float first_part(float v) {
+    constexpr float MOST = 3.38953139e38f;
+    return fabsf(v) > MOST && fabsf(v) <= 3.402823466e38f ? copysignf(MOST, v) : v;
+}
 template <int PARTS> __device__ __forceinline__ void split_store(__nv_bfloat16 *dst, int64_t part_cols, int64_t c, float v) {
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
-        const __nv_bfloat16 h = __float2bfloat16_rn(v);
+        const __nv_bfloat16 h = __float2bfloat16_rn(PARTS > 1 && p == 0 ? first_part(v) : v);
         dst[p * part_cols + c] = h;
         v -= __bfloat162float(h);
     }
@@ -782,7 +787,10 @@ __device__ __forceinline__ uint4 pack_f8(const float (&f)[8]) {
 template <int PARTS> __device__ __forceinline__ void split_store8(__nv_bfloat16 *dst, int64_t part_cols, float (&f)[8]) {
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
-        const uint4 v = pack_f8(f);
+        float h[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[k] = PARTS > 1 && p == 0 ? first_part(f[k]) : f[k];
+        const uint4 v = pack_f8(h);
         *reinterpret_cast<uint4 *>(dst + p * part_cols) = v;
         if (p + 1 < PARTS) {
             float g[8];

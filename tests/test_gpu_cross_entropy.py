@@ -778,3 +778,28 @@ def test_traced_by_torch_compile(rb):
         got = torch.compile(f, backend="aot_eager", fullgraph=True)()
         assert torch.equal(got, want)
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves), torch.autograd.grad(want, leaves)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [3, 70, 700])
+def test_vocabulary_rows_masked_by_the_lowest_value(rb, dtype, T):
+    """The same with the type's lowest finite value: the masked rows' logits are -1e38 or below, and all gradients are finite."""
+    R, V, seed = 40, 300, 2
+    x, w, target = inputs("linear", T, R, V, dtype, seed)
+    x[:, 0] = x[:, 0].abs() + 0.5
+    off = torch.tensor([7, 100, 299], device="cuda")
+    target[torch.isin(target, off)] = 3
+    w[off, 0] = torch.finfo(dtype).min
+    keep = torch.ones(V, dtype=torch.bool, device="cuda")
+    keep[off] = False
+    place = keep.cumsum(0) - 1
+    xl, wl, xk, kl = (t.clone().requires_grad_() for t in (x, w, x, w[keep]))
+    loss, want = rb.linear_cross_entropy(xl, wl, target), rb.linear_cross_entropy(xk, kl, place[target])
+    with torch.no_grad():
+        alone = rb.linear_cross_entropy(x, w, target)
+    (dx, dw), (dk_x, dk) = torch.autograd.grad(loss, [xl, wl]), torch.autograd.grad(want, [xk, kl])
+    # the same numbers added in another order
+    assert abs(loss.item() / want.item() - 1) < 2.0 ** -19 and abs(alone.item() / want.item() - 1) < 2.0 ** -19
+    step = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -18
+    assert (dw[off] == 0).all() and (dw[keep].double() - dk.double()).abs().max() <= step * dk.double().abs().max()
+    assert (dx.double() - dk_x.double()).abs().max() <= step * dk_x.double().abs().max()
