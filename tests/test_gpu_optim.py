@@ -540,3 +540,16 @@ def test_the_first_step_is_not_captured(rb):
     graph.replay()
     torch.cuda.synchronize()
     assert opt.state[p]["step"].item() == 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sizes", [(1e25,), (1e-25,), (1e20, 1e-3), (1e-25, 1e-22, 0.0)])
+def test_grad_norm_of_values_whose_squares_leave_the_range(rb, dtype, sizes):
+    """g^2 is infinite or 0 in float32, the norm is neither."""
+    g = torch.Generator().manual_seed(1)
+    grads = [(torch.randn(k, generator=g).double() * s).to(dtype).cuda() for k in (3, 8192, 20001) for s in sizes]
+    want = math.sqrt(sum(float((t.double() ** 2).sum()) for t in grads))
+    norm, f = rb.optim.grad_norm(grads, max_norm=0.5)
+    # the eight squares a lane adds, as in test_grad_norm
+    assert abs(norm.item() / want - 1) <= 8 * U
+    assert abs(f.item() / min(1.0, 0.5 / (want + 1e-6)) - 1) <= 12 * U
