@@ -9,10 +9,11 @@
 // so no running maximum is needed: the sum never falls below the target's own 1, and small losses and the gradients of tokens
 // the model already knows come out of log1p and of a sum without the target, not of a difference of nearly equal numbers.  Float32
 // holds e_v up to 69 above the target's logit (s below 2^100 leaves room for the gradient).  Where the row's length says that the
-// largest of V random logits may lie 40 or more above the target's (|x| |w_t| / sqrt(R) is their standard deviation, largest_of(V)
-// of those the mean of the largest), a few sampled logits are computed, and where they say so too (sampled_top), the estimate takes the
-// target's place:  e_v = exp(l_v - l_t - d),  loss = log(1 + s exp(d)).  A row that leaves the range all the same, at either end, or
-// whose target then turns out to be likelier than all others together, is noticed and done again with its true maximum (ce_far_rows).
+// largest of V random logits will lie 40 or more above the target's (|x| |w_t| / sqrt(R) is their standard deviation, largest_of(V)
+// of those the mean of the largest), or over a stored matrix, whose logits need be neither independent nor about 0, where a few sampled
+// ones say so (sampled_top), that estimate takes the target's place:  e_v = exp(l_v - l_t - d),  loss = log(1 + s exp(d)).  A row that
+// leaves the range all the same, at either end, or whose target then turns out to be likelier than all others together, is noticed
+// and done again with its true maximum (ce_far_rows).
 //
 // Rows whose target is ignored are left out: the remaining rows are gathered to the front, and every later kernel works on that
 // many rows, a number that only the device knows.
@@ -824,17 +825,19 @@ template <int N> __device__ __forceinline__ float warp_sums(float (&v)[N], int l
     return l;
 }
 
-// Where the largest logit of a row will lie, from SAMPLES vocabulary rows spread evenly (the target's left out; exact where there are no
-// more): the logits' mean plus `spread` deviations, and at least the largest one seen.  `sigma` is the deviation that the row's length gives, which
-// holds for logits that are independent with mean 0.  Where the matrix's rows share a component, as trained ones do, it is too large, for
-// that lengthens all of them and spreads none: the samples' mean counts where it is four standard errors off 0, their deviation where it differs from
-// sigma by a factor of two.  Four samples are enough where they look as the length says, or where even sigma about their mean stays below `enough`.
-// By a warp, and for rows alone whose length says that they may need it.  8192 rows of 768, V = 50257, loss, logits of deviation 3 about -100: without
-// the samples every row was redone, 61 ms; with them none is, 0.55 (0.45 for logits about 0).
+// Where the largest logit of a row over a stored matrix will lie, from SAMPLES vocabulary rows spread evenly (the target's left out; exact
+// where there are no more): the logits' mean plus `spread` deviations, and at least the largest one seen.  `sigma` is the deviation that the row's
+// length gives, which holds for logits that are independent with mean 0 (over a noise matrix they are).  Where the matrix's rows share a component,
+// as trained ones do, it is too large, for that lengthens all of them and spreads none: so the samples' mean counts where it is four standard errors
+// off 0, and their deviation (which 32 samples know to 13 %) where sigma is 1.6 times as large, or half.  Four samples are enough where even sigma,
+// four standard errors above their mean, stays below `enough`: minus infinity then.  By a warp.  8192 rows of 768, V = 50257, loss, ms, by the length
+// alone -> with samples: logits of deviation 3 about -100, or of deviation 10 about 60 beside a common component that the rows of x do not have, 61
+// (every row was redone) -> 0.53; deviation 20 about 60 35 -> 0.54, about -300 61 -> 10; independent logits of deviation 2 0.49 -> 0.49, of deviation 8
+// to 40 0.49 -> 0.51 to 0.55.
 constexpr int SAMPLES = 32;
 template <typename T>
 __device__ __noinline__ float sampled_top(const CeRowArgs &a, const Vocab &voc, const T *src, int64_t target, float sigma, float enough, int lane) {
-    const bool vec = rows_aligned<T>(a.x, a.ldx) && (!voc.w || rows_aligned<T>(voc.w, voc.ldw));
+    const bool vec = rows_aligned<T>(a.x, a.ldx) && rows_aligned<T>(voc.w, voc.ldw);
     const int64_t done = vec ? a.R / 8 * 8 : 0;
     auto sample = [&](int k) -> int64_t {         // in the order 0, 1/2, 1/4, 3/4, ...
         if (a.V <= SAMPLES) return k < a.V ? k : a.V - 1;
@@ -865,12 +868,7 @@ __device__ __noinline__ float sampled_top(const CeRowArgs &a, const Vocab &voc, 
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int64_t v = sample(k0 + q);
-                if (voc.w) load_f8(w, reinterpret_cast<const T *>(voc.w) + v * voc.ldw + c);
-                else {
-                    const uint32_t h = sq5_lin_rows(voc.seed, voc.row0 + (uint32_t)v, (uint32_t)c).base;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = to_f32<T>(from_f32<T>(sq5_to_float(sq5_tail(h + (uint32_t)e * SQ5_N1))));
-                }
+                load_f8(w, reinterpret_cast<const T *>(voc.w) + v * voc.ldw + c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) acc[q] = fmaf(f[e], w[e], acc[q]);
             }
@@ -878,14 +876,13 @@ __device__ __noinline__ float sampled_top(const CeRowArgs &a, const Vocab &voc, 
         for (int64_t c = done + lane; c < a.R; c += 32) {
             const float f = to_f32<T>(src[c]);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[q] = fmaf(f, vocab_at<T>(voc, sample(k0 + q), c), acc[q]);
+            for (int q = 0; q < 4; ++q) acc[q] = fmaf(f, to_f32<T>(reinterpret_cast<const T *>(voc.w)[sample(k0 + q) * voc.ldw + c]), acc[q]);
         }
         const float l = warp_sums(acc, lane);
         if (lane / 4 == k0 / 4) mine = l;
         if (k0 == 0 && a.V > SAMPLES) {
             spread_of(mine, on && lane < 4, mean, dev);
-            if (dev < 2.0f * sigma && ((dev > 0.5f * sigma && fabsf(mean) < 2.0f * sigma) || mean + (a.spread + 1.0f) * sigma < enough))
-                return (dev > 0.5f * sigma && fabsf(mean) < 2.0f * sigma ? 0.0f : mean) + a.spread * sigma;
+            if (dev < 2.0f * sigma && mean + (a.spread + 2.0f) * sigma < enough) return -INFINITY;
         }
     }
     float most = on ? mine : -INFINITY;
@@ -894,8 +891,9 @@ __device__ __noinline__ float sampled_top(const CeRowArgs &a, const Vocab &voc, 
     if (a.V <= SAMPLES) return most;
     const float n = spread_of(mine, on, mean, dev);
     if (fabsf(mean) * sqrtf(n) < 4.0f * dev) mean = 0.0f;
-    if (dev > 0.5f * sigma && dev < 2.0f * sigma) dev = sigma;
-    return fmaxf(most, mean + a.spread * dev);
+    if (sigma > 1.6f * dev) sigma = 1.3f * dev;
+    else if (dev > 2.0f * sigma) sigma = dev;
+    return fmaxf(most, mean + a.spread * sigma);
 }
 
 // One warp per gathered row: the row in bf16 parts, its target's logit (forward), or exponent offset, factor and target value of
@@ -973,10 +971,10 @@ __global__ void __launch_bounds__(256, 4) ce_gather_kernel(const __grid_constant
     if (!a.dloss) {                                   // (the whole warp holds the sums)
         if (!known) dot = NAN;                        // a target outside the vocabulary: the row's loss says so
         const float sigma = sqrtf(xx) * sqrtf(ww / (float)a.R), top = sigma * a.spread;
-        if (top - dot >= 40.0f && top < 1e6f) {
-            d = sampled_top<T>(a, voc, src, t, sigma, dot + 40.0f, lane) - dot;
-            if (!(d >= 40.0f && d < 1e6f)) d = 0.0f;
-        }
+        if (!voc.w) d = top - dot;
+        // (stored: where the logits' mean is not 0, the target's may be high and the largest far above it all the same)
+        else if ((top - dot >= 40.0f || sigma * (a.spread + 3.0f) >= 60.0f) && top < 1e6f) d = sampled_top<T>(a, voc, src, t, sigma, dot + 60.0f, lane) - dot;
+        if (!(d >= 40.0f && d < 1e6f)) d = 0.0f;
     }
     if (lane == 0) {
         a.tcol[j] = known ? (int32_t)t : -1;

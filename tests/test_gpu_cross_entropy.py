@@ -803,3 +803,36 @@ def test_vocabulary_rows_masked_by_the_lowest_value(rb, dtype, T):
     step = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -18
     assert (dw[off] == 0).all() and (dw[keep].double() - dk.double()).abs().max() <= step * dk.double().abs().max()
     assert (dx.double() - dk_x.double()).abs().max() <= step * dk_x.double().abs().max()
+
+
+@pytest.mark.parametrize("mean,dev,idle", [(60.0, 15.0, 0.0), (400.0, 10.0, 0.0), (0.0, 10.0, 30.0), (-300.0, 10.0, 100.0), (0.0, 20.0, 0.0)])
+def test_logits_of_any_mean_take_the_ordinary_way(rb, mean, dev, idle):
+    """Logits of the given mean and deviation; `idle`: a common component of the matrix's rows that the rows of x do not have, which lengthens the
+    first and moves no logit.  No row needs the slow way, and losses are those of 64 bits."""
+    T, R, V = 2048, 256, 20000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, _ = torch.linalg.qr(torch.randn(R, 2, device="cuda", generator=g))
+    u, away = q[:, 0], q[:, 1]
+    x = torch.randn(T, R, device="cuda", generator=g)
+    x += (10 - x @ u)[:, None] * u
+    x -= (x @ away)[:, None] * away
+    target = torch.randint(0, V, (T,), device="cuda", generator=g)
+    noise = torch.randn(V, R, device="cuda", generator=g) / R ** 0.5
+    took = []
+    for m, s, i in ((0.0, 1.0, 0.0), (mean, dev, idle)):
+        w = noise * s
+        w = (w + (m / 10 - w @ u)[:, None] * u + (i - w @ away)[:, None] * away).bfloat16()
+        xx = x.bfloat16()
+        times = []
+        with torch.no_grad():
+            for _ in range(8):
+                a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                a.record()
+                loss = rb.linear_cross_entropy(xx, w, target, reduction="none")
+                b.record()
+                b.synchronize()
+                times.append(a.elapsed_time(b))
+        took.append(sorted(times)[2])
+        _, losses, *_, terms = plain(xx, w, target, None, "none", torch.ones(T, device="cuda"))
+        assert ((loss.double() - losses).abs() <= 2.0 ** -21 * losses + tolerances(torch.bfloat16, R, V, terms)[0]).all()
+    assert took[1] < 8 * took[0], took
