@@ -425,8 +425,8 @@ int rdb_gemm_dense_scatter(void *const *dst_ptrs, int ndst, size_t dst_offset_by
                            const rdb_call_options *options, int32_t *status, void *stream);
 
 /*
- * AdamW over a list of tensors in one launch (no counterpart in the reference, which calls torch.optim: modded-nanogpt/
- * train_gpt2.py:354-372).  For every element, with t the tensor's step count after this call has raised it by one:
+ * AdamW over a list of tensors, one update launch for up to 384 of them (no counterpart in the reference, which calls torch.optim:
+ * modded-nanogpt/train_gpt2.py:354-372).  For every element, with t the tensor's step count after this call has raised it by one:
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2          g: gradient times *grad_scale (1 when null)
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * in float32.  `lists` and `h` are HOST memory, read before the call returns; the pointers in them (`step`: the tensor's
@@ -440,15 +440,15 @@ int rdb_gemm_dense_scatter(void *const *dst_ptrs, int ndst, size_t dst_offset_by
  *                 (ceil(numel / RDB_ADAMW_BLOCK) of them).  exp_avg: float8 e4m3, rounded to nearest, scale = largest
  *                 magnitude * float32(1/448).  exp_avg_sq: no sign, 4 exponent bits (bias 15) and 4 mantissa bits, scale = largest value *
  *                 float32(1/1.9375), rounded down or up at random with the odds that keep the expectation (nearest would never let it
- *                 decay: 1 - beta2 is below half a step of any 8-bit format), never to 0 when positive.  The random bits are
- *                 the upper 19 of the 1-D noise word of (element index mod 2^32) under the seed
+ *                 decay: 1 - beta2 is below half a step of any 8-bit format), never to code 0 when positive (under a
+ *                 scale of 2^-131 the smallest values are 0 all the same).  The random bits are the upper 19 of the 1-D noise word of (element index mod 2^32) under the seed
  *                 h->seed + t * 0x9E3779B1 + i * 0x85EBCA6B (tensor i of the list): the same call gives the same bytes.
  *                 An element whose new moments leave float32's range (an infinite gradient, one whose square is infinite) is left out of its
  *                 block's scales; its first moment is NaN from then on, the other elements are as if its gradient had been 0.  So is
  *                 an element whose gradient is NaN (its second moment, whose code has no NaN, is stored as the block's largest).
  * Tensors may start at any address their element type allows (vector accesses where all of a tensor's pointers allow them).
- * Entries of the list must not overlap.  rdb_grad_norm (grads, numels, dtypes: HOST arrays): 2-norm over all gradients in float64 partial sums, repeatable;
- * coef (may be null) = min(1, max_norm / (norm + 1e-6)), the factor to pass as grad_scale.  workspace: 8-byte aligned.
+ * Entries of the list must not overlap.  rdb_grad_norm (grads, numels, dtypes: HOST arrays): 2-norm over all gradients in float64 partial sums
+ * (squares that leave float32's range included), repeatable; coef (may be null) = min(1, max_norm / (norm + 1e-6)), the factor to pass as grad_scale.  workspace: 8-byte aligned.
  */
 #define RDB_ADAMW_BLOCK 256
 #define RDB_NORM_BLOCKS 1184

@@ -7,7 +7,7 @@ reference package ``rten_cpp``):
 * ``ops``      torch.library operators (``rten::rlinear_fwd`` ..., ``rten::materialize_fwd`` ...)
 * ``RandumbTensor`` / ``CreateRandumbTensor``   storage-less tensor subclass + differentiable constructor
 * ``RandumbLinear`` / ``SillyLinear`` / ``SillyEmbedding`` / ``SillyConv2d`` / ``stepgen`` / ``listgen``   modules
-* ``optim``    AdamW over all tensors in one launch (moments in 32 or 8 bits), norm of all gradients
+* ``optim``    AdamW over up to 384 tensors in one update launch (moments in 32 or 8 bits), norm of all gradients
 * ``parallel`` row sharding over GPUs and the dC all-reduce
 * ``kernels``  tensor-level wrappers over the C ABI (``include/randumb_b200.h``)
 

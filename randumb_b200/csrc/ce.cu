@@ -1074,8 +1074,8 @@ __device__ __forceinline__ float loss_above(float up, float s) {
 // Rows whose sum left float32's range: their logits once more on CUDA cores, first the maximum and the sum relative to it, then, with
 // slots, the gradient itself, which goes to a row's first slot.  By the whole block (512 threads), for up to FAR of its rows at a time
 // (`far`: bit r is row j0 + r): a warp multiplies FAR_ROWS rows of the matrix with all of them.  Bound by what one SM can load
-// (stored) or hash (noise).  Among 8192 rows of 768, V = 50257, the call takes, ms: stored, loss, no such row 0.5, one 3.6, 1024 7.7 (one row at a
-// time, a logit per warp: 25 and 84); noise, loss and gradient 1.0, 16, 52 (53, 337); all logits of standard deviation 150, loss, 15 (478).
+// (stored) or hash (noise).  Among 8192 rows of 768, V = 50257, the call takes, ms: stored, loss, no such row 0.5, one 3.8, every eighth 8.0, the first 1024 in
+// a row 59 (one row at a time, a logit per warp: 25 and 84 for the first two); noise, loss and gradient 1.0, 16, 53, 412.
 constexpr int FAR = 2, FAR_ROWS = 4, FAR_COLS = 4;
 
 template <typename T>
@@ -1654,8 +1654,9 @@ static int ce_kb(const CePlan &p) { return p.nterm * (int)cdiv64(p.piece, BK); }
 // Rows per tile.  float32: 256 (the registers hold one sub-tile).  bf16: 512-row tiles are the faster ones where rows fill them (8192
 // rows; 4000 of R = 1024, V = 50257, loss and gradient: 683 against 724 us), by about a tenth: 256-row tiles win when they round the
 // rows up to a tenth less (600 rows: 183 against 214; 2100: 410 against 454; 1200: even), and for short contractions of few rows, where
-// the exponentials bound the logits and twice the tiles spread better (R = 200, V = 32003: 512 rows 61 against 64, 1600 rows 99 against
-// 106, 2100 rows 117 against 125; 4000 rows 177 against 173).
+// the exponentials bound the logits and twice the tiles spread better (V = 32003, us, loss and gradient: R = 200 512 rows 66 against 69, 1600 rows
+// 105 against 113; R = 512 82 against 87, 146 against 158, 2048 rows 159 against 160; R = 640 95 against 98, 179 against 189, but 2048 rows 196 against
+// 194; R = 200 4000 rows 177 against 173).
 static int ce_tile_rows(int64_t T, int64_t R, int dtype) {
     if (dtype == RDB_F32) return CE_TILE;
     const int64_t r256 = round_up(T, CE_TILE), r512 = round_up(T, 2 * CE_TILE);

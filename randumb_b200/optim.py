@@ -1,4 +1,4 @@
-"""Optimiser of a training step: AdamW over all tensors in one launch, and the norm of all gradients.
+"""Optimiser of a training step: AdamW over lists of tensors (one update launch for up to 384), and the norm of all gradients.
 
 ``adamw_step`` / ``grad_norm`` are the functional forms over lists of tensors; ``AdamW`` is the ``torch.optim.Optimizer`` on top of
 them.  Everything a step depends on that changes from step to step (gradients, step counts, clipping factor, optionally the
@@ -206,7 +206,8 @@ def _like(codes: torch.Tensor, values: torch.Tensor) -> torch.Tensor:
 
 
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW`` on one launch per (parameter type, gradient type) and group, with 32-bit or 8-bit moments.
+    """``torch.optim.AdamW`` on two launches (step counts, update) per (parameter type, gradient type), group and 384 tensors, with 32-bit or
+    8-bit moments.
 
     Args:
         params, lr, betas, eps, weight_decay: as torch.optim.AdamW; ``lr`` may be a one-element float32 CUDA tensor, read when the
