@@ -553,3 +553,31 @@ def test_grad_norm_of_values_whose_squares_leave_the_range(rb, dtype, sizes):
     # the eight squares a lane adds, as in test_grad_norm
     assert abs(norm.item() / want - 1) <= 8 * U
     assert abs(f.item() / min(1.0, 0.5 / (want + 1e-6)) - 1) <= 12 * U
+
+
+@pytest.mark.parametrize("gdtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_masters_step_as_float32_parameters_do(rb, gdtype, bits, shift):
+    """bf16 parameters with masters, either moments, either gradient type: masters and state are bit for bit those of float32 parameters, the
+    parameters their rounding."""
+    n = sum(SIZES)
+    runs = []
+    for pdtype in (torch.float32, torch.bfloat16):
+        ps, grads, ms, vs, carve = make(SIZES, pdtype, gdtype, 11, shift)
+        start = carve(torch.randn(n, generator=torch.Generator().manual_seed(12)))
+        kw = {}
+        if bits == 8:
+            ms, vs = [t.view(torch.float8_e4m3fn) for t in carve(torch.zeros(n, dtype=torch.uint8))], carve(torch.zeros(n, dtype=torch.uint8))
+            kw = {k: [torch.zeros(-(-t.numel() // 256), device="cuda") for t in ps] for k in ("exp_avg_scales", "exp_avg_sq_scales")}
+        if pdtype == torch.bfloat16:
+            kw["masters"] = start
+        else:
+            ps = start
+        steps = torch.zeros(len(SIZES), device="cuda")
+        for _ in range(3):
+            rb.optim.adamw_step(ps, grads, ms, vs, steps, lr=1e-2, seed=5, **kw)
+        runs.append((start, [t.view(torch.uint8) for t in ms], [t.view(torch.uint8) for t in vs]))
+    for a, b in zip(*runs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert all(torch.equal(p, w.to(torch.bfloat16)) for p, w in zip(ps, runs[1][0]))
